@@ -303,6 +303,28 @@ int peco_place_heads(const void* input, int64_t stride_batch, int64_t stride_hea
                      const float* cos, const float* sin, int norm, const void* weight, float eps, int batch,
                      int heads, int rows, int first, int length, int dims, int dtype, void* stream);
 
+/* Rotary positions with several axes. No counterpart in the reference, which takes tables. input and output
+ * [batch, heads, rows, dims] (dtype fp16/bf16/fp32, element strides of batch, head and row, channels adjacent,
+ * every row 16-byte aligned; dims a multiple of 8 up to 512): the first 2 * P channels of a row form P pairs,
+ * adjacent channels or (halves != 0, P a multiple of 8) channels i and i + P, and pair i turns by
+ * 2 pi * positions[batch, axis of i, row] * turns[i] (inverse != 0: back), in fp32, rounded once; later channels
+ * are copied. Axis a (of up to 4) has the next axis_pairs[a] pairs, P = their sum <= 128. positions: device memory,
+ * position_type 0 int32, 1 int64, 2 fp32, element strides of batch and axis, rows adjacent. turns [P] and
+ * axis_pairs [axes] are host memory, read during the call.
+ * input == output with the same strides is allowed. */
+int peco_rotary_axes(const void* input, int64_t in_batch, int64_t in_head, int64_t in_row, void* output,
+                     int64_t out_batch, int64_t out_head, int64_t out_row, const void* positions, int position_type,
+                     int64_t position_batch, int64_t position_axis, const double* turns, const int* axis_pairs,
+                     int axes, int halves, int inverse, int batch, int heads, int rows, int dims, int dtype,
+                     void* stream);
+
+/* peco_place_heads with the rotation of peco_rotary_axes (adjacent channels; halves must be 0) in place of tables. */
+int peco_place_heads_axes(const void* input, int64_t stride_batch, int64_t stride_head, int64_t stride_row,
+                          void* output, const void* positions, int position_type, int64_t position_batch,
+                          int64_t position_axis, const double* turns, const int* axis_pairs, int axes, int halves,
+                          int inverse, int norm, const void* weight, float eps, int batch, int heads, int rows,
+                          int first, int length, int dims, int dtype, void* stream);
+
 /* peco_sparse_attention without a workspace argument. No counterpart in the reference: it is
  * for callers that cannot allocate device memory (code under HIP graph capture, serving loops
  * that forbid hipMalloc). The work list lives in a static per-device array of 1048576 int32

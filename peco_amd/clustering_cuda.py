@@ -13,7 +13,7 @@ import itertools
 
 import torch
 
-from . import _native
+from . import _native, rotary
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
@@ -506,17 +506,28 @@ def pack_clustered(tensors, indices, labels, centroids, bits, video):
 def place_heads(part, output, first, tables=None, rms=None):
     """Write a projected tensor [B,H,R,D] (16-bit, any strides with adjacent channels and 16-byte
     aligned rows) to rows [first, first + R) of the head-major output [B,H,S,D], RMS-normalised over
-    the channels by rms = (weight [D] or None, eps) and rotated by tables = (cos, sin), fp32 [R, D],
-    over interleaved channel pairs when given (peco/processor.py:159-190)."""
+    the channels by rms = (weight [D] or None, eps) and rotated when tables are given: (cos, sin), fp32
+    [R, D], over interleaved channel pairs (peco/processor.py:159-190), or a ``rotary.RotaryPositions``
+    whose axes have the interleaved layout."""
     library = _library()
     b, h, rows, d = part.shape
-    cos, sin = tables if tables is not None else (None, None)
     weight, eps = rms if rms is not None else (None, 0.0)
+    norm = (int(rms is not None), _native.ptr(weight), eps)
+    sizes = (b, h, rows, first, output.shape[2], d, _DTYPES[part.dtype])
     with torch.cuda.device(part.device):
-        status = library.peco_place_heads(
-            _native.ptr(part), *part.stride()[:3], _native.ptr(output), _native.ptr(cos), _native.ptr(sin),
-            int(rms is not None), _native.ptr(weight), eps, b, h, rows, first, output.shape[2], d, _DTYPES[part.dtype],
-            _retain_on_current_stream(part.device, part, output, cos, sin, weight))
+        if isinstance(tables, rotary.RotaryPositions):
+            if tables.axes.layout != "interleaved":
+                raise ValueError("place_heads rotates interleaved channel pairs")
+            positions = rotary.check_positions(tables.axes, tables.positions, b, rows, d, part.device)
+            status = library.peco_place_heads_axes(
+                _native.ptr(part), *part.stride()[:3], _native.ptr(output),
+                *rotary.plan_arguments(tables.axes, positions), *norm, *sizes,
+                _retain_on_current_stream(part.device, part, output, positions, weight))
+        else:
+            cos, sin = tables if tables is not None else (None, None)
+            status = library.peco_place_heads(
+                _native.ptr(part), *part.stride()[:3], _native.ptr(output), _native.ptr(cos), _native.ptr(sin), *norm,
+                *sizes, _retain_on_current_stream(part.device, part, output, cos, sin, weight))
     _raise_cluster_error(status)
 
 

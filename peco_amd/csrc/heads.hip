@@ -18,8 +18,11 @@
 // heads, a dozen passes for the rotary embedding, most in fp32) took about 0.6 ms of the call. The
 // norm costs a reduction over the row's lanes by DPP moves and no memory pass; as a module of its own
 // it took 118 us per tensor of that shape (0.7 TB/s), the launch with it takes 22 us; the whole
-// double-stream call 1870 -> 1550 us.
-#include "common.hpp"
+// double-stream call 1870 -> 1550 us. With axes in place of tables (peco_place_heads_axes) a lane computes its
+// row's four angles itself (rotary.hpp) once for its heads and no table is read.
+#include "rotary.hpp"
+
+#include <type_traits>
 
 namespace peco {
 namespace {
@@ -66,8 +69,10 @@ template <int G> __device__ __forceinline__ float row_squares(const float (&v)[8
     return s[0] + s[1];
 }
 
-template <int DT, int D>
-__global__ __launch_bounds__(256) void place_heads_kernel(PlaceArgs a) {
+struct NoPlan {};  // rows rotated from tables, or not at all
+
+template <int DT, int D, typename Plan>
+__global__ __launch_bounds__(256) void place_heads_kernel(PlaceArgs a, Plan plan) {
     constexpr int G = D / 8;
     const int b = blockIdx.z;
     const int row = blockIdx.x * (256 / G) + threadIdx.x / G;
@@ -127,6 +132,18 @@ __global__ __launch_bounds__(256) void place_heads_kernel(PlaceArgs a) {
                 x[i][k + 1] = f32_to_half<DT>(im_c + re_s);
             }
     }
+    if constexpr (!std::is_same_v<Plan, NoPlan>) {
+        if (c0 < 2 * plan.pairs) {
+            float c[4], s[4];
+            rotary_angles<4>(plan, b, row, c0 / 2, c, s);
+#pragma unroll
+            for (int i = 0; i < kPlaceHeads; ++i) {
+                Chunk<DT> y{x[i]};
+                turn_adjacent(y, c0 / 2, plan.pairs, c, s);
+                x[i] = y.raw;
+            }
+        }
+    }
     uint16_t* dst = a.out + (static_cast<int64_t>(b) * a.heads + h0) * a.out_head + static_cast<int64_t>(row) * D + c0;
 #pragma unroll
     for (int i = 0; i < kPlaceHeads; ++i)
@@ -135,15 +152,10 @@ __global__ __launch_bounds__(256) void place_heads_kernel(PlaceArgs a) {
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-}  // namespace
-}  // namespace peco
-
-using namespace peco;
-
-PECO_API int peco_place_heads(const void* input, int64_t stride_batch, int64_t stride_head, int64_t stride_row,
-                              void* output, const float* cos, const float* sin, int norm, const void* weight, float eps,
-                              int batch, int heads, int rows, int first, int length, int dims, int dtype,
-                              void* stream) {
+template <typename Plan>
+int launch_place(const void* input, int64_t stride_batch, int64_t stride_head, int64_t stride_row, void* output,
+                 const float* cos, const float* sin, const Plan& plan, int norm, const void* weight, float eps,
+                 int batch, int heads, int rows, int first, int length, int dims, int dtype, void* stream) {
     if (!input || !output || !cos != !sin || (weight && !norm) || batch < 1 || heads < 1 || rows < 1 || first < 0 || length < rows ||
         first > length - rows)
         return kInvalidValue;
@@ -171,7 +183,7 @@ PECO_API int peco_place_heads(const void* input, int64_t stride_batch, int64_t s
     const dim3 grid(static_cast<unsigned>(ceil_div(rows, 256 / (dims / 8))),
                     static_cast<unsigned>(ceil_div(heads, kPlaceHeads)), static_cast<unsigned>(batch));
     const auto s = static_cast<hipStream_t>(stream);
-#define PECO_PLACE(DT_, D_) hipLaunchKernelGGL((place_heads_kernel<DT_, D_>), grid, dim3(256), 0, s, a)
+#define PECO_PLACE(DT_, D_) hipLaunchKernelGGL((place_heads_kernel<DT_, D_, Plan>), grid, dim3(256), 0, s, a, plan)
     if (dtype == kBF16) {
         if (dims == 128) PECO_PLACE(kBF16, 128);
         else PECO_PLACE(kBF16, 64);
@@ -181,4 +193,30 @@ PECO_API int peco_place_heads(const void* input, int64_t stride_batch, int64_t s
     }
 #undef PECO_PLACE
     return hipGetLastError();
+}
+
+}  // namespace
+}  // namespace peco
+
+using namespace peco;
+
+PECO_API int peco_place_heads(const void* input, int64_t stride_batch, int64_t stride_head, int64_t stride_row,
+                              void* output, const float* cos, const float* sin, int norm, const void* weight, float eps,
+                              int batch, int heads, int rows, int first, int length, int dims, int dtype,
+                              void* stream) {
+    return launch_place(input, stride_batch, stride_head, stride_row, output, cos, sin, NoPlan{}, norm, weight, eps,
+                        batch, heads, rows, first, length, dims, dtype, stream);
+}
+
+PECO_API int peco_place_heads_axes(const void* input, int64_t stride_batch, int64_t stride_head, int64_t stride_row,
+                                   void* output, const void* positions, int position_type, int64_t position_batch,
+                                   int64_t position_axis, const double* turns, const int* axis_pairs, int axes,
+                                   int halves, int inverse, int norm, const void* weight, float eps, int batch,
+                                   int heads, int rows, int first, int length, int dims, int dtype, void* stream) {
+    RotaryPlan plan;
+    if (halves || !make_plan(plan, positions, position_type, position_batch, position_axis, turns, axis_pairs, axes,
+                             halves, inverse, dims))
+        return kInvalidValue;
+    return launch_place(input, stride_batch, stride_head, stride_row, output, nullptr, nullptr, plan, norm, weight, eps,
+                        batch, heads, rows, first, length, dims, dtype, stream);
 }

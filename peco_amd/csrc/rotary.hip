@@ -1,0 +1,124 @@
+// Rotary positions with several axes over strided rows, forward and (with the inverse rotation) backward.
+//
+// x [batch, heads, rows, D] (any strides, channels adjacent, rows on 16 bytes) to an output of the same
+// shape and its own strides. The first 2 P channels of a row form P pairs, adjacent channels (2 i, 2 i + 1)
+// or halves (i, i + P), and pair i turns by its axis's position times its frequency (rotary.hpp):
+//   (a, b) -> (a cos - b sin, b cos + a sin), in fp32, rounded once to the type.
+// The rotation is orthogonal, so the gradient of the rows is the gradient of the output turned back.
+//
+// HBM-bound: each row is read and written once and the angles are computed, so no tables are read (fp32
+// tables of 118800 rows x 128 channels are 122 MB, a sixth of what 24 bf16 heads move, for each group of
+// heads that reads them). A lane holds 8 channels (16 for halves: 8 of each) of one row of kHeads heads with
+// all loads in flight and computes its 4 (8) angles once for all of them.
+#include "rotary.hpp"
+
+namespace peco {
+namespace {
+
+struct RotaryArgs {
+    const void* in;
+    void* out;
+    int64_t in_batch, in_head, in_row;  // strides in elements
+    int64_t out_batch, out_head, out_row;
+    int batch, heads, dims;
+    uint32_t rows;
+    uint32_t lanes;  // lanes per row
+};
+
+template <int DT, bool kHalves, int kHeads>
+__global__ __launch_bounds__(256) void rotary_axes_kernel(RotaryArgs a, RotaryPlan plan) {
+    const uint32_t item = blockIdx.x * 256u + threadIdx.x;
+    const uint32_t row = item / a.lanes;
+    if (row >= a.rows) return;
+    const int lane = static_cast<int>(item - row * a.lanes);
+    const int h0 = blockIdx.y * kHeads;
+    constexpr int kChunks = kHalves ? 2 : 1;
+    constexpr int kPairs = kHalves ? 8 : 4;
+    // Channels of this lane's chunks. Halves: chunk `lane` of either half, then one chunk a lane behind them.
+    const int half_lanes = plan.pairs / 8;
+    const bool tail = kHalves ? lane >= half_lanes : 4 * lane >= plan.pairs;
+    const int c0 = kHalves && tail ? 8 * (lane + half_lanes) : 8 * lane;
+    const int c1 = kHalves && !tail ? plan.pairs + 8 * lane : c0;
+    for (int b = blockIdx.z; b < a.batch; b += gridDim.z) {
+        const int64_t src = b * a.in_batch + static_cast<int64_t>(row) * a.in_row;
+        const int64_t dst = b * a.out_batch + static_cast<int64_t>(row) * a.out_row;
+        Chunk<DT> x[kHeads][kChunks];
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {  // clamped, unconditional: all loads in flight
+            const int64_t at = src + static_cast<int64_t>(min(h0 + i, a.heads - 1)) * a.in_head;
+            x[i][0].load(a.in, at + c0);
+            if constexpr (kHalves) x[i][1].load(a.in, at + c1);
+        }
+        if (!tail) {
+            float c[kPairs], s[kPairs];
+            rotary_angles<kPairs>(plan, b, row, kPairs * lane, c, s);
+#pragma unroll
+            for (int i = 0; i < kHeads; ++i) {
+                if constexpr (kHalves) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float u = x[i][0].get(k), v = x[i][1].get(k);
+                        x[i][0].set(k, u * c[k] - v * s[k]);
+                        x[i][1].set(k, v * c[k] + u * s[k]);
+                    }
+                } else {
+                    turn_adjacent(x[i][0], 4 * lane, plan.pairs, c, s);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+            if (h0 + i >= a.heads) break;
+            const int64_t at = dst + static_cast<int64_t>(h0 + i) * a.out_head;
+            x[i][0].store(a.out, at + c0);
+            if constexpr (kHalves) {
+                if (!tail) x[i][1].store(a.out, at + c1);
+            }
+        }
+    }
+}
+
+// Heads per lane: 8 keep 128 bytes a lane in flight for 16-bit rows; the wider forms take 4 for the registers.
+template <int DT, bool kHalves> int launch_rotary(const RotaryArgs& a, const RotaryPlan& plan, hipStream_t s) {
+    constexpr int kHeads = DT == kF32 || kHalves ? 4 : 8;
+    const int64_t blocks = ceil_div(static_cast<int64_t>(a.rows) * a.lanes, 256);
+    const int64_t groups = ceil_div(a.heads, kHeads);
+    if (groups > 65535) return kUnsupportedShape;
+    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(groups),
+                    static_cast<unsigned>(a.batch < 65535 ? a.batch : 65535));
+    hipLaunchKernelGGL((rotary_axes_kernel<DT, kHalves, kHeads>), grid, dim3(256), 0, s, a, plan);
+    return hipGetLastError();
+}
+
+}  // namespace
+}  // namespace peco
+
+using namespace peco;
+
+PECO_API int peco_rotary_axes(const void* input, int64_t in_batch, int64_t in_head, int64_t in_row, void* output,
+                              int64_t out_batch, int64_t out_head, int64_t out_row, const void* positions,
+                              int position_type, int64_t position_batch, int64_t position_axis, const double* turns,
+                              const int* axis_pairs, int axes, int halves, int inverse, int batch, int heads, int rows,
+                              int dims, int dtype, void* stream) {
+    RotaryPlan plan;
+    if (!input || !output || batch < 1 || heads < 1 || rows < 1 ||
+        !make_plan(plan, positions, position_type, position_batch, position_axis, turns, axis_pairs, axes, halves,
+                   inverse, dims))
+        return kInvalidValue;
+    if (dims < 8 || dims > 512 || dims % 8) return kUnsupportedShape;
+    if (dtype != kBF16 && dtype != kF16 && dtype != kF32) return kUnsupportedDtype;
+    const int64_t lanes = halves ? plan.pairs / 8 + (dims - 2 * plan.pairs) / 8 : dims / 8;
+    if (static_cast<int64_t>(rows) * lanes > 0x7fffff00) return kUnsupportedShape;
+    const int per16 = dtype == kF32 ? 4 : 8;  // elements in 16 bytes: every row of every head must start on them
+    const int64_t strides = in_batch | in_head | in_row | out_batch | out_head | out_row;
+    if (strides % per16 || reinterpret_cast<uintptr_t>(input) % 16 || reinterpret_cast<uintptr_t>(output) % 16)
+        return kInvalidValue;
+    RotaryArgs a{input,     output,   in_batch, in_head, in_row, out_batch, out_head,
+                 out_row,   batch,    heads,    dims,    static_cast<uint32_t>(rows), static_cast<uint32_t>(lanes)};
+    const auto s = static_cast<hipStream_t>(stream);
+    switch (dtype) {
+        case kBF16: return halves ? launch_rotary<kBF16, true>(a, plan, s) : launch_rotary<kBF16, false>(a, plan, s);
+        case kF16: return halves ? launch_rotary<kF16, true>(a, plan, s) : launch_rotary<kF16, false>(a, plan, s);
+        default: return halves ? launch_rotary<kF32, true>(a, plan, s) : launch_rotary<kF32, false>(a, plan, s);
+    }
+}

@@ -26,6 +26,7 @@ from . import _native, clustering_cuda
 from .attention_cuda import base_offset_attention, dense_supported, sparse_attention, sparse_attention_work
 from .attention_cuda import dense_attention as dense_attention_hip
 from .quantization import _validate_bits
+from .rotary import RotaryPositions, check_positions, rotary_axes
 
 
 @dataclass(frozen=True)
@@ -153,9 +154,20 @@ def _published_rotary(fn):
                                        getattr(fn, "__name__", "") == "apply_rotary_emb")
 
 
-def _rotary_tables(fn, freqs, rows, dim, device):
-    """(cos, sin) when the rotary embedding is the published one over plain fp32 [rows, dim] tables
-    that the placing kernel can read, else None."""
+def _rotate(fn, part, freqs):
+    """The rows of ``part`` [B, H, rows, D] turned: by their positions, or by ``fn`` with the caller's tables."""
+    return rotary_axes(part, freqs.positions, freqs.axes) if isinstance(freqs, RotaryPositions) else fn(part, freqs)
+
+
+def _rotary_tables(fn, freqs, part):
+    """What the placing kernel rotates ``part`` [B, H, rows, D] with: (cos, sin) when the rotary embedding is the
+    published one over plain fp32 [rows, D] tables that it can read, positions whose axes pair adjacent channels,
+    else None."""
+    batch, _, rows, dim = part.shape
+    device = part.device
+    if isinstance(freqs, RotaryPositions):
+        check_positions(freqs.axes, freqs.positions, batch, rows, dim, device)
+        return freqs if freqs.axes.layout == "interleaved" else None
     if not _published_rotary(fn) or not isinstance(freqs, (tuple, list)) or len(freqs) != 2 or \
             not all(isinstance(t, torch.Tensor) for t in freqs) or not _native.plain_tensors(*freqs):
         return None
@@ -376,7 +388,8 @@ class PecoAttention:
         part is written once, head-major, into its slot of one [3, B, H, S, D] buffer, so no
         concatenation copies are made; one launch per projection splits the heads, applies a plain
         RMS norm and the rotary embedding and places the rows (torch operations do it for tensors that
-        launch does not take). Video rows get the rotary embedding; text rows never do. Double-stream blocks
+        launch does not take). Video rows get the rotary embedding (``image_rotary_emb``: (cos, sin) tables, or a
+        ``rotary.RotaryPositions`` whose angles that launch computes); text rows never do. Double-stream blocks
         (``add_q_proj`` set) project the text with their added projections and norms,
         single-stream blocks with the same ones as the video.
         """
@@ -404,7 +417,7 @@ class PecoAttention:
                 place = (turn or size > (_COPY_ELEMENTS if norm is None else _NORM_ELEMENTS)) and _placeable(part, None)
                 projected, tables, rms = part, None, None
                 if place and turn:
-                    tables = _rotary_tables(rotary, freqs, rows, part.shape[3], part.device)
+                    tables = _rotary_tables(rotary, freqs, part)
                     turn = tables is None  # by torch
                 if place and norm is not None and not turn:
                     rms = _rms_norm(norm, part)
@@ -413,7 +426,7 @@ class PecoAttention:
                     swap = part.is_cuda and _per_channel_norm(norm)
                     part = norm(part.transpose(1, 2)).transpose(1, 2) if swap else norm(part)
                 if turn:
-                    part = rotary(part, freqs)
+                    part = _rotate(rotary, part, freqs)
                 if qkv is None:
                     batch, heads, _, dim = part.shape
                     qkv = torch.empty((3, batch, heads, length, dim), dtype=part.dtype, device=part.device)
@@ -422,7 +435,7 @@ class PecoAttention:
                     clustering_cuda.place_heads(part, qkv[slot], first, tables, rms)
                 else:
                     part = part if rms is None else norm(part)
-                    qkv[slot, :, :, first:first + rows] = part if tables is None else rotary(part, freqs)
+                    qkv[slot, :, :, first:first + rows] = part if tables is None else _rotate(rotary, part, freqs)
             first += rows
         output = self.attention(qkv[0], qkv[1], qkv[2]).transpose(1, 2)  # [B, S, H, D] view
         video = hidden_states.shape[1]
