@@ -325,6 +325,41 @@ int peco_place_heads_axes(const void* input, int64_t stride_batch, int64_t strid
                           int inverse, int norm, const void* weight, float eps, int batch, int heads, int rows,
                           int first, int length, int dims, int dtype, void* stream);
 
+/* Attention with a sliding window and sinks. No counterpart in the reference. q and output [batch, q_heads,
+ * queries, d], k and v [batch, kv_heads, keys, d] (fp16/bf16, d 64 or 128; q_heads a multiple of kv_heads, query
+ * head h reads key head h / (q_heads / kv_heads)). strides: host memory, element strides of batch, head and row
+ * of q, k, v and output (12 values, multiples of 8; channels adjacent, tensors 16-byte aligned). Queries and keys
+ * end together: query i stands at p = i + keys - queries and sees key j when j <= p + right and (j >= p - left or
+ * j < sinks); left or right -1 is without limit. A query that sees no key gives 0. lengths (nullable, device,
+ * int32 [batch], needs queries == keys): tokens of each sequence of a padded batch (clamped to [0, keys]); later
+ * keys are not seen and later queries give 0. scale: positive, of the scores. row_max and row_log (both or
+ * neither, fp32 [batch, q_heads, queries]) receive each row's largest unscaled score and the log2 of its sum for
+ * peco_window_attention_grad. workspace: peco_window_attention_workspace_size floats, 16-byte aligned (calls that
+ * overlap need one each; may be null when that is 0). */
+size_t peco_window_attention_workspace_size(int batch, int q_heads, int kv_heads, int queries, int keys, int left,
+                                            int right, int sinks, int d);
+int peco_window_attention(const void* q, const void* k, const void* v, void* output, const int64_t* strides,
+                          const int32_t* lengths, float* row_max, float* row_log, float* workspace,
+                          size_t workspace_floats, int batch, int q_heads, int kv_heads, int queries, int keys,
+                          int left, int right, int sinks, float scale, int d, int dtype, void* stream);
+
+/* Attention of new tokens over a paged cache, with the same window (right 0) and sinks. q and output [tokens,
+ * q_heads, d] hold the new tokens of `batch` sequences in a row: sequence b has rows offsets[b] .. offsets[b+1]-1
+ * (int32 [batch + 1], ascending) and lengths[b] tokens in the cache (int32 [batch]), the new ones, already
+ * appended, last. Token t of a sequence is slot t % page of page page_table[b * table_stride + t / page] (int32,
+ * table_width entries) of k_pages and v_pages [pages, kv_heads, page, d]. strides: host memory, element strides of
+ * head and token of q, of page, head and row of k_pages and of v_pages, of head
+ * and token of output (10 values). Keys on a page outside [0, pages) are not seen; lengths and offsets are clamped
+ * to the table and to the tokens, so no entry of theirs reads or writes out of bounds. Rows of no sequence are
+ * left as they were, or cleared with clear_tail != 0. workspace as above. */
+size_t peco_paged_attention_workspace_size(int batch, int q_heads, int kv_heads, int tokens, int table_width, int page,
+                                           int left, int sinks, int d);
+int peco_paged_attention(const void* q, const void* k_pages, const void* v_pages, void* output,
+                         const int64_t* strides, const int32_t* page_table, int64_t table_stride,
+                         const int32_t* offsets, const int32_t* lengths, int clear_tail, float* workspace,
+                         size_t workspace_floats, int batch, int q_heads, int kv_heads, int tokens, int pages, int page,
+                         int table_width, int left, int sinks, float scale, int d, int dtype, void* stream);
+
 /* peco_sparse_attention without a workspace argument. No counterpart in the reference: it is
  * for callers that cannot allocate device memory (code under HIP graph capture, serving loops
  * that forbid hipMalloc). The work list lives in a static per-device array of 1048576 int32

@@ -8,7 +8,8 @@ so state such as the loaded HIP library is shared between the two names.
 import importlib
 import sys
 
-_MODULES = ("processor", "clustering", "quantization", "clustering_cuda", "attention_cuda", "model", "rotary")
+_MODULES = ("processor", "clustering", "quantization", "clustering_cuda", "attention_cuda", "model", "rotary",
+            "window", "paged")
 
 for _name in _MODULES:
     _module = importlib.import_module(f"peco_amd.{_name}")

@@ -99,6 +99,7 @@ def build_library(force: bool = False, jobs: int | None = None) -> Path:
 P, I, Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
 PP = ctypes.POINTER(ctypes.c_void_p)
 IP = ctypes.POINTER(ctypes.c_int)
+LP = ctypes.POINTER(ctypes.c_int64)
 # Rotary positions: positions, their type and strides (batch, axis), turns and pairs of the axes (host), their
 # number, the layout and the direction.
 PLAN = [P, I, ctypes.c_int64, ctypes.c_int64, ctypes.POINTER(ctypes.c_double), IP, I, I, I]
@@ -143,6 +144,10 @@ SIGNATURES = {
     "peco_dense_attention_workspace_size": (Z, [I, I]),
     "peco_dense_attention": (I, [P] * 4 + [I, P, Z] + [I] * 4 + [P]),
     "peco_place_heads": (I, [P] + [ctypes.c_int64] * 3 + [P] * 3 + [I, P, ctypes.c_float] + [I] * 7 + [P]),
+    "peco_window_attention_workspace_size": (Z, [I] * 9),
+    "peco_window_attention": (I, [P] * 4 + [LP] + [P] * 4 + [Z] + [I] * 8 + [ctypes.c_float, I, I, P]),
+    "peco_paged_attention_workspace_size": (Z, [I] * 9),
+    "peco_paged_attention": (I, [P] * 4 + [LP, P, ctypes.c_int64, P, P, I, P, Z] + [I] * 9 + [ctypes.c_float, I, I, P]),
     "peco_rotary_axes": (I, [P] + [ctypes.c_int64] * 3 + [P] + [ctypes.c_int64] * 3 + PLAN + [I] * 5 + [P]),
     "peco_place_heads_axes": (I, [P] + [ctypes.c_int64] * 3 + [P] + PLAN + [I, P, ctypes.c_float] + [I] * 7 + [P]),
     "peco_base_offset_attention": (I, [P, P, P, I] + [P] * 9 + [I, I] + [P] * 5 + [Z] + [I] * 8 + [P]),

@@ -30,6 +30,7 @@
 // (fusing restore_sequence_order, peco/clustering.py:128-136).
 #include "base_offset.hpp"
 #include "common.hpp"
+#include "mfma.hpp"
 #include "work.hpp"
 
 #include <algorithm>
@@ -217,41 +218,6 @@ __global__ __launch_bounds__(kBuildWaves * kWave) void build_work_kernel(const u
                         tmp);
 }
 
-template <int DT> struct Mfma;
-template <> struct Mfma<kBF16> {
-    static __device__ __forceinline__ f32x16 run(u16x8 a, u16x8 b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
-                                                       0, 0, 0);
-    }
-    // Two fp32 -> packed pair with round-to-nearest-even (v_cvt_pk_bf16_f32).
-    static __device__ __forceinline__ uint32_t pack2(float a, float b) {
-        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-        typedef float f2 __attribute__((ext_vector_type(2)));
-        return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{a, b}, b2));
-    }
-    // acc + lo(p) + hi(p) of a packed pair (v_dot2_f32_bf16 against (1, 1)).
-    static __device__ __forceinline__ float sum2(uint32_t p, float acc) {
-        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, p), __builtin_bit_cast(b2, 0x3f803f80u), acc,
-                                               false);
-    }
-};
-template <> struct Mfma<kF16> {
-    static __device__ __forceinline__ f32x16 run(u16x8 a, u16x8 b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c,
-                                                      0, 0, 0);
-    }
-    static __device__ __forceinline__ uint32_t pack2(float a, float b) {
-        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-        typedef float f2 __attribute__((ext_vector_type(2)));
-        return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{a, b}, h2));
-    }
-    static __device__ __forceinline__ float sum2(uint32_t p, float acc) {
-        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-        return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, p), __builtin_bit_cast(h2, 0x3c003c00u), acc, false);
-    }
-};
-
 // K and V tiles live in LDS row-major ([64 keys][D], no padding) and are filled straight
 // from global memory with 16-byte global_load_lds, which writes each wave's 64 lanes to one
 // contiguous 1 KB span. Bank conflicts are avoided by XOR-swizzling the 16-byte chunks of a
@@ -306,8 +272,6 @@ __device__ __forceinline__ void load_tile_lds(uint16_t* ks, uint16_t* vs, const 
     }
 #endif
 }
-
-typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // Input modes:
 //   kPacked: Q, K and V in cluster order (out_index, when given, only scatters the output);

@@ -1,0 +1,745 @@
+// Attention with a sliding window and sinks, over tensors or over a paged cache: forward.
+//
+//   out_i = sum_j softmax_j(scale q_i . k_j) v_j over the keys j that query i sees (window.hpp), 0 for a query
+//   that sees none.
+//
+// A workgroup of 4 wavefronts takes 128 rows of one key head's row stream (its `group` query heads, token by
+// token) and walks the keys that any of them sees in 64-row tiles: direct loads of the next tile's K and V
+// into the other LDS buffer are in flight during the products of the current one, one barrier a tile.
+//   S^T = K Q^T (32x32x16 MFMA, A = K tile rows, B = Q^T in registers): lane l holds query l % 32, keys
+//         8 (i / 4) + 4 (l / 32) + i % 4 of a 32-key half;
+//   softmax with the running maximum and sum in fp32, a lane's query its own column;
+//   O^T += V^T P^T (A = V tile by transpose reads, B = P^T straight from the S^T accumulators).
+// Tiles that every row of a wave sees whole run without any mask; those at the edges of the window, of the
+// causal triangle and of the stream take per-element comparisons, halves that no row of the wave sees are left
+// out. Items of at most 64 rows pair the waves: two waves take the same 32 rows and one 32-key half of every
+// tile each, and join their states at the end.
+//
+// With few items the key stream is cut into `splits` parts, whose unnormalised fp32 outputs, maxima and sums
+// a second launch joins.
+//
+// Roundings: scores, softmax statistics and O are fp32. P is rounded to the type for the second product (the
+// sum takes the rounded values, so that the weights still add up to 1), out once at the end. O is rescaled at
+// every new maximum, so a row's largest weight is 1 when it is rounded.
+#include "window.hpp"
+
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+#include <type_traits>
+
+namespace peco {
+namespace {
+
+// Scaled scores past which the maximum is subtracted before the multiplication: exp2(fma(s, scale, -m scale))
+// rounds m * scale first, 2^-14 of an exponent off at this size.
+constexpr float kWideScores = 0x1p10f;
+
+struct WindowArgs {
+    const uint16_t *q, *k, *v;
+    uint16_t* out;
+    Strides qs, os, ks, vs;  // paged: ks.b, vs.b are the page strides, qs.b, os.b are 0
+    int heads, group;        // key heads, query heads of each
+    int batch, queries, keys;  // paged: sequences, all new tokens, capacity of a table row in keys
+    int left, right, sinks;
+    float scale_log2;
+    const int32_t* lengths;  // contiguous: nullable valid tokens [batch]; paged: tokens held [batch]
+    const int32_t* offsets;  // paged: first new token of each sequence [batch + 1]
+    const int32_t* table;    // paged: page of each `page` tokens [batch, table_width]
+    int64_t table_stride;
+    int table_width, page, pages;
+    int tiles;               // row tiles per key head (paged: an upper bound)
+    int splits;
+    int clear_tail;          // paged: rows outside every sequence are cleared
+    float* part_o;           // [splits, rows, D] with splits > 1
+    float2* part_ml;         // [splits, rows]
+    float* row_max;          // nullable: raw maximum and log2 of the sum of every row (for the backward pass)
+    float* row_log;
+};
+
+// Where a workgroup's rows are.
+struct Item {
+    int b, kvh, split;
+    int row0, rows;    // rows of the stream of (b, kvh)
+    int first_token;   // of the sequence within q/out
+    int position0;     // position of the sequence's first query
+    int queries;       // queries of the sequence that take part (later rows see nothing)
+    int keys;
+};
+
+enum WindowMode : int {
+    kNear = 0,   // tensors whose heads' rows lie within 2^32 bytes: 32-bit offsets from the head
+    kFar = 1,    // tensors of any size
+    kPaged = 2,  // pages of a cache
+};
+
+// Item of workgroup g. Contiguous: heads fastest (with a multiple of 8 of them every head stays on one XCD),
+// the last row tiles, which see most under a causal mask, first. Paged: heads fastest, then splits, then
+// the row tiles of the sequences in order; false past the last of them.
+template <int kMode> __device__ __forceinline__ bool find_item(const WindowArgs& A, int64_t g, Item& it) {
+    if constexpr (kMode != kPaged) {
+        const int heads = A.batch * A.heads;
+        const int bh = static_cast<int>(g % heads);
+        const int64_t rest = g / heads;
+        it.split = static_cast<int>(rest % A.splits);
+        const int tile = A.tiles - 1 - static_cast<int>(rest / A.splits);
+        it.b = bh / A.heads;
+        it.kvh = bh % A.heads;
+        it.first_token = 0;
+        it.row0 = tile * kWinRows;
+        it.rows = min(kWinRows, A.queries * A.group - it.row0);
+        it.queries = A.queries;
+        it.keys = A.keys;
+        it.position0 = A.keys - A.queries;
+        if (A.lengths) it.keys = it.queries = max(0, min(A.lengths[it.b], A.keys));  // (queries == keys)
+        return true;
+    } else {
+        it.kvh = static_cast<int>(g % A.heads);
+        const int64_t rest = g / A.heads;
+        it.split = static_cast<int>(rest % A.splits);
+        int tile = static_cast<int>(rest / A.splits);
+        const int lane = threadIdx.x % kWave;
+        for (int b0 = 0; b0 < A.batch; b0 += kWave) {
+            const int b = min(b0 + lane, A.batch - 1);
+            const int o0 = max(0, min(A.offsets[b], A.queries)), o1 = max(0, min(A.offsets[b + 1], A.queries));
+            const int n = b0 + lane < A.batch ? max(0, o1 - o0) : 0;
+            const int tiles = static_cast<int>(ceil_div(static_cast<int64_t>(n) * A.group, kWinRows));
+            int upto = tiles;  // tiles of the sequences up to this lane's
+#pragma unroll
+            for (int d = 1; d < kWave; d *= 2) {
+                const int below = __shfl_up(upto, d, kWave);
+                if (lane >= d) upto += below;
+            }
+            const uint64_t past = __ballot(upto > tile);
+            if (past) {
+                const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
+                it.b = b0 + at;
+                it.first_token = __shfl(o0, at, kWave);
+                it.queries = __shfl(n, at, kWave);
+                it.row0 = (tile - __shfl(upto - tiles, at, kWave)) * kWinRows;
+                it.rows = min(kWinRows, it.queries * A.group - it.row0);
+                it.keys = max(0, min(A.lengths[it.b], A.keys));
+                it.position0 = it.keys - it.queries;
+                return true;
+            }
+            tile -= __shfl(upto, kWave - 1, kWave);
+        }
+        it.row0 = tile;  // number among the workgroups without rows
+        return false;
+    }
+}
+
+// Clears the output rows that belong to no sequence (those before the first offset and behind the last). There
+// is always a workgroup without rows (A.tiles is larger than any number of row tiles): the first one does it.
+template <int D> __device__ void clear_tail(const WindowArgs& A, int kvh) {
+    const int o0 = max(0, min(A.offsets[0], A.queries)), o1 = max(o0, min(A.offsets[A.batch], A.queries));
+    constexpr int CH = D / 8;
+    const int64_t n = (static_cast<int64_t>(o0) + (A.queries - o1)) * A.group * CH;
+    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
+        const int64_t r = i / CH, t = r / A.group;
+        const int64_t token = t < o0 ? t : t - o0 + o1, head = static_cast<int64_t>(kvh) * A.group + r % A.group;
+        *reinterpret_cast<u16x8*>(A.out + head * A.os.h + token * A.os.s + 8 * (i % CH)) = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    }
+}
+
+template <int DT, int D, int kMode>
+__global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
+    using T = WinTile<D>;
+    constexpr int S = D / 16, NB = D / 32, H = 2;
+    __shared__ __align__(16) uint16_t kvs[4][T::kElems];
+    uint16_t(*const ks)[T::kElems] = kvs;
+    uint16_t(*const vs)[T::kElems] = kvs + 2;
+    static_assert(2 * kWave * (NB * 16 + 2) * sizeof(float) <= sizeof(kvs), "pair exchange exceeds the tile LDS");
+    // Far and paged rows: offsets (bytes) of a tile's K and V rows, whether each row counts, and page numbers
+    // on their way (loaded two tiles before they are used).
+    constexpr int kRowLds = kMode == kNear ? 1 : kWinTile;
+    __shared__ int64_t k_off[2][kRowLds], v_off[2][kRowLds];
+    __shared__ uint16_t counts[4][4];  // (read during a tile, when those two tiles on are written)
+    __shared__ int page_of[2][kRowLds];
+
+    Item it;
+    const bool found = find_item<kMode>(A, blockIdx.x, it);
+    if (kMode == kPaged && !found) {
+        if (A.clear_tail && it.split == 0 && it.row0 == 0) clear_tail<D>(A, it.kvh);
+        return;
+    }
+    const int tid = threadIdx.x, lane = tid % kWave, h = lane / 32;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    it.keys = __builtin_amdgcn_readfirstlane(it.keys);
+    it.queries = __builtin_amdgcn_readfirstlane(it.queries);
+    it.position0 = __builtin_amdgcn_readfirstlane(it.position0);
+    it.row0 = __builtin_amdgcn_readfirstlane(it.row0);
+    it.rows = __builtin_amdgcn_readfirstlane(it.rows);
+    it.b = __builtin_amdgcn_readfirstlane(it.b);
+    it.first_token = __builtin_amdgcn_readfirstlane(it.first_token);
+
+    const bool split = it.rows <= 32 * H;
+    const int rb = split ? wave % H : wave;
+    const int hb = split ? wave / H : 0;
+    const bool wave_active = rb * 32 < it.rows;
+    const int lrow = it.row0 + rb * 32 + lane % 32;  // this lane's row of the stream
+    const bool qvalid = rb * 32 + lane % 32 < it.rows;
+    const int token = min(lrow, it.row0 + it.rows - 1) / A.group;
+    const int head = it.kvh * A.group + (min(lrow, it.row0 + it.rows - 1) - token * A.group);
+
+    u16x8 qf[S];
+    {
+        const int64_t bq = kMode == kPaged ? 0 : it.b;
+        const uint16_t* qrow = A.q + bq * A.qs.b + head * A.qs.h + static_cast<int64_t>(it.first_token + token) * A.qs.s;
+#pragma unroll
+        for (int s = 0; s < S; ++s) qf[s] = *reinterpret_cast<const u16x8*>(qrow + 16 * s + 8 * h);
+    }
+    // Keys of this tile of rows, and in stream rows what this lane's query and the wave's rows see.
+    const int t_first = it.row0 / A.group, t_last = min((it.row0 + it.rows - 1) / A.group, it.queries - 1);
+    const KeyStream stream = t_first > t_last ? KeyStream{0, 0, 0}
+                                              : key_stream(it.position0 + t_first, it.position0 + t_last, it.keys,
+                                                           A.left, A.right, A.sinks);
+    const int L = stream.length;
+    const int all_tiles = static_cast<int>(ceil_div(L, kWinTile));
+    const int per = static_cast<int>(ceil_div(all_tiles, A.splits));
+    const int tile0 = min(it.split * per, all_tiles), tile1 = min(tile0 + per, all_tiles);
+    const int pos = it.position0 + token;
+    const bool sees = qvalid && token < it.queries;
+    const int last_r = sees ? min(min(pos + A.right, it.keys - 1) - stream.delta, L - 1) : -1;
+    const int first_r = pos - A.left - stream.delta;
+    // Of the wave's rows that exist: every one sees [w_first, w_last] and the sinks up to w_last; rows past
+    // w_any, and between the sinks and w_from, none of them sees.
+    const int w_row0 = min(it.row0 + rb * 32, it.row0 + it.rows - 1);
+    const int w_row1 = min(it.row0 + rb * 32 + 31, it.row0 + it.rows - 1);
+    const int w_tok0 = w_row0 / A.group, w_tok1 = w_row1 / A.group;
+    const int w_last = w_tok1 < it.queries
+                           ? min(min(it.position0 + w_tok0 + A.right, it.keys - 1) - stream.delta, L - 1) : -1;
+    const int w_first = it.position0 + w_tok1 - A.left - stream.delta;
+    const int w_any = min(min(it.position0 + w_tok1 + A.right, it.keys - 1) - stream.delta, L - 1);
+    const int w_from = it.position0 + w_tok0 - A.left - stream.delta;
+
+    // Heads' first rows.
+    const uint16_t* kh = A.k + (kMode == kPaged ? 0 : it.b) * A.ks.b + it.kvh * A.ks.h;
+    const uint16_t* vh = A.v + (kMode == kPaged ? 0 : it.b) * A.vs.b + it.kvh * A.vs.h;
+    const int32_t* trow = kMode == kPaged ? A.table + it.b * A.table_stride : nullptr;
+    auto key_of = [&](int r) { return r < stream.a1 ? r : r + stream.delta; };
+    // Tile rows 16 * wave + lane % 16 are this wave's to look up (lanes 0..15).
+    constexpr int kLook = kWinTile / 4;
+    const int own = kLook * wave + lane % kLook;
+    const bool owner = lane < kLook;
+    const int l_last = max(L - 1, 0);
+    auto table_entry = [&](int r) { return trow + min(key_of(min(r, l_last)) / A.page, A.table_width - 1); };
+    // Publishes this wave's rows of tile t (page: the row's page number, paged only).
+    auto publish = [&](int t, int buf, int page) {
+        const int r = t * kWinTile + own;
+        const int key = key_of(min(r, l_last));  // rows past the stream repeat its last row
+        bool ok = r < L;
+        int64_t ko, vo;
+        if constexpr (kMode == kPaged) {
+            ok = ok && page >= 0 && page < A.pages;  // a page that is not held: its keys are not seen
+            const int64_t p = max(0, min(page, A.pages - 1)), slot = key % A.page;
+            ko = p * A.ks.b + slot * A.ks.s;
+            vo = p * A.vs.b + slot * A.vs.s;
+        } else {
+            ko = key * A.ks.s;
+            vo = key * A.vs.s;
+        }
+        const uint64_t bits = __ballot(ok);
+        if (owner) {
+            k_off[buf][own] = 2 * ko;
+            v_off[buf][own] = 2 * vo;
+        }
+        if (lane == 0) counts[t % 4][wave] = static_cast<uint16_t>(bits);
+    };
+    auto load_tile = [&](int t, int buf) __attribute__((always_inline)) {
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+        for (int i = 0; i < T::kLoads; ++i) {
+            const int span = i * 4 + wave;
+            const int r = span * T::kWaveRows + lane / T::CH, p = lane % T::CH;
+            const uint32_t chunk = (p ^ T::swz(r)) * 16;
+            const uint32_t kdst = lds_addr(ks[buf] + span * kWave * 8), vdst = lds_addr(vs[buf] + span * kWave * 8);
+            if constexpr (kMode == kNear) {
+                const uint32_t key = key_of(min(t * kWinTile + r, l_last));
+                dma16_off(kh, key * static_cast<uint32_t>(2 * A.ks.s) + chunk, kdst);
+                dma16_off(vh, key * static_cast<uint32_t>(2 * A.vs.s) + chunk, vdst);
+            } else {
+                dma16(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(kh) + k_off[buf][r] + chunk), kdst);
+                dma16(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(vh) + v_off[buf][r] + chunk), vdst);
+            }
+        }
+#endif
+    };
+
+    f32x16 oacc[NB];
+    float m_run, l_run, neg_m;
+    bool wide, dirty = false;
+    const int arow = lane % 32;
+
+    // One 32-key half (cb) of tile t in buffer buf; after_s() runs once the score products are issued.
+    auto compute = [&](auto careful, int t, int buf, int cb, auto&& after_s) __attribute__((always_inline)) {
+        constexpr bool kCareful = decltype(careful)::value;
+        const uint16_t *kt = ks[buf], *vt = vs[buf];
+        const int r0 = t * kWinTile + 32 * cb;
+        if (r0 > w_any || (r0 + 31 < w_from && r0 >= A.sinks)) {  // no row of the wave sees any of it
+            after_s();
+            return;
+        }
+        uint32_t held = 0xffffffffu;
+        if constexpr (kMode == kPaged) {
+            held = __builtin_amdgcn_readfirstlane(counts[t % 4][2 * cb] | static_cast<uint32_t>(counts[t % 4][2 * cb + 1]) << 16);
+        }
+        const bool whole = r0 + 31 <= w_last && (r0 >= w_first || r0 + 31 < A.sinks) && held == 0xffffffffu;
+        f32x16 sacc{};
+        const int krow = 32 * cb + arow;
+#pragma unroll
+        for (int s = 0; s < S; ++s) sacc = Mfma<DT>::run(T::rows(kt, krow, s, h), qf[s], sacc);
+        {
+            constexpr int kAhead = 4;  // K fragments are read this many products ahead
+            __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+            for (int i = 0; i < S - kAhead; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        after_s();
+        auto seen_at = [&](int row) {  // tile half's row -> whether this lane's query sees it
+            const int r = r0 + row;
+            return r <= last_r && (r >= first_r || r < A.sinks) && (held >> row & 1);
+        };
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (!seen_at(8 * (i / 4) + 4 * h + i % 4)) sacc[i] = -INFINITY;
+        }
+        float tmax = sacc[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) tmax = fmaxf(tmax, sacc[i]);
+        if (__any(tmax > m_run)) {
+            tmax = fmaxf(tmax, __shfl_xor(tmax, 32, kWave));
+            const float m_new = fmaxf(m_run, tmax);
+            const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * A.scale_log2);
+            m_run = m_new;
+            // (A query that has seen nothing yet keeps its maximum at the lowest value; its weights are all 0.)
+            neg_m = m_new == -FLT_MAX ? 0.0f : -m_new * A.scale_log2;
+            wide = __any(fabsf(neg_m) > kWideScores);
+            l_run *= alpha;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) oacc[nb][i] *= alpha;
+        }
+        float offset = neg_m;
+        if (wide) {
+            offset = 0.0f;
+            if (m_run != -FLT_MAX) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sacc[i] -= m_run;
+            }
+        }
+        uint32_t pp[8];
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[i], A.scale_log2, offset));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[i + 1], A.scale_log2, offset));
+            pp[i / 2] = Mfma<DT>::pack2(p0, p1);
+            l_run = Mfma<DT>::sum2(pp[i / 2], l_run);
+        }
+        if constexpr (kCareful) {
+            if (!whole && tile_not_finite<DT, D>(vt, 32 * cb, lane)) {
+                add_rows_seen<DT, D>(oacc, vt, 32 * cb, pp, lane, seen_at);
+                return;
+            }
+        } else if (!whole) {
+            dirty |= tile_not_finite<DT, D>(vt, 32 * cb, lane);
+        }
+        add_rows<DT, D>(oacc, vt, 32 * cb, pp, lane);
+    };
+
+    // One walk over the tiles. The careful one is taken again from the start when the first met an infinity or NaN
+    // in a value that some query must not see.
+    auto walk = [&](auto careful) __attribute__((always_inline)) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) oacc[nb] = f32x16{};
+        m_run = -FLT_MAX;
+        l_run = neg_m = 0.0f;
+        wide = false;
+        if (tile0 >= tile1) return;
+        if constexpr (kMode != kNear) {
+            int p0 = 0, p1 = 0;
+            if constexpr (kMode == kPaged) {
+                p0 = *table_entry(tile0 * kWinTile + own);
+                p1 = *table_entry((tile0 + 1) * kWinTile + own);
+                if (owner) page_of[0][own] = *table_entry((tile0 + 2) * kWinTile + own);
+            }
+            publish(tile0, 0, p0);
+            publish(tile0 + 1, 1, p1);
+            __syncthreads();
+        }
+        // The query rows must have arrived before the tile loads are issued: the compiler does not count those,
+        // so a later wait for the rows would also wait for the tile.
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+        for (int s = 0; s < S; ++s) asm volatile("" ::"v"(qf[s]));
+#endif
+        load_tile(tile0, 0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        auto step = [&](auto bufc, int t) __attribute__((always_inline)) {
+            const int buf = bufc;
+            const bool more = t + 1 < tile1;
+            auto next = [&]() __attribute__((always_inline)) {
+                if (more) load_tile(t + 1, buf ^ 1);
+            };
+            if (wave_active) {
+                if constexpr (decltype(careful)::value) {
+                    next();
+#pragma unroll 1
+                    for (int cb = hb; cb < (split ? hb + 1 : 2); ++cb) compute(careful, t, buf, cb, [] {});
+                } else {
+                    compute(careful, t, buf, hb, next);
+                    if (!split) compute(careful, t, buf, 1, [] {});
+                }
+            } else {
+                next();
+            }
+            if constexpr (kMode == kPaged) {
+                // Page numbers of tile t + 3 start on their way to LDS; those of tile t + 2 and this wave's share of
+                // tile t + 1 have landed.
+                const int32_t* e = table_entry((t + 3) * kWinTile + own);
+                if (owner) dma4(e, lds_addr(&page_of[buf ^ 1][kLook * wave]));
+                asm volatile("s_waitcnt vmcnt(1)" ::: "memory");
+            } else {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
+            if constexpr (kMode != kNear) {
+                // (This tile's row offsets were last read a tile ago, when its loads were issued.)
+                int page = 0;
+                if constexpr (kMode == kPaged) page = page_of[buf][own];
+                publish(t + 2, buf, page);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+        };
+        if constexpr (decltype(careful)::value) {
+#pragma unroll 1
+            for (int t = tile0; t < tile1; ++t) step((t - tile0) & 1, t);
+        } else {
+            for (int t = tile0; t < tile1; t += 2) {
+                step(std::integral_constant<int, 0>{}, t);
+                if (t + 1 < tile1) step(std::integral_constant<int, 1>{}, t + 1);
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last page numbers
+    };
+    walk(std::false_type{});
+    if (__syncthreads_or(dirty)) walk(std::true_type{});
+    if (split) {
+        // The wave of the second halves leaves its state in the tile LDS (free after the last barrier), the wave of
+        // the first halves joins both at the larger maximum.
+        float* xch = reinterpret_cast<float*>(&kvs[0][0]) + (rb * kWave + lane) * (NB * 16 + 2);
+        __syncthreads();
+        if (hb == 1 && wave_active) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) xch[nb * 16 + i] = oacc[nb][i];
+            xch[NB * 16] = m_run;
+            xch[NB * 16 + 1] = l_run;
+        }
+        __syncthreads();
+        if (hb == 1) return;
+        if (wave_active) {
+            const float m1 = xch[NB * 16], m = fmaxf(m_run, m1);
+            const float a0 = __builtin_amdgcn_exp2f((m_run - m) * A.scale_log2);
+            const float a1 = __builtin_amdgcn_exp2f((m1 - m) * A.scale_log2);
+            m_run = m;
+            l_run = l_run * a0 + xch[NB * 16 + 1] * a1;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) oacc[nb][i] = oacc[nb][i] * a0 + xch[nb * 16 + i] * a1;
+        }
+    }
+    if (!qvalid) return;
+    const float l_tot = l_run + __shfl_xor(l_run, 32, kWave);
+    // Row number among the partial results and statistics: query head major (paged: token major).
+    const int64_t rows_all = static_cast<int64_t>(kMode == kPaged ? 1 : A.batch) * A.queries * A.heads * A.group;
+    const int64_t row_id = kMode == kPaged
+                               ? static_cast<int64_t>(it.first_token + token) * (A.heads * A.group) + head
+                               : (static_cast<int64_t>(it.b) * (A.heads * A.group) + head) * A.queries + token;
+    if (A.splits > 1) {
+        if (h == 0) A.part_ml[it.split * rows_all + row_id] = float2{m_run, l_tot};
+        if (l_tot == 0.0f) return;  // (the join does not read it)
+        float* o = A.part_o + (it.split * rows_all + row_id) * D;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<f32x4*>(o + 32 * nb + 8 * g + 4 * h) =
+                    f32x4{oacc[nb][4 * g], oacc[nb][4 * g + 1], oacc[nb][4 * g + 2], oacc[nb][4 * g + 3]};
+        return;
+    }
+    const float inv = l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
+    if (A.row_max && h == 0) {
+        A.row_max[row_id] = m_run;
+        A.row_log[row_id] = l_tot == 0.0f ? INFINITY : log2f(l_tot);
+    }
+    uint16_t* o = A.out + (kMode == kPaged ? 0 : it.b) * A.os.b + head * A.os.h +
+                  static_cast<int64_t>(it.first_token + token) * A.os.s;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const uint32_t w0 = Mfma<DT>::pack2(oacc[nb][4 * g] * inv, oacc[nb][4 * g + 1] * inv);
+            const uint32_t w1 = Mfma<DT>::pack2(oacc[nb][4 * g + 2] * inv, oacc[nb][4 * g + 3] * inv);
+            *reinterpret_cast<u32x2*>(o + 32 * nb + 8 * g + 4 * h) = u32x2{w0, w1};
+        }
+}
+
+// Joins the parts of every row: out = sum_s 2^((m_s - M) scale) O_s / sum_s 2^((m_s - M) scale) l_s, parts in
+// order. D / 4 lanes a row.
+template <int DT, int D, bool kPagedRows>
+__global__ __launch_bounds__(256) void window_join_kernel(WindowArgs A) {
+    constexpr int kLanes = D / 4;
+    const int64_t rows_all = static_cast<int64_t>(kPagedRows ? 1 : A.batch) * A.queries * A.heads * A.group;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
+    if (row >= rows_all) return;
+    const int c = threadIdx.x % kLanes * 4, hq = A.heads * A.group;
+    int64_t b = 0, head, token;
+    if constexpr (kPagedRows) {
+        token = row / hq;
+        head = row % hq;
+        const int o0 = max(0, min(A.offsets[0], A.queries)), o1 = min(A.offsets[A.batch], A.queries);
+        if (token < o0 || token >= o1) return;  // of no sequence: no parts were written
+    } else {
+        token = row % A.queries;
+        head = row / A.queries % hq;
+        b = row / A.queries / hq;
+    }
+    float m = -FLT_MAX;
+    for (int s = 0; s < A.splits; ++s) m = fmaxf(m, A.part_ml[s * rows_all + row].x);
+    float l = 0.0f;
+    f32x4 o{};
+    for (int s = 0; s < A.splits; ++s) {
+        const float2 ml = A.part_ml[s * rows_all + row];
+        if (ml.y == 0.0f) continue;
+        const float w = __builtin_amdgcn_exp2f((ml.x - m) * A.scale_log2);
+        const f32x4 part = *reinterpret_cast<const f32x4*>(A.part_o + (s * rows_all + row) * D + c);
+        l += w * ml.y;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] += w * part[k];
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (A.row_max && c == 0) {
+        A.row_max[row] = m;
+        A.row_log[row] = l == 0.0f ? INFINITY : log2f(l);
+    }
+    uint16_t* dst = A.out + b * A.os.b + head * A.os.h + token * A.os.s + c;
+    *reinterpret_cast<u32x2*>(dst) = u32x2{Mfma<DT>::pack2(o[0] * inv, o[1] * inv), Mfma<DT>::pack2(o[2] * inv, o[3] * inv)};
+}
+
+template <int DT, int D> int launch_window(const WindowArgs& A, WindowMode mode, hipStream_t s) {
+    const int64_t heads = mode == kPaged ? A.heads : static_cast<int64_t>(A.heads) * A.batch;
+    const int64_t blocks = heads * A.tiles * A.splits;
+    if (blocks > 0x7fffffff) return kUnsupportedShape;
+    const dim3 grid(static_cast<unsigned>(blocks));
+    switch (mode) {
+        case kNear: hipLaunchKernelGGL((window_forward_kernel<DT, D, kNear>), grid, dim3(256), 0, s, A); break;
+        case kFar: hipLaunchKernelGGL((window_forward_kernel<DT, D, kFar>), grid, dim3(256), 0, s, A); break;
+        default: hipLaunchKernelGGL((window_forward_kernel<DT, D, kPaged>), grid, dim3(256), 0, s, A); break;
+    }
+    int status = hipGetLastError();
+    if (status || A.splits == 1) return status;
+    const int64_t rows = static_cast<int64_t>(mode == kPaged ? 1 : A.batch) * A.queries * A.heads * A.group;
+    const dim3 join(static_cast<unsigned>(ceil_div(rows, 256 / (D / 4))));
+    if (mode == kPaged) hipLaunchKernelGGL((window_join_kernel<DT, D, true>), join, dim3(256), 0, s, A);
+    else hipLaunchKernelGGL((window_join_kernel<DT, D, false>), join, dim3(256), 0, s, A);
+    return hipGetLastError();
+}
+
+int launch(const WindowArgs& A, WindowMode mode, int d, int dtype, hipStream_t s) {
+    if (dtype == kBF16) return d == 128 ? launch_window<kBF16, 128>(A, mode, s) : launch_window<kBF16, 64>(A, mode, s);
+    return d == 128 ? launch_window<kF16, 128>(A, mode, s) : launch_window<kF16, 64>(A, mode, s);
+}
+
+// Parts of the key stream. A workgroup's walk over its tiles is a chain of latencies, so calls whose items
+// leave compute units idle cut the stream, into parts of at least kPartTiles tiles (below that a part costs
+// more in its start, its 64 KB of fp32 output and the join than its tiles do).
+constexpr int kPartTiles = 4;
+constexpr int kMaxSplits = 64;
+int split_count(int64_t items, int64_t seen_keys) {
+    const int64_t slots = 2 * static_cast<int64_t>(device_compute_units());
+    const int64_t most = std::min<int64_t>(kMaxSplits, ceil_div(seen_keys, kWinTile) / kPartTiles);
+    if (items >= slots / 2 || most < 2) return 1;
+    return static_cast<int>(std::min(most, ceil_div(2 * slots, items)));
+}
+
+struct Shape {
+    int splits;
+    int64_t rows;  // all query rows
+    int64_t tiles;
+};
+
+// Most keys that a tile of rows may see.
+int64_t seen_keys(int64_t keys, int64_t tokens, int left, int right, int sinks) {
+    const int64_t window = left < 0 || right < 0 ? keys : std::min<int64_t>(keys, int64_t{left} + right + tokens + sinks);
+    return std::max<int64_t>(window, 0);
+}
+
+Shape window_shape(int batch, int q_heads, int kv_heads, int queries, int keys, int left, int right, int sinks) {
+    const int group = q_heads / kv_heads;
+    const int64_t tiles = ceil_div(static_cast<int64_t>(queries) * group, kWinRows);
+    const int64_t tokens = std::min<int64_t>(queries, kWinRows / group + 1);
+    const int splits = split_count(tiles * batch * kv_heads, seen_keys(keys, tokens, left, right, sinks));
+    return Shape{splits, static_cast<int64_t>(batch) * q_heads * queries, tiles};
+}
+
+// Row tiles of a ragged batch: each sequence has at most one that is not full; one more, so that some
+// workgroup always finds no rows and clears those outside every sequence.
+Shape paged_shape(int batch, int q_heads, int kv_heads, int tokens, int64_t capacity, int left, int sinks) {
+    const int group = q_heads / kv_heads;
+    const int64_t tiles = static_cast<int64_t>(tokens) * group / kWinRows + batch + 1;
+    const int64_t some = std::min<int64_t>(tokens, kWinRows / group + 1);
+    const int splits = split_count((tiles - 1) * kv_heads, seen_keys(capacity, some, left, 0, sinks));
+    return Shape{splits, static_cast<int64_t>(tokens) * q_heads, tiles};
+}
+
+size_t workspace_floats(const Shape& s, int d) {
+    return s.splits > 1 ? static_cast<size_t>(s.splits) * s.rows * (d + 2) : 0;
+}
+
+bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+bool aligned(const Strides& s) { return (s.b | s.h | s.s) % 8 == 0; }
+
+bool mask_ok(int left, int right, int sinks) {
+    return left >= -1 && right >= -1 && sinks >= 0 && left <= kUnbounded && right <= kUnbounded && sinks <= kUnbounded;
+}
+// (A negative scale would turn the running maximum into a minimum, 0 times a masked score is NaN.)
+bool scale_ok(float scale) { return scale >= FLT_MIN && scale <= FLT_MAX; }
+int unbounded(int n) { return n < 0 ? kUnbounded : n; }
+
+void set_parts(WindowArgs& A, const Shape& s, float* workspace, int d) {
+    A.splits = s.splits;
+    A.tiles = static_cast<int>(s.tiles);
+    A.part_o = workspace;
+    A.part_ml = reinterpret_cast<float2*>(workspace + static_cast<int64_t>(s.splits) * s.rows * d);
+}
+
+Strides strides_of(const int64_t* s) { return Strides{s[0], s[1], s[2]}; }
+
+}  // namespace
+}  // namespace peco
+
+using namespace peco;
+
+PECO_API size_t peco_window_attention_workspace_size(int batch, int q_heads, int kv_heads, int queries, int keys,
+                                                     int left, int right, int sinks, int d) {
+    if (batch < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || queries < 1 || keys < 0) return 0;
+    return workspace_floats(window_shape(batch, q_heads, kv_heads, queries, keys, left, right, sinks), d);
+}
+
+PECO_API int peco_window_attention(const void* q, const void* k, const void* v, void* output, const int64_t* strides,
+                                   const int32_t* lengths, float* row_max, float* row_log, float* workspace,
+                                   size_t workspace_floats_given, int batch, int q_heads, int kv_heads, int queries,
+                                   int keys, int left, int right, int sinks, float scale, int d, int dtype,
+                                   void* stream) {
+    if (!q || !k || !v || !output || !strides || !row_max != !row_log || batch < 1 || kv_heads < 1 ||
+        q_heads < kv_heads || q_heads % kv_heads || queries < 1 || keys < 1 || !mask_ok(left, right, sinks) ||
+        !scale_ok(scale) || (lengths && queries != keys))
+        return kInvalidValue;
+    if (d != 64 && d != 128) return kUnsupportedShape;
+    if (dtype != kBF16 && dtype != kF16) return kUnsupportedDtype;
+    if (keys > kUnbounded - 1 || queries > kUnbounded - 1 ||
+        static_cast<int64_t>(queries) * (q_heads / kv_heads) > 0x7fffff00)
+        return kUnsupportedShape;
+    WindowArgs A{};
+    A.qs = strides_of(strides);
+    A.ks = strides_of(strides + 3);
+    A.vs = strides_of(strides + 6);
+    A.os = strides_of(strides + 9);
+    if (!aligned(q) || !aligned(k) || !aligned(v) || !aligned(output) || !aligned(A.qs) || !aligned(A.ks) ||
+        !aligned(A.vs) || !aligned(A.os))
+        return kInvalidValue;
+    A.q = static_cast<const uint16_t*>(q);
+    A.k = static_cast<const uint16_t*>(k);
+    A.v = static_cast<const uint16_t*>(v);
+    A.out = static_cast<uint16_t*>(output);
+    A.heads = kv_heads;
+    A.group = q_heads / kv_heads;
+    A.batch = batch;
+    A.queries = queries;
+    A.keys = keys;
+    A.left = unbounded(left);
+    A.right = unbounded(right);
+    A.sinks = sinks;
+    A.scale_log2 = static_cast<float>(1.4426950408889634 * static_cast<double>(scale));
+    A.lengths = lengths;
+    A.row_max = row_max;
+    A.row_log = row_log;
+    const Shape shape = window_shape(batch, q_heads, kv_heads, queries, keys, left, right, sinks);
+    if (workspace_floats(shape, d) > workspace_floats_given) return kWorkspaceTooSmall;
+    if (shape.splits > 1 && !aligned(workspace)) return kInvalidValue;
+    set_parts(A, shape, workspace, d);
+    const int64_t reach = std::max(A.ks.s, A.vs.s) * 2 * keys + 2 * d;
+    return launch(A, reach < (int64_t{1} << 32) ? kNear : kFar, d, dtype, static_cast<hipStream_t>(stream));
+}
+
+PECO_API size_t peco_paged_attention_workspace_size(int batch, int q_heads, int kv_heads, int tokens, int table_width,
+                                                    int page, int left, int sinks, int d) {
+    if (batch < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || tokens < 1 || table_width < 1 || page < 1)
+        return 0;
+    const int64_t capacity = static_cast<int64_t>(table_width) * page;
+    return workspace_floats(paged_shape(batch, q_heads, kv_heads, tokens, capacity, left, sinks), d);
+}
+
+PECO_API int peco_paged_attention(const void* q, const void* k_pages, const void* v_pages, void* output,
+                                  const int64_t* strides, const int32_t* page_table, int64_t table_stride,
+                                  const int32_t* offsets, const int32_t* lengths, int clear_tail, float* workspace,
+                                  size_t workspace_floats_given, int batch, int q_heads, int kv_heads, int tokens,
+                                  int pages, int page, int table_width, int left, int sinks, float scale, int d,
+                                  int dtype, void* stream) {
+    if (!q || !k_pages || !v_pages || !output || !strides || !page_table || !offsets || !lengths || batch < 1 ||
+        kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || tokens < 1 || pages < 1 || page < 1 ||
+        table_width < 1 || table_stride < 0 || !mask_ok(left, 0, sinks) || !scale_ok(scale))
+        return kInvalidValue;
+    if (d != 64 && d != 128) return kUnsupportedShape;
+    if (dtype != kBF16 && dtype != kF16) return kUnsupportedDtype;
+    const int64_t capacity = static_cast<int64_t>(table_width) * page;
+    if (capacity > kUnbounded - 1 || tokens > kUnbounded - 1 ||
+        static_cast<int64_t>(tokens) * (q_heads / kv_heads) > 0x7fffff00)
+        return kUnsupportedShape;
+    WindowArgs A{};
+    A.qs = Strides{0, strides[0], strides[1]};
+    A.ks = strides_of(strides + 2);
+    A.vs = strides_of(strides + 5);
+    A.os = Strides{0, strides[8], strides[9]};
+    if (!aligned(q) || !aligned(k_pages) || !aligned(v_pages) || !aligned(output) || !aligned(A.qs) || !aligned(A.ks) ||
+        !aligned(A.vs) || !aligned(A.os))
+        return kInvalidValue;
+    A.q = static_cast<const uint16_t*>(q);
+    A.k = static_cast<const uint16_t*>(k_pages);
+    A.v = static_cast<const uint16_t*>(v_pages);
+    A.out = static_cast<uint16_t*>(output);
+    A.heads = kv_heads;
+    A.group = q_heads / kv_heads;
+    A.batch = batch;
+    A.queries = tokens;
+    A.keys = static_cast<int>(capacity);
+    A.left = unbounded(left);
+    A.right = 0;
+    A.sinks = sinks;
+    A.scale_log2 = static_cast<float>(1.4426950408889634 * static_cast<double>(scale));
+    A.lengths = lengths;
+    A.offsets = offsets;
+    A.table = page_table;
+    A.table_stride = table_stride;
+    A.table_width = table_width;
+    A.page = page;
+    A.pages = pages;
+    A.clear_tail = clear_tail;
+    const Shape shape = paged_shape(batch, q_heads, kv_heads, tokens, capacity, left, sinks);
+    if (workspace_floats(shape, d) > workspace_floats_given) return kWorkspaceTooSmall;
+    if (shape.splits > 1 && !aligned(workspace)) return kInvalidValue;
+    set_parts(A, shape, workspace, d);
+    return launch(A, kPaged, d, dtype, static_cast<hipStream_t>(stream));
+}

@@ -1,0 +1,95 @@
+"""A paged key/value cache on gfx950: new tokens' keys and values appended, new queries' attention over it.
+
+A cache is two tensors of pages, K and V [pages, heads, page, D] (any strides with adjacent channels), and per
+sequence a row of page numbers: token t of sequence b is slot t % page of page ``page_table[b, t // page]``. A call
+takes the new tokens of a batch of sequences in a row, sequence b's at ``offsets[b]`` to ``offsets[b + 1]``, and
+every sequence's number of tokens with the new ones, ``lengths``. All of these are on the GPU and are not read by
+the host, so a captured graph serves any batch that fits its sizes.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _native
+from .attention_cuda import _device_is_gfx950
+from .window import check_mask, raise_error, rows16, strides_of
+
+
+def _check_cache(k_pages, v_pages, page_table, offsets, lengths, rows, name):
+    tensors = (rows, k_pages, v_pages, page_table, offsets, lengths)
+    if not all(isinstance(t, torch.Tensor) for t in tensors):
+        raise TypeError("All paged cache inputs must be torch tensors")
+    if k_pages.ndim != 4 or v_pages.shape != k_pages.shape or min(k_pages.shape[:3]) < 1:
+        raise ValueError("Expected equal-shaped K/V pages [pages,HK,page,D] that are not empty")
+    if rows.ndim != 3 or rows.shape[2] != k_pages.shape[3]:
+        raise ValueError(f"Expected {name} [tokens,heads,D] with the pages' feature dimension")
+    if k_pages.shape[3] not in (64, 128):
+        raise ValueError("HIP attention supports head dimensions 64 and 128")
+    if rows.dtype not in (torch.float16, torch.bfloat16) or k_pages.dtype != rows.dtype or v_pages.dtype != rows.dtype:
+        raise TypeError(f"{name} and the pages must share dtype torch.float16 or torch.bfloat16")
+    if page_table.ndim != 2 or min(page_table.shape) < 1:
+        raise ValueError("page_table must have shape [sequences,entries] and not be empty")
+    if offsets.shape != (page_table.shape[0] + 1,) or lengths.shape != (page_table.shape[0],):
+        raise ValueError("offsets and lengths must have shapes [sequences + 1] and [sequences]")
+    if any(t.dtype != torch.int32 for t in (page_table, offsets, lengths)):
+        raise TypeError("page_table, offsets and lengths must be int32")
+    if not rows.is_cuda or any(t.device != rows.device for t in tensors):
+        raise ValueError("All paged cache inputs must reside on the same GPU device")
+    if not _native.plain_tensors(*tensors):
+        raise RuntimeError("a paged cache takes ordinary tensors (no tracing, transforms or tangents)")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (rows, k_pages, v_pages)):
+        raise RuntimeError("a paged cache supports inference only; use torch.no_grad()")
+    if any(rows16(t) is not t for t in (k_pages[:1], v_pages[:1])) or \
+            any(t.stride(0) % 8 for t in (k_pages, v_pages)):
+        raise ValueError("pages must have adjacent channels and rows on 16 bytes")
+    if page_table.shape[1] * k_pages.shape[2] >= 1 << 30 or rows.shape[0] >= 1 << 30:
+        raise ValueError("sequences must be shorter than 2^30")
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                    offsets: torch.Tensor, lengths: torch.Tensor, *, window: int = -1, sinks: int = 0,
+                    scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of new tokens q [tokens,HQ,D] over the cache, causal, with ``window.window_attention``'s mask.
+
+    The new tokens are the last ones of their sequences and are in the cache already (``append_pages``): new token
+    i of n of a sequence of ``lengths[b]`` tokens stands at p = lengths[b] - n + i and sees token j when j <= p and
+    (j >= p - window or j < sinks); ``window`` -1 is without limit. HQ is a multiple of the pages' heads HK, query
+    head h reads key head h // (HQ / HK). Keys on a page whose number in ``page_table`` is outside [0, pages) (one
+    that left the window and was given back, say) are not seen. A query that sees no key gives 0. ``offsets``
+    ascend; ``lengths`` are taken within [0, table's tokens]. Rows of q of no sequence, those behind
+    ``offsets[-1]`` of a padded batch, give 0, or with ``out`` (a tensor like q) are left there as they were.
+    """
+    _check_cache(k_pages, v_pages, page_table, offsets, lengths, q, "q")
+    tokens, heads, dim = q.shape
+    pages, kv_heads, page, _ = k_pages.shape
+    if heads < 1 or heads % kv_heads:
+        raise ValueError("the query heads must be a multiple of the pages' heads")
+    left, _, sinks, scale = check_mask((window, 0), sinks, scale, dim)
+    if out is not None:
+        if not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+            raise ValueError("out must be a tensor like q")
+        if not _native.plain_tensors(out) or (torch.is_grad_enabled() and out.requires_grad):
+            raise RuntimeError("out must be an ordinary tensor without gradient")
+        if rows16(out) is not out:
+            raise ValueError("out must have adjacent channels and rows on 16 bytes")
+    result = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device) if out is None else out
+    if tokens == 0:
+        return result
+    with torch.cuda.device(q.device):
+        if not _device_is_gfx950(q.device):
+            raise RuntimeError("This HIP build requires an MI355X-class gfx950 GPU")
+        library = _native.library()
+        q, table = rows16(q), page_table if page_table.stride(1) == 1 else page_table.contiguous()
+        offsets, lengths = offsets.contiguous(), lengths.contiguous()
+        batch, width = table.shape
+        floats = library.peco_paged_attention_workspace_size(batch, heads, kv_heads, tokens, width, page, left, sinks, dim)
+        workspace = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+        # (q and the output count head before token.)
+        strides = strides_of(q.transpose(0, 1), k_pages, v_pages, result.transpose(0, 1))
+        raise_error(library.peco_paged_attention(
+            _native.ptr(q), _native.ptr(k_pages), _native.ptr(v_pages), _native.ptr(result), strides, _native.ptr(table),
+            table.stride(0), _native.ptr(offsets), _native.ptr(lengths), int(out is None), _native.ptr(workspace), floats,
+            batch, heads, kv_heads, tokens, pages, page, width, left, sinks, scale, dim, _native.dtype_code(q.dtype),
+            _native.current_stream(q.device, q, k_pages, v_pages, result, table, offsets, lengths, workspace)),
+            "paged attention")
+    return result

@@ -1,0 +1,124 @@
+"""Attention with a sliding window and sinks on gfx950 MFMA: forward and backward.
+
+For clips that are generated or fine-tuned piece by piece: a token sees the tokens of a window around it (causal
+or to both sides) and the first tokens of its sequence (the prompt's, say), which stay visible to every later one.
+``paged.paged_attention`` is the same attention over a cache.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _native
+from .attention_cuda import _device_is_gfx950
+
+
+def rows16(t):
+    """t with adjacent channels and every row on 16 bytes (a copy when it is laid out otherwise)."""
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def strides_of(*tensors):
+    """The strides of all but the last axis of the tensors, as the C-ABI's host array."""
+    values = [s for t in tensors for s in t.stride()[:-1]]
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+def raise_error(error, what):
+    if error:
+        message = _native.library().peco_attention_error_string(error).decode("utf-8", errors="replace")
+        raise RuntimeError(f"PECO HIP {what} launch failed: {message} ({error})")
+
+
+def check_mask(window, sinks, scale, dim):
+    """(left, right, sinks, scale) as the kernels take them: limits in [-1, 2^30], a positive scale."""
+    if not isinstance(window, (tuple, list)) or len(window) != 2 or \
+            any(isinstance(n, bool) or not isinstance(n, int) or n < -1 for n in window):
+        raise ValueError("window must be (left, right), nonnegative integers or -1 for no limit")
+    if isinstance(sinks, bool) or not isinstance(sinks, int) or sinks < 0:
+        raise ValueError("sinks must be a nonnegative integer")
+    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError("scale must be a positive finite number")
+    most = 1 << 30
+    return min(window[0], most), min(window[1], most), min(sinks, most), scale
+
+
+def _check(q, k, v, lengths):
+    tensors = (q, k, v) if lengths is None else (q, k, v, lengths)
+    if not all(isinstance(t, torch.Tensor) for t in tensors):
+        raise TypeError("All window attention inputs must be torch tensors")
+    if q.ndim != 4 or k.ndim != 4 or v.shape != k.shape:
+        raise ValueError("Expected Q [B,HQ,SQ,D] and equal-shaped K/V [B,HK,SK,D]")
+    batch, heads, sq, dim = q.shape
+    if k.shape[0] != batch or k.shape[3] != dim:
+        raise ValueError("Q and K/V batch and feature dimensions must match")
+    if k.shape[1] < 1 or heads < 1 or heads % k.shape[1]:
+        raise ValueError("the query heads must be a multiple of the key heads")
+    if dim not in (64, 128):
+        raise ValueError("HIP attention supports head dimensions 64 and 128")
+    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("Q/K/V must share dtype torch.float16 or torch.bfloat16")
+    if lengths is not None:
+        if sq != k.shape[2]:
+            raise ValueError("lengths needs as many queries as keys")
+        if lengths.dtype != torch.int32 or lengths.shape != (batch,):
+            raise TypeError("lengths must be int32 [B]")
+    if not q.is_cuda or any(t.device != q.device for t in tensors):
+        raise ValueError("All window attention inputs must reside on the same GPU device")
+    if not _native.plain_tensors(*tensors):
+        raise RuntimeError("window_attention takes ordinary tensors (no tracing, transforms or tangents)")
+    if max(sq, k.shape[2]) >= 1 << 30:
+        raise ValueError("sequences must be shorter than 2^30")
+
+
+def _forward(q, k, v, lengths, left, right, sinks, scale, stats):
+    """(output, row maxima, log2 of the row sums); the last two None without ``stats``."""
+    batch, heads, sq, dim = q.shape
+    out = torch.empty_like(q)
+    row_max = row_log = None
+    if q.numel() == 0:
+        return out, row_max, row_log
+    if k.shape[2] == 0:
+        return out.zero_(), row_max, row_log
+    with torch.cuda.device(q.device):
+        if not _device_is_gfx950(q.device):
+            raise RuntimeError("This HIP build requires an MI355X-class gfx950 GPU")
+        library = _native.library()
+        q, k, v = rows16(q), rows16(k), rows16(v)
+        target = out if rows16(out) is out else torch.empty(out.shape, dtype=out.dtype, device=out.device)
+        if stats:
+            row_max, row_log = torch.empty((2, batch, heads, sq), dtype=torch.float32, device=q.device).unbind()
+        shape = (batch, heads, k.shape[1], sq, k.shape[2], left, right, sinks)
+        floats = library.peco_window_attention_workspace_size(*shape, dim)
+        workspace = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+        raise_error(library.peco_window_attention(
+            _native.ptr(q), _native.ptr(k), _native.ptr(v), _native.ptr(target), strides_of(q, k, v, target),
+            _native.ptr(lengths), _native.ptr(row_max), _native.ptr(row_log), _native.ptr(workspace), floats, *shape,
+            scale, dim, _native.dtype_code(q.dtype),
+            _native.current_stream(q.device, q, k, v, target, lengths, row_max, row_log, workspace)),
+            "window attention")
+        return (out if target is out else out.copy_(target)), row_max, row_log
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window, sinks: int = 0, *,
+                     lengths: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
+    """softmax(scale Q K^T) V over the keys that each query sees.
+
+    Q [B,HQ,SQ,D] and K/V [B,HK,SK,D], fp16 or bf16, D 64 or 128, any strides (tensors whose rows do not lie on
+    16 bytes with adjacent channels are copied first); HQ a multiple of HK, query head h reads key head
+    h // (HQ / HK). Queries and keys end together: query i stands at position p = i + SK - SQ and sees key j when
+    j <= p + right and (j >= p - left or j < sinks), with ``window = (left, right)``, -1 for no limit: (-1, 0) is
+    causal, (n - 1, 0) a causal window of n tokens, (n, n) one to both sides. A query that sees no key gives 0.
+    ``lengths`` (int32 [B], needs SQ == SK): valid tokens of each sequence of a right-padded batch; later keys are
+    not seen, later rows give 0 and take no gradient, whatever they hold. ``scale`` defaults to 1 / sqrt(D).
+    The result has the strides of ``empty_like(q)``. Differentiable once in Q, K and V.
+    """
+    _check(q, k, v, lengths)
+    mask = check_mask(window, sinks, scale, q.shape[3])
+    lengths = None if lengths is None else lengths.contiguous()
+    return _forward(q, k, v, lengths, *mask, False)[0]
