@@ -360,6 +360,18 @@ int peco_paged_attention(const void* q, const void* k_pages, const void* v_pages
                          size_t workspace_floats, int batch, int q_heads, int kv_heads, int tokens, int pages, int page,
                          int table_width, int left, int sinks, float scale, int d, int dtype, void* stream);
 
+/* New tokens' keys and values into the pages of such a cache: k and v [tokens, heads, dims] (dims 64 or 128), laid
+ * out over sequences by offsets as q above, to places lengths[b] - n .. lengths[b] - 1 of sequence b's n new tokens.
+ * strides: host memory, element strides of token and head of k and of v, of page, head and row of k_pages and of
+ * v_pages (10 values). With positions (else null) the keys are turned first, as by peco_rotary_axes with rows =
+ * tokens (position_batch is unused). Tokens of no sequence, places outside the table and pages outside [0, pages)
+ * are passed over. */
+int peco_append_pages(const void* k, const void* v, void* k_pages, void* v_pages, const int64_t* strides,
+                      const int32_t* page_table, int64_t table_stride, const int32_t* offsets, const int32_t* lengths,
+                      const void* positions, int position_type, int64_t position_batch, int64_t position_axis,
+                      const double* turns, const int* axis_pairs, int axes, int halves, int inverse, int batch,
+                      int heads, int tokens, int pages, int page, int table_width, int dims, int dtype, void* stream);
+
 /* peco_sparse_attention without a workspace argument. No counterpart in the reference: it is
  * for callers that cannot allocate device memory (code under HIP graph capture, serving loops
  * that forbid hipMalloc). The work list lives in a static per-device array of 1048576 int32

@@ -148,6 +148,7 @@ SIGNATURES = {
     "peco_window_attention": (I, [P] * 4 + [LP] + [P] * 4 + [Z] + [I] * 8 + [ctypes.c_float, I, I, P]),
     "peco_paged_attention_workspace_size": (Z, [I] * 9),
     "peco_paged_attention": (I, [P] * 4 + [LP, P, ctypes.c_int64, P, P, I, P, Z] + [I] * 9 + [ctypes.c_float, I, I, P]),
+    "peco_append_pages": (I, [P] * 4 + [LP, P, ctypes.c_int64, P, P] + PLAN + [I] * 8 + [P]),
     "peco_rotary_axes": (I, [P] + [ctypes.c_int64] * 3 + [P] + [ctypes.c_int64] * 3 + PLAN + [I] * 5 + [P]),
     "peco_place_heads_axes": (I, [P] + [ctypes.c_int64] * 3 + [P] + PLAN + [I, P, ctypes.c_float] + [I] * 7 + [P]),
     "peco_base_offset_attention": (I, [P, P, P, I] + [P] * 9 + [I, I] + [P] * 5 + [Z] + [I] * 8 + [P]),

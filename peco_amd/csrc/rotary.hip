@@ -90,6 +90,100 @@ template <int DT, bool kHalves> int launch_rotary(const RotaryArgs& a, const Rot
     return hipGetLastError();
 }
 
+// New tokens' keys (rotated) and values into the pages of a cache. k and v [tokens, heads, D] hold the tokens of
+// `batch` sequences in a row (offsets), token i of n of sequence b goes to place lengths[b] - n + i of its row of
+// the page table. Every lane moves 8 channels of K and of V of kHeads heads of one token; with halves it reads
+// its partner chunk as well (from the L1, where the partner's own read puts it).
+struct AppendArgs {
+    const uint16_t *k, *v;
+    uint16_t *k_pages, *v_pages;
+    int64_t k_token, k_head, v_token, v_head;         // strides in elements
+    int64_t kp_page, kp_head, kp_row, vp_page, vp_head, vp_row;
+    const int32_t *table, *offsets, *lengths;
+    int64_t table_stride;
+    int batch, heads, tokens, pages, page, width;
+    int halves;
+};
+
+template <int DT, int D, int kHeads>
+__global__ __launch_bounds__(256) void append_pages_kernel(AppendArgs a, RotaryPlan plan) {
+    constexpr int G = D / 8;               // lanes a token
+    constexpr int kTokens = kWave / G;     // tokens a wavefront
+    const int lane = threadIdx.x % kWave;
+    const int first = (blockIdx.x * (256 / kWave) + threadIdx.x / kWave) * kTokens;
+    if (first >= a.tokens) return;
+    const int token = first + lane / G;
+    // The token's sequence: the offsets up to it, counted 64 at a time for all the wavefront's tokens.
+    int upto = 0;
+    for (int b0 = 0; b0 <= a.batch; b0 += kWave) {
+        const int at = b0 + lane;
+        const int offset = at <= a.batch ? a.offsets[at] : 0x7fffffff;
+#pragma unroll
+        for (int t = 0; t < kTokens; ++t) {
+            const int n = __popcll(__ballot(offset <= first + t));
+            upto += lane / G == t ? n : 0;
+        }
+    }
+    const int b = upto - 1;
+    if (token >= a.tokens || b < 0 || b >= a.batch) return;  // of no sequence
+    const int begin = max(0, a.offsets[b]), end = min(a.offsets[b + 1], a.tokens);
+    const int64_t place = static_cast<int64_t>(a.lengths[b]) - (end - begin) + (token - begin);
+    if (place < 0 || place >= static_cast<int64_t>(a.width) * a.page) return;
+    const int page = a.table[b * a.table_stride + place / a.page];
+    if (page < 0 || page >= a.pages) return;  // not held
+    const int64_t slot = place % a.page;
+    const int c = 8 * (lane % G), chunk = lane % G, h0 = blockIdx.y * kHeads;
+    const int half = plan.pairs / 8;  // chunks of a half
+    const bool turns = a.halves ? chunk < 2 * half : c < 2 * plan.pairs;
+    const int partner = a.halves && turns ? (chunk < half ? c + plan.pairs : c - plan.pairs) : c;
+    Chunk<DT> kx[kHeads], px[kHeads], vx[kHeads];
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+        const int head = min(h0 + i, a.heads - 1);
+        kx[i].load(a.k, token * a.k_token + head * a.k_head + c);
+        if (a.halves) px[i].load(a.k, token * a.k_token + head * a.k_head + partner);
+        vx[i].load(a.v, token * a.v_token + head * a.v_head + c);
+    }
+    if (turns) {
+        if (a.halves) {
+            const bool upper = chunk >= half;
+            float cs[8], sn[8];
+            rotary_angles<8>(plan, 0, token, 8 * (upper ? chunk - half : chunk), cs, sn);
+#pragma unroll
+            for (int i = 0; i < kHeads; ++i)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float own = kx[i].get(k), other = px[i].get(k);
+                    kx[i].set(k, upper ? own * cs[k] + other * sn[k] : own * cs[k] - other * sn[k]);
+                }
+        } else {
+            float cs[4], sn[4];
+            rotary_angles<4>(plan, 0, token, c / 2, cs, sn);
+#pragma unroll
+            for (int i = 0; i < kHeads; ++i) turn_adjacent(kx[i], c / 2, plan.pairs, cs, sn);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+        if (h0 + i >= a.heads) break;
+        kx[i].store(a.k_pages, page * a.kp_page + (h0 + i) * a.kp_head + slot * a.kp_row + c);
+        vx[i].store(a.v_pages, page * a.vp_page + (h0 + i) * a.vp_head + slot * a.vp_row + c);
+    }
+}
+
+// Heads per lane: 4 share a token's angles and keep 128 bytes a lane in flight; 1 where that leaves fewer
+// than two workgroups for each CU.
+template <int DT, int D> int launch_append(const AppendArgs& a, const RotaryPlan& plan, hipStream_t s) {
+    const int64_t blocks = ceil_div(a.tokens, 256 / (D / 8));
+    const bool wide = blocks * ceil_div(a.heads, 4) >= 2 * device_compute_units();
+    const int64_t groups = wide ? ceil_div(a.heads, 4) : a.heads;
+    if (groups > 65535) return kUnsupportedShape;
+    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(groups));
+    if (wide) hipLaunchKernelGGL((append_pages_kernel<DT, D, 4>), grid, dim3(256), 0, s, a, plan);
+    else hipLaunchKernelGGL((append_pages_kernel<DT, D, 1>), grid, dim3(256), 0, s, a, plan);
+    return hipGetLastError();
+}
+
 }  // namespace
 }  // namespace peco
 
@@ -121,4 +215,33 @@ PECO_API int peco_rotary_axes(const void* input, int64_t in_batch, int64_t in_he
         case kF16: return halves ? launch_rotary<kF16, true>(a, plan, s) : launch_rotary<kF16, false>(a, plan, s);
         default: return halves ? launch_rotary<kF32, true>(a, plan, s) : launch_rotary<kF32, false>(a, plan, s);
     }
+}
+
+PECO_API int peco_append_pages(const void* k, const void* v, void* k_pages, void* v_pages, const int64_t* strides,
+                               const int32_t* page_table, int64_t table_stride, const int32_t* offsets,
+                               const int32_t* lengths, const void* positions, int position_type,
+                               int64_t position_batch, int64_t position_axis, const double* turns,
+                               const int* axis_pairs, int axes, int halves, int inverse, int batch, int heads,
+                               int tokens, int pages, int page, int table_width, int dims, int dtype, void* stream) {
+    RotaryPlan plan{};
+    if (!k || !v || !k_pages || !v_pages || !strides || !page_table || !offsets || !lengths || batch < 1 || heads < 1 ||
+        tokens < 1 || pages < 1 || page < 1 || table_width < 1 || table_stride < 0 ||
+        (positions && !make_plan(plan, positions, position_type, 0, position_axis, turns, axis_pairs, axes, halves,
+                                 inverse, dims)))
+        return kInvalidValue;
+    if (dims != 64 && dims != 128) return kUnsupportedShape;
+    if (dtype != kBF16 && dtype != kF16) return kUnsupportedDtype;
+    if (tokens > 0x3fffffff || static_cast<int64_t>(table_width) * page > 0x3fffffff) return kUnsupportedShape;
+    int64_t all = 0;
+    for (int i = 0; i < 10; ++i) all |= strides[i];
+    for (const void* p : {k, v, static_cast<const void*>(k_pages), static_cast<const void*>(v_pages)})
+        if (reinterpret_cast<uintptr_t>(p) % 16) return kInvalidValue;
+    if (all % 8) return kInvalidValue;
+    AppendArgs a{static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), static_cast<uint16_t*>(k_pages),
+                 static_cast<uint16_t*>(v_pages), strides[0], strides[1], strides[2], strides[3], strides[4], strides[5],
+                 strides[6], strides[7], strides[8], strides[9], page_table, offsets, lengths, table_stride, batch, heads,
+                 tokens, pages, page, table_width, positions ? halves : 0};
+    const auto s = static_cast<hipStream_t>(stream);
+    if (dtype == kBF16) return dims == 128 ? launch_append<kBF16, 128>(a, plan, s) : launch_append<kBF16, 64>(a, plan, s);
+    return dims == 128 ? launch_append<kF16, 128>(a, plan, s) : launch_append<kF16, 64>(a, plan, s);
 }

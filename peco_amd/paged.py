@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import torch
 
-from . import _native
+from . import _native, rotary as rotary_module
 from .attention_cuda import _device_is_gfx950
 from .window import check_mask, raise_error, rows16, strides_of
 
@@ -44,6 +44,47 @@ def _check_cache(k_pages, v_pages, page_table, offsets, lengths, rows, name):
         raise ValueError("pages must have adjacent channels and rows on 16 bytes")
     if page_table.shape[1] * k_pages.shape[2] >= 1 << 30 or rows.shape[0] >= 1 << 30:
         raise ValueError("sequences must be shorter than 2^30")
+
+
+_NO_PLAN = (None, 0, 0, 0, None, None, 0, 0, 0)
+
+
+def append_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                 page_table: torch.Tensor, offsets: torch.Tensor, lengths: torch.Tensor, *,
+                 rotary: rotary_module.RotaryPositions | None = None) -> None:
+    """Write new tokens' keys and values k, v [tokens,HK,D] to their places in the cache.
+
+    Token i of n new ones of sequence b goes to place lengths[b] - n + i (``lengths`` count the new tokens).
+    With ``rotary`` (positions [axes,tokens]) the keys are turned first, as ``rotary.rotary_axes`` turns them.
+    Tokens of no sequence, places outside the table and pages outside [0, pages) are passed over; two places that
+    share a page's row (a page given twice) are written in no order.
+    """
+    _check_cache(k_pages, v_pages, page_table, offsets, lengths, k, "k and v")
+    if not isinstance(v, torch.Tensor) or v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
+        raise ValueError("k and v must be tensors of one shape, dtype and device")
+    if not _native.plain_tensors(v) or (torch.is_grad_enabled() and v.requires_grad):
+        raise RuntimeError("a paged cache supports inference only; use torch.no_grad()")
+    tokens, heads, dim = k.shape
+    pages, kv_heads, page, _ = k_pages.shape
+    if heads != kv_heads:
+        raise ValueError("k and v must have the pages' heads")
+    positions, plan = None, _NO_PLAN
+    if rotary is not None:
+        if not isinstance(rotary, rotary_module.RotaryPositions):
+            raise TypeError("rotary must be a RotaryPositions")
+        positions = rotary_module.check_positions(rotary.axes, rotary.positions, 1, tokens, dim, k.device)
+        plan = rotary_module.plan_arguments(rotary.axes, positions)
+    if tokens == 0:
+        return
+    with torch.cuda.device(k.device):
+        k, v, table = rows16(k), rows16(v), page_table if page_table.stride(1) == 1 else page_table.contiguous()
+        offsets, lengths = offsets.contiguous(), lengths.contiguous()
+        _native.check(_native.library().peco_append_pages(
+            _native.ptr(k), _native.ptr(v), _native.ptr(k_pages), _native.ptr(v_pages), strides_of(k, v, k_pages, v_pages),
+            _native.ptr(table), table.stride(0), _native.ptr(offsets), _native.ptr(lengths), *plan, table.shape[0], heads,
+            tokens, pages, page, table.shape[1], dim, _native.dtype_code(k.dtype),
+            _native.current_stream(k.device, k, v, k_pages, v_pages, table, offsets, lengths, positions)),
+            "PECO HIP append to pages")
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
