@@ -343,6 +343,18 @@ int peco_window_attention(const void* q, const void* k, const void* v, void* out
                           size_t workspace_floats, int batch, int q_heads, int kv_heads, int queries, int keys,
                           int left, int right, int sinks, float scale, int d, int dtype, void* stream);
 
+/* Its gradients: dq, dk, dv (of the shapes of q, k, v) from grad, the gradient of output, with the inputs, output,
+ * row_max and row_log of the forward call. strides: of q, k, v, output, grad, dq, dk, dv (24 values). Written with
+ * lengths: every row of dq, dk and dv, 0 behind a sequence's length. workspace:
+ * peco_window_attention_grad_workspace_size floats, 16-byte aligned (calls that overlap need one each). */
+size_t peco_window_attention_grad_workspace_size(int batch, int q_heads, int kv_heads, int queries, int keys, int left,
+                                                 int right, int sinks, int d, int dtype);
+int peco_window_attention_grad(const void* q, const void* k, const void* v, const void* output, const void* grad,
+                               void* dq, void* dk, void* dv, const int64_t* strides, const int32_t* lengths,
+                               const float* row_max, const float* row_log, float* workspace, size_t workspace_floats,
+                               int batch, int q_heads, int kv_heads, int queries, int keys, int left, int right,
+                               int sinks, float scale, int d, int dtype, void* stream);
+
 /* Attention of new tokens over a paged cache, with the same window (right 0) and sinks. q and output [tokens,
  * q_heads, d] hold the new tokens of `batch` sequences in a row: sequence b has rows offsets[b] .. offsets[b+1]-1
  * (int32 [batch + 1], ascending) and lengths[b] tokens in the cache (int32 [batch]), the new ones, already

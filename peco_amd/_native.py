@@ -146,6 +146,8 @@ SIGNATURES = {
     "peco_place_heads": (I, [P] + [ctypes.c_int64] * 3 + [P] * 3 + [I, P, ctypes.c_float] + [I] * 7 + [P]),
     "peco_window_attention_workspace_size": (Z, [I] * 9),
     "peco_window_attention": (I, [P] * 4 + [LP] + [P] * 4 + [Z] + [I] * 8 + [ctypes.c_float, I, I, P]),
+    "peco_window_attention_grad_workspace_size": (Z, [I] * 10),
+    "peco_window_attention_grad": (I, [P] * 8 + [LP] + [P] * 4 + [Z] + [I] * 8 + [ctypes.c_float, I, I, P]),
     "peco_paged_attention_workspace_size": (Z, [I] * 9),
     "peco_paged_attention": (I, [P] * 4 + [LP, P, ctypes.c_int64, P, P, I, P, Z] + [I] * 9 + [ctypes.c_float, I, I, P]),
     "peco_append_pages": (I, [P] * 4 + [LP, P, ctypes.c_int64, P, P] + PLAN + [I] * 8 + [P]),

@@ -150,9 +150,9 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
     uint16_t(*const ks)[T::kElems] = kvs;
     uint16_t(*const vs)[T::kElems] = kvs + 2;
     static_assert(2 * kWave * (NB * 16 + 2) * sizeof(float) <= sizeof(kvs), "pair exchange exceeds the tile LDS");
-    // Far and paged rows: offsets (bytes) of a tile's K and V rows, whether each row counts, and page numbers
-    // on their way (loaded two tiles before they are used).
-    constexpr int kRowLds = kMode == kNear ? 1 : kWinTile;
+    // Paged rows: offsets (bytes) of a tile's K and V rows, whether each row counts, and page numbers on their
+    // way (loaded two tiles before they are used).
+    constexpr int kRowLds = kMode == kPaged ? kWinTile : 1;
     __shared__ int64_t k_off[2][kRowLds], v_off[2][kRowLds];
     __shared__ uint16_t counts[4][4];  // (read during a tile, when those two tiles on are written)
     __shared__ int page_of[2][kRowLds];
@@ -224,25 +224,16 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
     const bool owner = lane < kLook;
     const int l_last = max(L - 1, 0);
     auto table_entry = [&](int r) { return trow + min(key_of(min(r, l_last)) / A.page, A.table_width - 1); };
-    // Publishes this wave's rows of tile t (page: the row's page number, paged only).
+    // Publishes this wave's rows of tile t, given the row's page number.
     auto publish = [&](int t, int buf, int page) {
         const int r = t * kWinTile + own;
         const int key = key_of(min(r, l_last));  // rows past the stream repeat its last row
-        bool ok = r < L;
-        int64_t ko, vo;
-        if constexpr (kMode == kPaged) {
-            ok = ok && page >= 0 && page < A.pages;  // a page that is not held: its keys are not seen
-            const int64_t p = max(0, min(page, A.pages - 1)), slot = key % A.page;
-            ko = p * A.ks.b + slot * A.ks.s;
-            vo = p * A.vs.b + slot * A.vs.s;
-        } else {
-            ko = key * A.ks.s;
-            vo = key * A.vs.s;
-        }
+        const bool ok = r < L && page >= 0 && page < A.pages;  // a page that is not held: its keys are not seen
+        const int64_t p = max(0, min(page, A.pages - 1)), slot = key % A.page;
         const uint64_t bits = __ballot(ok);
         if (owner) {
-            k_off[buf][own] = 2 * ko;
-            v_off[buf][own] = 2 * vo;
+            k_off[buf][own] = 2 * (p * A.ks.b + slot * A.ks.s);
+            v_off[buf][own] = 2 * (p * A.vs.b + slot * A.vs.s);
         }
         if (lane == 0) counts[t % 4][wave] = static_cast<uint16_t>(bits);
     };
@@ -254,10 +245,10 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
             const int r = span * T::kWaveRows + lane / T::CH, p = lane % T::CH;
             const uint32_t chunk = (p ^ T::swz(r)) * 16;
             const uint32_t kdst = lds_addr(ks[buf] + span * kWave * 8), vdst = lds_addr(vs[buf] + span * kWave * 8);
-            if constexpr (kMode == kNear) {
-                const uint32_t key = key_of(min(t * kWinTile + r, l_last));
-                dma16_off(kh, key * static_cast<uint32_t>(2 * A.ks.s) + chunk, kdst);
-                dma16_off(vh, key * static_cast<uint32_t>(2 * A.vs.s) + chunk, vdst);
+            if constexpr (kMode != kPaged) {
+                const int key = key_of(min(t * kWinTile + r, l_last));
+                load_row16<kMode == kFar>(kh, key, A.ks.s, chunk, kdst);
+                load_row16<kMode == kFar>(vh, key, A.vs.s, chunk, vdst);
             } else {
                 dma16(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(kh) + k_off[buf][r] + chunk), kdst);
                 dma16(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(vh) + v_off[buf][r] + chunk), vdst);
@@ -269,15 +260,14 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
     f32x16 oacc[NB];
     float m_run, l_run, neg_m;
     bool wide, dirty = false;
-    const int arow = lane % 32;
+    const WinLane<D> at(lane);
 
-    // One 32-key half (cb) of tile t in buffer buf; after_s() runs once the score products are issued.
-    auto compute = [&](auto careful, int t, int buf, int cb, auto&& after_s) __attribute__((always_inline)) {
+    // One 32-key half (cb) of tile t in buffer buf;
+    auto compute = [&](auto careful, int t, int buf, int cb) __attribute__((always_inline)) {
         constexpr bool kCareful = decltype(careful)::value;
         const uint16_t *kt = ks[buf], *vt = vs[buf];
         const int r0 = t * kWinTile + 32 * cb;
         if (r0 > w_any || (r0 + 31 < w_from && r0 >= A.sinks)) {  // no row of the wave sees any of it
-            after_s();
             return;
         }
         uint32_t held = 0xffffffffu;
@@ -286,21 +276,10 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
         }
         const bool whole = r0 + 31 <= w_last && (r0 >= w_first || r0 + 31 < A.sinks) && held == 0xffffffffu;
         f32x16 sacc{};
-        const int krow = 32 * cb + arow;
 #pragma unroll
-        for (int s = 0; s < S; ++s) sacc = Mfma<DT>::run(T::rows(kt, krow, s, h), qf[s], sacc);
-        {
-            constexpr int kAhead = 4;  // K fragments are read this many products ahead
-            __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
-#pragma unroll
-            for (int i = 0; i < S - kAhead; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            }
-            __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
-        }
+        for (int s = 0; s < S; ++s) sacc = Mfma<DT>::run(at.rows(kt, 32 * cb, s), qf[s], sacc);
+        read_ahead<S>();
         __builtin_amdgcn_sched_barrier(0);
-        after_s();
         auto seen_at = [&](int row) {  // tile half's row -> whether this lane's query sees it
             const int r = r0 + row;
             return r <= last_r && (r >= first_r || r < A.sinks) && (held >> row & 1);
@@ -345,13 +324,14 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
         }
         if constexpr (kCareful) {
             if (!whole && tile_not_finite<DT, D>(vt, 32 * cb, lane)) {
-                add_rows_seen<DT, D>(oacc, vt, 32 * cb, pp, lane, seen_at);
+                add_rows_seen<DT, D>(oacc, vt, 32 * cb, pp, at, h, seen_at);
                 return;
             }
         } else if (!whole) {
             dirty |= tile_not_finite<DT, D>(vt, 32 * cb, lane);
         }
-        add_rows<DT, D>(oacc, vt, 32 * cb, pp, lane);
+        __builtin_amdgcn_sched_barrier(0);
+        add_rows<DT, D>(oacc, vt, 32 * cb, pp, at);
     };
 
     // One walk over the tiles. The careful one is taken again from the start when the first met an infinity or NaN
@@ -363,13 +343,9 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
         l_run = neg_m = 0.0f;
         wide = false;
         if (tile0 >= tile1) return;
-        if constexpr (kMode != kNear) {
-            int p0 = 0, p1 = 0;
-            if constexpr (kMode == kPaged) {
-                p0 = *table_entry(tile0 * kWinTile + own);
-                p1 = *table_entry((tile0 + 1) * kWinTile + own);
-                if (owner) page_of[0][own] = *table_entry((tile0 + 2) * kWinTile + own);
-            }
+        if constexpr (kMode == kPaged) {
+            const int p0 = *table_entry(tile0 * kWinTile + own), p1 = *table_entry((tile0 + 1) * kWinTile + own);
+            if (owner) page_of[0][own] = *table_entry((tile0 + 2) * kWinTile + own);
             publish(tile0, 0, p0);
             publish(tile0 + 1, 1, p1);
             __syncthreads();
@@ -385,21 +361,15 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
         __syncthreads();
         auto step = [&](auto bufc, int t) __attribute__((always_inline)) {
             const int buf = bufc;
-            const bool more = t + 1 < tile1;
-            auto next = [&]() __attribute__((always_inline)) {
-                if (more) load_tile(t + 1, buf ^ 1);
-            };
+            if (t + 1 < tile1) load_tile(t + 1, buf ^ 1);
             if (wave_active) {
                 if constexpr (decltype(careful)::value) {
-                    next();
 #pragma unroll 1
-                    for (int cb = hb; cb < (split ? hb + 1 : 2); ++cb) compute(careful, t, buf, cb, [] {});
+                    for (int cb = hb; cb < (split ? hb + 1 : 2); ++cb) compute(careful, t, buf, cb);
                 } else {
-                    compute(careful, t, buf, hb, next);
-                    if (!split) compute(careful, t, buf, 1, [] {});
+                    compute(careful, t, buf, hb);
+                    if (!split) compute(careful, t, buf, 1);
                 }
-            } else {
-                next();
             }
             if constexpr (kMode == kPaged) {
                 // Page numbers of tile t + 3 start on their way to LDS; those of tile t + 2 and this wave's share of
@@ -407,14 +377,10 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
                 const int32_t* e = table_entry((t + 3) * kWinTile + own);
                 if (owner) dma4(e, lds_addr(&page_of[buf ^ 1][kLook * wave]));
                 asm volatile("s_waitcnt vmcnt(1)" ::: "memory");
+                // (This tile's row offsets were last read a tile ago, when its loads were issued.)
+                publish(t + 2, buf, page_of[buf][own]);
             } else {
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            }
-            if constexpr (kMode != kNear) {
-                // (This tile's row offsets were last read a tile ago, when its loads were issued.)
-                int page = 0;
-                if constexpr (kMode == kPaged) page = page_of[buf][own];
-                publish(t + 2, buf, page);
             }
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
             __builtin_amdgcn_s_barrier();

@@ -32,19 +32,39 @@ template <int D> struct WinTile {
     static __device__ __forceinline__ int swz(int row) {
         return CH == 16 ? 4 * (row % 4) + ((row >> 2) & 3) : 4 * ((row >> 1) & 1) + ((row >> 2) & 3);
     }
-    // A operand with the tile's rows along M: row, channels 16 s + 8 h .. + 7.
-    static __device__ __forceinline__ u16x8 rows(const uint16_t* t, int row, int s, int h) {
-        return *reinterpret_cast<const u16x8*>(t + row * D + ((2 * s + h) ^ swz(row)) * 8);
+};
+
+// Where a lane's fragments lie in a tile (bytes from its first row). Kept apart from the tile and the row block,
+// which are constants of the unrolled loops and go into the LDS reads' immediate offsets.
+template <int D> struct WinLane {
+    using T = WinTile<D>;
+    int row[D / 16];        // A operand with rows along M: row l % 32, channels 16 s + 8 (l / 32) .. + 7
+    int channel[D / 32][2]; // A operand with channels along M (see channels below)
+    __device__ __forceinline__ explicit WinLane(int lane) {
+        const int h = lane / 32, r = lane % 32;
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) row[s] = 2 * (r * D + ((2 * s + h) ^ T::swz(r)) * 8);
+        const int src = lane % 16;
+#pragma unroll
+        for (int nb = 0; nb < D / 32; ++nb)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int d = 32 * nb + 16 * ((lane / 16) % 2) + 4 * (src % 4), at = 8 * u + 4 * h + src / 4;
+                channel[nb][u] = 2 * (at * D + ((d / 8) ^ T::swz(at)) * 8 + d % 8);
+            }
     }
-    // A operand with channels along M: channel 32 nb + l % 32, tile rows row0 + 8 t + 4 h + (0..3), t = 0, 1.
-    // Source lane r of each 16-lane group points at row r / 4, channels 32 nb + 16 ((l / 16) % 2) + 4 (r % 4).
-    static __device__ __forceinline__ u16x8 channels(const uint16_t* t, int row0, int nb, int lane) {
-        const int src = lane % 16, d = 32 * nb + 16 * ((lane / 16) % 2) + 4 * (src % 4);
+    // Rows row0 .. row0 + 31 (row0 a multiple of 32; the swizzle repeats every 16 rows), step s.
+    __device__ __forceinline__ u16x8 rows(const uint16_t* t, int row0, int s) const {
+        return *reinterpret_cast<const u16x8*>(reinterpret_cast<const char*>(t) + (row[s] + 2 * row0 * D));
+    }
+    // Channel 32 nb + l % 32 of tile rows row0 + 8 u + 4 (l / 32) + (0..3), u = 0, 1 (row0 a multiple of 16), by
+    // transpose reads: source lane r of each 16-lane group points at row r / 4, channels 32 nb + 16 ((l / 16) % 2) +
+    // 4 (r % 4).
+    __device__ __forceinline__ u16x8 channels(const uint16_t* t, int row0, int nb) const {
         u32x2 part[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const int row = row0 + 8 * u + 4 * (lane / 32) + src / 4;
-            const uint16_t* a = t + row * D + ((d / 8) ^ swz(row)) * 8 + (d % 8);
+            const char* a = reinterpret_cast<const char*>(t) + (channel[nb][u] + 2 * row0 * D);
             part[u] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                                     (__attribute__((address_space(3))) s16x4*)(a)));
         }
@@ -61,7 +81,7 @@ template <int DT> __device__ __forceinline__ bool not_finite(uint16_t b) {
 template <int DT, int D>
 __device__ __forceinline__ bool tile_not_finite(const uint16_t* t, int row0, int lane) {
     bool bad = false;
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < 32 * D / 8 / kWave; ++i) {
         const u16x8 x = *reinterpret_cast<const u16x8*>(t + row0 * D + (i * kWave + lane) * 8);
 #pragma unroll
@@ -70,18 +90,44 @@ __device__ __forceinline__ bool tile_not_finite(const uint16_t* t, int row0, int
     return __any(bad);
 }
 
+// Schedules the N products before it with their A fragments, one LDS read each, read four products ahead (LDS
+// latency is longer than a product; more in flight costs registers).
+template <int N> __device__ __forceinline__ void read_ahead() {
+    constexpr int kAhead = 4;
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);  // LDS reads
+#pragma unroll
+    for (int i = 0; i < N - kAhead; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+}
+
+// The same for N products whose A fragments are two transpose reads each.
+template <int N> __device__ __forceinline__ void read_channels_ahead() {
+    constexpr int kAhead = 3;
+    __builtin_amdgcn_sched_group_barrier(0x100, 2 * kAhead, 0);
+#pragma unroll
+    for (int i = 0; i < N - kAhead; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+}
+
 // acc += (tile rows row0 .. row0 + 31, channels along M) x w, where w holds this lane's column: packed weight
 // pairs of rows 8 (i / 4) + 4 h + i % 4.
 template <int DT, int D>
 __device__ __forceinline__ void add_rows(f32x16 (&acc)[D / 32], const uint16_t* t, int row0, const uint32_t (&w)[8],
-                                         int lane) {
+                                         const WinLane<D>& at) {
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
         const u16x8 b = __builtin_bit_cast(u16x8, u32x4{w[4 * kk], w[4 * kk + 1], w[4 * kk + 2], w[4 * kk + 3]});
 #pragma unroll
         for (int nb = 0; nb < D / 32; ++nb)
-            acc[nb] = Mfma<DT>::run(WinTile<D>::channels(t, row0 + 16 * kk, nb, lane), b, acc[nb]);
+            acc[nb] = Mfma<DT>::run(at.channels(t, row0 + 16 * kk, nb), b, acc[nb]);
     }
+    read_channels_ahead<D / 16>();
 }
 
 // The same for a tile with infinities or NaN in rows that some column hides: a hidden row's weight is 0, but 0
@@ -89,8 +135,7 @@ __device__ __forceinline__ void add_rows(f32x16 (&acc)[D / 32], const uint16_t* 
 // here only in a second walk over their tiles, after a first one met such a tile.
 template <int DT, int D, typename Seen>
 __device__ __forceinline__ void add_rows_seen(f32x16 (&acc)[D / 32], const uint16_t* t, int row0,
-                                              const uint32_t (&w)[8], int lane, const Seen& seen) {
-    const int h = lane / 32;
+                                              const uint32_t (&w)[8], const WinLane<D>& at, int h, const Seen& seen) {
 #pragma unroll 1
     for (int row = 0; row < 32; ++row) {
         const bool add = seen(row);
@@ -99,7 +144,7 @@ __device__ __forceinline__ void add_rows_seen(f32x16 (&acc)[D / 32], const uint1
             f32x16 one{};
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
-                u16x8 a = WinTile<D>::channels(t, row0 + 16 * kk, nb, lane);
+                u16x8 a = at.channels(t, row0 + 16 * kk, nb);
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                     if (16 * kk + 8 * (e / 4) + 4 * h + e % 4 != row) a[e] = 0;
@@ -111,6 +156,14 @@ __device__ __forceinline__ void add_rows_seen(f32x16 (&acc)[D / 32], const uint1
             for (int i = 0; i < 16; ++i) acc[nb][i] += add ? one[i] : 0.0f;
         }
     }
+}
+
+// 16 bytes a lane of row `row` (`stride` elements apart) of a head, at byte `chunk`, into LDS. kFar: the head's
+// rows span more than 2^32 bytes.
+template <bool kFar>
+__device__ __forceinline__ void load_row16(const uint16_t* head, int row, int64_t stride, uint32_t chunk, uint32_t lds) {
+    if constexpr (kFar) dma16(head + row * stride + chunk / 2, lds);
+    else dma16_off(head, static_cast<uint32_t>(row) * static_cast<uint32_t>(2 * stride) + chunk, lds);
 }
 
 // Row strides (elements) of a [batch, heads, rows, D] tensor.

@@ -1,0 +1,683 @@
+// Attention with a sliding window and sinks: gradients.
+//
+// With P the weights, g the gradient of the output and delta_i = g_i . out_i (= sum_j P_ij dP_ij):
+//   dV = P^T g,   dP = g V^T,   dS = P (dP - delta),   dQ = scale dS K,   dK = scale dS^T Q.
+// P is computed again from Q, K and the forward's row statistics: P = 2^((s - m) scale log2 e - log2 l).
+//
+// Two launches, both without atomics (every sum has one order):
+//   dQ: a workgroup takes 128 rows as in the forward and walks their keys; per 32-key half S^T = K Q^T and
+//       dP^T = V g^T (A = tile rows, B in registers), dQ^T += K^T dS^T (A = the K tile by transpose reads, B =
+//       dS^T straight from the accumulators). It also forms delta, which the second launch reads.
+//   dK/dV: a workgroup takes 128 keys, 32 a wave, and walks the rows that see any of them in 64-row tiles of Q
+//       and g; S = Q K^T and dP = g V^T (B = K, V in registers), dV^T += g^T P, dK^T += Q^T dS. The rows of all
+//       query heads of the key head pass by, so shared heads need no further sum. Keys that are sinks are seen
+//       by every later row: their walk is cut into parts, which a third launch adds up in order.
+//
+// Roundings: scores, dP, P and all sums are fp32; P and dS are rounded to the type for the products.
+// fp16: its smallest normal number, 2^-14, is large for a weight among thousands and for a gradient, so P enters
+// its product times 2^14 and dS times a power of two taken from |dS| <= 2 max|g_i| max|V_j| (lengths of rows); both
+// are divided out of the fp32 sums. bf16 has fp32's exponents and needs neither.
+#include "window.hpp"
+
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+#include <type_traits>
+
+namespace peco {
+namespace {
+
+struct GradArgs {
+    const uint16_t *q, *k, *v, *out, *grad;
+    uint16_t *dq, *dk, *dv;
+    Strides qs, ks, vs, os, gs, dqs, dks, dvs;
+    int heads, group, batch, queries, keys, left, right, sinks;
+    float scale_log2, scale;
+    const int32_t* lengths;
+    const float *row_max, *row_log;  // [batch, query heads, queries]
+    float* delta;                    // the same shape
+    int row_tiles, key_tiles;
+    // fp16: longest rows (squared) of V, per block of kWinRows of a key head, and of g, per row tile of one
+    float *v_long, *g_long;
+    int sink_tiles, sink_parts, parts;  // key tiles that hold sinks come first; parts of their walks and of the others'
+    float* part;                        // [batch * heads, split items, 128, 2, D]
+};
+
+struct Sequence {
+    int queries, keys, position0;
+};
+__device__ __forceinline__ Sequence sequence_of(const GradArgs& A, int b) {
+    Sequence s{A.queries, A.keys, A.keys - A.queries};
+    if (A.lengths) {
+        s.keys = s.queries = __builtin_amdgcn_readfirstlane(max(0, min(A.lengths[b], A.keys)));
+        s.position0 = 0;
+    }
+    return s;
+}
+
+// fp16: dS is multiplied by this power of two (never more than 2^14 then).
+__device__ __forceinline__ float dscale(float g2, float v2) {
+    const float bound = 2.0f * sqrtf(g2) * sqrtf(v2);
+    if (!(bound > 0x1p-80f && bound < 0x1p80f)) return 1.0f;
+    int e;
+    frexpf(bound, &e);  // bound < 2^e
+    return ldexpf(1.0f, 14 - e);
+}
+
+template <int n> __device__ __forceinline__ float block_max(float v, float* tmp) {
+#pragma unroll
+    for (int m = kWave / 2; m; m /= 2) v = fmaxf(v, __shfl_xor(v, m, kWave));
+    __syncthreads();
+    if (threadIdx.x % kWave == 0) tmp[threadIdx.x / kWave] = v;
+    __syncthreads();
+    v = tmp[0];
+#pragma unroll
+    for (int i = 1; i < n; ++i) v = fmaxf(v, tmp[i]);
+    return v;
+}
+
+// fp16: the longest of each block of kWinRows rows of V.
+template <int D> __global__ __launch_bounds__(256) void value_lengths_kernel(GradArgs A) {
+    __shared__ float tmp[4];
+    const int bh = blockIdx.x / A.key_tiles, tile = blockIdx.x % A.key_tiles;
+    const int b = bh / A.heads;
+    const Sequence q = sequence_of(A, b);
+    constexpr int G = D / 8;
+    float most = 0.0f;
+    for (int r = threadIdx.x / G; r < kWinRows; r += 256 / G) {
+        const int key = tile * kWinRows + r;
+        float sq = 0.0f;
+        if (key < q.keys) {
+            const u16x8 x = *reinterpret_cast<const u16x8*>(A.v + b * A.vs.b + (bh % A.heads) * A.vs.h +
+                                                            static_cast<int64_t>(key) * A.vs.s + 8 * (threadIdx.x % G));
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sq += f16_bits_to_f32(x[k]) * f16_bits_to_f32(x[k]);
+        }
+#pragma unroll
+        for (int m = G / 2; m; m /= 2) sq += __shfl_xor(sq, m, kWave);
+        most = fmaxf(most, sq);
+    }
+    most = block_max<4>(most, tmp);
+    if (threadIdx.x == 0) A.v_long[blockIdx.x] = most;
+}
+
+template <int DT, int D, bool kFar>
+__global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
+    using T = WinTile<D>;
+    constexpr int S = D / 16, NB = D / 32;
+    __shared__ __align__(16) uint16_t kvs[4][T::kElems];
+    uint16_t(*const ks)[T::kElems] = kvs;
+    uint16_t(*const vs)[T::kElems] = kvs + 2;
+    __shared__ float tmp[4];
+
+    const int heads = A.batch * A.heads;
+    const int bh = blockIdx.x % heads, tile = A.row_tiles - 1 - static_cast<int>(blockIdx.x / heads);
+    const int b = bh / A.heads, kvh = bh % A.heads;
+    const Sequence q = sequence_of(A, b);
+    const int row0 = tile * kWinRows, rows = min(kWinRows, A.queries * A.group - row0);
+    const int tid = threadIdx.x, lane = tid % kWave, h = lane / 32;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const bool wave_active = wave * 32 < rows;
+    const bool qvalid = wave * 32 + lane % 32 < rows;
+    const int lrow = min(row0 + wave * 32 + lane % 32, row0 + rows - 1);
+    const int token = lrow / A.group, head = kvh * A.group + (lrow - token * A.group);
+    const bool takes = qvalid && token < q.queries;
+
+    const int t_first = row0 / A.group, t_last = min((row0 + rows - 1) / A.group, q.queries - 1);
+    const KeyStream stream = t_first > t_last ? KeyStream{0, 0, 0}
+                                              : key_stream(q.position0 + t_first, q.position0 + t_last, q.keys, A.left,
+                                                           A.right, A.sinks);
+    const int L = stream.length, l_last = max(L - 1, 0);
+    const int tiles = static_cast<int>(ceil_div(L, kWinTile));
+    const int pos = q.position0 + token;
+    const int last_r = takes ? min(min(pos + A.right, q.keys - 1) - stream.delta, L - 1) : -1;
+    const int first_r = pos - A.left - stream.delta;
+    const int w_tok0 = min(row0 + wave * 32, row0 + rows - 1) / A.group;
+    const int w_tok1 = min(row0 + wave * 32 + 31, row0 + rows - 1) / A.group;
+    const int w_last =
+        w_tok1 < q.queries ? min(min(q.position0 + w_tok0 + A.right, q.keys - 1) - stream.delta, L - 1) : -1;
+    const int w_first = q.position0 + w_tok1 - A.left - stream.delta;
+    const int w_any = min(min(q.position0 + w_tok1 + A.right, q.keys - 1) - stream.delta, L - 1);
+    const int w_from = q.position0 + w_tok0 - A.left - stream.delta;
+
+    // This lane's half of its query's rows: channels 16 s + 8 h .. + 7.
+    u16x8 qf[S], gf[S];
+    const int64_t row_id = (static_cast<int64_t>(b) * (A.heads * A.group) + head) * A.queries + token;
+    float delta = 0.0f, g2 = 0.0f;
+    {
+        const uint16_t* qrow = A.q + b * A.qs.b + head * A.qs.h + token * A.qs.s;
+        const uint16_t* grow = A.grad + b * A.gs.b + head * A.gs.h + token * A.gs.s;
+        const uint16_t* orow = A.out + b * A.os.b + head * A.os.h + token * A.os.s;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            qf[s] = *reinterpret_cast<const u16x8*>(qrow + 16 * s + 8 * h);
+            gf[s] = *reinterpret_cast<const u16x8*>(grow + 16 * s + 8 * h);
+            const u16x8 of = *reinterpret_cast<const u16x8*>(orow + 16 * s + 8 * h);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float g = half_to_f32<DT>(gf[s][k]);
+                delta += g * half_to_f32<DT>(of[k]);
+                if constexpr (DT == kF16) g2 += g * g;
+            }
+        }
+    }
+    delta += __shfl_xor(delta, 32, kWave);
+    if (!takes) delta = 0.0f;
+    if (qvalid && h == 0) A.delta[row_id] = delta;
+    float dmul = 1.0f;
+    if constexpr (DT == kF16) {
+        g2 += __shfl_xor(g2, 32, kWave);
+        if (!takes) g2 = 0.0f;
+        const float longest = block_max<4>(g2, tmp);
+        if (tid == 0) A.g_long[static_cast<int64_t>(bh) * A.row_tiles + tile] = longest;
+        float v2 = 0.0f;
+        for (int i = tid; i < A.key_tiles; i += 256) v2 = fmaxf(v2, A.v_long[static_cast<int64_t>(bh) * A.key_tiles + i]);
+        dmul = dscale(g2, block_max<4>(v2, tmp));
+    }
+    const float m = A.row_max[row_id], log_l = A.row_log[row_id];
+
+    const uint16_t* kh = A.k + b * A.ks.b + kvh * A.ks.h;
+    const uint16_t* vh = A.v + b * A.vs.b + kvh * A.vs.h;
+    auto load_tile = [&](int t, int buf) __attribute__((always_inline)) {
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+        for (int i = 0; i < T::kLoads; ++i) {
+            const int span = i * 4 + wave;
+            const int r = span * T::kWaveRows + lane / T::CH, p = lane % T::CH;
+            const uint32_t chunk = (p ^ T::swz(r)) * 16;
+            const int sr = min(t * kWinTile + r, l_last);
+            load_row16<kFar>(kh, sr < stream.a1 ? sr : sr + stream.delta, A.ks.s, chunk, lds_addr(ks[buf] + span * kWave * 8));
+            load_row16<kFar>(vh, sr < stream.a1 ? sr : sr + stream.delta, A.vs.s, chunk, lds_addr(vs[buf] + span * kWave * 8));
+        }
+#endif
+    };
+    f32x16 acc[NB];
+    bool dirty = false;
+    const WinLane<D> at(lane);
+    auto compute = [&](auto careful, int t, int buf, int cb) __attribute__((always_inline)) {
+        const uint16_t *kt = ks[buf], *vt = vs[buf];
+        const int r0 = t * kWinTile + 32 * cb;
+        if (r0 > w_any || (r0 + 31 < w_from && r0 >= A.sinks)) {
+            return;
+        }
+        const bool whole = r0 + 31 <= w_last && (r0 >= w_first || r0 + 31 < A.sinks);
+        f32x16 sacc{}, pacc{};
+#pragma unroll
+        for (int s = 0; s < S; ++s) sacc = Mfma<DT>::run(at.rows(kt, 32 * cb, s), qf[s], sacc);
+#pragma unroll
+        for (int s = 0; s < S; ++s) pacc = Mfma<DT>::run(at.rows(vt, 32 * cb, s), gf[s], pacc);
+        read_ahead<2 * S>();
+        __builtin_amdgcn_sched_barrier(0);
+        auto seen_at = [&](int row) {
+            const int r = r0 + row;
+            return r <= last_r && (r >= first_r || r < A.sinks);
+        };
+        float ds[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[i] - m, A.scale_log2, -log_l));
+            ds[i] = p * (pacc[i] - delta);
+            if constexpr (DT == kF16) ds[i] *= dmul;
+        }
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (!seen_at(8 * (i / 4) + 4 * h + i % 4)) ds[i] = 0.0f;
+        }
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = Mfma<DT>::pack2(ds[2 * i], ds[2 * i + 1]);
+        if constexpr (decltype(careful)::value) {
+            if (!whole && tile_not_finite<DT, D>(kt, 32 * cb, lane)) {
+                add_rows_seen<DT, D>(acc, kt, 32 * cb, w, at, h, seen_at);
+                return;
+            }
+        } else if (!whole) {
+            dirty |= tile_not_finite<DT, D>(kt, 32 * cb, lane);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        add_rows<DT, D>(acc, kt, 32 * cb, w, at);
+    };
+    auto walk = [&](auto careful) __attribute__((always_inline)) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) acc[nb] = f32x16{};
+        if (tiles == 0) return;
+#if defined(__HIP_DEVICE_COMPILE__)
+        // (What the loop reads from registers has arrived: the compiler does not count the tile loads.)
+#pragma unroll
+        for (int s = 0; s < S; ++s) asm volatile("" ::"v"(qf[s]), "v"(gf[s]));
+        asm volatile("" ::"v"(m), "v"(log_l));
+#endif
+        load_tile(0, 0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        auto step = [&](auto bufc, int t) __attribute__((always_inline)) {
+            const int buf = bufc;
+            if (t + 1 < tiles) load_tile(t + 1, buf ^ 1);
+            if (!wave_active) {
+            } else if constexpr (decltype(careful)::value) {
+#pragma unroll 1
+                for (int cb = 0; cb < 2; ++cb) compute(careful, t, buf, cb);
+            } else {
+                compute(careful, t, buf, 0);
+                compute(careful, t, buf, 1);
+            }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+        };
+        if constexpr (decltype(careful)::value) {
+#pragma unroll 1
+            for (int t = 0; t < tiles; ++t) step(t & 1, t);
+        } else {
+            for (int t = 0; t < tiles; t += 2) {
+                step(std::integral_constant<int, 0>{}, t);
+                if (t + 1 < tiles) step(std::integral_constant<int, 1>{}, t + 1);
+            }
+        }
+    };
+    walk(std::false_type{});
+    if (__syncthreads_or(dirty)) walk(std::true_type{});
+    if (!qvalid) return;
+    const float mul = A.scale / dmul;
+    uint16_t* o = A.dq + b * A.dqs.b + head * A.dqs.h + token * A.dqs.s;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const uint32_t w0 = Mfma<DT>::pack2(acc[nb][4 * g] * mul, acc[nb][4 * g + 1] * mul);
+            const uint32_t w1 = Mfma<DT>::pack2(acc[nb][4 * g + 2] * mul, acc[nb][4 * g + 3] * mul);
+            *reinterpret_cast<u32x2*>(o + 32 * nb + 8 * g + 4 * h) = takes ? u32x2{w0, w1} : u32x2{0, 0};
+        }
+}
+
+// Items of a head: the sink tiles' parts, then the other tiles' parts.
+__host__ __device__ __forceinline__ int64_t grad_items(const GradArgs& A) {
+    return static_cast<int64_t>(A.sink_tiles) * A.sink_parts + static_cast<int64_t>(A.key_tiles - A.sink_tiles) * A.parts;
+}
+// Items of a head whose results are partial (the first ones of the list).
+__host__ __device__ __forceinline__ int64_t partial_items(const GradArgs& A) {
+    if (A.parts > 1) return grad_items(A);
+    return A.sink_parts > 1 ? static_cast<int64_t>(A.sink_tiles) * A.sink_parts : 0;
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(256, 1) void window_dkv_kernel(GradArgs A) {
+    using T = WinTile<D>;
+    constexpr int S = D / 16, NB = D / 32;
+    __shared__ __align__(16) uint16_t tiles_lds[4][T::kElems];
+    uint16_t(*const qt_)[T::kElems] = tiles_lds;
+    uint16_t(*const gt_)[T::kElems] = tiles_lds + 2;
+    __shared__ __align__(16) float stat[2][3][kWinTile];  // row maxima, log2 sums and deltas of a tile
+    __shared__ float tmp[4];
+
+    const int heads = A.batch * A.heads;
+    const int bh = blockIdx.x % heads;
+    const int item = static_cast<int>(blockIdx.x / heads);
+    const int sink_items = A.sink_tiles * A.sink_parts;
+    const bool sink = item < sink_items;
+    const int parts = sink ? A.sink_parts : A.parts;
+    const int tile = sink ? item / parts : A.sink_tiles + (item - sink_items) / parts;
+    const int part = sink ? item % parts : (item - sink_items) % parts;
+    const int b = bh / A.heads, kvh = bh % A.heads;
+    const Sequence q = sequence_of(A, b);
+    const int tid = threadIdx.x, lane = tid % kWave, h = lane / 32;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int key0 = tile * kWinRows, wkey0 = key0 + 32 * wave;
+    const int key = wkey0 + lane % 32;  // this lane's column
+
+    // Rows of the stream that see key j: [row_from(j), row_to(j)).
+    const int all_rows = q.queries * A.group;
+    auto row_from = [&](int j) {
+        const int64_t t = max(static_cast<int64_t>(j) - A.right - q.position0, int64_t{0});
+        return static_cast<int>(min(t * A.group, static_cast<int64_t>(all_rows)));
+    };
+    auto row_to = [&](int j) {
+        const int64_t t = j < A.sinks ? int64_t{1} << 31 : static_cast<int64_t>(j) + A.left - q.position0 + 1;
+        return static_cast<int>(max(min(t * A.group, static_cast<int64_t>(all_rows)), int64_t{0}));
+    };
+    const int last_key = min(key0 + kWinRows, q.keys) - 1;
+    int r_begin = 0, r_end = 0;
+    if (last_key >= key0) {
+        r_begin = row_from(key0);
+        r_end = key0 < A.sinks ? all_rows : row_to(last_key);
+    }
+    // 64-row tiles of this part.
+    const int all_tiles = r_end > r_begin ? static_cast<int>(ceil_div(r_end - r_begin, kWinTile)) : 0;
+    const int per = static_cast<int>(ceil_div(all_tiles, parts));
+    const int tile0 = min(part * per, all_tiles), tile1 = min(tile0 + per, all_tiles);
+    const bool held = key < q.keys;
+    const int from = held ? row_from(key) : 0x7fffffff, to = held ? row_to(key) : 0;
+    // Of the wave's keys: every one is seen by the rows [w_from, w_to), none by rows outside [w_first, w_last).
+    const bool wave_active = wkey0 < q.keys;
+    const int wlast = min(wkey0 + 31, q.keys - 1);
+    const int w_from = wkey0 + 31 < q.keys ? row_from(wlast) : 0x7fffffff, w_to = row_to(wkey0 + 31 < A.sinks ? wkey0 : max(wkey0, A.sinks));
+    const int w_first = row_from(wkey0), w_last = wkey0 < A.sinks ? all_rows : row_to(wlast);
+
+    u16x8 kf[S], vf[S];
+    {
+        const int row = min(key, A.keys - 1);
+        const uint16_t* krow = A.k + b * A.ks.b + kvh * A.ks.h + row * A.ks.s;
+        const uint16_t* vrow = A.v + b * A.vs.b + kvh * A.vs.h + row * A.vs.s;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            kf[s] = *reinterpret_cast<const u16x8*>(krow + 16 * s + 8 * h);
+            vf[s] = *reinterpret_cast<const u16x8*>(vrow + 16 * s + 8 * h);
+        }
+    }
+    float dmul = 1.0f;
+    constexpr float kShift = DT == kF16 ? 14.0f : 0.0f;  // P times 2^14
+    if constexpr (DT == kF16) {
+        float g2 = 0.0f, v2 = 0.0f;
+        for (int i = tid; i < A.row_tiles; i += 256) g2 = fmaxf(g2, A.g_long[static_cast<int64_t>(bh) * A.row_tiles + i]);
+        for (int i = tid; i < A.key_tiles; i += 256) v2 = fmaxf(v2, A.v_long[static_cast<int64_t>(bh) * A.key_tiles + i]);
+        g2 = block_max<4>(g2, tmp);
+        dmul = dscale(g2, block_max<4>(v2, tmp));
+    }
+
+    const uint16_t* qh = A.q + b * A.qs.b + static_cast<int64_t>(kvh) * A.group * A.qs.h;
+    const uint16_t* gh = A.grad + b * A.gs.b + static_cast<int64_t>(kvh) * A.group * A.gs.h;
+    const int64_t stat0 = (static_cast<int64_t>(b) * A.heads + kvh) * A.group * A.queries;
+    auto load_tile = [&](int t, int buf) __attribute__((always_inline)) {
+#if defined(__HIP_DEVICE_COMPILE__)
+        const int first = r_begin + t * kWinTile;
+#pragma unroll
+        for (int i = 0; i < T::kLoads; ++i) {
+            const int span = i * 4 + wave;
+            const int r = span * T::kWaveRows + lane / T::CH, p = lane % T::CH;
+            const int chunk = (p ^ T::swz(r)) * 8;
+            const int row = min(first + r, r_end - 1);  // rows past the walk repeat its last row
+            const int token = A.group == 1 ? row : row / A.group, head = row - token * A.group;
+            dma16(qh + head * A.qs.h + token * A.qs.s + chunk, lds_addr(qt_[buf] + span * kWave * 8));
+            dma16(gh + head * A.gs.h + token * A.gs.s + chunk, lds_addr(gt_[buf] + span * kWave * 8));
+        }
+        if (wave < 3) {
+            const int row = min(first + lane, r_end - 1);
+            const int token = A.group == 1 ? row : row / A.group, head = row - token * A.group;
+            const float* from = wave == 0 ? A.row_max : wave == 1 ? A.row_log : A.delta;
+            dma4(from + stat0 + static_cast<int64_t>(head) * A.queries + token, lds_addr(stat[buf][wave]));
+        }
+#endif
+    };
+
+    f32x16 dk[NB], dv[NB];
+    bool dirty = false;
+    const WinLane<D> at(lane);
+    auto compute = [&](auto careful, int t, int buf, int cb) __attribute__((always_inline)) {
+        const uint16_t *qt = qt_[buf], *gt = gt_[buf];
+        const int r0 = r_begin + t * kWinTile + 32 * cb;
+        if (r0 + 31 < w_first || r0 >= w_last) {
+            return;
+        }
+        const bool whole = r0 >= w_from && r0 + 31 < w_to;
+        f32x16 sacc{}, pacc{};
+#pragma unroll
+        for (int s = 0; s < S; ++s) sacc = Mfma<DT>::run(at.rows(qt, 32 * cb, s), kf[s], sacc);
+#pragma unroll
+        for (int s = 0; s < S; ++s) pacc = Mfma<DT>::run(at.rows(gt, 32 * cb, s), vf[s], pacc);
+        read_ahead<2 * S>();
+        __builtin_amdgcn_sched_barrier(0);
+        auto seen_at = [&](int row) { return r0 + row >= from && r0 + row < to; };
+        uint32_t wp[8], wd[8];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int row = 32 * cb + 8 * g + 4 * h;
+            const f32x4 m = *reinterpret_cast<const f32x4*>(&stat[buf][0][row]);
+            const f32x4 log_l = *reinterpret_cast<const f32x4*>(&stat[buf][1][row]);
+            const f32x4 delta = *reinterpret_cast<const f32x4*>(&stat[buf][2][row]);
+            float p[4], ds[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[4 * g + i] - m[i], A.scale_log2, kShift - log_l[i]));
+                ds[i] = p[i] * (pacc[4 * g + i] - delta[i]);
+                if constexpr (DT == kF16) ds[i] *= dmul * 0x1p-14f;
+                if (!whole && !seen_at(8 * g + 4 * h + i)) p[i] = ds[i] = 0.0f;
+            }
+            wp[2 * g] = Mfma<DT>::pack2(p[0], p[1]);
+            wp[2 * g + 1] = Mfma<DT>::pack2(p[2], p[3]);
+            wd[2 * g] = Mfma<DT>::pack2(ds[0], ds[1]);
+            wd[2 * g + 1] = Mfma<DT>::pack2(ds[2], ds[3]);
+        }
+        if constexpr (decltype(careful)::value) {
+            if (!whole && (tile_not_finite<DT, D>(qt, 32 * cb, lane) || tile_not_finite<DT, D>(gt, 32 * cb, lane))) {
+                add_rows_seen<DT, D>(dv, gt, 32 * cb, wp, at, h, seen_at);
+                add_rows_seen<DT, D>(dk, qt, 32 * cb, wd, at, h, seen_at);
+                return;
+            }
+        } else if (!whole) {
+            dirty |= tile_not_finite<DT, D>(qt, 32 * cb, lane) || tile_not_finite<DT, D>(gt, 32 * cb, lane);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        add_rows<DT, D>(dv, gt, 32 * cb, wp, at);
+        add_rows<DT, D>(dk, qt, 32 * cb, wd, at);
+    };
+    auto walk = [&](auto careful) __attribute__((always_inline)) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) dk[nb] = dv[nb] = f32x16{};
+        if (tile0 >= tile1) return;
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+        for (int s = 0; s < S; ++s) asm volatile("" ::"v"(kf[s]), "v"(vf[s]));
+#endif
+        load_tile(tile0, 0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        auto step = [&](auto bufc, int t) __attribute__((always_inline)) {
+            const int buf = bufc;
+            if (t + 1 < tile1) load_tile(t + 1, buf ^ 1);
+            if (!wave_active) {
+            } else if constexpr (decltype(careful)::value) {
+#pragma unroll 1
+                for (int cb = 0; cb < 2; ++cb) compute(careful, t, buf, cb);
+            } else {
+                compute(careful, t, buf, 0);
+                compute(careful, t, buf, 1);
+            }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+        };
+        if constexpr (decltype(careful)::value) {
+#pragma unroll 1
+            for (int t = tile0; t < tile1; ++t) step((t - tile0) & 1, t);
+        } else {
+            for (int t = tile0; t < tile1; t += 2) {
+                step(std::integral_constant<int, 0>{}, t);
+                if (t + 1 < tile1) step(std::integral_constant<int, 1>{}, t + 1);
+            }
+        }
+    };
+    walk(std::false_type{});
+    if (__syncthreads_or(dirty)) walk(std::true_type{});
+    const float kmul = A.scale / dmul, vmul = DT == kF16 ? 0x1p-14f : 1.0f;
+    if (parts > 1) {
+        // [head, item, key, dK | dV, D]; every key of the tile, so that the join reads nothing unwritten.
+        float* o = A.part + ((static_cast<int64_t>(bh) * partial_items(A) + item) * kWinRows + 32 * wave + lane % 32) * 2 * D;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int d = 32 * nb + 8 * g + 4 * h;
+                *reinterpret_cast<f32x4*>(o + d) = f32x4{dk[nb][4 * g] * kmul, dk[nb][4 * g + 1] * kmul,
+                                                         dk[nb][4 * g + 2] * kmul, dk[nb][4 * g + 3] * kmul};
+                *reinterpret_cast<f32x4*>(o + D + d) = f32x4{dv[nb][4 * g] * vmul, dv[nb][4 * g + 1] * vmul,
+                                                             dv[nb][4 * g + 2] * vmul, dv[nb][4 * g + 3] * vmul};
+            }
+        return;
+    }
+    if (key >= A.keys) return;
+    uint16_t* ok = A.dk + b * A.dks.b + kvh * A.dks.h + key * A.dks.s;
+    uint16_t* ov = A.dv + b * A.dvs.b + kvh * A.dvs.h + key * A.dvs.s;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int d = 32 * nb + 8 * g + 4 * h;
+            *reinterpret_cast<u32x2*>(ok + d) = u32x2{Mfma<DT>::pack2(dk[nb][4 * g] * kmul, dk[nb][4 * g + 1] * kmul),
+                                                      Mfma<DT>::pack2(dk[nb][4 * g + 2] * kmul, dk[nb][4 * g + 3] * kmul)};
+            *reinterpret_cast<u32x2*>(ov + d) = u32x2{Mfma<DT>::pack2(dv[nb][4 * g] * vmul, dv[nb][4 * g + 1] * vmul),
+                                                      Mfma<DT>::pack2(dv[nb][4 * g + 2] * vmul, dv[nb][4 * g + 3] * vmul)};
+        }
+}
+
+// dK and dV of the key tiles whose walks were cut: the parts' sums, in order. D / 2 lanes a key (4 values each of
+// dK, then of dV).
+template <int DT, int D> __global__ __launch_bounds__(256) void window_dkv_join_kernel(GradArgs A) {
+    constexpr int kLanes = D / 2;
+    const int heads = A.batch * A.heads;
+    const int split_tiles = A.parts > 1 ? A.key_tiles : A.sink_tiles;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
+    const int64_t per_head = static_cast<int64_t>(split_tiles) * kWinRows;
+    if (row >= heads * per_head) return;
+    const int bh = static_cast<int>(row / per_head), key = static_cast<int>(row % per_head);
+    const int tile = key / kWinRows;
+    if (key >= A.keys || (tile < A.sink_tiles ? A.sink_parts : A.parts) == 1) return;
+    const bool sink = tile < A.sink_tiles;
+    const int parts = sink ? A.sink_parts : A.parts;
+    const int64_t item = sink ? static_cast<int64_t>(tile) * parts
+                              : static_cast<int64_t>(A.sink_tiles) * A.sink_parts + static_cast<int64_t>(tile - A.sink_tiles) * parts;
+    const int c = 4 * (threadIdx.x % kLanes);
+    const float* p = A.part + ((static_cast<int64_t>(bh) * partial_items(A) + item) * kWinRows + key % kWinRows) * 2 * D + c;
+    f32x4 sum{};
+    for (int i = 0; i < parts; ++i) sum += *reinterpret_cast<const f32x4*>(p + static_cast<int64_t>(i) * kWinRows * 2 * D);
+    const int b = bh / A.heads, kvh = bh % A.heads;
+    uint16_t* o = c < D ? A.dk + b * A.dks.b + kvh * A.dks.h + key * A.dks.s + c
+                        : A.dv + b * A.dvs.b + kvh * A.dvs.h + key * A.dvs.s + (c - D);
+    *reinterpret_cast<u32x2*>(o) = u32x2{Mfma<DT>::pack2(sum[0], sum[1]), Mfma<DT>::pack2(sum[2], sum[3])};
+}
+
+// Parts of the key tiles' walks. Under a window a tile without sinks is seen by about left + right + 128 tokens,
+// one with sinks by every later token: the latter's walk is cut to about the former's length, so that no
+// workgroup walks on alone. Calls of few key tiles cut the other walks too, into parts of at least
+// kGradPartTiles tiles (a part writes and reads 128 KB of fp32).
+constexpr int kGradPartTiles = 8;
+constexpr int kMaxParts = 64;
+void plan_parts(GradArgs& A) {
+    A.row_tiles = static_cast<int>(ceil_div(static_cast<int64_t>(A.queries) * A.group, kWinRows));
+    A.key_tiles = static_cast<int>(ceil_div(A.keys, kWinRows));
+    const int64_t all = ceil_div(static_cast<int64_t>(A.queries) * A.group, kWinTile);
+    const int64_t window = std::min<int64_t>(A.queries, static_cast<int64_t>(A.left) + A.right + kWinRows);
+    const int64_t walk = std::max<int64_t>(1, std::min(all, ceil_div(window * A.group, kWinTile)));
+    A.sink_tiles = static_cast<int>(std::min<int64_t>(A.key_tiles, ceil_div(A.sinks, kWinRows)));
+    const int64_t items = static_cast<int64_t>(A.batch) * A.heads * A.key_tiles;
+    const int64_t slots = device_compute_units();
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kMaxParts, walk / kGradPartTiles));
+    A.parts = items >= slots ? 1 : static_cast<int>(std::min(most, ceil_div(2 * slots, items)));
+    const int64_t per = std::max<int64_t>(kGradPartTiles, ceil_div(walk, A.parts));
+    A.sink_parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMaxParts, ceil_div(all, per))));
+    if (A.sink_tiles == 0) A.sink_parts = 1;
+}
+
+struct GradLayout {
+    int64_t delta, v_long, g_long, part, floats;
+};
+GradLayout grad_layout(const GradArgs& A, int d, int dtype) {
+    const int64_t heads = static_cast<int64_t>(A.batch) * A.heads;
+    auto up = [](int64_t n) { return ceil_div(n, 4) * 4; };
+    GradLayout l{};
+    l.v_long = up(heads * A.group * A.queries);
+    l.g_long = l.v_long + (dtype == kF16 ? up(heads * A.key_tiles) : 0);
+    l.part = l.g_long + (dtype == kF16 ? up(heads * A.row_tiles) : 0);
+    l.floats = l.part + heads * partial_items(A) * kWinRows * 2 * d;
+    return l;
+}
+
+template <int DT, int D> int launch_grad(const GradArgs& A, bool far, hipStream_t s) {
+    const int64_t heads = static_cast<int64_t>(A.batch) * A.heads;
+    const int64_t dq = heads * A.row_tiles, dkv = heads * grad_items(A);
+    if (std::max(dq, dkv) > 0x7fffffff || heads * A.key_tiles > 0x7fffffff) return kUnsupportedShape;
+    if constexpr (DT == kF16)
+        hipLaunchKernelGGL((value_lengths_kernel<D>), dim3(static_cast<unsigned>(heads * A.key_tiles)), dim3(256), 0, s, A);
+    if (far) hipLaunchKernelGGL((window_dq_kernel<DT, D, true>), dim3(static_cast<unsigned>(dq)), dim3(256), 0, s, A);
+    else hipLaunchKernelGGL((window_dq_kernel<DT, D, false>), dim3(static_cast<unsigned>(dq)), dim3(256), 0, s, A);
+    hipLaunchKernelGGL((window_dkv_kernel<DT, D>), dim3(static_cast<unsigned>(dkv)), dim3(256), 0, s, A);
+    if (partial_items(A)) {
+        const int64_t rows = heads * (A.parts > 1 ? A.key_tiles : A.sink_tiles) * kWinRows;
+        hipLaunchKernelGGL((window_dkv_join_kernel<DT, D>), dim3(static_cast<unsigned>(ceil_div(rows, 256 / (D / 2)))),
+                           dim3(256), 0, s, A);
+    }
+    return hipGetLastError();
+}
+
+Strides strides_of(const int64_t* s) { return Strides{s[0], s[1], s[2]}; }
+bool shape_ok(int batch, int q_heads, int kv_heads, int queries, int keys, int left, int right, int sinks) {
+    return batch >= 1 && kv_heads >= 1 && q_heads >= kv_heads && q_heads % kv_heads == 0 && queries >= 1 && keys >= 1 &&
+           left >= -1 && right >= -1 && sinks >= 0 && left <= kUnbounded && right <= kUnbounded && sinks <= kUnbounded;
+}
+GradArgs sizes_of(int batch, int q_heads, int kv_heads, int queries, int keys, int left, int right, int sinks) {
+    GradArgs A{};
+    A.batch = batch;
+    A.heads = kv_heads;
+    A.group = q_heads / kv_heads;
+    A.queries = queries;
+    A.keys = keys;
+    A.left = left < 0 ? kUnbounded : left;
+    A.right = right < 0 ? kUnbounded : right;
+    A.sinks = sinks;
+    plan_parts(A);
+    return A;
+}
+
+}  // namespace
+}  // namespace peco
+
+using namespace peco;
+
+PECO_API size_t peco_window_attention_grad_workspace_size(int batch, int q_heads, int kv_heads, int queries, int keys,
+                                                          int left, int right, int sinks, int d, int dtype) {
+    if (!shape_ok(batch, q_heads, kv_heads, queries, keys, left, right, sinks)) return 0;
+    return static_cast<size_t>(
+        grad_layout(sizes_of(batch, q_heads, kv_heads, queries, keys, left, right, sinks), d, dtype).floats);
+}
+
+PECO_API int peco_window_attention_grad(const void* q, const void* k, const void* v, const void* output,
+                                        const void* grad, void* dq, void* dk, void* dv, const int64_t* strides,
+                                        const int32_t* lengths, const float* row_max, const float* row_log,
+                                        float* workspace, size_t workspace_floats, int batch, int q_heads, int kv_heads,
+                                        int queries, int keys, int left, int right, int sinks, float scale, int d,
+                                        int dtype, void* stream) {
+    if (!q || !k || !v || !output || !grad || !dq || !dk || !dv || !strides || !row_max || !row_log || !workspace ||
+        !shape_ok(batch, q_heads, kv_heads, queries, keys, left, right, sinks) ||
+        !(scale >= FLT_MIN && scale <= FLT_MAX) || (lengths && queries != keys))
+        return kInvalidValue;
+    if (d != 64 && d != 128) return kUnsupportedShape;
+    if (dtype != kBF16 && dtype != kF16) return kUnsupportedDtype;
+    if (keys > kUnbounded - 1 || queries > kUnbounded - 1 ||
+        static_cast<int64_t>(queries) * (q_heads / kv_heads) > 0x7fffff00)
+        return kUnsupportedShape;
+    int64_t all = 0;
+    for (int i = 0; i < 24; ++i) all |= strides[i];
+    uintptr_t at = 0;
+    for (const void* p : {q, k, v, output, grad, static_cast<const void*>(dq), static_cast<const void*>(dk),
+                          static_cast<const void*>(dv), static_cast<const void*>(workspace)})
+        at |= reinterpret_cast<uintptr_t>(p);
+    if (all % 8 || at % 16) return kInvalidValue;
+    GradArgs A = sizes_of(batch, q_heads, kv_heads, queries, keys, left, right, sinks);
+    const GradLayout l = grad_layout(A, d, dtype);
+    if (workspace_floats < static_cast<size_t>(l.floats)) return kWorkspaceTooSmall;
+    A.q = static_cast<const uint16_t*>(q);
+    A.k = static_cast<const uint16_t*>(k);
+    A.v = static_cast<const uint16_t*>(v);
+    A.out = static_cast<const uint16_t*>(output);
+    A.grad = static_cast<const uint16_t*>(grad);
+    A.dq = static_cast<uint16_t*>(dq);
+    A.dk = static_cast<uint16_t*>(dk);
+    A.dv = static_cast<uint16_t*>(dv);
+    Strides* const to[8] = {&A.qs, &A.ks, &A.vs, &A.os, &A.gs, &A.dqs, &A.dks, &A.dvs};
+    for (int i = 0; i < 8; ++i) *to[i] = strides_of(strides + 3 * i);
+    A.lengths = lengths;
+    A.row_max = row_max;
+    A.row_log = row_log;
+    A.scale = scale;
+    A.scale_log2 = static_cast<float>(1.4426950408889634 * static_cast<double>(scale));
+    A.delta = workspace;
+    A.v_long = workspace + l.v_long;
+    A.g_long = workspace + l.g_long;
+    A.part = workspace + l.part;
+    const bool far = std::max(A.ks.s, A.vs.s) * 2 * keys + 2 * d >= (int64_t{1} << 32);
+    const auto s = static_cast<hipStream_t>(stream);
+    if (dtype == kBF16) return d == 128 ? launch_grad<kBF16, 128>(A, far, s) : launch_grad<kBF16, 64>(A, far, s);
+    return d == 128 ? launch_grad<kF16, 128>(A, far, s) : launch_grad<kF16, 64>(A, far, s);
+}

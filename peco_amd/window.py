@@ -105,6 +105,41 @@ def _forward(q, k, v, lengths, left, right, sinks, scale, stats):
         return (out if target is out else out.copy_(target)), row_max, row_log
 
 
+def _backward(q, k, v, out, row_max, row_log, lengths, grad, left, right, sinks, scale):
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    if row_max is None:  # no query or no key: nothing is seen
+        return dq.zero_(), dk.zero_(), dv.zero_()
+    batch, heads, sq, dim = q.shape
+    with torch.cuda.device(q.device):
+        library = _native.library()
+        tensors = [rows16(t) for t in (q, k, v, out, grad)] + [dq, dk, dv]
+        shape = (batch, heads, k.shape[1], sq, k.shape[2], left, right, sinks)
+        code = _native.dtype_code(q.dtype)
+        floats = library.peco_window_attention_grad_workspace_size(*shape, dim, code)
+        workspace = torch.empty(floats, dtype=torch.float32, device=q.device)
+        raise_error(library.peco_window_attention_grad(
+            *[_native.ptr(t) for t in tensors], strides_of(*tensors), _native.ptr(lengths), _native.ptr(row_max),
+            _native.ptr(row_log), _native.ptr(workspace), floats, *shape, scale, dim, code,
+            _native.current_stream(q.device, *tensors, lengths, row_max, row_log, workspace)),
+            "window attention gradient")
+    return dq, dk, dv
+
+
+class _WindowAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lengths, mask):
+        out, row_max, row_log = _forward(q, k, v, lengths, *mask, True)
+        ctx.save_for_backward(q, k, v, lengths, out, row_max, row_log)
+        ctx.mask = mask
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        q, k, v, lengths, out, row_max, row_log = ctx.saved_tensors
+        return (*_backward(q, k, v, out, row_max, row_log, lengths, grad, *ctx.mask), None, None)
+
+
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window, sinks: int = 0, *,
                      lengths: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
     """softmax(scale Q K^T) V over the keys that each query sees.
@@ -121,4 +156,6 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window, 
     _check(q, k, v, lengths)
     mask = check_mask(window, sinks, scale, q.shape[3])
     lengths = None if lengths is None else lengths.contiguous()
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+        return _WindowAttention.apply(q, k, v, lengths, mask)
     return _forward(q, k, v, lengths, *mask, False)[0]

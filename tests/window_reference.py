@@ -53,3 +53,53 @@ def attention(q, k, v, left, right, sinks, scale=None, lengths=None):
             out[b, h, :last], bound[b, h, :last] = rows(q[b, h, :last], k[b, h // group, :n], v[b, h // group, :n], seen,
                                                         scale)[:2]
     return out, bound
+
+
+def rows_grad(q, k, v, g, seen, scale):
+    """((dq, dk, dv), (their bounds)) of one head, g [n, d] the gradient of out.
+
+    A weight computed again is off by e - u and by the forward's sum of rounded weights, u: e in all; rounded for
+    dV, u more. dP is off by (D + 2) 2^-24 sum |g||v|, delta by the bound of out under |g| and D 2^-24 sum |g||out|;
+    dS takes both, the weight's e, its rounding u and (fp16) half a smallest step of its scaled value, 2^-37 of
+    2 max|g| max|v|. The products' sums are fp32 (n 2^-24), the results rounded once.
+    """
+    unit, d = UNIT[q.dtype], q.shape[1]
+    out, off, w, e = rows(q, k, v, seen, scale)
+    q, k, v, g = q.double(), k.double(), v.double(), g.double()
+    dp = g @ v.T
+    delta = (g * out).sum(1, keepdim=True)
+    ds = w * (dp - delta)
+    dp_off = (d + 2) * 2.0 ** -24 * (g.abs() @ v.abs().T)
+    delta_off = (g.abs() * (off + d * 2.0 ** -24 * out.abs())).sum(1, keepdim=True)
+    ds_off = w * (e * (dp.abs() + delta.abs()) + dp_off + delta_off) + unit * ds.abs()
+    if unit == 2.0 ** -11 and seen.numel():
+        ds_off = ds_off + seen * (2.0 ** -36 * float(g.norm(dim=1).max()) * float(v.norm(dim=1).max()))
+    tiny = 2.0 ** -25 if unit == 2.0 ** -11 else 0.0
+    results, bounds = [], []
+    for weight, weight_off, x, mul in ((ds, ds_off, k, scale), (ds.T, ds_off.T, q, scale),
+                                       (w.T, ((e + unit) * w).T + seen.T * tiny * 2.0 ** -14, g, 1.0)):
+        r = mul * (weight @ x)
+        b = mul * (weight_off @ x.abs() + x.shape[0] * 2.0 ** -24 * (weight.abs() @ x.abs()))
+        results.append(r)
+        bounds.append(1.05 * b + unit * 1.05 * r.abs() + tiny + 2.0 ** -60)
+    return results, bounds
+
+
+def gradients(q, k, v, g, left, right, sinks, scale=None, lengths=None):
+    """((dq, dk, dv), (bounds)) of the whole tensors; the bound of a shared head is the sum of its heads'."""
+    batch, heads, sq, d = q.shape
+    group, sk = heads // k.shape[1], k.shape[2]
+    scale = d ** -0.5 if scale is None else scale
+    results = [torch.zeros(t.shape, dtype=torch.float64, device=q.device) for t in (q, k, v)]
+    bounds = [torch.zeros_like(t) for t in results]
+    for b in range(batch):
+        n = sk if lengths is None else max(0, min(int(lengths[b]), sk))
+        first, last = (sk - sq, sq) if lengths is None else (0, n)
+        seen = seen_keys(torch.arange(first, first + last, device=q.device), n, left, right, sinks)
+        for h in range(heads):
+            r, o = rows_grad(q[b, h, :last], k[b, h // group, :n], v[b, h // group, :n], g[b, h, :last], seen, scale)
+            for to, part in ((results, r), (bounds, o)):
+                to[0][b, h, :last] = part[0]
+                to[1][b, h // group, :n] += part[1]
+                to[2][b, h // group, :n] += part[2]
+    return results, bounds
