@@ -332,26 +332,28 @@ int peco_place_heads_axes(const void* input, int64_t stride_batch, int64_t strid
  * end together: query i stands at p = i + keys - queries and sees key j when j <= p + right and (j >= p - left or
  * j < sinks); left or right -1 is without limit. A query that sees no key gives 0. lengths (nullable, device,
  * int32 [batch], needs queries == keys): tokens of each sequence of a padded batch (clamped to [0, keys]); later
- * keys are not seen and later queries give 0. scale: positive, of the scores. row_max and row_log (both or
- * neither, fp32 [batch, q_heads, queries]) receive each row's largest unscaled score and the log2 of its sum for
- * peco_window_attention_grad. workspace: peco_window_attention_workspace_size floats, 16-byte aligned (calls that
+ * keys are not seen and later queries give 0. scale: positive, of the scores. row_max, row_log (fp32
+ * [batch, q_heads, queries]) and output_rest (the output's dtype, contiguous [batch, q_heads, queries, d]; all three
+ * or none) receive each row's largest unscaled score, the log2 of its sum and what the rounding of its output left,
+ * for peco_window_attention_grad. workspace: peco_window_attention_workspace_size floats, 16-byte aligned (calls that
  * overlap need one each; may be null when that is 0). */
 size_t peco_window_attention_workspace_size(int batch, int q_heads, int kv_heads, int queries, int keys, int left,
                                             int right, int sinks, int d);
 int peco_window_attention(const void* q, const void* k, const void* v, void* output, const int64_t* strides,
-                          const int32_t* lengths, float* row_max, float* row_log, float* workspace,
-                          size_t workspace_floats, int batch, int q_heads, int kv_heads, int queries, int keys,
+                          const int32_t* lengths, float* row_max, float* row_log, void* output_rest,
+                          float* workspace, size_t workspace_floats, int batch, int q_heads, int kv_heads, int queries, int keys,
                           int left, int right, int sinks, float scale, int d, int dtype, void* stream);
 
 /* Its gradients: dq, dk, dv (of the shapes of q, k, v) from grad, the gradient of output, with the inputs, output,
- * row_max and row_log of the forward call. strides: of q, k, v, output, grad, dq, dk, dv (24 values). Written with
+ * row_max, row_log and output_rest of the forward call. strides: of q, k, v, output, grad, dq, dk, dv (24 values). Written with
  * lengths: every row of dq, dk and dv, 0 behind a sequence's length. workspace:
  * peco_window_attention_grad_workspace_size floats, 16-byte aligned (calls that overlap need one each). */
 size_t peco_window_attention_grad_workspace_size(int batch, int q_heads, int kv_heads, int queries, int keys, int left,
                                                  int right, int sinks, int d, int dtype);
 int peco_window_attention_grad(const void* q, const void* k, const void* v, const void* output, const void* grad,
                                void* dq, void* dk, void* dv, const int64_t* strides, const int32_t* lengths,
-                               const float* row_max, const float* row_log, float* workspace, size_t workspace_floats,
+                               const float* row_max, const float* row_log, const void* output_rest,
+                               float* workspace, size_t workspace_floats,
                                int batch, int q_heads, int kv_heads, int queries, int keys, int left, int right,
                                int sinks, float scale, int d, int dtype, void* stream);
 

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import fcntl
+import functools
 import os
 import shutil
 import subprocess
@@ -145,9 +146,9 @@ SIGNATURES = {
     "peco_dense_attention": (I, [P] * 4 + [I, P, Z] + [I] * 4 + [P]),
     "peco_place_heads": (I, [P] + [ctypes.c_int64] * 3 + [P] * 3 + [I, P, ctypes.c_float] + [I] * 7 + [P]),
     "peco_window_attention_workspace_size": (Z, [I] * 9),
-    "peco_window_attention": (I, [P] * 4 + [LP] + [P] * 4 + [Z] + [I] * 8 + [ctypes.c_float, I, I, P]),
+    "peco_window_attention": (I, [P] * 4 + [LP] + [P] * 5 + [Z] + [I] * 8 + [ctypes.c_float, I, I, P]),
     "peco_window_attention_grad_workspace_size": (Z, [I] * 10),
-    "peco_window_attention_grad": (I, [P] * 8 + [LP] + [P] * 4 + [Z] + [I] * 8 + [ctypes.c_float, I, I, P]),
+    "peco_window_attention_grad": (I, [P] * 8 + [LP] + [P] * 5 + [Z] + [I] * 8 + [ctypes.c_float, I, I, P]),
     "peco_paged_attention_workspace_size": (Z, [I] * 9),
     "peco_paged_attention": (I, [P] * 4 + [LP, P, ctypes.c_int64, P, P, I, P, Z] + [I] * 9 + [ctypes.c_float, I, I, P]),
     "peco_append_pages": (I, [P] * 4 + [LP, P, ctypes.c_int64, P, P] + PLAN + [I] * 8 + [P]),
@@ -203,6 +204,55 @@ def current_stream(device, *tensors) -> ctypes.c_void_p:
         if t is not None:
             t.record_stream(stream)
     return ctypes.c_void_p(stream.cuda_stream)
+
+
+def address(t):
+    """A tensor's address as the ctypes calls take it (None: a null pointer)."""
+    return None if t is None else t.data_ptr()
+
+
+def retain(device, *tensors) -> int:
+    """``current_stream`` for callers that time their host work: the stream's handle as an integer. For tensors that
+    the caller passed in; one allocated on the current stream in the same call needs no record."""
+    import torch
+
+    stream = torch.cuda.current_stream(device)
+    for t in tensors:
+        if t is not None:
+            t.record_stream(stream)
+    return stream.cuda_stream
+
+
+class _Here:
+    """The scope of the current device."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *_):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(device):
+    """``torch.cuda.device(device)``, without its cost where that device is the current one."""
+    import torch
+
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+@functools.lru_cache(maxsize=None)
+def _is_gfx950(index) -> bool:
+    import torch
+
+    return getattr(torch.cuda.get_device_properties(index), "gcnArchName", "").split(":")[0] == "gfx950"
+
+
+def require_gfx950(device) -> None:
+    if not _is_gfx950(device.index):
+        raise RuntimeError("This HIP build requires an MI355X-class gfx950 GPU")
 
 
 def plain_tensors(*tensors) -> bool:

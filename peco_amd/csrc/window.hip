@@ -53,8 +53,10 @@ struct WindowArgs {
     int clear_tail;          // paged: rows outside every sequence are cleared
     float* part_o;           // [splits, rows, D] with splits > 1
     float2* part_ml;         // [splits, rows]
-    float* row_max;          // nullable: raw maximum and log2 of the sum of every row (for the backward pass)
-    float* row_log;
+    // For the backward pass (all or none): raw maximum and log2 of the sum of every row, and what the rounding of
+    // its output left (output rows one after another).
+    float *row_max, *row_log;
+    uint16_t* out_rest;
 };
 
 // Where a workgroup's rows are.
@@ -142,11 +144,21 @@ template <int D> __device__ void clear_tail(const WindowArgs& A, int kvh) {
     }
 }
 
+// Four values of an output row, and with `rest` what their rounding left.
+template <int DT> __device__ __forceinline__ void store_output(f32x4 x, uint16_t* out, uint16_t* rest) {
+    const u32x2 w{Mfma<DT>::pack2(x[0], x[1]), Mfma<DT>::pack2(x[2], x[3])};
+    *reinterpret_cast<u32x2*>(out) = w;
+    if (!rest) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] -= half_to_f32<DT>(static_cast<uint16_t>(w[i / 2] >> (16 * (i % 2))));
+    *reinterpret_cast<u32x2*>(rest) = u32x2{Mfma<DT>::pack2(x[0], x[1]), Mfma<DT>::pack2(x[2], x[3])};
+}
+
 template <int DT, int D, int kMode>
 __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
     using T = WinTile<D>;
     constexpr int S = D / 16, NB = D / 32, H = 2;
-    __shared__ __align__(16) uint16_t kvs[4][T::kElems];
+    __shared__ __align__(256) uint16_t kvs[4][T::kElems];  // K tiles, V tiles
     uint16_t(*const ks)[T::kElems] = kvs;
     uint16_t(*const vs)[T::kElems] = kvs + 2;
     static_assert(2 * kWave * (NB * 16 + 2) * sizeof(float) <= sizeof(kvs), "pair exchange exceeds the tile LDS");
@@ -260,12 +272,12 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
     f32x16 oacc[NB];
     float m_run, l_run, neg_m;
     bool wide, dirty = false;
-    const WinLane<D> at(lane);
+    const WinLane<D> at(lane, kvs[0]);
 
     // One 32-key half (cb) of tile t in buffer buf;
     auto compute = [&](auto careful, int t, int buf, int cb) __attribute__((always_inline)) {
         constexpr bool kCareful = decltype(careful)::value;
-        const uint16_t *kt = ks[buf], *vt = vs[buf];
+        const int kt = 2 * (buf * T::kElems + 32 * cb * D), vt = kt + 4 * T::kElems;  // bytes from the first tile
         const int r0 = t * kWinTile + 32 * cb;
         if (r0 > w_any || (r0 + 31 < w_from && r0 >= A.sinks)) {  // no row of the wave sees any of it
             return;
@@ -277,8 +289,8 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
         const bool whole = r0 + 31 <= w_last && (r0 >= w_first || r0 + 31 < A.sinks) && held == 0xffffffffu;
         f32x16 sacc{};
 #pragma unroll
-        for (int s = 0; s < S; ++s) sacc = Mfma<DT>::run(at.rows(kt, 32 * cb, s), qf[s], sacc);
-        read_ahead<S>();
+        for (int s = 0; s < S; ++s) sacc = Mfma<DT>::run(at.rows(kt, s), qf[s], sacc);
+        read_ahead<S, S, 4>();
         __builtin_amdgcn_sched_barrier(0);
         auto seen_at = [&](int row) {  // tile half's row -> whether this lane's query sees it
             const int r = r0 + row;
@@ -323,15 +335,15 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
             l_run = Mfma<DT>::sum2(pp[i / 2], l_run);
         }
         if constexpr (kCareful) {
-            if (!whole && tile_not_finite<DT, D>(vt, 32 * cb, lane)) {
-                add_rows_seen<DT, D>(oacc, vt, 32 * cb, pp, at, h, seen_at);
+            if (!whole && rows_not_finite<DT, D>(kvs[0], vt, lane)) {
+                add_rows_seen<DT, D>(oacc, vt, pp, at, h, seen_at);
                 return;
             }
         } else if (!whole) {
-            dirty |= tile_not_finite<DT, D>(vt, 32 * cb, lane);
+            dirty |= rows_not_finite<DT, D>(kvs[0], vt, lane);
         }
         __builtin_amdgcn_sched_barrier(0);
-        add_rows<DT, D>(oacc, vt, 32 * cb, pp, at);
+        add_rows<DT, D>(oacc, vt, pp, at);
     };
 
     // One walk over the tiles. The careful one is taken again from the start when the first met an infinity or NaN
@@ -456,9 +468,9 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const uint32_t w0 = Mfma<DT>::pack2(oacc[nb][4 * g] * inv, oacc[nb][4 * g + 1] * inv);
-            const uint32_t w1 = Mfma<DT>::pack2(oacc[nb][4 * g + 2] * inv, oacc[nb][4 * g + 3] * inv);
-            *reinterpret_cast<u32x2*>(o + 32 * nb + 8 * g + 4 * h) = u32x2{w0, w1};
+            f32x4 x{oacc[nb][4 * g], oacc[nb][4 * g + 1], oacc[nb][4 * g + 2], oacc[nb][4 * g + 3]};
+            store_output<DT>(x * inv, o + 32 * nb + 8 * g + 4 * h,
+                             A.row_max ? A.out_rest + row_id * D + 32 * nb + 8 * g + 4 * h : nullptr);
         }
 }
 
@@ -501,7 +513,7 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs A) {
         A.row_log[row] = l == 0.0f ? INFINITY : log2f(l);
     }
     uint16_t* dst = A.out + b * A.os.b + head * A.os.h + token * A.os.s + c;
-    *reinterpret_cast<u32x2*>(dst) = u32x2{Mfma<DT>::pack2(o[0] * inv, o[1] * inv), Mfma<DT>::pack2(o[2] * inv, o[3] * inv)};
+    store_output<DT>(o * inv, dst, A.row_max ? A.out_rest + row * D + c : nullptr);
 }
 
 template <int DT, int D> int launch_window(const WindowArgs& A, WindowMode mode, hipStream_t s) {
@@ -605,11 +617,11 @@ PECO_API size_t peco_window_attention_workspace_size(int batch, int q_heads, int
 }
 
 PECO_API int peco_window_attention(const void* q, const void* k, const void* v, void* output, const int64_t* strides,
-                                   const int32_t* lengths, float* row_max, float* row_log, float* workspace,
-                                   size_t workspace_floats_given, int batch, int q_heads, int kv_heads, int queries,
+                                   const int32_t* lengths, float* row_max, float* row_log, void* output_rest,
+                                   float* workspace, size_t workspace_floats_given, int batch, int q_heads, int kv_heads, int queries,
                                    int keys, int left, int right, int sinks, float scale, int d, int dtype,
                                    void* stream) {
-    if (!q || !k || !v || !output || !strides || !row_max != !row_log || batch < 1 || kv_heads < 1 ||
+    if (!q || !k || !v || !output || !strides || !row_max != !row_log || !row_max != !output_rest || batch < 1 || kv_heads < 1 ||
         q_heads < kv_heads || q_heads % kv_heads || queries < 1 || keys < 1 || !mask_ok(left, right, sinks) ||
         !scale_ok(scale) || (lengths && queries != keys))
         return kInvalidValue;
@@ -642,6 +654,8 @@ PECO_API int peco_window_attention(const void* q, const void* k, const void* v, 
     A.lengths = lengths;
     A.row_max = row_max;
     A.row_log = row_log;
+    A.out_rest = static_cast<uint16_t*>(output_rest);
+    if (!aligned(output_rest)) return kInvalidValue;
     const Shape shape = window_shape(batch, q_heads, kv_heads, queries, keys, left, right, sinks);
     if (workspace_floats(shape, d) > workspace_floats_given) return kWorkspaceTooSmall;
     if (shape.splits > 1 && !aligned(workspace)) return kInvalidValue;

@@ -34,40 +34,43 @@ template <int D> struct WinTile {
     }
 };
 
-// Where a lane's fragments lie in a tile (bytes from its first row). Kept apart from the tile and the row block,
-// which are constants of the unrolled loops and go into the LDS reads' immediate offsets.
+// LDS addresses (bytes) of a lane's fragments of the tile at address 0 of the workgroup's tiles. The steps of a row
+// of fragments differ from one another in bits of the swizzled chunk alone, so one address each and exclusive ors
+// give all of them; a tile's and a half's distance from the first tile are constants that go into the LDS reads'
+// immediate offsets. The tiles start on a multiple of 256 bytes.
+typedef __attribute__((address_space(3))) const u16x8* LdsChunk;
 template <int D> struct WinLane {
-    using T = WinTile<D>;
-    int row[D / 16];        // A operand with rows along M: row l % 32, channels 16 s + 8 (l / 32) .. + 7
-    int channel[D / 32][2]; // A operand with channels along M (see channels below)
-    __device__ __forceinline__ explicit WinLane(int lane) {
-        const int h = lane / 32, r = lane % 32;
-#pragma unroll
-        for (int s = 0; s < D / 16; ++s) row[s] = 2 * (r * D + ((2 * s + h) ^ T::swz(r)) * 8);
-        const int src = lane % 16;
-#pragma unroll
-        for (int nb = 0; nb < D / 32; ++nb)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int d = 32 * nb + 16 * ((lane / 16) % 2) + 4 * (src % 4), at = 8 * u + 4 * h + src / 4;
-                channel[nb][u] = 2 * (at * D + ((d / 8) ^ T::swz(at)) * 8 + d % 8);
-            }
+    int row;      // A operand with rows along M: row l % 32, channels 8 (l / 32) .. + 7
+    int channel;  // A operand with channels along M: see channels()
+    __device__ __forceinline__ WinLane(int lane, const uint16_t* tiles) {
+        using T = WinTile<D>;
+        const int h = lane / 32, r = lane % 32, src = lane % 16, at = 4 * h + src / 4;
+        const int base = static_cast<int>(lds_addr(tiles));
+        row = base + 2 * (r * D + (h ^ T::swz(r)) * 8);
+        const int d = 16 * ((lane / 16) % 2) + 4 * (src % 4);
+        channel = base + 2 * (at * D + ((d / 8) ^ T::swz(at)) * 8 + d % 8);
     }
-    // Rows row0 .. row0 + 31 (row0 a multiple of 32; the swizzle repeats every 16 rows), step s.
-    __device__ __forceinline__ u16x8 rows(const uint16_t* t, int row0, int s) const {
-        return *reinterpret_cast<const u16x8*>(reinterpret_cast<const char*>(t) + (row[s] + 2 * row0 * D));
+    // The same `bytes` (a multiple of 256) further on.
+    __device__ __forceinline__ WinLane moved(int bytes) const {
+        WinLane x = *this;
+        x.row += bytes;
+        x.channel += bytes;
+        return x;
     }
-    // Channel 32 nb + l % 32 of tile rows row0 + 8 u + 4 (l / 32) + (0..3), u = 0, 1 (row0 a multiple of 16), by
-    // transpose reads: source lane r of each 16-lane group points at row r / 4, channels 32 nb + 16 ((l / 16) % 2) +
-    // 4 (r % 4).
-    __device__ __forceinline__ u16x8 channels(const uint16_t* t, int row0, int nb) const {
+    // Keeps the compiler from computing every address once and holding them all through a loop.
+    __device__ __forceinline__ void fresh() { asm volatile("" : "+v"(row), "+v"(channel)); }
+    // The 32 rows at byte `off` (a multiple of 16 rows: the swizzle repeats every 16), channels 16 s + 8 (l / 32) ...
+    __device__ __forceinline__ u16x8 rows(int off, int s) const { return *LdsChunk((row ^ (32 * s)) + off); }
+    // Channel 32 nb + l % 32 of rows 8 u + 4 (l / 32) + (0..3), u = 0, 1, from byte `off` on (a multiple of 16 rows),
+    // by transpose reads: source lane r of each 16-lane group points at row r / 4, channels 32 nb + 16 ((l / 16) % 2)
+    // + 4 (r % 4).
+    __device__ __forceinline__ u16x8 channels(int off, int nb) const {
         u32x2 part[2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const char* a = reinterpret_cast<const char*>(t) + (channel[nb][u] + 2 * row0 * D);
-            part[u] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                    (__attribute__((address_space(3))) s16x4*)(a)));
-        }
+        for (int u = 0; u < 2; ++u)
+            part[u] = __builtin_bit_cast(
+                u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(
+                           (channel ^ (64 * nb + 32 * u)) + (off + 16 * u * D))));
         return __builtin_bit_cast(u16x8, u32x4{part[0][0], part[0][1], part[1][0], part[1][1]});
     }
 };
@@ -77,65 +80,53 @@ template <int DT> __device__ __forceinline__ bool not_finite(uint16_t b) {
     return (b & kExp) == kExp;
 }
 
-// Whether any of the 32 tile rows from row0 holds an infinity or NaN.
+// Whether any of the 32 rows at byte `off` of the tiles holds an infinity or NaN.
 template <int DT, int D>
-__device__ __forceinline__ bool tile_not_finite(const uint16_t* t, int row0, int lane) {
+__device__ __forceinline__ bool rows_not_finite(const uint16_t* tiles, int off, int lane) {
     bool bad = false;
 #pragma unroll 1
     for (int i = 0; i < 32 * D / 8 / kWave; ++i) {
-        const u16x8 x = *reinterpret_cast<const u16x8*>(t + row0 * D + (i * kWave + lane) * 8);
+        const u16x8 x = *reinterpret_cast<const u16x8*>(tiles + off / 2 + (i * kWave + lane) * 8);
 #pragma unroll
         for (int k = 0; k < 8; ++k) bad |= not_finite<DT>(x[k]);
     }
     return __any(bad);
 }
 
-// Schedules the N products before it with their A fragments, one LDS read each, read four products ahead (LDS
-// latency is longer than a product; more in flight costs registers).
-template <int N> __device__ __forceinline__ void read_ahead() {
-    constexpr int kAhead = 4;
+// Schedules the kProducts products before it with the kReads LDS reads of their operands, kAhead of them before the
+// first product and the others spread over the products (LDS latency is longer than a product; more in flight costs
+// registers).
+template <int kProducts, int kReads, int kAhead> __device__ __forceinline__ void read_ahead() {
     __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);  // LDS reads
+    constexpr int kRest = kReads - kAhead, kEach = (kRest + kProducts - 1) / kProducts;
 #pragma unroll
-    for (int i = 0; i < N - kAhead; ++i) {
+    for (int i = 0; i < kProducts; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        if (i * kEach < kRest) __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
 }
 
-// The same for N products whose A fragments are two transpose reads each.
-template <int N> __device__ __forceinline__ void read_channels_ahead() {
-    constexpr int kAhead = 3;
-    __builtin_amdgcn_sched_group_barrier(0x100, 2 * kAhead, 0);
-#pragma unroll
-    for (int i = 0; i < N - kAhead; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
-}
-
-// acc += (tile rows row0 .. row0 + 31, channels along M) x w, where w holds this lane's column: packed weight
-// pairs of rows 8 (i / 4) + 4 h + i % 4.
+// acc += (the 32 rows at byte `off`, channels along M) x w, where w holds this lane's column: packed weight pairs of
+// rows 8 (i / 4) + 4 h + i % 4.
 template <int DT, int D>
-__device__ __forceinline__ void add_rows(f32x16 (&acc)[D / 32], const uint16_t* t, int row0, const uint32_t (&w)[8],
+__device__ __forceinline__ void add_rows(f32x16 (&acc)[D / 32], int off, const uint32_t (&w)[8],
                                          const WinLane<D>& at) {
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
         const u16x8 b = __builtin_bit_cast(u16x8, u32x4{w[4 * kk], w[4 * kk + 1], w[4 * kk + 2], w[4 * kk + 3]});
 #pragma unroll
         for (int nb = 0; nb < D / 32; ++nb)
-            acc[nb] = Mfma<DT>::run(at.channels(t, row0 + 16 * kk, nb), b, acc[nb]);
+            acc[nb] = Mfma<DT>::run(at.channels(off + 32 * kk * D, nb), b, acc[nb]);
     }
-    read_channels_ahead<D / 16>();
+    read_ahead<D / 16, D / 8, 6>();
 }
 
-// The same for a tile with infinities or NaN in rows that some column hides: a hidden row's weight is 0, but 0
-// times them is NaN. Each tile row is multiplied by itself and added where seen(row) holds. The kernels come
-// here only in a second walk over their tiles, after a first one met such a tile.
+// The same for rows with infinities or NaN that some column hides: a hidden row's weight is 0, but 0 times them is
+// NaN. Each row is multiplied by itself and added where seen(row) holds. The kernels come here only in a second walk
+// over their tiles, after a first one met such a row.
 template <int DT, int D, typename Seen>
-__device__ __forceinline__ void add_rows_seen(f32x16 (&acc)[D / 32], const uint16_t* t, int row0,
-                                              const uint32_t (&w)[8], const WinLane<D>& at, int h, const Seen& seen) {
+__device__ __forceinline__ void add_rows_seen(f32x16 (&acc)[D / 32], int off, const uint32_t (&w)[8],
+                                              const WinLane<D>& at, int h, const Seen& seen) {
 #pragma unroll 1
     for (int row = 0; row < 32; ++row) {
         const bool add = seen(row);
@@ -144,7 +135,7 @@ __device__ __forceinline__ void add_rows_seen(f32x16 (&acc)[D / 32], const uint1
             f32x16 one{};
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
-                u16x8 a = at.channels(t, row0 + 16 * kk, nb);
+                u16x8 a = at.channels(off + 32 * kk * D, nb);
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                     if (16 * kk + 8 * (e / 4) + 4 * h + e % 4 != row) a[e] = 0;

@@ -8,12 +8,15 @@
 //   dQ: a workgroup takes 128 rows as in the forward and walks their keys; per 32-key half S^T = K Q^T and
 //       dP^T = V g^T (A = tile rows, B in registers), dQ^T += K^T dS^T (A = the K tile by transpose reads, B =
 //       dS^T straight from the accumulators). It also forms delta, which the second launch reads.
-//   dK/dV: a workgroup takes 128 keys, 32 a wave, and walks the rows that see any of them in 64-row tiles of Q
-//       and g; S = Q K^T and dP = g V^T (B = K, V in registers), dV^T += g^T P, dK^T += Q^T dS. The rows of all
+//   dK/dV: a workgroup of 8 waves takes 256 keys, 32 a wave, and walks the rows that see any of them in 64-row
+//       tiles of Q and g; S = Q K^T (B = K in registers) and dP = g V^T (B = V in LDS: with V in registers too the
+//       sums of both leave room for one wave a SIMD only), dV^T += g^T P, dK^T += Q^T dS. The rows of all
 //       query heads of the key head pass by, so shared heads need no further sum. Keys that are sinks are seen
 //       by every later row: their walk is cut into parts, which a third launch adds up in order.
 //
-// Roundings: scores, dP, P and all sums are fp32; P and dS are rounded to the type for the products.
+// Roundings: scores, dP, P and all sums are fp32; P and dS are rounded to the type for the products. delta takes out
+// with what its rounding left: where a query sees a few keys dS is a small difference, and out's rounding alone
+// would put as much error into it as dS's own.
 // fp16: its smallest normal number, 2^-14, is large for a weight among thousands and for a gradient, so P enters
 // its product times 2^14 and dS times a power of two taken from |dS| <= 2 max|g_i| max|V_j| (lengths of rows); both
 // are divided out of the fp32 sums. bf16 has fp32's exponents and needs neither.
@@ -27,8 +30,12 @@
 namespace peco {
 namespace {
 
+constexpr int kGradWaves = 8;               // of a dK/dV workgroup
+constexpr int kGradKeys = 32 * kGradWaves;  // its keys
+constexpr int kGradTile = 64;               // query rows of its tiles
+
 struct GradArgs {
-    const uint16_t *q, *k, *v, *out, *grad;
+    const uint16_t *q, *k, *v, *out, *out_rest, *grad;
     uint16_t *dq, *dk, *dv;
     Strides qs, ks, vs, os, gs, dqs, dks, dvs;
     int heads, group, batch, queries, keys, left, right, sinks;
@@ -36,11 +43,11 @@ struct GradArgs {
     const int32_t* lengths;
     const float *row_max, *row_log;  // [batch, query heads, queries]
     float* delta;                    // the same shape
-    int row_tiles, key_tiles;
+    int row_tiles, key_tiles, v_blocks;  // tiles of kWinRows rows, of kGradKeys keys, blocks of kWinRows keys
     // fp16: longest rows (squared) of V, per block of kWinRows of a key head, and of g, per row tile of one
     float *v_long, *g_long;
     int sink_tiles, sink_parts, parts;  // key tiles that hold sinks come first; parts of their walks and of the others'
-    float* part;                        // [batch * heads, split items, 128, 2, D]
+    float* part;                        // [batch * heads, partial items, kGradKeys, 2, D]
 };
 
 struct Sequence {
@@ -79,7 +86,7 @@ template <int n> __device__ __forceinline__ float block_max(float v, float* tmp)
 // fp16: the longest of each block of kWinRows rows of V.
 template <int D> __global__ __launch_bounds__(256) void value_lengths_kernel(GradArgs A) {
     __shared__ float tmp[4];
-    const int bh = blockIdx.x / A.key_tiles, tile = blockIdx.x % A.key_tiles;
+    const int bh = blockIdx.x / A.v_blocks, tile = blockIdx.x % A.v_blocks;
     const int b = bh / A.heads;
     const Sequence q = sequence_of(A, b);
     constexpr int G = D / 8;
@@ -105,7 +112,7 @@ template <int DT, int D, bool kFar>
 __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
     using T = WinTile<D>;
     constexpr int S = D / 16, NB = D / 32;
-    __shared__ __align__(16) uint16_t kvs[4][T::kElems];
+    __shared__ __align__(256) uint16_t kvs[4][T::kElems];  // K tiles, V tiles
     uint16_t(*const ks)[T::kElems] = kvs;
     uint16_t(*const vs)[T::kElems] = kvs + 2;
     __shared__ float tmp[4];
@@ -153,10 +160,11 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
             qf[s] = *reinterpret_cast<const u16x8*>(qrow + 16 * s + 8 * h);
             gf[s] = *reinterpret_cast<const u16x8*>(grow + 16 * s + 8 * h);
             const u16x8 of = *reinterpret_cast<const u16x8*>(orow + 16 * s + 8 * h);
+            const u16x8 rest = *reinterpret_cast<const u16x8*>(A.out_rest + row_id * D + 16 * s + 8 * h);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const float g = half_to_f32<DT>(gf[s][k]);
-                delta += g * half_to_f32<DT>(of[k]);
+                delta += g * (half_to_f32<DT>(of[k]) + half_to_f32<DT>(rest[k]));
                 if constexpr (DT == kF16) g2 += g * g;
             }
         }
@@ -171,7 +179,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
         const float longest = block_max<4>(g2, tmp);
         if (tid == 0) A.g_long[static_cast<int64_t>(bh) * A.row_tiles + tile] = longest;
         float v2 = 0.0f;
-        for (int i = tid; i < A.key_tiles; i += 256) v2 = fmaxf(v2, A.v_long[static_cast<int64_t>(bh) * A.key_tiles + i]);
+        for (int i = tid; i < A.v_blocks; i += 256) v2 = fmaxf(v2, A.v_long[static_cast<int64_t>(bh) * A.v_blocks + i]);
         dmul = dscale(g2, block_max<4>(v2, tmp));
     }
     const float m = A.row_max[row_id], log_l = A.row_log[row_id];
@@ -193,9 +201,9 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
     };
     f32x16 acc[NB];
     bool dirty = false;
-    const WinLane<D> at(lane);
+    const WinLane<D> at(lane, kvs[0]);
     auto compute = [&](auto careful, int t, int buf, int cb) __attribute__((always_inline)) {
-        const uint16_t *kt = ks[buf], *vt = vs[buf];
+        const int kt = 2 * (buf * T::kElems + 32 * cb * D), vt = kt + 4 * T::kElems;  // bytes from the first tile
         const int r0 = t * kWinTile + 32 * cb;
         if (r0 > w_any || (r0 + 31 < w_from && r0 >= A.sinks)) {
             return;
@@ -203,10 +211,10 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
         const bool whole = r0 + 31 <= w_last && (r0 >= w_first || r0 + 31 < A.sinks);
         f32x16 sacc{}, pacc{};
 #pragma unroll
-        for (int s = 0; s < S; ++s) sacc = Mfma<DT>::run(at.rows(kt, 32 * cb, s), qf[s], sacc);
+        for (int s = 0; s < S; ++s) sacc = Mfma<DT>::run(at.rows(kt, s), qf[s], sacc);
 #pragma unroll
-        for (int s = 0; s < S; ++s) pacc = Mfma<DT>::run(at.rows(vt, 32 * cb, s), gf[s], pacc);
-        read_ahead<2 * S>();
+        for (int s = 0; s < S; ++s) pacc = Mfma<DT>::run(at.rows(vt, s), gf[s], pacc);
+        read_ahead<2 * S, 2 * S, 4>();
         __builtin_amdgcn_sched_barrier(0);
         auto seen_at = [&](int row) {
             const int r = r0 + row;
@@ -228,15 +236,15 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = Mfma<DT>::pack2(ds[2 * i], ds[2 * i + 1]);
         if constexpr (decltype(careful)::value) {
-            if (!whole && tile_not_finite<DT, D>(kt, 32 * cb, lane)) {
-                add_rows_seen<DT, D>(acc, kt, 32 * cb, w, at, h, seen_at);
+            if (!whole && rows_not_finite<DT, D>(kvs[0], kt, lane)) {
+                add_rows_seen<DT, D>(acc, kt, w, at, h, seen_at);
                 return;
             }
         } else if (!whole) {
-            dirty |= tile_not_finite<DT, D>(kt, 32 * cb, lane);
+            dirty |= rows_not_finite<DT, D>(kvs[0], kt, lane);
         }
         __builtin_amdgcn_sched_barrier(0);
-        add_rows<DT, D>(acc, kt, 32 * cb, w, at);
+        add_rows<DT, D>(acc, kt, w, at);
     };
     auto walk = [&](auto careful) __attribute__((always_inline)) {
 #pragma unroll
@@ -303,14 +311,19 @@ __host__ __device__ __forceinline__ int64_t partial_items(const GradArgs& A) {
 }
 
 template <int DT, int D>
-__global__ __launch_bounds__(256, 1) void window_dkv_kernel(GradArgs A) {
+__global__ __launch_bounds__(kGradWaves * kWave, 2) void window_dkv_kernel(GradArgs A) {
     using T = WinTile<D>;
     constexpr int S = D / 16, NB = D / 32;
-    __shared__ __align__(16) uint16_t tiles_lds[4][T::kElems];
-    uint16_t(*const qt_)[T::kElems] = tiles_lds;
-    uint16_t(*const gt_)[T::kElems] = tiles_lds + 2;
-    __shared__ __align__(16) float stat[2][3][kWinTile];  // row maxima, log2 sums and deltas of a tile
-    __shared__ float tmp[4];
+    constexpr int kTile = kGradTile, kElems = kTile * D, kLoads = kTile / (kGradWaves * T::kWaveRows);
+    __shared__ __align__(256) uint16_t tiles_lds[4][kElems];  // Q tiles, g tiles
+    uint16_t(*const qt_)[kElems] = tiles_lds;
+    uint16_t(*const gt_)[kElems] = tiles_lds + 2;
+    // Operands of the workgroup's keys, as each lane takes them: V, and the last kSpilled steps of K. (With all of K
+    // in registers the compiler spills some of it to memory, whose loads wait for the tile loads before them.)
+    constexpr int kSpilled = D == 128 ? 3 : 0, kHeld = S - kSpilled;
+    __shared__ u16x8 operands[kGradWaves][S + kSpilled][kWave];
+    __shared__ __align__(16) float stat[2][3][kTile];  // row maxima, log2 sums and deltas of a tile
+    __shared__ float tmp[kGradWaves];
 
     const int heads = A.batch * A.heads;
     const int bh = blockIdx.x % heads;
@@ -324,7 +337,7 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(GradArgs A) {
     const Sequence q = sequence_of(A, b);
     const int tid = threadIdx.x, lane = tid % kWave, h = lane / 32;
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-    const int key0 = tile * kWinRows, wkey0 = key0 + 32 * wave;
+    const int key0 = tile * kGradKeys, wkey0 = key0 + 32 * wave;
     const int key = wkey0 + lane % 32;  // this lane's column
 
     // Rows of the stream that see key j: [row_from(j), row_to(j)).
@@ -337,14 +350,14 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(GradArgs A) {
         const int64_t t = j < A.sinks ? int64_t{1} << 31 : static_cast<int64_t>(j) + A.left - q.position0 + 1;
         return static_cast<int>(max(min(t * A.group, static_cast<int64_t>(all_rows)), int64_t{0}));
     };
-    const int last_key = min(key0 + kWinRows, q.keys) - 1;
+    const int last_key = min(key0 + kGradKeys, q.keys) - 1;
     int r_begin = 0, r_end = 0;
     if (last_key >= key0) {
         r_begin = row_from(key0);
         r_end = key0 < A.sinks ? all_rows : row_to(last_key);
     }
-    // 64-row tiles of this part.
-    const int all_tiles = r_end > r_begin ? static_cast<int>(ceil_div(r_end - r_begin, kWinTile)) : 0;
+    // Tiles of this part.
+    const int all_tiles = r_end > r_begin ? static_cast<int>(ceil_div(r_end - r_begin, kTile)) : 0;
     const int per = static_cast<int>(ceil_div(all_tiles, parts));
     const int tile0 = min(part * per, all_tiles), tile1 = min(tile0 + per, all_tiles);
     const bool held = key < q.keys;
@@ -355,25 +368,27 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(GradArgs A) {
     const int w_from = wkey0 + 31 < q.keys ? row_from(wlast) : 0x7fffffff, w_to = row_to(wkey0 + 31 < A.sinks ? wkey0 : max(wkey0, A.sinks));
     const int w_first = row_from(wkey0), w_last = wkey0 < A.sinks ? all_rows : row_to(wlast);
 
-    u16x8 kf[S], vf[S];
+    u16x8 kf[kHeld];
     {
         const int row = min(key, A.keys - 1);
         const uint16_t* krow = A.k + b * A.ks.b + kvh * A.ks.h + row * A.ks.s;
         const uint16_t* vrow = A.v + b * A.vs.b + kvh * A.vs.h + row * A.vs.s;
+        u16x8(*const own)[kWave] = operands[wave];  // (a wave reads what it wrote: no barrier)
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            kf[s] = *reinterpret_cast<const u16x8*>(krow + 16 * s + 8 * h);
-            vf[s] = *reinterpret_cast<const u16x8*>(vrow + 16 * s + 8 * h);
+            own[s][lane] = *reinterpret_cast<const u16x8*>(vrow + 16 * s + 8 * h);
+            const u16x8 x = *reinterpret_cast<const u16x8*>(krow + 16 * s + 8 * h);
+            if (s < kHeld) kf[s] = x;
+            else own[S + s - kHeld][lane] = x;
         }
     }
     float dmul = 1.0f;
-    constexpr float kShift = DT == kF16 ? 14.0f : 0.0f;  // P times 2^14
     if constexpr (DT == kF16) {
         float g2 = 0.0f, v2 = 0.0f;
-        for (int i = tid; i < A.row_tiles; i += 256) g2 = fmaxf(g2, A.g_long[static_cast<int64_t>(bh) * A.row_tiles + i]);
-        for (int i = tid; i < A.key_tiles; i += 256) v2 = fmaxf(v2, A.v_long[static_cast<int64_t>(bh) * A.key_tiles + i]);
-        g2 = block_max<4>(g2, tmp);
-        dmul = dscale(g2, block_max<4>(v2, tmp));
+        for (int i = tid; i < A.row_tiles; i += kGradWaves * kWave) g2 = fmaxf(g2, A.g_long[static_cast<int64_t>(bh) * A.row_tiles + i]);
+        for (int i = tid; i < A.v_blocks; i += kGradWaves * kWave) v2 = fmaxf(v2, A.v_long[static_cast<int64_t>(bh) * A.v_blocks + i]);
+        g2 = block_max<kGradWaves>(g2, tmp);
+        dmul = dscale(g2, block_max<kGradWaves>(v2, tmp));
     }
 
     const uint16_t* qh = A.q + b * A.qs.b + static_cast<int64_t>(kvh) * A.group * A.qs.h;
@@ -381,10 +396,12 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(GradArgs A) {
     const int64_t stat0 = (static_cast<int64_t>(b) * A.heads + kvh) * A.group * A.queries;
     auto load_tile = [&](int t, int buf) __attribute__((always_inline)) {
 #if defined(__HIP_DEVICE_COMPILE__)
-        const int first = r_begin + t * kWinTile;
+        const int first = r_begin + t * kTile;
+        int lane = threadIdx.x % kWave;
+        asm volatile("" : "+v"(lane));  // (the lane's shares of the addresses are computed again, not held)
 #pragma unroll
-        for (int i = 0; i < T::kLoads; ++i) {
-            const int span = i * 4 + wave;
+        for (int i = 0; i < kLoads; ++i) {
+            const int span = i * kGradWaves + wave;
             const int r = span * T::kWaveRows + lane / T::CH, p = lane % T::CH;
             const int chunk = (p ^ T::swz(r)) * 8;
             const int row = min(first + r, r_end - 1);  // rows past the walk repeat its last row
@@ -392,7 +409,7 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(GradArgs A) {
             dma16(qh + head * A.qs.h + token * A.qs.s + chunk, lds_addr(qt_[buf] + span * kWave * 8));
             dma16(gh + head * A.gs.h + token * A.gs.s + chunk, lds_addr(gt_[buf] + span * kWave * 8));
         }
-        if (wave < 3) {
+        if (wave < 3 && lane < kTile) {
             const int row = min(first + lane, r_end - 1);
             const int token = A.group == 1 ? row : row / A.group, head = row - token * A.group;
             const float* from = wave == 0 ? A.row_max : wave == 1 ? A.row_log : A.delta;
@@ -403,54 +420,73 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(GradArgs A) {
 
     f32x16 dk[NB], dv[NB];
     bool dirty = false;
-    const WinLane<D> at(lane);
+    const WinLane<D> at0(lane, tiles_lds[0]);
+    // One 32-row half of a tile: S and P, then dV, then dP and dS, then dK, which keeps one 32 x 32 result and its packed form alive
+    // at a time beside the sums.
     auto compute = [&](auto careful, int t, int buf, int cb) __attribute__((always_inline)) {
-        const uint16_t *qt = qt_[buf], *gt = gt_[buf];
-        const int r0 = r_begin + t * kWinTile + 32 * cb;
-        if (r0 + 31 < w_first || r0 >= w_last) {
-            return;
-        }
+        const int qoff = 2 * (buf * kElems + 32 * cb * D), goff = qoff + 4 * kElems;  // bytes from the first tile
+        constexpr int qt = 0, gt = 4 * kElems;  // (`at` holds the buffer and the half)
+        const int r0 = r_begin + t * kTile + 32 * cb;
+        if (r0 + 31 < w_first || r0 >= w_last) return;
         const bool whole = r0 >= w_from && r0 + 31 < w_to;
-        f32x16 sacc{}, pacc{};
-#pragma unroll
-        for (int s = 0; s < S; ++s) sacc = Mfma<DT>::run(at.rows(qt, 32 * cb, s), kf[s], sacc);
-#pragma unroll
-        for (int s = 0; s < S; ++s) pacc = Mfma<DT>::run(at.rows(gt, 32 * cb, s), vf[s], pacc);
-        read_ahead<2 * S>();
-        __builtin_amdgcn_sched_barrier(0);
+        constexpr bool kCareful = decltype(careful)::value;
+        if (!kCareful && !whole) dirty |= rows_not_finite<DT, D>(tiles_lds[0], qoff, lane) || rows_not_finite<DT, D>(tiles_lds[0], goff, lane);
         auto seen_at = [&](int row) { return r0 + row >= from && r0 + row < to; };
-        uint32_t wp[8], wd[8];
+        f32x16 p{}, ds{};
+        WinLane<D> at = at0.moved(qoff);
+        at.fresh();
+#pragma unroll
+        for (int s = S - 1; s >= kHeld; --s)
+            p = Mfma<DT>::run(at.rows(qt, s), operands[wave][S + s - kHeld][lane], p);
+#pragma unroll
+        for (int s = 0; s < kHeld; ++s) p = Mfma<DT>::run(at.rows(qt, s), kf[s], p);
+        read_ahead<S, S + kSpilled, 6>();
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const int row = 32 * cb + 8 * g + 4 * h;
-            const f32x4 m = *reinterpret_cast<const f32x4*>(&stat[buf][0][row]);
-            const f32x4 log_l = *reinterpret_cast<const f32x4*>(&stat[buf][1][row]);
-            const f32x4 delta = *reinterpret_cast<const f32x4*>(&stat[buf][2][row]);
-            float p[4], ds[4];
+            const f32x4 m = *reinterpret_cast<const f32x4*>(&stat[buf][0][32 * cb + 8 * g + 4 * h]);
+            const f32x4 log_l = *reinterpret_cast<const f32x4*>(&stat[buf][1][32 * cb + 8 * g + 4 * h]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[4 * g + i] - m[i], A.scale_log2, kShift - log_l[i]));
-                ds[i] = p[i] * (pacc[4 * g + i] - delta[i]);
-                if constexpr (DT == kF16) ds[i] *= dmul * 0x1p-14f;
-                if (!whole && !seen_at(8 * g + 4 * h + i)) p[i] = ds[i] = 0.0f;
+                const float x = __builtin_fmaf(p[4 * g + i] - m[i], A.scale_log2, DT == kF16 ? 14.0f - log_l[i] : -log_l[i]);
+                p[4 * g + i] = __builtin_amdgcn_exp2f(x);  // (fp16: times 2^14)
             }
-            wp[2 * g] = Mfma<DT>::pack2(p[0], p[1]);
-            wp[2 * g + 1] = Mfma<DT>::pack2(p[2], p[3]);
-            wd[2 * g] = Mfma<DT>::pack2(ds[0], ds[1]);
-            wd[2 * g + 1] = Mfma<DT>::pack2(ds[2], ds[3]);
         }
-        if constexpr (decltype(careful)::value) {
-            if (!whole && (tile_not_finite<DT, D>(qt, 32 * cb, lane) || tile_not_finite<DT, D>(gt, 32 * cb, lane))) {
-                add_rows_seen<DT, D>(dv, gt, 32 * cb, wp, at, h, seen_at);
-                add_rows_seen<DT, D>(dk, qt, 32 * cb, wd, at, h, seen_at);
-                return;
-            }
-        } else if (!whole) {
-            dirty |= tile_not_finite<DT, D>(qt, 32 * cb, lane) || tile_not_finite<DT, D>(gt, 32 * cb, lane);
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (!seen_at(8 * (i / 4) + 4 * h + i % 4)) p[i] = 0.0f;
         }
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = Mfma<DT>::pack2(p[2 * i], p[2 * i + 1]);
         __builtin_amdgcn_sched_barrier(0);
-        add_rows<DT, D>(dv, gt, 32 * cb, wp, at);
-        add_rows<DT, D>(dk, qt, 32 * cb, wd, at);
+        if constexpr (kCareful) add_rows_seen<DT, D>(dv, gt, w, at, h, seen_at);
+        else add_rows<DT, D>(dv, gt, w, at);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < S; ++s) ds = Mfma<DT>::run(at.rows(gt, s), operands[wave][s][lane], ds);
+        read_ahead<S, 2 * S, 6>();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const f32x4 delta = *reinterpret_cast<const f32x4*>(&stat[buf][2][32 * cb + 8 * g + 4 * h]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                ds[4 * g + i] = p[4 * g + i] * (ds[4 * g + i] - delta[i]);
+                if constexpr (DT == kF16) ds[4 * g + i] *= dmul * 0x1p-14f;
+            }
+        }
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (!seen_at(8 * (i / 4) + 4 * h + i % 4)) ds[i] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = Mfma<DT>::pack2(ds[2 * i], ds[2 * i + 1]);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (kCareful) add_rows_seen<DT, D>(dk, qt, w, at, h, seen_at);
+        else add_rows<DT, D>(dk, qt, w, at);
     };
     auto walk = [&](auto careful) __attribute__((always_inline)) {
 #pragma unroll
@@ -458,43 +494,31 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(GradArgs A) {
         if (tile0 >= tile1) return;
 #if defined(__HIP_DEVICE_COMPILE__)
 #pragma unroll
-        for (int s = 0; s < S; ++s) asm volatile("" ::"v"(kf[s]), "v"(vf[s]));
+        for (int s = 0; s < kHeld; ++s) asm volatile("" ::"v"(kf[s]));
 #endif
         load_tile(tile0, 0);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        auto step = [&](auto bufc, int t) __attribute__((always_inline)) {
-            const int buf = bufc;
+        auto step = [&](int buf, int t) __attribute__((always_inline)) {
             if (t + 1 < tile1) load_tile(t + 1, buf ^ 1);
-            if (!wave_active) {
-            } else if constexpr (decltype(careful)::value) {
+            if (wave_active) {
 #pragma unroll 1
-                for (int cb = 0; cb < 2; ++cb) compute(careful, t, buf, cb);
-            } else {
-                compute(careful, t, buf, 0);
-                compute(careful, t, buf, 1);
+                for (int cb = 0; cb < kTile / 32; ++cb) compute(careful, t, buf, cb);
             }
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
             __builtin_amdgcn_s_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
         };
-        if constexpr (decltype(careful)::value) {
 #pragma unroll 1
-            for (int t = tile0; t < tile1; ++t) step((t - tile0) & 1, t);
-        } else {
-            for (int t = tile0; t < tile1; t += 2) {
-                step(std::integral_constant<int, 0>{}, t);
-                if (t + 1 < tile1) step(std::integral_constant<int, 1>{}, t + 1);
-            }
-        }
+        for (int t = tile0; t < tile1; ++t) step((t - tile0) & 1, t);
     };
     walk(std::false_type{});
     if (__syncthreads_or(dirty)) walk(std::true_type{});
     const float kmul = A.scale / dmul, vmul = DT == kF16 ? 0x1p-14f : 1.0f;
     if (parts > 1) {
         // [head, item, key, dK | dV, D]; every key of the tile, so that the join reads nothing unwritten.
-        float* o = A.part + ((static_cast<int64_t>(bh) * partial_items(A) + item) * kWinRows + 32 * wave + lane % 32) * 2 * D;
+        float* o = A.part + ((static_cast<int64_t>(bh) * partial_items(A) + item) * kGradKeys + 32 * wave + lane % 32) * 2 * D;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -529,38 +553,39 @@ template <int DT, int D> __global__ __launch_bounds__(256) void window_dkv_join_
     const int heads = A.batch * A.heads;
     const int split_tiles = A.parts > 1 ? A.key_tiles : A.sink_tiles;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
-    const int64_t per_head = static_cast<int64_t>(split_tiles) * kWinRows;
+    const int64_t per_head = static_cast<int64_t>(split_tiles) * kGradKeys;
     if (row >= heads * per_head) return;
     const int bh = static_cast<int>(row / per_head), key = static_cast<int>(row % per_head);
-    const int tile = key / kWinRows;
+    const int tile = key / kGradKeys;
     if (key >= A.keys || (tile < A.sink_tiles ? A.sink_parts : A.parts) == 1) return;
     const bool sink = tile < A.sink_tiles;
     const int parts = sink ? A.sink_parts : A.parts;
     const int64_t item = sink ? static_cast<int64_t>(tile) * parts
                               : static_cast<int64_t>(A.sink_tiles) * A.sink_parts + static_cast<int64_t>(tile - A.sink_tiles) * parts;
     const int c = 4 * (threadIdx.x % kLanes);
-    const float* p = A.part + ((static_cast<int64_t>(bh) * partial_items(A) + item) * kWinRows + key % kWinRows) * 2 * D + c;
+    const float* p = A.part + ((static_cast<int64_t>(bh) * partial_items(A) + item) * kGradKeys + key % kGradKeys) * 2 * D + c;
     f32x4 sum{};
-    for (int i = 0; i < parts; ++i) sum += *reinterpret_cast<const f32x4*>(p + static_cast<int64_t>(i) * kWinRows * 2 * D);
+    for (int i = 0; i < parts; ++i) sum += *reinterpret_cast<const f32x4*>(p + static_cast<int64_t>(i) * kGradKeys * 2 * D);
     const int b = bh / A.heads, kvh = bh % A.heads;
     uint16_t* o = c < D ? A.dk + b * A.dks.b + kvh * A.dks.h + key * A.dks.s + c
                         : A.dv + b * A.dvs.b + kvh * A.dvs.h + key * A.dvs.s + (c - D);
     *reinterpret_cast<u32x2*>(o) = u32x2{Mfma<DT>::pack2(sum[0], sum[1]), Mfma<DT>::pack2(sum[2], sum[3])};
 }
 
-// Parts of the key tiles' walks. Under a window a tile without sinks is seen by about left + right + 128 tokens,
+// Parts of the key tiles' walks. Under a window a tile without sinks is seen by about left + right + 256 tokens,
 // one with sinks by every later token: the latter's walk is cut to about the former's length, so that no
 // workgroup walks on alone. Calls of few key tiles cut the other walks too, into parts of at least
-// kGradPartTiles tiles (a part writes and reads 128 KB of fp32).
-constexpr int kGradPartTiles = 8;
+// kGradPartTiles tiles (a part writes and reads 256 KB of fp32).
+constexpr int kGradPartTiles = 512 / kGradTile;
 constexpr int kMaxParts = 64;
 void plan_parts(GradArgs& A) {
     A.row_tiles = static_cast<int>(ceil_div(static_cast<int64_t>(A.queries) * A.group, kWinRows));
-    A.key_tiles = static_cast<int>(ceil_div(A.keys, kWinRows));
-    const int64_t all = ceil_div(static_cast<int64_t>(A.queries) * A.group, kWinTile);
-    const int64_t window = std::min<int64_t>(A.queries, static_cast<int64_t>(A.left) + A.right + kWinRows);
-    const int64_t walk = std::max<int64_t>(1, std::min(all, ceil_div(window * A.group, kWinTile)));
-    A.sink_tiles = static_cast<int>(std::min<int64_t>(A.key_tiles, ceil_div(A.sinks, kWinRows)));
+    A.key_tiles = static_cast<int>(ceil_div(A.keys, kGradKeys));
+    A.v_blocks = static_cast<int>(ceil_div(A.keys, kWinRows));
+    const int64_t all = ceil_div(static_cast<int64_t>(A.queries) * A.group, kGradTile);
+    const int64_t window = std::min<int64_t>(A.queries, static_cast<int64_t>(A.left) + A.right + kGradKeys);
+    const int64_t walk = std::max<int64_t>(1, std::min(all, ceil_div(window * A.group, kGradTile)));
+    A.sink_tiles = static_cast<int>(std::min<int64_t>(A.key_tiles, ceil_div(A.sinks, kGradKeys)));
     const int64_t items = static_cast<int64_t>(A.batch) * A.heads * A.key_tiles;
     const int64_t slots = device_compute_units();
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kMaxParts, walk / kGradPartTiles));
@@ -578,23 +603,24 @@ GradLayout grad_layout(const GradArgs& A, int d, int dtype) {
     auto up = [](int64_t n) { return ceil_div(n, 4) * 4; };
     GradLayout l{};
     l.v_long = up(heads * A.group * A.queries);
-    l.g_long = l.v_long + (dtype == kF16 ? up(heads * A.key_tiles) : 0);
+    l.g_long = l.v_long + (dtype == kF16 ? up(heads * A.v_blocks) : 0);
     l.part = l.g_long + (dtype == kF16 ? up(heads * A.row_tiles) : 0);
-    l.floats = l.part + heads * partial_items(A) * kWinRows * 2 * d;
+    l.floats = l.part + heads * partial_items(A) * kGradKeys * 2 * d;
     return l;
 }
 
 template <int DT, int D> int launch_grad(const GradArgs& A, bool far, hipStream_t s) {
     const int64_t heads = static_cast<int64_t>(A.batch) * A.heads;
     const int64_t dq = heads * A.row_tiles, dkv = heads * grad_items(A);
-    if (std::max(dq, dkv) > 0x7fffffff || heads * A.key_tiles > 0x7fffffff) return kUnsupportedShape;
+    if (std::max(dq, dkv) > 0x7fffffff || heads * A.v_blocks > 0x7fffffff) return kUnsupportedShape;
     if constexpr (DT == kF16)
-        hipLaunchKernelGGL((value_lengths_kernel<D>), dim3(static_cast<unsigned>(heads * A.key_tiles)), dim3(256), 0, s, A);
+        hipLaunchKernelGGL((value_lengths_kernel<D>), dim3(static_cast<unsigned>(heads * A.v_blocks)), dim3(256), 0, s, A);
     if (far) hipLaunchKernelGGL((window_dq_kernel<DT, D, true>), dim3(static_cast<unsigned>(dq)), dim3(256), 0, s, A);
     else hipLaunchKernelGGL((window_dq_kernel<DT, D, false>), dim3(static_cast<unsigned>(dq)), dim3(256), 0, s, A);
-    hipLaunchKernelGGL((window_dkv_kernel<DT, D>), dim3(static_cast<unsigned>(dkv)), dim3(256), 0, s, A);
+    hipLaunchKernelGGL((window_dkv_kernel<DT, D>), dim3(static_cast<unsigned>(dkv)),
+                       dim3(kGradWaves * kWave), 0, s, A);
     if (partial_items(A)) {
-        const int64_t rows = heads * (A.parts > 1 ? A.key_tiles : A.sink_tiles) * kWinRows;
+        const int64_t rows = heads * (A.parts > 1 ? A.key_tiles : A.sink_tiles) * kGradKeys;
         hipLaunchKernelGGL((window_dkv_join_kernel<DT, D>), dim3(static_cast<unsigned>(ceil_div(rows, 256 / (D / 2)))),
                            dim3(256), 0, s, A);
     }
@@ -635,10 +661,11 @@ PECO_API size_t peco_window_attention_grad_workspace_size(int batch, int q_heads
 PECO_API int peco_window_attention_grad(const void* q, const void* k, const void* v, const void* output,
                                         const void* grad, void* dq, void* dk, void* dv, const int64_t* strides,
                                         const int32_t* lengths, const float* row_max, const float* row_log,
-                                        float* workspace, size_t workspace_floats, int batch, int q_heads, int kv_heads,
+                                        const void* output_rest, float* workspace, size_t workspace_floats, int batch, int q_heads, int kv_heads,
                                         int queries, int keys, int left, int right, int sinks, float scale, int d,
                                         int dtype, void* stream) {
-    if (!q || !k || !v || !output || !grad || !dq || !dk || !dv || !strides || !row_max || !row_log || !workspace ||
+    if (!q || !k || !v || !output || !grad || !dq || !dk || !dv || !strides || !row_max || !row_log ||
+        !output_rest || !workspace ||
         !shape_ok(batch, q_heads, kv_heads, queries, keys, left, right, sinks) ||
         !(scale >= FLT_MIN && scale <= FLT_MAX) || (lengths && queries != keys))
         return kInvalidValue;
@@ -651,7 +678,7 @@ PECO_API int peco_window_attention_grad(const void* q, const void* k, const void
     for (int i = 0; i < 24; ++i) all |= strides[i];
     uintptr_t at = 0;
     for (const void* p : {q, k, v, output, grad, static_cast<const void*>(dq), static_cast<const void*>(dk),
-                          static_cast<const void*>(dv), static_cast<const void*>(workspace)})
+                          static_cast<const void*>(dv), output_rest, static_cast<const void*>(workspace)})
         at |= reinterpret_cast<uintptr_t>(p);
     if (all % 8 || at % 16) return kInvalidValue;
     GradArgs A = sizes_of(batch, q_heads, kv_heads, queries, keys, left, right, sinks);
@@ -661,6 +688,7 @@ PECO_API int peco_window_attention_grad(const void* q, const void* k, const void
     A.k = static_cast<const uint16_t*>(k);
     A.v = static_cast<const uint16_t*>(v);
     A.out = static_cast<const uint16_t*>(output);
+    A.out_rest = static_cast<const uint16_t*>(output_rest);
     A.grad = static_cast<const uint16_t*>(grad);
     A.dq = static_cast<uint16_t*>(dq);
     A.dk = static_cast<uint16_t*>(dk);

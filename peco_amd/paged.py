@@ -11,8 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _native, rotary as rotary_module
-from .attention_cuda import _device_is_gfx950
-from .window import check_mask, raise_error, rows16, strides_of
+from .window import check_mask, raise_error, rows16, strides_of, workspace_floats
 
 
 def _check_cache(k_pages, v_pages, page_table, offsets, lengths, rows, name):
@@ -31,17 +30,20 @@ def _check_cache(k_pages, v_pages, page_table, offsets, lengths, rows, name):
         raise ValueError("page_table must have shape [sequences,entries] and not be empty")
     if offsets.shape != (page_table.shape[0] + 1,) or lengths.shape != (page_table.shape[0],):
         raise ValueError("offsets and lengths must have shapes [sequences + 1] and [sequences]")
-    if any(t.dtype != torch.int32 for t in (page_table, offsets, lengths)):
+    if page_table.dtype != torch.int32 or offsets.dtype != torch.int32 or lengths.dtype != torch.int32:
         raise TypeError("page_table, offsets and lengths must be int32")
-    if not rows.is_cuda or any(t.device != rows.device for t in tensors):
+    device = rows.device
+    if not rows.is_cuda or k_pages.device != device or v_pages.device != device or page_table.device != device or \
+            offsets.device != device or lengths.device != device:
         raise ValueError("All paged cache inputs must reside on the same GPU device")
     if not _native.plain_tensors(*tensors):
         raise RuntimeError("a paged cache takes ordinary tensors (no tracing, transforms or tangents)")
     if torch.is_grad_enabled() and any(t.requires_grad for t in (rows, k_pages, v_pages)):
         raise RuntimeError("a paged cache supports inference only; use torch.no_grad()")
-    if any(rows16(t) is not t for t in (k_pages[:1], v_pages[:1])) or \
-            any(t.stride(0) % 8 for t in (k_pages, v_pages)):
-        raise ValueError("pages must have adjacent channels and rows on 16 bytes")
+    for t in (k_pages, v_pages):
+        a, b, c, inner = t.stride()
+        if inner != 1 or (a | b | c) % 8 or t.data_ptr() % 16:
+            raise ValueError("pages must have adjacent channels and rows on 16 bytes")
     if page_table.shape[1] * k_pages.shape[2] >= 1 << 30 or rows.shape[0] >= 1 << 30:
         raise ValueError("sequences must be shorter than 2^30")
 
@@ -76,15 +78,16 @@ def append_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
         plan = rotary_module.plan_arguments(rotary.axes, positions)
     if tokens == 0:
         return
-    with torch.cuda.device(k.device):
+    device = k.device
+    with _native.on_device(device):
+        _native.require_gfx950(device)
         k, v, table = rows16(k), rows16(v), page_table if page_table.stride(1) == 1 else page_table.contiguous()
         offsets, lengths = offsets.contiguous(), lengths.contiguous()
         _native.check(_native.library().peco_append_pages(
-            _native.ptr(k), _native.ptr(v), _native.ptr(k_pages), _native.ptr(v_pages), strides_of(k, v, k_pages, v_pages),
-            _native.ptr(table), table.stride(0), _native.ptr(offsets), _native.ptr(lengths), *plan, table.shape[0], heads,
+            k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), strides_of(k, v, k_pages, v_pages),
+            table.data_ptr(), table.stride(0), offsets.data_ptr(), lengths.data_ptr(), *plan, table.shape[0], heads,
             tokens, pages, page, table.shape[1], dim, _native.dtype_code(k.dtype),
-            _native.current_stream(k.device, k, v, k_pages, v_pages, table, offsets, lengths, positions)),
-            "PECO HIP append to pages")
+            _native.retain(device, k, v, k_pages, v_pages, table, offsets, lengths, positions)), "PECO HIP append to pages")
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -116,21 +119,20 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     result = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device) if out is None else out
     if tokens == 0:
         return result
-    with torch.cuda.device(q.device):
-        if not _device_is_gfx950(q.device):
-            raise RuntimeError("This HIP build requires an MI355X-class gfx950 GPU")
-        library = _native.library()
+    device = q.device
+    with _native.on_device(device):
+        _native.require_gfx950(device)
         q, table = rows16(q), page_table if page_table.stride(1) == 1 else page_table.contiguous()
         offsets, lengths = offsets.contiguous(), lengths.contiguous()
         batch, width = table.shape
-        floats = library.peco_paged_attention_workspace_size(batch, heads, kv_heads, tokens, width, page, left, sinks, dim)
-        workspace = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+        floats = workspace_floats("peco_paged_attention_workspace_size", device.index, batch, heads, kv_heads, tokens, width,
+                                  page, left, sinks, dim)
+        workspace = torch.empty(floats, dtype=torch.float32, device=device) if floats else None
         # (q and the output count head before token.)
         strides = strides_of(q.transpose(0, 1), k_pages, v_pages, result.transpose(0, 1))
-        raise_error(library.peco_paged_attention(
-            _native.ptr(q), _native.ptr(k_pages), _native.ptr(v_pages), _native.ptr(result), strides, _native.ptr(table),
-            table.stride(0), _native.ptr(offsets), _native.ptr(lengths), int(out is None), _native.ptr(workspace), floats,
+        raise_error(_native.library().peco_paged_attention(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), result.data_ptr(), strides, table.data_ptr(),
+            table.stride(0), offsets.data_ptr(), lengths.data_ptr(), int(out is None), _native.address(workspace), floats,
             batch, heads, kv_heads, tokens, pages, page, width, left, sinks, scale, dim, _native.dtype_code(q.dtype),
-            _native.current_stream(q.device, q, k_pages, v_pages, result, table, offsets, lengths, workspace)),
-            "paged attention")
+            _native.retain(device, q, k_pages, v_pages, out, table, offsets, lengths)), "paged attention")
     return result

@@ -88,7 +88,7 @@ def plan_arguments(axes, positions, inverse=False):
     """The plan's arguments of the C-ABI entries, for positions that ``check_positions`` returned."""
     turns, pairs = _plan(axes)
     batch = positions.stride(0) if positions.dim() == 3 and positions.shape[0] > 1 else 0
-    return (_native.ptr(positions), _POSITION_TYPES[positions.dtype], batch, positions.stride(-2), turns, pairs,
+    return (positions.data_ptr(), _POSITION_TYPES[positions.dtype], batch, positions.stride(-2), turns, pairs,
             len(axes.dims), int(axes.layout == "halves"), int(inverse))
 
 
@@ -114,8 +114,8 @@ def check_positions(axes, positions, batch, rows, dim, device):
 
 def _rows16(x):
     """x with adjacent channels and every row of every head on 16 bytes (a copy when it is laid out otherwise)."""
-    per16 = 16 // x.element_size()
-    if x.stride(3) == 1 and x.data_ptr() % 16 == 0 and all(s % per16 == 0 for s in x.stride()[:3]):
+    b, h, r, inner = x.stride()
+    if inner == 1 and x.data_ptr() % 16 == 0 and (b | h | r) * x.element_size() % 16 == 0:
         return x
     return x.clone(memory_format=torch.contiguous_format)
 
@@ -125,14 +125,16 @@ def _launch(x, positions, axes, inverse):
     if x.numel() == 0:
         return out
     batch, heads, rows, dim = x.shape
-    with torch.cuda.device(x.device):
+    device = x.device
+    with _native.on_device(device):
+        _native.require_gfx950(device)
         source, target = _rows16(x), out
         if _rows16(target) is not target:
-            target = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            target = torch.empty(x.shape, dtype=x.dtype, device=device)
         status = _native.library().peco_rotary_axes(
-            _native.ptr(source), *source.stride()[:3], _native.ptr(target), *target.stride()[:3],
+            source.data_ptr(), *source.stride()[:3], target.data_ptr(), *target.stride()[:3],
             *plan_arguments(axes, positions, inverse), batch, heads, rows, dim, _native.dtype_code(x.dtype),
-            _native.current_stream(x.device, source, target, positions))
+            _native.retain(device, source, positions))
         _native.check(status, "PECO HIP rotary positions")
         return out if target is out else out.copy_(target)
 

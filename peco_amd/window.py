@@ -7,25 +7,43 @@ or to both sides) and the first tokens of its sequence (the prompt's, say), whic
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
 
 from . import _native
-from .attention_cuda import _device_is_gfx950
 
 
 def rows16(t):
     """t with adjacent channels and every row on 16 bytes (a copy when it is laid out otherwise)."""
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1]):
-        return t
+    *outer, inner = t.stride()
+    if inner == 1 and t.data_ptr() % 16 == 0:
+        low = 0
+        for s in outer:
+            low |= s
+        if low % 8 == 0:
+            return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
 def strides_of(*tensors):
     """The strides of all but the last axis of the tensors, as the C-ABI's host array."""
-    values = [s for t in tensors for s in t.stride()[:-1]]
-    return (ctypes.c_int64 * len(values))(*values)
+    values = []
+    for t in tensors:
+        values += t.stride()[:-1]
+    return _long_array(len(values))(*values)
+
+
+@functools.lru_cache(maxsize=None)
+def _long_array(n):
+    return ctypes.c_int64 * n
+
+
+@functools.lru_cache(maxsize=1024)
+def workspace_floats(entry, device_index, *sizes):
+    """A workspace size query's answer; it depends on the sizes and on the device's compute units alone."""
+    return getattr(_native.library(), entry)(*sizes)
 
 
 def raise_error(error, what):
@@ -68,7 +86,8 @@ def _check(q, k, v, lengths):
             raise ValueError("lengths needs as many queries as keys")
         if lengths.dtype != torch.int32 or lengths.shape != (batch,):
             raise TypeError("lengths must be int32 [B]")
-    if not q.is_cuda or any(t.device != q.device for t in tensors):
+    device = q.device
+    if not q.is_cuda or k.device != device or v.device != device or (lengths is not None and lengths.device != device):
         raise ValueError("All window attention inputs must reside on the same GPU device")
     if not _native.plain_tensors(*tensors):
         raise RuntimeError("window_attention takes ordinary tensors (no tracing, transforms or tangents)")
@@ -77,67 +96,67 @@ def _check(q, k, v, lengths):
 
 
 def _forward(q, k, v, lengths, left, right, sinks, scale, stats):
-    """(output, row maxima, log2 of the row sums); the last two None without ``stats``."""
+    """(output, row maxima, log2 of the row sums, rest of the output); the last three None without ``stats``."""
     batch, heads, sq, dim = q.shape
+    kv_heads, sk = k.shape[1:3]
     out = torch.empty_like(q)
-    row_max = row_log = None
+    row_max = row_log = rest = workspace = None
     if q.numel() == 0:
-        return out, row_max, row_log
-    if k.shape[2] == 0:
-        return out.zero_(), row_max, row_log
-    with torch.cuda.device(q.device):
-        if not _device_is_gfx950(q.device):
-            raise RuntimeError("This HIP build requires an MI355X-class gfx950 GPU")
-        library = _native.library()
+        return out, row_max, row_log, rest
+    if sk == 0:
+        return out.zero_(), row_max, row_log, rest
+    device, address = q.device, _native.address
+    with _native.on_device(device):
+        _native.require_gfx950(device)
         q, k, v = rows16(q), rows16(k), rows16(v)
-        target = out if rows16(out) is out else torch.empty(out.shape, dtype=out.dtype, device=out.device)
+        target = out if rows16(out) is out else torch.empty(out.shape, dtype=out.dtype, device=device)
         if stats:
-            row_max, row_log = torch.empty((2, batch, heads, sq), dtype=torch.float32, device=q.device).unbind()
-        shape = (batch, heads, k.shape[1], sq, k.shape[2], left, right, sinks)
-        floats = library.peco_window_attention_workspace_size(*shape, dim)
-        workspace = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-        raise_error(library.peco_window_attention(
-            _native.ptr(q), _native.ptr(k), _native.ptr(v), _native.ptr(target), strides_of(q, k, v, target),
-            _native.ptr(lengths), _native.ptr(row_max), _native.ptr(row_log), _native.ptr(workspace), floats, *shape,
-            scale, dim, _native.dtype_code(q.dtype),
-            _native.current_stream(q.device, q, k, v, target, lengths, row_max, row_log, workspace)),
-            "window attention")
-        return (out if target is out else out.copy_(target)), row_max, row_log
+            row_max, row_log = torch.empty((2, batch, heads, sq), dtype=torch.float32, device=device).unbind()
+            rest = torch.empty((batch, heads, sq, dim), dtype=q.dtype, device=device)
+        shape = (batch, heads, kv_heads, sq, sk, left, right, sinks)
+        floats = workspace_floats("peco_window_attention_workspace_size", device.index, *shape, dim)
+        if floats:
+            workspace = torch.empty(floats, dtype=torch.float32, device=device)
+        raise_error(_native.library().peco_window_attention(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), target.data_ptr(), strides_of(q, k, v, target),
+            address(lengths), address(row_max), address(row_log), address(rest), address(workspace), floats, *shape, scale,
+            dim, _native.dtype_code(q.dtype), _native.retain(device, q, k, v, lengths)), "window attention")
+        return (out if target is out else out.copy_(target)), row_max, row_log, rest
 
 
-def _backward(q, k, v, out, row_max, row_log, lengths, grad, left, right, sinks, scale):
+def _backward(q, k, v, out, row_max, row_log, rest, lengths, grad, left, right, sinks, scale):
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
     if row_max is None:  # no query or no key: nothing is seen
         return dq.zero_(), dk.zero_(), dv.zero_()
     batch, heads, sq, dim = q.shape
-    with torch.cuda.device(q.device):
-        library = _native.library()
-        tensors = [rows16(t) for t in (q, k, v, out, grad)] + [dq, dk, dv]
+    device, address = q.device, _native.address
+    with _native.on_device(device):
+        given = [rows16(t) for t in (q, k, v, out, grad)]
         shape = (batch, heads, k.shape[1], sq, k.shape[2], left, right, sinks)
         code = _native.dtype_code(q.dtype)
-        floats = library.peco_window_attention_grad_workspace_size(*shape, dim, code)
-        workspace = torch.empty(floats, dtype=torch.float32, device=q.device)
-        raise_error(library.peco_window_attention_grad(
-            *[_native.ptr(t) for t in tensors], strides_of(*tensors), _native.ptr(lengths), _native.ptr(row_max),
-            _native.ptr(row_log), _native.ptr(workspace), floats, *shape, scale, dim, code,
-            _native.current_stream(q.device, *tensors, lengths, row_max, row_log, workspace)),
-            "window attention gradient")
+        floats = workspace_floats("peco_window_attention_grad_workspace_size", device.index, *shape, dim, code)
+        workspace = torch.empty(floats, dtype=torch.float32, device=device)
+        raise_error(_native.library().peco_window_attention_grad(
+            *[t.data_ptr() for t in given], dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+            strides_of(*given, dq, dk, dv), address(lengths), row_max.data_ptr(), row_log.data_ptr(), rest.data_ptr(),
+            workspace.data_ptr(), floats, *shape, scale, dim, code,
+            _native.retain(device, *given, lengths, row_max, row_log, rest)), "window attention gradient")
     return dq, dk, dv
 
 
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, mask):
-        out, row_max, row_log = _forward(q, k, v, lengths, *mask, True)
-        ctx.save_for_backward(q, k, v, lengths, out, row_max, row_log)
+        out, row_max, row_log, rest = _forward(q, k, v, lengths, *mask, True)
+        ctx.save_for_backward(q, k, v, lengths, out, row_max, row_log, rest)
         ctx.mask = mask
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        q, k, v, lengths, out, row_max, row_log = ctx.saved_tensors
-        return (*_backward(q, k, v, out, row_max, row_log, lengths, grad, *ctx.mask), None, None)
+        q, k, v, lengths, out, row_max, row_log, rest = ctx.saved_tensors
+        return (*_backward(q, k, v, out, row_max, row_log, rest, lengths, grad, *ctx.mask), None, None)
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window, sinks: int = 0, *,

@@ -251,7 +251,7 @@ def test_entry_refuses_bad_arguments():
 
     lib, null, some = _native.library(), ctypes.c_void_p(0), ctypes.c_void_p(4096)  # refused before it is read
     good = dict(q=some, k=some, v=some, out=some, strides=[1024, 512, 64] * 4, lengths=null, row_max=null, row_log=null,
-                work=null, floats=0, batch=1, q_heads=2, kv_heads=1, queries=5, keys=5, left=1, right=0, sinks=0,
+                rest=null, work=null, floats=0, batch=1, q_heads=2, kv_heads=1, queries=5, keys=5, left=1, right=0, sinks=0,
                 scale=0.125, d=64, dtype=1)
 
     def call(**changes):
@@ -261,7 +261,7 @@ def test_entry_refuses_bad_arguments():
 
     for change in (dict(q=null), dict(out=null), dict(batch=0), dict(kv_heads=0), dict(q_heads=3, kv_heads=2),
                    dict(queries=0), dict(keys=0), dict(left=-2), dict(right=-2), dict(sinks=-1), dict(scale=0.0),
-                   dict(scale=-1.0), dict(scale=float("nan")), dict(row_max=some), dict(lengths=some, queries=4),
+                   dict(scale=-1.0), dict(scale=float("nan")), dict(row_max=some), dict(row_max=some, row_log=some), dict(lengths=some, queries=4),
                    dict(strides=[1024, 512, 60] * 4), dict(k=ctypes.c_void_p(4104))):
         assert call(**change) == 1, change
     assert call(d=96) == 20002 and call(dtype=2) == 20003 and call(keys=1 << 30) == 20002

@@ -270,7 +270,7 @@ def test_entry_refuses_bad_arguments():
     floats = lib.peco_window_attention_grad_workspace_size(1, 2, 1, 5, 5, 1, 0, 0, 64, 1)
     assert floats >= 10
     good = dict(q=some, k=some, v=some, out=some, grad=some, dq=some, dk=some, dv=some, strides=[1024, 512, 64] * 8,
-                lengths=null, row_max=some, row_log=some, work=some, floats=floats, batch=1, q_heads=2, kv_heads=1,
+                lengths=null, row_max=some, row_log=some, rest=some, work=some, floats=floats, batch=1, q_heads=2, kv_heads=1,
                 queries=5, keys=5, left=1, right=0, sinks=0, scale=0.125, d=64, dtype=1)
 
     def call(**changes):
@@ -278,7 +278,7 @@ def test_entry_refuses_bad_arguments():
         a["strides"] = (ctypes.c_int64 * 24)(*a["strides"])
         return lib.peco_window_attention_grad(*a.values(), null)
 
-    for name in ("q", "k", "v", "out", "grad", "dq", "dk", "dv", "row_max", "row_log", "work"):
+    for name in ("q", "k", "v", "out", "grad", "dq", "dk", "dv", "row_max", "row_log", "rest", "work"):
         assert call(**{name: null}) == 1, name
     for change in (dict(batch=0), dict(q_heads=3, kv_heads=2), dict(queries=0), dict(keys=0), dict(left=-2), dict(sinks=-1),
                    dict(scale=0.0), dict(lengths=some, queries=4), dict(strides=[1024, 512, 60] * 8),
