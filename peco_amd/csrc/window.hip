@@ -15,8 +15,12 @@
 // out. Items of at most 64 rows pair the waves: two waves take the same 32 rows and one 32-key half of every
 // tile each, and join their states at the end.
 //
-// With few items the key stream is cut into `splits` parts, whose unnormalised fp32 outputs, maxima and sums
-// a second launch joins.
+// Where items leave workgroup slots empty, their key streams are cut into `splits` parts, whose unnormalised fp32
+// outputs, maxima and sums a second launch joins.
+//
+// A value that a query must not see has a weight of 0, but 0 times an infinity or NaN is NaN. A workgroup whose
+// sums come out other than finite takes its item again in a careful walk, which multiplies the rows of halves that are
+// seen in part and hold such values one by one.
 //
 // Roundings: scores, softmax statistics and O are fp32. P is rounded to the type for the second product (the
 // sum takes the rounded values, so that the weights still add up to 1), out once at the end. O is rescaled at
@@ -49,19 +53,19 @@ struct WindowArgs {
     int64_t table_stride;
     int table_width, page, pages;
     int tiles;               // row tiles per key head (paged: an upper bound)
-    int splits;
+    int splits;              // parts of every item's key stream
     int clear_tail;          // paged: rows outside every sequence are cleared
-    float* part_o;           // [splits, rows, D] with splits > 1
-    float2* part_ml;         // [splits, rows]
+    float* part_o;           // parts' results [splits, rows, D]
+    float2* part_ml;         // and [splits, rows]: largest score, sum
     // For the backward pass (all or none): raw maximum and log2 of the sum of every row, and what the rounding of
     // its output left (output rows one after another).
     float *row_max, *row_log;
     uint16_t* out_rest;
 };
 
-// Where a workgroup's rows are.
+// A tile of rows, and where they are.
 struct Item {
-    int b, kvh, split;
+    int b, kvh;
     int row0, rows;    // rows of the stream of (b, kvh)
     int first_token;   // of the sequence within q/out
     int position0;     // position of the sequence's first query
@@ -75,16 +79,14 @@ enum WindowMode : int {
     kPaged = 2,  // pages of a cache
 };
 
-// Item of workgroup g. Contiguous: heads fastest (with a multiple of 8 of them every head stays on one XCD),
-// the last row tiles, which see most under a causal mask, first. Paged: heads fastest, then splits, then
-// the row tiles of the sequences in order; false past the last of them.
-template <int kMode> __device__ __forceinline__ bool find_item(const WindowArgs& A, int64_t g, Item& it) {
+// Item i. Contiguous: heads fastest (with a multiple of 8 of them every head stays on one XCD), the last row tiles,
+// which see most under a causal mask, first. Paged: heads fastest, then the row tiles of the sequences in order; false
+// past the last of them.
+template <int kMode> __device__ __forceinline__ bool find_rows(const WindowArgs& A, int64_t i, Item& it) {
     if constexpr (kMode != kPaged) {
         const int heads = A.batch * A.heads;
-        const int bh = static_cast<int>(g % heads);
-        const int64_t rest = g / heads;
-        it.split = static_cast<int>(rest % A.splits);
-        const int tile = A.tiles - 1 - static_cast<int>(rest / A.splits);
+        const int bh = static_cast<int>(i % heads);
+        const int tile = A.tiles - 1 - static_cast<int>(i / heads);
         it.b = bh / A.heads;
         it.kvh = bh % A.heads;
         it.first_token = 0;
@@ -96,10 +98,8 @@ template <int kMode> __device__ __forceinline__ bool find_item(const WindowArgs&
         if (A.lengths) it.keys = it.queries = max(0, min(A.lengths[it.b], A.keys));  // (queries == keys)
         return true;
     } else {
-        it.kvh = static_cast<int>(g % A.heads);
-        const int64_t rest = g / A.heads;
-        it.split = static_cast<int>(rest % A.splits);
-        int tile = static_cast<int>(rest / A.splits);
+        it.kvh = static_cast<int>(i % A.heads);
+        int tile = static_cast<int>(i / A.heads);
         const int lane = threadIdx.x % kWave;
         for (int b0 = 0; b0 < A.batch; b0 += kWave) {
             const int b = min(b0 + lane, A.batch - 1);
@@ -129,6 +129,17 @@ template <int kMode> __device__ __forceinline__ bool find_item(const WindowArgs&
         it.row0 = tile;  // number among the workgroups without rows
         return false;
     }
+}
+
+// Number of a query row: query head major (paged: token major).
+template <int kMode>
+__device__ __forceinline__ int64_t row_number(const WindowArgs& A, const Item& it, int token, int head) {
+    if constexpr (kMode == kPaged) return static_cast<int64_t>(it.first_token + token) * (A.heads * A.group) + head;
+    else return (static_cast<int64_t>(it.b) * (A.heads * A.group) + head) * A.queries + token;
+}
+
+template <int kMode> __device__ __forceinline__ int64_t all_rows(const WindowArgs& A) {
+    return static_cast<int64_t>(kMode == kPaged ? 1 : A.batch) * A.heads * A.group * A.queries;
 }
 
 // Clears the output rows that belong to no sequence (those before the first offset and behind the last). There
@@ -169,10 +180,13 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
     __shared__ uint16_t counts[4][4];  // (read during a tile, when those two tiles on are written)
     __shared__ int page_of[2][kRowLds];
 
+    // Parts of one item are as many workgroups apart as there are items.
+    const int64_t items = static_cast<int64_t>(kMode == kPaged ? 1 : A.batch) * A.heads * A.tiles;
+    const int part = static_cast<int>(blockIdx.x / items);
     Item it;
-    const bool found = find_item<kMode>(A, blockIdx.x, it);
+    const bool found = find_rows<kMode>(A, blockIdx.x % items, it);
     if (kMode == kPaged && !found) {
-        if (A.clear_tail && it.split == 0 && it.row0 == 0) clear_tail<D>(A, it.kvh);
+        if (A.clear_tail && part == 0 && it.row0 == 0) clear_tail<D>(A, it.kvh);
         return;
     }
     const int tid = threadIdx.x, lane = tid % kWave, h = lane / 32;
@@ -209,7 +223,7 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
     const int L = stream.length;
     const int all_tiles = static_cast<int>(ceil_div(L, kWinTile));
     const int per = static_cast<int>(ceil_div(all_tiles, A.splits));
-    const int tile0 = min(it.split * per, all_tiles), tile1 = min(tile0 + per, all_tiles);
+    const int tile0 = min(part * per, all_tiles), tile1 = min(tile0 + per, all_tiles);
     const int pos = it.position0 + token;
     const bool sees = qvalid && token < it.queries;
     const int last_r = sees ? min(min(pos + A.right, it.keys - 1) - stream.delta, L - 1) : -1;
@@ -271,14 +285,15 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
 
     f32x16 oacc[NB];
     float m_run, l_run, neg_m;
-    bool wide, dirty = false;
-    const WinLane<D> at(lane, kvs[0]);
+    bool wide;
+    // (From the half that the wave begins with: the second half of a tile is taken by unpaired waves, whose hb is 0.)
+    const WinLane<D> at = WinLane<D>(lane, kvs[0]).moved(hb * 64 * D);
 
     // One 32-key half (cb) of tile t in buffer buf;
-    auto compute = [&](auto careful, int t, int buf, int cb) __attribute__((always_inline)) {
+    auto compute = [&](auto careful, int t, int buf, int second) __attribute__((always_inline)) {
         constexpr bool kCareful = decltype(careful)::value;
-        const int kt = 2 * (buf * T::kElems + 32 * cb * D), vt = kt + 4 * T::kElems;  // bytes from the first tile
-        const int r0 = t * kWinTile + 32 * cb;
+        const int kt = 2 * (buf * T::kElems + 32 * second * D), vt = kt + 4 * T::kElems;  // bytes from `at`'s tile
+        const int cb = hb + second, r0 = t * kWinTile + 32 * cb;
         if (r0 > w_any || (r0 + 31 < w_from && r0 >= A.sinks)) {  // no row of the wave sees any of it
             return;
         }
@@ -297,9 +312,14 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
             return r <= last_r && (r >= first_r || r < A.sinks) && (held >> row & 1);
         };
         if (!whole) {
+            // (Element i is row 8 (i / 4) + 4 h + i % 4: the lane's 4 h is taken off the limits, the rest is uniform.)
+            const int last = last_r - 4 * h, from = first_r - 4 * h, sinks = A.sinks - 4 * h;
+            const uint32_t mine = held >> (4 * h);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (!seen_at(8 * (i / 4) + 4 * h + i % 4)) sacc[i] = -INFINITY;
+            for (int i = 0; i < 16; ++i) {
+                const int c = 8 * (i / 4) + i % 4, r = r0 + c;
+                if (!(r <= last && (r >= from || r < sinks) && (mine >> c & 1))) sacc[i] = -INFINITY;
+            }
         }
         float tmax = sacc[0];
 #pragma unroll
@@ -335,19 +355,16 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
             l_run = Mfma<DT>::sum2(pp[i / 2], l_run);
         }
         if constexpr (kCareful) {
-            if (!whole && rows_not_finite<DT, D>(kvs[0], vt, lane)) {
+            if (!whole && rows_not_finite<DT, D>(kvs[0], vt + hb * 64 * D, lane)) {
                 add_rows_seen<DT, D>(oacc, vt, pp, at, h, seen_at);
                 return;
             }
-        } else if (!whole) {
-            dirty |= rows_not_finite<DT, D>(kvs[0], vt, lane);
         }
         __builtin_amdgcn_sched_barrier(0);
         add_rows<DT, D>(oacc, vt, pp, at);
     };
 
-    // One walk over the tiles. The careful one is taken again from the start when the first met an infinity or NaN
-    // in a value that some query must not see.
+    // One walk over the tiles.
     auto walk = [&](auto careful) __attribute__((always_inline)) {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) oacc[nb] = f32x16{};
@@ -377,9 +394,9 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
             if (wave_active) {
                 if constexpr (decltype(careful)::value) {
 #pragma unroll 1
-                    for (int cb = hb; cb < (split ? hb + 1 : 2); ++cb) compute(careful, t, buf, cb);
+                    for (int second = 0; second < (split ? 1 : 2); ++second) compute(careful, t, buf, second);
                 } else {
-                    compute(careful, t, buf, hb);
+                    compute(careful, t, buf, 0);
                     if (!split) compute(careful, t, buf, 1);
                 }
             }
@@ -410,7 +427,7 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last page numbers
     };
     walk(std::false_type{});
-    if (__syncthreads_or(dirty)) walk(std::true_type{});
+    if (__syncthreads_or(wave_active && !all_finite(oacc))) walk(std::true_type{});
     if (split) {
         // The wave of the second halves leaves its state in the tile LDS (free after the last barrier), the wave of
         // the first halves joins both at the larger maximum.
@@ -440,15 +457,12 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
     }
     if (!qvalid) return;
     const float l_tot = l_run + __shfl_xor(l_run, 32, kWave);
-    // Row number among the partial results and statistics: query head major (paged: token major).
-    const int64_t rows_all = static_cast<int64_t>(kMode == kPaged ? 1 : A.batch) * A.queries * A.heads * A.group;
-    const int64_t row_id = kMode == kPaged
-                               ? static_cast<int64_t>(it.first_token + token) * (A.heads * A.group) + head
-                               : (static_cast<int64_t>(it.b) * (A.heads * A.group) + head) * A.queries + token;
+    const int64_t row_id = row_number<kMode>(A, it, token, head);
     if (A.splits > 1) {
-        if (h == 0) A.part_ml[it.split * rows_all + row_id] = float2{m_run, l_tot};
+        const int64_t at = part * all_rows<kMode>(A) + row_id;
+        if (h == 0) A.part_ml[at] = float2{m_run, l_tot};
         if (l_tot == 0.0f) return;  // (the join does not read it)
-        float* o = A.part_o + (it.split * rows_all + row_id) * D;
+        float* o = A.part_o + at * D;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -474,17 +488,20 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
         }
 }
 
-// Joins the parts of every row: out = sum_s 2^((m_s - M) scale) O_s / sum_s 2^((m_s - M) scale) l_s, parts in
-// order. D / 4 lanes a row.
-template <int DT, int D, bool kPagedRows>
+// Joins the parts of every row: out = sum_s 2^((m_s - M) scale) O_s / sum_s 2^((m_s - M) scale) l_s, in a fixed
+// order. D / 4 lanes a row; kWide: one row a workgroup, whose lane groups take the parts in turn and are joined in LDS
+// (a call with many parts has few rows, and one lane group would wait for one part after another).
+template <int DT, int D, int kMode, bool kWide>
 __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs A) {
-    constexpr int kLanes = D / 4;
-    const int64_t rows_all = static_cast<int64_t>(kPagedRows ? 1 : A.batch) * A.queries * A.heads * A.group;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
+    constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
+    __shared__ f32x4 group_o[kWide ? kGroups : 1][kLanes];
+    __shared__ float2 group_ml[kWide ? kGroups : 1];
+    const int group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes, c = 4 * lane, hq = A.heads * A.group;
+    const int64_t rows_all = all_rows<kMode>(A);
+    const int64_t row = kWide ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * kGroups + group;
     if (row >= rows_all) return;
-    const int c = threadIdx.x % kLanes * 4, hq = A.heads * A.group;
     int64_t b = 0, head, token;
-    if constexpr (kPagedRows) {
+    if constexpr (kMode == kPaged) {
         token = row / hq;
         head = row % hq;
         const int o0 = max(0, min(A.offsets[0], A.queries)), o1 = min(A.offsets[A.batch], A.queries);
@@ -494,11 +511,11 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs A) {
         head = row / A.queries % hq;
         b = row / A.queries / hq;
     }
-    float m = -FLT_MAX;
-    for (int s = 0; s < A.splits; ++s) m = fmaxf(m, A.part_ml[s * rows_all + row].x);
-    float l = 0.0f;
+    float m = -FLT_MAX, l = 0.0f;
     f32x4 o{};
-    for (int s = 0; s < A.splits; ++s) {
+    const int first = kWide ? group : 0, step = kWide ? kGroups : 1;
+    for (int s = first; s < A.splits; s += step) m = fmaxf(m, A.part_ml[s * rows_all + row].x);
+    for (int s = first; s < A.splits; s += step) {
         const float2 ml = A.part_ml[s * rows_all + row];
         if (ml.y == 0.0f) continue;
         const float w = __builtin_amdgcn_exp2f((ml.x - m) * A.scale_log2);
@@ -506,6 +523,28 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs A) {
         l += w * ml.y;
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[k] += w * part[k];
+    }
+    if constexpr (kWide) {
+        group_o[group][lane] = o;
+        if (lane == 0) group_ml[group] = float2{m, l};
+        __syncthreads();
+        if (group) return;
+        const float own = m;
+#pragma unroll
+        for (int i = 1; i < kGroups; ++i) m = fmaxf(m, group_ml[i].x);
+        const float w0 = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f((own - m) * A.scale_log2);
+        l *= w0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = l == 0.0f ? 0.0f : o[k] * w0;
+        for (int i = 1; i < kGroups; ++i) {
+            const float2 ml = group_ml[i];
+            if (ml.y == 0.0f) continue;
+            const float w = __builtin_amdgcn_exp2f((ml.x - m) * A.scale_log2);
+            l += w * ml.y;
+            const f32x4 x = group_o[i][lane];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] += w * x[k];
+        }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (A.row_max && c == 0) {
@@ -516,23 +555,35 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs A) {
     store_output<DT>(o * inv, dst, A.row_max ? A.out_rest + row * D + c : nullptr);
 }
 
-template <int DT, int D> int launch_window(const WindowArgs& A, WindowMode mode, hipStream_t s) {
-    const int64_t heads = mode == kPaged ? A.heads : static_cast<int64_t>(A.heads) * A.batch;
-    const int64_t blocks = heads * A.tiles * A.splits;
-    if (blocks > 0x7fffffff) return kUnsupportedShape;
-    const dim3 grid(static_cast<unsigned>(blocks));
-    switch (mode) {
-        case kNear: hipLaunchKernelGGL((window_forward_kernel<DT, D, kNear>), grid, dim3(256), 0, s, A); break;
-        case kFar: hipLaunchKernelGGL((window_forward_kernel<DT, D, kFar>), grid, dim3(256), 0, s, A); break;
-        default: hipLaunchKernelGGL((window_forward_kernel<DT, D, kPaged>), grid, dim3(256), 0, s, A); break;
-    }
-    int status = hipGetLastError();
-    if (status || A.splits == 1) return status;
-    const int64_t rows = static_cast<int64_t>(mode == kPaged ? 1 : A.batch) * A.queries * A.heads * A.group;
-    const dim3 join(static_cast<unsigned>(ceil_div(rows, 256 / (D / 4))));
-    if (mode == kPaged) hipLaunchKernelGGL((window_join_kernel<DT, D, true>), join, dim3(256), 0, s, A);
-    else hipLaunchKernelGGL((window_join_kernel<DT, D, false>), join, dim3(256), 0, s, A);
+constexpr int kWideParts = 8;  // parts from which the join takes a workgroup a row
+
+template <int DT, int D, int kMode> int launch_join(const WindowArgs& A, int64_t rows, hipStream_t s) {
+    constexpr int kGroups = 256 / (D / 4);
+    if (A.splits >= kWideParts)
+        hipLaunchKernelGGL((window_join_kernel<DT, D, kMode, true>), dim3(static_cast<unsigned>(rows)), dim3(256), 0, s, A);
+    else
+        hipLaunchKernelGGL((window_join_kernel<DT, D, kMode, false>), dim3(static_cast<unsigned>(ceil_div(rows, kGroups))),
+                           dim3(256), 0, s, A);
     return hipGetLastError();
+}
+
+template <int DT, int D, int kMode> int launch_mode(const WindowArgs& A, hipStream_t s) {
+    const int64_t rows = (kMode == kPaged ? int64_t{1} : int64_t{A.batch}) * A.heads * A.group * A.queries;
+    const int64_t blocks = (kMode == kPaged ? int64_t{1} : int64_t{A.batch}) * A.heads * A.tiles * A.splits;
+    if (blocks > 0x7fffffff || rows > 0x7fffffff) return kUnsupportedShape;
+    const dim3 grid(static_cast<unsigned>(blocks));
+    hipLaunchKernelGGL((window_forward_kernel<DT, D, kMode>), grid, dim3(256), 0, s, A);
+    const int status = hipGetLastError();
+    if (status || A.splits == 1) return status;
+    return launch_join<DT, D, kMode == kFar ? kNear : kMode>(A, rows, s);
+}
+
+template <int DT, int D> int launch_window(const WindowArgs& A, WindowMode mode, hipStream_t s) {
+    switch (mode) {
+        case kNear: return launch_mode<DT, D, kNear>(A, s);
+        case kFar: return launch_mode<DT, D, kFar>(A, s);
+        default: return launch_mode<DT, D, kPaged>(A, s);
+    }
 }
 
 int launch(const WindowArgs& A, WindowMode mode, int d, int dtype, hipStream_t s) {
@@ -540,23 +591,46 @@ int launch(const WindowArgs& A, WindowMode mode, int d, int dtype, hipStream_t s
     return d == 128 ? launch_window<kF16, 128>(A, mode, s) : launch_window<kF16, 64>(A, mode, s);
 }
 
-// Parts of the key stream. A workgroup's walk over its tiles is a chain of latencies, so calls whose items
-// leave compute units idle cut the stream, into parts of at least kPartTiles tiles (below that a part costs
-// more in its start, its 64 KB of fp32 output and the join than its tiles do).
+// Into how many parts (of at least kPartTiles tiles) the key streams are cut.
+// Items of a few rows (single tokens) are bound by what they read: about four workgroups a slot (two slots a CU) keep
+// the reads even where sequences differ in length. Measured, 128 channels: 32 x 8 heads of one token over up to 7006
+// keys 176 us uncut, 106 in 8 parts and 5 for the join; one token over 119056 keys, 24 heads, 298 us in 12 parts, 359
+// in 21 (one even round, whose last workgroups read alone), 271 in 64 and 13 for the join.
+// Other items are bound by their products. A call takes as long as its busiest CU: the count of workgroups there times
+// a workgroup's tiles (and kStartTiles for its start and end), in units of what a CU takes for a tile with two
+// workgroups sharing it (1.4 us with 128 channels, half with 64; one alone is a third faster than that, not twice),
+// plus the join, which writes and reads the parts' fp32 rows.
+constexpr int kFewRows = 32;
 constexpr int kPartTiles = 4;
+constexpr int kStartTiles = 4;
 constexpr int kMaxSplits = 64;
-int split_count(int64_t items, int64_t seen_keys) {
-    const int64_t slots = 2 * static_cast<int64_t>(device_compute_units());
-    const int64_t most = std::min<int64_t>(kMaxSplits, ceil_div(seen_keys, kWinTile) / kPartTiles);
-    if (items >= slots / 2 || most < 2) return 1;
-    return static_cast<int>(std::min(most, ceil_div(2 * slots, items)));
-}
-
 struct Shape {
+    int64_t tiles, rows, blocks;  // row tiles of a key head, query rows, workgroups
     int splits;
-    int64_t rows;  // all query rows
-    int64_t tiles;
 };
+// `heads` key heads of `tiles` row tiles, `items` of them with rows, which hold `rows` in all.
+Shape shape_of(int64_t heads, int64_t tiles, int64_t items, int64_t seen_keys, int64_t rows, int d) {
+    const int64_t cus = device_compute_units(), n = ceil_div(seen_keys, kWinTile);
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, n / kPartTiles));
+    Shape best{tiles, rows, 0, 1};
+    if (rows <= items * kFewRows) {
+        best.splits = static_cast<int>(std::min(most, ceil_div(8 * cus, items)));
+    } else {
+        const double tile_us = d == 128 ? 1.4 : 0.7;
+        double least = 1e30;
+        for (int s = 1; s <= most; ++s) {
+            const int64_t k = ceil_div(items * s, cus);
+            double cost = (k == 1 ? 4.0 / 3.0 : static_cast<double>(k)) * static_cast<double>(ceil_div(n, s) + kStartTiles);
+            if (s > 1) cost += (4.0 + static_cast<double>(rows) * s * (d + 2) * 8.0 / 5.0e6) / tile_us;  // 4 us and 5 TB/s
+            else cost *= 0.93;  // (less than that a cut is not worth: the busiest CU's last workgroup runs the faster)
+            if (cost >= least) continue;
+            least = cost;
+            best.splits = s;
+        }
+    }
+    best.blocks = heads * tiles * best.splits;
+    return best;
+}
 
 // Most keys that a tile of rows may see.
 int64_t seen_keys(int64_t keys, int64_t tokens, int left, int right, int sinks) {
@@ -564,22 +638,21 @@ int64_t seen_keys(int64_t keys, int64_t tokens, int left, int right, int sinks) 
     return std::max<int64_t>(window, 0);
 }
 
-Shape window_shape(int batch, int q_heads, int kv_heads, int queries, int keys, int left, int right, int sinks) {
+Shape window_shape(int batch, int q_heads, int kv_heads, int queries, int keys, int left, int right, int sinks, int d) {
     const int group = q_heads / kv_heads;
-    const int64_t tiles = ceil_div(static_cast<int64_t>(queries) * group, kWinRows);
+    const int64_t tiles = ceil_div(static_cast<int64_t>(queries) * group, kWinRows), heads = int64_t{batch} * kv_heads;
     const int64_t tokens = std::min<int64_t>(queries, kWinRows / group + 1);
-    const int splits = split_count(tiles * batch * kv_heads, seen_keys(keys, tokens, left, right, sinks));
-    return Shape{splits, static_cast<int64_t>(batch) * q_heads * queries, tiles};
+    return shape_of(heads, tiles, heads * tiles, seen_keys(keys, tokens, left, right, sinks), heads * group * queries, d);
 }
 
 // Row tiles of a ragged batch: each sequence has at most one that is not full; one more, so that some
 // workgroup always finds no rows and clears those outside every sequence.
-Shape paged_shape(int batch, int q_heads, int kv_heads, int tokens, int64_t capacity, int left, int sinks) {
+Shape paged_shape(int batch, int q_heads, int kv_heads, int tokens, int64_t capacity, int left, int sinks, int d) {
     const int group = q_heads / kv_heads;
-    const int64_t tiles = static_cast<int64_t>(tokens) * group / kWinRows + batch + 1;
+    const int64_t full = static_cast<int64_t>(tokens) * group / kWinRows, tiles = full + batch + 1;
     const int64_t some = std::min<int64_t>(tokens, kWinRows / group + 1);
-    const int splits = split_count((tiles - 1) * kv_heads, seen_keys(capacity, some, left, 0, sinks));
-    return Shape{splits, static_cast<int64_t>(tokens) * q_heads, tiles};
+    return shape_of(kv_heads, tiles, (tiles - 1) * kv_heads, seen_keys(capacity, some, left, 0, sinks),
+                 static_cast<int64_t>(tokens) * q_heads, d);
 }
 
 size_t workspace_floats(const Shape& s, int d) {
@@ -613,7 +686,7 @@ using namespace peco;
 PECO_API size_t peco_window_attention_workspace_size(int batch, int q_heads, int kv_heads, int queries, int keys,
                                                      int left, int right, int sinks, int d) {
     if (batch < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || queries < 1 || keys < 0) return 0;
-    return workspace_floats(window_shape(batch, q_heads, kv_heads, queries, keys, left, right, sinks), d);
+    return workspace_floats(window_shape(batch, q_heads, kv_heads, queries, keys, left, right, sinks, d), d);
 }
 
 PECO_API int peco_window_attention(const void* q, const void* k, const void* v, void* output, const int64_t* strides,
@@ -656,9 +729,10 @@ PECO_API int peco_window_attention(const void* q, const void* k, const void* v, 
     A.row_log = row_log;
     A.out_rest = static_cast<uint16_t*>(output_rest);
     if (!aligned(output_rest)) return kInvalidValue;
-    const Shape shape = window_shape(batch, q_heads, kv_heads, queries, keys, left, right, sinks);
+    const Shape shape = window_shape(batch, q_heads, kv_heads, queries, keys, left, right, sinks, d);
+    if (shape.blocks > 0x7fffffff) return kUnsupportedShape;
     if (workspace_floats(shape, d) > workspace_floats_given) return kWorkspaceTooSmall;
-    if (shape.splits > 1 && !aligned(workspace)) return kInvalidValue;
+    if (workspace_floats(shape, d) && (!workspace || !aligned(workspace))) return kInvalidValue;
     set_parts(A, shape, workspace, d);
     const int64_t reach = std::max(A.ks.s, A.vs.s) * 2 * keys + 2 * d;
     return launch(A, reach < (int64_t{1} << 32) ? kNear : kFar, d, dtype, static_cast<hipStream_t>(stream));
@@ -669,7 +743,7 @@ PECO_API size_t peco_paged_attention_workspace_size(int batch, int q_heads, int 
     if (batch < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || tokens < 1 || table_width < 1 || page < 1)
         return 0;
     const int64_t capacity = static_cast<int64_t>(table_width) * page;
-    return workspace_floats(paged_shape(batch, q_heads, kv_heads, tokens, capacity, left, sinks), d);
+    return workspace_floats(paged_shape(batch, q_heads, kv_heads, tokens, capacity, left, sinks, d), d);
 }
 
 PECO_API int peco_paged_attention(const void* q, const void* k_pages, const void* v_pages, void* output,
@@ -717,9 +791,10 @@ PECO_API int peco_paged_attention(const void* q, const void* k_pages, const void
     A.page = page;
     A.pages = pages;
     A.clear_tail = clear_tail;
-    const Shape shape = paged_shape(batch, q_heads, kv_heads, tokens, capacity, left, sinks);
+    const Shape shape = paged_shape(batch, q_heads, kv_heads, tokens, capacity, left, sinks, d);
+    if (shape.blocks > 0x7fffffff) return kUnsupportedShape;
     if (workspace_floats(shape, d) > workspace_floats_given) return kWorkspaceTooSmall;
-    if (shape.splits > 1 && !aligned(workspace)) return kInvalidValue;
+    if (workspace_floats(shape, d) && (!workspace || !aligned(workspace))) return kInvalidValue;
     set_parts(A, shape, workspace, d);
     return launch(A, kPaged, d, dtype, static_cast<hipStream_t>(stream));
 }

@@ -80,6 +80,15 @@ template <int DT> __device__ __forceinline__ bool not_finite(uint16_t b) {
     return (b & kExp) == kExp;
 }
 
+template <int N> __device__ __forceinline__ bool all_finite(const f32x16 (&acc)[N]) {
+    float zero = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) zero = __builtin_fmaf(acc[n][i], 0.0f, zero);
+    return zero == 0.0f;
+}
+
 // Whether any of the 32 rows at byte `off` of the tiles holds an infinity or NaN.
 template <int DT, int D>
 __device__ __forceinline__ bool rows_not_finite(const uint16_t* tiles, int off, int lane) {
@@ -123,7 +132,7 @@ __device__ __forceinline__ void add_rows(f32x16 (&acc)[D / 32], int off, const u
 
 // The same for rows with infinities or NaN that some column hides: a hidden row's weight is 0, but 0 times them is
 // NaN. Each row is multiplied by itself and added where seen(row) holds. The kernels come here only in a second walk
-// over their tiles, after a first one met such a row.
+// over their tiles, after the sums of a first one came out other than finite.
 template <int DT, int D, typename Seen>
 __device__ __forceinline__ void add_rows_seen(f32x16 (&acc)[D / 32], int off, const uint32_t (&w)[8],
                                               const WinLane<D>& at, int h, const Seen& seen) {

@@ -200,7 +200,6 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
 #endif
     };
     f32x16 acc[NB];
-    bool dirty = false;
     const WinLane<D> at(lane, kvs[0]);
     auto compute = [&](auto careful, int t, int buf, int cb) __attribute__((always_inline)) {
         const int kt = 2 * (buf * T::kElems + 32 * cb * D), vt = kt + 4 * T::kElems;  // bytes from the first tile
@@ -228,9 +227,13 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
             if constexpr (DT == kF16) ds[i] *= dmul;
         }
         if (!whole) {
+            // (Element i is row 8 (i / 4) + 4 h + i % 4: the lane's 4 h is taken off the limits, the rest is uniform.)
+            const int last = last_r - 4 * h, from = first_r - 4 * h, sinks = A.sinks - 4 * h;
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (!seen_at(8 * (i / 4) + 4 * h + i % 4)) ds[i] = 0.0f;
+            for (int i = 0; i < 16; ++i) {
+                const int r = r0 + 8 * (i / 4) + i % 4;
+                if (!(r <= last && (r >= from || r < sinks))) ds[i] = 0.0f;
+            }
         }
         uint32_t w[8];
 #pragma unroll
@@ -240,8 +243,6 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
                 add_rows_seen<DT, D>(acc, kt, w, at, h, seen_at);
                 return;
             }
-        } else if (!whole) {
-            dirty |= rows_not_finite<DT, D>(kvs[0], kt, lane);
         }
         __builtin_amdgcn_sched_barrier(0);
         add_rows<DT, D>(acc, kt, w, at);
@@ -286,7 +287,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
         }
     };
     walk(std::false_type{});
-    if (__syncthreads_or(dirty)) walk(std::true_type{});
+    if (__syncthreads_or(wave_active && !all_finite(acc))) walk(std::true_type{});
     if (!qvalid) return;
     const float mul = A.scale / dmul;
     uint16_t* o = A.dq + b * A.dqs.b + head * A.dqs.h + token * A.dqs.s;
@@ -419,7 +420,6 @@ __global__ __launch_bounds__(kGradWaves * kWave, 2) void window_dkv_kernel(GradA
     };
 
     f32x16 dk[NB], dv[NB];
-    bool dirty = false;
     const WinLane<D> at0(lane, tiles_lds[0]);
     // One 32-row half of a tile: S and P, then dV, then dP and dS, then dK, which keeps one 32 x 32 result and its packed form alive
     // at a time beside the sums.
@@ -429,8 +429,9 @@ __global__ __launch_bounds__(kGradWaves * kWave, 2) void window_dkv_kernel(GradA
         const int r0 = r_begin + t * kTile + 32 * cb;
         if (r0 + 31 < w_first || r0 >= w_last) return;
         const bool whole = r0 >= w_from && r0 + 31 < w_to;
-        constexpr bool kCareful = decltype(careful)::value;
-        if (!kCareful && !whole) dirty |= rows_not_finite<DT, D>(tiles_lds[0], qoff, lane) || rows_not_finite<DT, D>(tiles_lds[0], goff, lane);
+        [[maybe_unused]] const bool one_by_one =
+            decltype(careful)::value && !whole &&
+            (rows_not_finite<DT, D>(tiles_lds[0], qoff, lane) || rows_not_finite<DT, D>(tiles_lds[0], goff, lane));
         auto seen_at = [&](int row) { return r0 + row >= from && r0 + row < to; };
         f32x16 p{}, ds{};
         WinLane<D> at = at0.moved(qoff);
@@ -454,14 +455,16 @@ __global__ __launch_bounds__(kGradWaves * kWave, 2) void window_dkv_kernel(GradA
         }
         if (!whole) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (!seen_at(8 * (i / 4) + 4 * h + i % 4)) p[i] = 0.0f;
+            for (int i = 0; i < 16; ++i) {
+                const int r = r0 + 8 * (i / 4) + i % 4;
+                if (!(r >= from - 4 * h && r < to - 4 * h)) p[i] = 0.0f;
+            }
         }
         uint32_t w[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = Mfma<DT>::pack2(p[2 * i], p[2 * i + 1]);
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (kCareful) add_rows_seen<DT, D>(dv, gt, w, at, h, seen_at);
+        if (one_by_one) add_rows_seen<DT, D>(dv, gt, w, at, h, seen_at);
         else add_rows<DT, D>(dv, gt, w, at);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -479,13 +482,15 @@ __global__ __launch_bounds__(kGradWaves * kWave, 2) void window_dkv_kernel(GradA
         }
         if (!whole) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (!seen_at(8 * (i / 4) + 4 * h + i % 4)) ds[i] = 0.0f;
+            for (int i = 0; i < 16; ++i) {
+                const int r = r0 + 8 * (i / 4) + i % 4;
+                if (!(r >= from - 4 * h && r < to - 4 * h)) ds[i] = 0.0f;
+            }
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = Mfma<DT>::pack2(ds[2 * i], ds[2 * i + 1]);
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (kCareful) add_rows_seen<DT, D>(dk, qt, w, at, h, seen_at);
+        if (one_by_one) add_rows_seen<DT, D>(dk, qt, w, at, h, seen_at);
         else add_rows<DT, D>(dk, qt, w, at);
     };
     auto walk = [&](auto careful) __attribute__((always_inline)) {
@@ -514,7 +519,7 @@ __global__ __launch_bounds__(kGradWaves * kWave, 2) void window_dkv_kernel(GradA
         for (int t = tile0; t < tile1; ++t) step((t - tile0) & 1, t);
     };
     walk(std::false_type{});
-    if (__syncthreads_or(dirty)) walk(std::true_type{});
+    if (__syncthreads_or(wave_active && !(all_finite(dk) && all_finite(dv)))) walk(std::true_type{});
     const float kmul = A.scale / dmul, vmul = DT == kF16 ? 0x1p-14f : 1.0f;
     if (parts > 1) {
         // [head, item, key, dK | dV, D]; every key of the tile, so that the join reads nothing unwritten.
@@ -617,8 +622,7 @@ template <int DT, int D> int launch_grad(const GradArgs& A, bool far, hipStream_
         hipLaunchKernelGGL((value_lengths_kernel<D>), dim3(static_cast<unsigned>(heads * A.v_blocks)), dim3(256), 0, s, A);
     if (far) hipLaunchKernelGGL((window_dq_kernel<DT, D, true>), dim3(static_cast<unsigned>(dq)), dim3(256), 0, s, A);
     else hipLaunchKernelGGL((window_dq_kernel<DT, D, false>), dim3(static_cast<unsigned>(dq)), dim3(256), 0, s, A);
-    hipLaunchKernelGGL((window_dkv_kernel<DT, D>), dim3(static_cast<unsigned>(dkv)),
-                       dim3(kGradWaves * kWave), 0, s, A);
+    hipLaunchKernelGGL((window_dkv_kernel<DT, D>), dim3(static_cast<unsigned>(dkv)), dim3(kGradWaves * kWave), 0, s, A);
     if (partial_items(A)) {
         const int64_t rows = heads * (A.parts > 1 ? A.key_tiles : A.sink_tiles) * kGradKeys;
         hipLaunchKernelGGL((window_dkv_join_kernel<DT, D>), dim3(static_cast<unsigned>(ceil_div(rows, 256 / (D / 2)))),

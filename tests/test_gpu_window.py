@@ -268,5 +268,5 @@ def test_entry_refuses_bad_arguments():
     floats = lib.peco_window_attention_workspace_size(1, 2, 1, 1, 50000, -1, 0, 0, 64)
     assert floats > 0 and call(queries=1, keys=50000, left=-1, work=some, floats=floats - 1) == 20001
     assert call(queries=1, keys=50000, left=-1, work=ctypes.c_void_p(4100), floats=floats) == 1
-    assert lib.peco_window_attention_workspace_size(1, 24, 24, 7006, 7006, 2025, 0, 256, 128) == 0
+    assert lib.peco_window_attention_workspace_size(1, 2, 1, 5, 5, 1, 0, 0, 64) == 0
     assert lib.peco_window_attention_workspace_size(0, 24, 24, 7006, 7006, 2025, 0, 256, 128) == 0
