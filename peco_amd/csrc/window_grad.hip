@@ -210,9 +210,10 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
         const bool whole = r0 + 31 <= w_last && (r0 >= w_first || r0 + 31 < A.sinks);
         f32x16 sacc{}, pacc{};
 #pragma unroll
-        for (int s = 0; s < S; ++s) sacc = Mfma<DT>::run(at.rows(kt, s), qf[s], sacc);
-#pragma unroll
-        for (int s = 0; s < S; ++s) pacc = Mfma<DT>::run(at.rows(vt, s), gf[s], pacc);
+        for (int s = 0; s < S; ++s) {  // in turn: two chains, each product behind the other chain's
+            sacc = Mfma<DT>::run(at.rows(kt, s), qf[s], sacc);
+            pacc = Mfma<DT>::run(at.rows(vt, s), gf[s], pacc);
+        }
         read_ahead<2 * S, 2 * S, 4>();
         __builtin_amdgcn_sched_barrier(0);
         auto seen_at = [&](int row) {
