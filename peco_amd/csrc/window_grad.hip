@@ -580,8 +580,9 @@ template <int DT, int D> __global__ __launch_bounds__(256) void window_dkv_join_
 
 // Parts of the key tiles' walks. Under a window a tile without sinks is seen by about left + right + 256 tokens,
 // one with sinks by every later token: the latter's walk is cut to about the former's length, so that no
-// workgroup walks on alone. Calls of few key tiles cut the other walks too, into parts of at least
-// kGradPartTiles tiles (a part writes and reads 256 KB of fp32).
+// workgroup walks on alone, but to no less than a quarter of a CU's share of the call (where the sinks are many there
+// are workgroups enough, and each part costs workspace). Calls of few key tiles cut the other walks too, into parts of
+// at least kGradPartTiles tiles (a part writes and reads 256 KB of fp32).
 constexpr int kGradPartTiles = 512 / kGradTile;
 constexpr int kMaxParts = 64;
 void plan_parts(GradArgs& A) {
@@ -596,7 +597,10 @@ void plan_parts(GradArgs& A) {
     const int64_t slots = device_compute_units();
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kMaxParts, walk / kGradPartTiles));
     A.parts = items >= slots ? 1 : static_cast<int>(std::min(most, ceil_div(2 * slots, items)));
-    const int64_t per = std::max<int64_t>(kGradPartTiles, ceil_div(walk, A.parts));
+    const int64_t total = static_cast<int64_t>(A.batch) * A.heads *
+                          (A.sink_tiles * all + (A.key_tiles - A.sink_tiles) * walk);
+    const int64_t per =
+        std::max({int64_t{kGradPartTiles}, ceil_div(walk, A.parts), ceil_div(total, 4 * slots)});
     A.sink_parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMaxParts, ceil_div(all, per))));
     if (A.sink_tiles == 0) A.sink_parts = 1;
 }

@@ -265,6 +265,25 @@ def test_second_derivatives_are_refused_and_empty_inputs(announce):
     assert (empty[0] == 0).all() and empty[1].shape == (1, 2, 0, 64)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,keys,sinks", [(3, 32896, 32896), (24, 118800, 118800), (1, 118800, 50000), (24, 7006, 256)])
+def test_many_sinks_need_little_workspace(heads, keys, sinks, announce):
+    """The walks of keys that every later token sees are cut for few heads only: at most 4 parts for each CU and one
+    for each tile of 256 keys, of 256 KB."""
+    announce()
+    floats = _native.library().peco_window_attention_grad_workspace_size(1, heads, heads, keys, keys, 255, 0, sinks, 128, 1)
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    assert floats <= heads * keys + 64 + (4 * cus + heads * (keys // 256 + 1)) * 256 * 256
+
+
+@pytest.mark.gpu
+def test_sinks_over_the_whole_sequence(announce):
+    announce()
+    q, k, v, g = _inputs(12, 1, 3, 3, 4000, 4000, 64, torch.bfloat16)
+    _, grads = _gradients(q, k, v, g, (63, 0), 4000)
+    _near(grads, *gradients(q, k, v, g, 63, 0, 4000))
+
+
 def test_entry_refuses_bad_arguments():
     lib, null, some = _native.library(), ctypes.c_void_p(0), ctypes.c_void_p(4096)  # refused before it is read
     floats = lib.peco_window_attention_grad_workspace_size(1, 2, 1, 5, 5, 1, 0, 0, 64, 1)
