@@ -143,12 +143,13 @@ template <int kMode> __device__ __forceinline__ int64_t all_rows(const WindowArg
 }
 
 // Clears the output rows that belong to no sequence (those before the first offset and behind the last). There
-// is always a workgroup without rows (A.tiles is larger than any number of row tiles): the first one does it.
-template <int D> __device__ void clear_tail(const WindowArgs& A, int kvh) {
+// is always a workgroup without rows (A.tiles is larger than any number of row tiles); number `at` of the `n` of a
+// key head clears its share.
+template <int D> __device__ void clear_tail(const WindowArgs& A, int kvh, int at, int n) {
     const int o0 = max(0, min(A.offsets[0], A.queries)), o1 = max(o0, min(A.offsets[A.batch], A.queries));
     constexpr int CH = D / 8;
-    const int64_t n = (static_cast<int64_t>(o0) + (A.queries - o1)) * A.group * CH;
-    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
+    const int64_t chunks = (static_cast<int64_t>(o0) + (A.queries - o1)) * A.group * CH;
+    for (int64_t i = at * int64_t{256} + threadIdx.x; i < chunks; i += n * int64_t{256}) {
         const int64_t r = i / CH, t = r / A.group;
         const int64_t token = t < o0 ? t : t - o0 + o1, head = static_cast<int64_t>(kvh) * A.group + r % A.group;
         *reinterpret_cast<u16x8*>(A.out + head * A.os.h + token * A.os.s + 8 * (i % CH)) = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
@@ -186,7 +187,8 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
     Item it;
     const bool found = find_rows<kMode>(A, blockIdx.x % items, it);
     if (kMode == kPaged && !found) {
-        if (A.clear_tail && part == 0 && it.row0 == 0) clear_tail<D>(A, it.kvh);
+        const int tile = static_cast<int>(blockIdx.x % items / A.heads);
+        if (A.clear_tail && part == 0) clear_tail<D>(A, it.kvh, it.row0, A.tiles - (tile - it.row0));
         return;
     }
     const int tid = threadIdx.x, lane = tid % kWave, h = lane / 32;

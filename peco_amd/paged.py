@@ -51,6 +51,10 @@ def _check_cache(k_pages, v_pages, page_table, offsets, lengths, rows, name):
 _NO_PLAN = (None, 0, 0, 0, None, None, 0, 0, 0)
 
 
+def _repeats_rows(t):
+    return any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape))
+
+
 def append_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                  page_table: torch.Tensor, offsets: torch.Tensor, lengths: torch.Tensor, *,
                  rotary: rotary_module.RotaryPositions | None = None) -> None:
@@ -70,6 +74,8 @@ def append_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     pages, kv_heads, page, _ = k_pages.shape
     if heads != kv_heads:
         raise ValueError("k and v must have the pages' heads")
+    if _repeats_rows(k_pages) or _repeats_rows(v_pages):
+        raise ValueError("pages that are written must not be expanded")
     positions, plan = None, _NO_PLAN
     if rotary is not None:
         if not isinstance(rotary, rotary_module.RotaryPositions):
@@ -114,8 +120,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             raise ValueError("out must be a tensor like q")
         if not _native.plain_tensors(out) or (torch.is_grad_enabled() and out.requires_grad):
             raise RuntimeError("out must be an ordinary tensor without gradient")
-        if rows16(out) is not out:
-            raise ValueError("out must have adjacent channels and rows on 16 bytes")
+        if rows16(out) is not out or _repeats_rows(out):
+            raise ValueError("out must have adjacent channels and rows on 16 bytes and not be expanded")
     result = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device) if out is None else out
     if tokens == 0:
         return result

@@ -261,6 +261,36 @@ def test_generation_as_it_runs(announce):
     assert (out.float() - whole.float()).abs().max() <= 2 * 2.0 ** -6 * v.abs().max()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("first,last", [(0, 1), (700, 1100), (2000, 2000)])
+def test_rows_of_no_sequence_in_a_wide_batch(first, last, announce):
+    """A batch captured for 5000 new tokens that holds few: all other rows give 0."""
+    announce()
+    cache = Cache(8, [500, 1200], 16, 2, 64, torch.bfloat16)
+    q = torch.randn(5000, 6, 64, device=DEV).bfloat16()
+    offsets = torch.tensor([first, last, last], dtype=torch.int32, device=DEV)
+    sizes = torch.tensor(cache.lengths, dtype=torch.int32, device=DEV)
+    soil = torch.full_like(q, float("nan"))
+    del soil  # (the result's memory, as a rule)
+    out = paged_attention(q, cache.k_pages, cache.v_pages, cache.table, offsets, sizes)
+    assert (out[:first] == 0).all() and (out[last:] == 0).all()
+    assert (out[first:last] != 0).any(-1).all()
+
+
+@pytest.mark.gpu
+def test_expanded_places_to_write_are_refused(announce):
+    announce()
+    cache = Cache(9, [40], 16, 2, 64, torch.bfloat16)
+    q, offsets, sizes = cache.queries([3], 2)
+    wide = cache.k_pages[:1].expand(cache.k_pages.shape)
+    args = (cache.table, offsets, sizes)
+    for pages in ((wide, cache.v_pages), (cache.k_pages, wide)):
+        with pytest.raises(ValueError, match="expanded"):
+            append_pages(q, q, *pages, *args)
+    with pytest.raises(ValueError, match="expanded"):
+        paged_attention(q, cache.k_pages, cache.v_pages, *args, out=torch.empty_like(q[:1]).expand(q.shape))
+
+
 def test_refusals():
     """No launch is reached: these run without a GPU."""
     q, pages = torch.zeros(3, 4, 64).bfloat16(), torch.zeros(5, 2, 16, 64).bfloat16()
