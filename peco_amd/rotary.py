@@ -157,7 +157,8 @@ def rotary_axes(x: torch.Tensor, positions: torch.Tensor, axes: RotaryAxes) -> t
 
     fp16, bf16 or fp32 rows, D a multiple of 8 up to 512, any strides (rows that are not laid out on 16 bytes
     with adjacent channels are copied first); the result has the strides of ``empty_like(x)``. Differentiable
-    once in x: its gradient is turned back. Rows are turned in fp32 and rounded once.
+    once in x: its gradient is turned back (a backward pass may be captured into a HIP graph while no eager graph
+    of the same leaf is alive, as with any torch operation). Rows are turned in fp32 and rounded once.
     """
     if not isinstance(x, torch.Tensor) or x.dim() != 4:
         raise ValueError("rotary_axes expects rows [B,H,S,D]")

@@ -170,7 +170,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window, 
     causal, (n - 1, 0) a causal window of n tokens, (n, n) one to both sides. A query that sees no key gives 0.
     ``lengths`` (int32 [B], needs SQ == SK): valid tokens of each sequence of a right-padded batch; later keys are
     not seen, later rows give 0 and take no gradient, whatever they hold. ``scale`` defaults to 1 / sqrt(D).
-    The result has the strides of ``empty_like(q)``. Differentiable once in Q, K and V.
+    The result has the strides of ``empty_like(q)``. Differentiable once in Q, K and V. A backward pass may be
+    captured into a HIP graph while no eager graph of the same leaves is alive (torch's engine would accumulate
+    their gradients on that graph's stream and end the process).
     """
     _check(q, k, v, lengths)
     mask = check_mask(window, sinks, scale, q.shape[3])
