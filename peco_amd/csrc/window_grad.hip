@@ -581,11 +581,15 @@ template <int DT, int D> __global__ __launch_bounds__(256) void window_dkv_join_
 // Parts of the key tiles' walks. Under a window a tile without sinks is seen by about left + right + 256 tokens,
 // one with sinks by every later token: the latter's walk is cut to about the former's length, so that no
 // workgroup walks on alone, but to no less than a quarter of a CU's share of the call (where the sinks are many there
-// are workgroups enough, and each part costs workspace). Calls of few key tiles cut the other walks too, into parts of
-// at least kGradPartTiles tiles (a part writes and reads 256 KB of fp32).
-constexpr int kGradPartTiles = 512 / kGradTile;
+// are workgroups enough, and each part costs workspace).
+// Calls of few key tiles cut the other walks too: a workgroup to a CU at a time, the rounds of workgroups times a
+// part's tiles and a fixed cost, plus the third launch, which reads the parts' fp32 sums. Measured (128 channels: 3.3 us
+// a tile and 15 fixed, 64 channels: 2.0 and 10): one head of 7006 tokens without a window (28 key tiles) 333 us uncut,
+// 80 in 6 parts, 69 in 12; 24 heads of 1800 tokens in windows of 512 (192) 55 uncut, 86 in 2 parts; 8 heads of 777
+// tokens in windows of 256 (32, 64 channels) 41 in 2 parts, 30 in 8.
+constexpr int kGradPartTiles = 2;  // of a part at least
 constexpr int kMaxParts = 64;
-void plan_parts(GradArgs& A) {
+void plan_parts(GradArgs& A, int d) {
     A.row_tiles = static_cast<int>(ceil_div(static_cast<int64_t>(A.queries) * A.group, kWinRows));
     A.key_tiles = static_cast<int>(ceil_div(A.keys, kGradKeys));
     A.v_blocks = static_cast<int>(ceil_div(A.keys, kWinRows));
@@ -596,7 +600,16 @@ void plan_parts(GradArgs& A) {
     const int64_t items = static_cast<int64_t>(A.batch) * A.heads * A.key_tiles;
     const int64_t slots = device_compute_units();
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kMaxParts, walk / kGradPartTiles));
-    A.parts = items >= slots ? 1 : static_cast<int>(std::min(most, ceil_div(2 * slots, items)));
+    const double tile_us = d == 128 ? 3.3 : 2.0, fixed_us = d == 128 ? 15.0 : 10.0;
+    double least = 1e30;
+    A.parts = 1;
+    for (int n = 1; n <= most; ++n) {
+        double cost = static_cast<double>(ceil_div(items * n, slots)) * (fixed_us + tile_us * static_cast<double>(ceil_div(walk, n)));
+        if (n > 1) cost += 4.0 + static_cast<double>(items) * n * kGradKeys * 2 * d * 4 / 6.0e6;  // 4 us and 6 TB/s
+        if (cost >= least) continue;
+        least = cost;
+        A.parts = n;
+    }
     const int64_t total = static_cast<int64_t>(A.batch) * A.heads *
                           (A.sink_tiles * all + (A.key_tiles - A.sink_tiles) * walk);
     const int64_t per =
@@ -641,7 +654,7 @@ bool shape_ok(int batch, int q_heads, int kv_heads, int queries, int keys, int l
     return batch >= 1 && kv_heads >= 1 && q_heads >= kv_heads && q_heads % kv_heads == 0 && queries >= 1 && keys >= 1 &&
            left >= -1 && right >= -1 && sinks >= 0 && left <= kUnbounded && right <= kUnbounded && sinks <= kUnbounded;
 }
-GradArgs sizes_of(int batch, int q_heads, int kv_heads, int queries, int keys, int left, int right, int sinks) {
+GradArgs sizes_of(int batch, int q_heads, int kv_heads, int queries, int keys, int left, int right, int sinks, int d) {
     GradArgs A{};
     A.batch = batch;
     A.heads = kv_heads;
@@ -651,7 +664,7 @@ GradArgs sizes_of(int batch, int q_heads, int kv_heads, int queries, int keys, i
     A.left = left < 0 ? kUnbounded : left;
     A.right = right < 0 ? kUnbounded : right;
     A.sinks = sinks;
-    plan_parts(A);
+    plan_parts(A, d);
     return A;
 }
 
@@ -664,7 +677,7 @@ PECO_API size_t peco_window_attention_grad_workspace_size(int batch, int q_heads
                                                           int left, int right, int sinks, int d, int dtype) {
     if (!shape_ok(batch, q_heads, kv_heads, queries, keys, left, right, sinks)) return 0;
     return static_cast<size_t>(
-        grad_layout(sizes_of(batch, q_heads, kv_heads, queries, keys, left, right, sinks), d, dtype).floats);
+        grad_layout(sizes_of(batch, q_heads, kv_heads, queries, keys, left, right, sinks, d), d, dtype).floats);
 }
 
 PECO_API int peco_window_attention_grad(const void* q, const void* k, const void* v, const void* output,
@@ -690,7 +703,7 @@ PECO_API int peco_window_attention_grad(const void* q, const void* k, const void
                           static_cast<const void*>(dv), output_rest, static_cast<const void*>(workspace)})
         at |= reinterpret_cast<uintptr_t>(p);
     if (all % 8 || at % 16) return kInvalidValue;
-    GradArgs A = sizes_of(batch, q_heads, kv_heads, queries, keys, left, right, sinks);
+    GradArgs A = sizes_of(batch, q_heads, kv_heads, queries, keys, left, right, sinks, d);
     const GradLayout l = grad_layout(A, d, dtype);
     if (workspace_floats < static_cast<size_t>(l.floats)) return kWorkspaceTooSmall;
     A.q = static_cast<const uint16_t*>(q);
