@@ -598,46 +598,20 @@ int launch(const WindowArgs& A, WindowMode mode, int d, int dtype, hipStream_t s
 // the reads even where sequences differ in length. Measured, 128 channels: 32 x 8 heads of one token over up to 7006
 // keys 176 us uncut, 106 in 8 parts and 5 for the join; one token over 119056 keys, 24 heads, 298 us in 12 parts, 359
 // in 21 (one even round, whose last workgroups read alone), 271 in 64 and 13 for the join.
-// Other items are bound by their products. A call takes as long as its busiest CU: the count of workgroups there times
-// a workgroup's tiles (and kStartTiles for its start and end), in units of what a CU takes for a tile with two
-// workgroups sharing it (1.4 us with 128 channels, half with 64; one alone is a third faster than that, not twice),
-// plus the join, which writes and reads the parts' fp32 rows.
+// Other items are bound by their products (cut_parts).
 constexpr int kFewRows = 32;
-constexpr int kPartTiles = 4;
-constexpr int kStartTiles = 4;
-constexpr int kMaxSplits = 64;
 struct Shape {
     int64_t tiles, rows, blocks;  // row tiles of a key head, query rows, workgroups
     int splits;
 };
 // `heads` key heads of `tiles` row tiles, `items` of them with rows, which hold `rows` in all.
 Shape shape_of(int64_t heads, int64_t tiles, int64_t items, int64_t seen_keys, int64_t rows, int d) {
-    const int64_t cus = device_compute_units(), n = ceil_div(seen_keys, kWinTile);
-    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, n / kPartTiles));
     Shape best{tiles, rows, 0, 1};
-    if (rows <= items * kFewRows) {
-        best.splits = static_cast<int>(std::min(most, ceil_div(8 * cus, items)));
-    } else {
-        const double tile_us = d == 128 ? 1.4 : 0.7;
-        double least = 1e30;
-        for (int s = 1; s <= most; ++s) {
-            const int64_t k = ceil_div(items * s, cus);
-            double cost = (k == 1 ? 4.0 / 3.0 : static_cast<double>(k)) * static_cast<double>(ceil_div(n, s) + kStartTiles);
-            if (s > 1) cost += (4.0 + static_cast<double>(rows) * s * (d + 2) * 8.0 / 5.0e6) / tile_us;  // 4 us and 5 TB/s
-            else cost *= 0.93;  // (less than that a cut is not worth: the busiest CU's last workgroup runs the faster)
-            if (cost >= least) continue;
-            least = cost;
-            best.splits = s;
-        }
-    }
+    if (rows <= items * kFewRows)
+        best.splits = static_cast<int>(std::min(most_parts(seen_keys), ceil_div(8 * int64_t{device_compute_units()}, items)));
+    else best.splits = cut_parts(items, seen_keys, rows, d);
     best.blocks = heads * tiles * best.splits;
     return best;
-}
-
-// Most keys that a tile of rows may see.
-int64_t seen_keys(int64_t keys, int64_t tokens, int left, int right, int sinks) {
-    const int64_t window = left < 0 || right < 0 ? keys : std::min<int64_t>(keys, int64_t{left} + right + tokens + sinks);
-    return std::max<int64_t>(window, 0);
 }
 
 Shape window_shape(int batch, int q_heads, int kv_heads, int queries, int keys, int left, int right, int sinks, int d) {

@@ -18,6 +18,8 @@
 
 #include "mfma.hpp"
 
+#include <algorithm>
+
 namespace peco {
 
 constexpr int kWinTile = 64;      // rows of an LDS tile
@@ -184,6 +186,41 @@ __device__ __forceinline__ KeyStream key_stream(int first, int last, int keys, i
     s.length = s.a1 + max(hi + 1 - lo, 0);
     s.delta = lo - s.a1;
     return s;
+}
+
+// Most keys that a tile of `tokens` tokens' rows may see.
+inline int64_t seen_keys(int64_t keys, int64_t tokens, int left, int right, int sinks) {
+    const int64_t window = left < 0 || right < 0 ? keys : std::min<int64_t>(keys, int64_t{left} + right + tokens + sinks);
+    return std::max<int64_t>(window, 0);
+}
+
+constexpr int kPartTiles = 4;   // of a part at least
+constexpr int kStartTiles = 4;
+constexpr int kMaxSplits = 64;
+inline int64_t most_parts(int64_t keys) {
+    return std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, ceil_div(keys, kWinTile) / kPartTiles));
+}
+
+// Into how many parts the walks of `items` row tiles, each over up to `keys` keys, `rows` query rows in all, are cut.
+// A call takes as long as its busiest CU: the count of workgroups there times a workgroup's tiles (and kStartTiles for
+// its start and end), in units of what a CU takes for a tile with two workgroups sharing it (1.4 us with 128 channels,
+// half with 64, in the forward and in dQ; one alone is a third faster than that, not twice), plus the join, which
+// writes and reads the parts' fp32 rows.
+inline int cut_parts(int64_t items, int64_t keys, int64_t rows, int d) {
+    const int64_t cus = device_compute_units(), n = ceil_div(keys, kWinTile), most = most_parts(keys);
+    const double tile_us = d == 128 ? 1.4 : 0.7;
+    double least = 1e30;
+    int best = 1;
+    for (int s = 1; s <= most; ++s) {
+        const int64_t k = ceil_div(items * s, cus);
+        double cost = (k == 1 ? 4.0 / 3.0 : static_cast<double>(k)) * static_cast<double>(ceil_div(n, s) + kStartTiles);
+        if (s > 1) cost += (4.0 + static_cast<double>(rows) * s * (d + 2) * 8.0 / 5.0e6) / tile_us;  // 4 us and 5 TB/s
+        else cost *= 0.93;  // (less than that a cut is not worth: the busiest CU's last workgroup runs the faster)
+        if (cost >= least) continue;
+        least = cost;
+        best = s;
+    }
+    return best;
 }
 
 }  // namespace peco

@@ -44,6 +44,8 @@ struct GradArgs {
     const float *row_max, *row_log;  // [batch, query heads, queries]
     float* delta;                    // the same shape
     int row_tiles, key_tiles, v_blocks;  // tiles of kWinRows rows, of kGradKeys keys, blocks of kWinRows keys
+    int row_parts;                       // of every row tile's walk
+    float* row_part;                     // dQ of each part [row_parts, query rows, D]
     // fp16: longest rows (squared) of V, per block of kWinRows of a key head, and of g, per row tile of one
     float *v_long, *g_long;
     int sink_tiles, sink_parts, parts;  // key tiles that hold sinks come first; parts of their walks and of the others'
@@ -117,8 +119,10 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
     uint16_t(*const vs)[T::kElems] = kvs + 2;
     __shared__ float tmp[4];
 
-    const int heads = A.batch * A.heads;
-    const int bh = blockIdx.x % heads, tile = A.row_tiles - 1 - static_cast<int>(blockIdx.x / heads);
+    // Parts of one row tile are as many workgroups apart as there are row tiles.
+    const int heads = A.batch * A.heads, items = heads * A.row_tiles;
+    const int part = static_cast<int>(blockIdx.x / items), item = static_cast<int>(blockIdx.x % items);
+    const int bh = item % heads, tile = A.row_tiles - 1 - item / heads;
     const int b = bh / A.heads, kvh = bh % A.heads;
     const Sequence q = sequence_of(A, b);
     const int row0 = tile * kWinRows, rows = min(kWinRows, A.queries * A.group - row0);
@@ -135,7 +139,9 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
                                               : key_stream(q.position0 + t_first, q.position0 + t_last, q.keys, A.left,
                                                            A.right, A.sinks);
     const int L = stream.length, l_last = max(L - 1, 0);
-    const int tiles = static_cast<int>(ceil_div(L, kWinTile));
+    const int all_tiles = static_cast<int>(ceil_div(L, kWinTile));
+    const int per = static_cast<int>(ceil_div(all_tiles, A.row_parts));
+    const int tile0 = min(part * per, all_tiles), tile1 = min(tile0 + per, all_tiles);
     const int pos = q.position0 + token;
     const int last_r = takes ? min(min(pos + A.right, q.keys - 1) - stream.delta, L - 1) : -1;
     const int first_r = pos - A.left - stream.delta;
@@ -171,13 +177,13 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
     }
     delta += __shfl_xor(delta, 32, kWave);
     if (!takes) delta = 0.0f;
-    if (qvalid && h == 0) A.delta[row_id] = delta;
+    if (qvalid && h == 0 && part == 0) A.delta[row_id] = delta;
     float dmul = 1.0f;
     if constexpr (DT == kF16) {
         g2 += __shfl_xor(g2, 32, kWave);
         if (!takes) g2 = 0.0f;
         const float longest = block_max<4>(g2, tmp);
-        if (tid == 0) A.g_long[static_cast<int64_t>(bh) * A.row_tiles + tile] = longest;
+        if (tid == 0 && part == 0) A.g_long[static_cast<int64_t>(bh) * A.row_tiles + tile] = longest;
         float v2 = 0.0f;
         for (int i = tid; i < A.v_blocks; i += 256) v2 = fmaxf(v2, A.v_long[static_cast<int64_t>(bh) * A.v_blocks + i]);
         dmul = dscale(g2, block_max<4>(v2, tmp));
@@ -251,19 +257,19 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
     auto walk = [&](auto careful) __attribute__((always_inline)) {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) acc[nb] = f32x16{};
-        if (tiles == 0) return;
+        if (tile0 >= tile1) return;
 #if defined(__HIP_DEVICE_COMPILE__)
         // (What the loop reads from registers has arrived: the compiler does not count the tile loads.)
 #pragma unroll
         for (int s = 0; s < S; ++s) asm volatile("" ::"v"(qf[s]), "v"(gf[s]));
         asm volatile("" ::"v"(m), "v"(log_l));
 #endif
-        load_tile(0, 0);
+        load_tile(tile0, 0);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         auto step = [&](auto bufc, int t) __attribute__((always_inline)) {
             const int buf = bufc;
-            if (t + 1 < tiles) load_tile(t + 1, buf ^ 1);
+            if (t + 1 < tile1) load_tile(t + 1, buf ^ 1);
             if (!wave_active) {
             } else if constexpr (decltype(careful)::value) {
 #pragma unroll 1
@@ -279,11 +285,11 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
         };
         if constexpr (decltype(careful)::value) {
 #pragma unroll 1
-            for (int t = 0; t < tiles; ++t) step(t & 1, t);
+            for (int t = tile0; t < tile1; ++t) step((t - tile0) & 1, t);
         } else {
-            for (int t = 0; t < tiles; t += 2) {
+            for (int t = tile0; t < tile1; t += 2) {
                 step(std::integral_constant<int, 0>{}, t);
-                if (t + 1 < tiles) step(std::integral_constant<int, 1>{}, t + 1);
+                if (t + 1 < tile1) step(std::integral_constant<int, 1>{}, t + 1);
             }
         }
     };
@@ -291,6 +297,18 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
     if (__syncthreads_or(wave_active && !all_finite(acc))) walk(std::true_type{});
     if (!qvalid) return;
     const float mul = A.scale / dmul;
+    if (A.row_parts > 1) {
+        const int64_t rows_all = static_cast<int64_t>(heads) * A.group * A.queries;
+        float* o = A.row_part + (part * rows_all + row_id) * D;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 x{acc[nb][4 * g] * mul, acc[nb][4 * g + 1] * mul, acc[nb][4 * g + 2] * mul, acc[nb][4 * g + 3] * mul};
+                *reinterpret_cast<f32x4*>(o + 32 * nb + 8 * g + 4 * h) = takes ? x : f32x4{};
+            }
+        return;
+    }
     uint16_t* o = A.dq + b * A.dqs.b + head * A.dqs.h + token * A.dqs.s;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
@@ -300,6 +318,21 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
             const uint32_t w1 = Mfma<DT>::pack2(acc[nb][4 * g + 2] * mul, acc[nb][4 * g + 3] * mul);
             *reinterpret_cast<u32x2*>(o + 32 * nb + 8 * g + 4 * h) = takes ? u32x2{w0, w1} : u32x2{0, 0};
         }
+}
+
+// dQ of the row tiles whose walks were cut: the parts' sums, in order. D / 4 lanes a row.
+template <int DT, int D> __global__ __launch_bounds__(256) void window_dq_join_kernel(GradArgs A) {
+    constexpr int kLanes = D / 4;
+    const int hq = A.heads * A.group;
+    const int64_t rows_all = static_cast<int64_t>(A.batch) * hq * A.queries;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
+    if (row >= rows_all) return;
+    const int c = 4 * (threadIdx.x % kLanes);
+    f32x4 sum{};
+    for (int i = 0; i < A.row_parts; ++i) sum += *reinterpret_cast<const f32x4*>(A.row_part + (i * rows_all + row) * D + c);
+    const int64_t token = row % A.queries, head = row / A.queries % hq, b = row / A.queries / hq;
+    *reinterpret_cast<u32x2*>(A.dq + b * A.dqs.b + head * A.dqs.h + token * A.dqs.s + c) =
+        u32x2{Mfma<DT>::pack2(sum[0], sum[1]), Mfma<DT>::pack2(sum[2], sum[3])};
 }
 
 // Items of a head: the sink tiles' parts, then the other tiles' parts.
@@ -593,6 +626,10 @@ void plan_parts(GradArgs& A, int d) {
     A.row_tiles = static_cast<int>(ceil_div(static_cast<int64_t>(A.queries) * A.group, kWinRows));
     A.key_tiles = static_cast<int>(ceil_div(A.keys, kGradKeys));
     A.v_blocks = static_cast<int>(ceil_div(A.keys, kWinRows));
+    const int64_t tokens = std::min<int64_t>(A.queries, kWinRows / A.group + 1);
+    A.row_parts = cut_parts(static_cast<int64_t>(A.batch) * A.heads * A.row_tiles,
+                            seen_keys(A.keys, tokens, A.left, A.right, A.sinks),
+                            static_cast<int64_t>(A.batch) * A.heads * A.group * A.queries, d);
     const int64_t all = ceil_div(static_cast<int64_t>(A.queries) * A.group, kGradTile);
     const int64_t window = std::min<int64_t>(A.queries, static_cast<int64_t>(A.left) + A.right + kGradKeys);
     const int64_t walk = std::max<int64_t>(1, std::min(all, ceil_div(window * A.group, kGradTile)));
@@ -628,18 +665,23 @@ GradLayout grad_layout(const GradArgs& A, int d, int dtype) {
     l.v_long = up(heads * A.group * A.queries);
     l.g_long = l.v_long + (dtype == kF16 ? up(heads * A.v_blocks) : 0);
     l.part = l.g_long + (dtype == kF16 ? up(heads * A.row_tiles) : 0);
-    l.floats = l.part + heads * partial_items(A) * kGradKeys * 2 * d;
+    // (One after the other: the parts of dQ are joined before the next launch writes its own.)
+    const int64_t row_parts = A.row_parts > 1 ? A.row_parts * heads * A.group * A.queries * d : 0;
+    l.floats = l.part + std::max(row_parts, heads * partial_items(A) * kGradKeys * 2 * d);
     return l;
 }
 
 template <int DT, int D> int launch_grad(const GradArgs& A, bool far, hipStream_t s) {
     const int64_t heads = static_cast<int64_t>(A.batch) * A.heads;
-    const int64_t dq = heads * A.row_tiles, dkv = heads * grad_items(A);
+    const int64_t dq = heads * A.row_tiles * A.row_parts, dkv = heads * grad_items(A);
     if (std::max(dq, dkv) > 0x7fffffff || heads * A.v_blocks > 0x7fffffff) return kUnsupportedShape;
     if constexpr (DT == kF16)
         hipLaunchKernelGGL((value_lengths_kernel<D>), dim3(static_cast<unsigned>(heads * A.v_blocks)), dim3(256), 0, s, A);
     if (far) hipLaunchKernelGGL((window_dq_kernel<DT, D, true>), dim3(static_cast<unsigned>(dq)), dim3(256), 0, s, A);
     else hipLaunchKernelGGL((window_dq_kernel<DT, D, false>), dim3(static_cast<unsigned>(dq)), dim3(256), 0, s, A);
+    if (A.row_parts > 1)
+        hipLaunchKernelGGL((window_dq_join_kernel<DT, D>),
+                           dim3(static_cast<unsigned>(ceil_div(heads * A.group * A.queries, 256 / (D / 4)))), dim3(256), 0, s, A);
     hipLaunchKernelGGL((window_dkv_kernel<DT, D>), dim3(static_cast<unsigned>(dkv)), dim3(kGradWaves * kWave), 0, s, A);
     if (partial_items(A)) {
         const int64_t rows = heads * (A.parts > 1 ? A.key_tiles : A.sink_tiles) * kGradKeys;
@@ -725,7 +767,7 @@ PECO_API int peco_window_attention_grad(const void* q, const void* k, const void
     A.delta = workspace;
     A.v_long = workspace + l.v_long;
     A.g_long = workspace + l.g_long;
-    A.part = workspace + l.part;
+    A.part = A.row_part = workspace + l.part;
     const bool far = std::max(A.ks.s, A.vs.s) * 2 * keys + 2 * d >= (int64_t{1} << 32);
     const auto s = static_cast<hipStream_t>(stream);
     if (dtype == kBF16) return d == 128 ? launch_grad<kBF16, 128>(A, far, s) : launch_grad<kBF16, 64>(A, far, s);

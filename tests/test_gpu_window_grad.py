@@ -130,6 +130,26 @@ def test_padded_batch(dtype, announce):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_padded_batch_in_parts(dim, dtype, announce):
+    """Few heads of long sequences: the walks of row tiles and of key tiles are cut, and parts beyond a sequence's
+    end have nothing to add."""
+    announce()
+    sizes = [2600, 900, 5]
+    q, k, v, g = _inputs(13, len(sizes), 2, 1, 2600, 2600, dim, dtype)
+    for b, n in enumerate(sizes):
+        for t, value in ((q, "nan"), (k, "inf"), (v, "-inf"), (g, "nan")):
+            t[b, :, n:] = float(value)
+    lengths = torch.tensor(sizes, dtype=torch.int32, device=DEV)
+    _, grads = _gradients(q, k, v, g, (-1, 0), 0, lengths=lengths)
+    for b, n in enumerate(sizes):
+        assert all((t[b, :, n:] == 0).all() for t in grads)
+        part = [t[b:b + 1, :, :n] for t in (q, k, v, g)]
+        _near([t[b:b + 1, :, :n] for t in grads], *gradients(*part, -1, 0, 0))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("which", range(4))
 @pytest.mark.parametrize("at", [3, 130, 200])
 def test_values_that_are_not_seen(which, at, announce):
