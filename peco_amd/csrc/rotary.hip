@@ -9,7 +9,8 @@
 // HBM-bound: each row is read and written once and the angles are computed, so no tables are read (fp32
 // tables of 118800 rows x 128 channels are 122 MB, a sixth of what 24 bf16 heads move, for each group of
 // heads that reads them). A lane holds 8 channels (16 for halves: 8 of each) of one row of kHeads heads with
-// all loads in flight and computes its 4 (8) angles once for all of them.
+// all loads in flight and computes its 4 (8) angles once for all of them. Measured, 24 heads x 128 channels, bf16:
+// 6750 rows 18 us (83 MB, 4.6 TB/s; a plain copy reaches 5.2), 118800 rows in halves 317 us (1.46 GB, 4.6 TB/s).
 #include "rotary.hpp"
 
 namespace peco {
@@ -93,7 +94,8 @@ template <int DT, bool kHalves> int launch_rotary(const RotaryArgs& a, const Rot
 // New tokens' keys (rotated) and values into the pages of a cache. k and v [tokens, heads, D] hold the tokens of
 // `batch` sequences in a row (offsets), token i of n of sequence b goes to place lengths[b] - n + i of its row of
 // the page table. Every lane moves 8 channels of K and of V of kHeads heads of one token; with halves it reads
-// its partner chunk as well (from the L1, where the partner's own read puts it).
+// its partner chunk as well (from the L1, where the partner's own read puts it). Measured, 128 channels, bf16: 5497
+// tokens of 24 heads 29 us (135 MB, 4.7 TB/s), 32 tokens of 8 heads 6 us.
 struct AppendArgs {
     const uint16_t *k, *v;
     uint16_t *k_pages, *v_pages;

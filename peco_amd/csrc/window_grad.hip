@@ -4,7 +4,7 @@
 //   dV = P^T g,   dP = g V^T,   dS = P (dP - delta),   dQ = scale dS K,   dK = scale dS^T Q.
 // P is computed again from Q, K and the forward's row statistics: P = 2^((s - m) scale log2 e - log2 l).
 //
-// Two launches, both without atomics (every sum has one order):
+// Two launches (and the joins of walks that are cut), without atomics (every sum has one order):
 //   dQ: a workgroup takes 128 rows as in the forward and walks their keys; per 32-key half S^T = K Q^T and
 //       dP^T = V g^T (A = tile rows, B in registers), dQ^T += K^T dS^T (A = the K tile by transpose reads, B =
 //       dS^T straight from the accumulators). It also forms delta, which the second launch reads.
@@ -13,6 +13,12 @@
 //       sums of both leave room for one wave a SIMD only), dV^T += g^T P, dK^T += Q^T dS. The rows of all
 //       query heads of the key head pass by, so shared heads need no further sum. Keys that are sinks are seen
 //       by every later row: their walk is cut into parts, which a third launch adds up in order.
+//
+// S and dP are taken in both launches: seven products where five would do, but no atomics, and no gradient is read
+// again. Measured with 128 channels, bf16, 24 heads of 7006 tokens in causal windows of 2026 with 256 sinks: dQ 268 us
+// (921 TFLOP/s of its three products, MFMA busy 51% of the time), dK/dV 417 us (789 of its four, 45%), its join 7 us.
+// Neither has LDS bank conflicts; what is left is the waves' waiting for LDS operands and for one another at the tiles'
+// ends. 4 waves of 64 keys, which read half as much from LDS, took 630 us for dK/dV (one wave a SIMD covers nothing).
 //
 // Roundings: scores, dP, P and all sums are fp32; P and dS are rounded to the type for the products. delta takes out
 // with what its rounding left: where a query sees a few keys dS is a small difference, and out's rounding alone
