@@ -334,8 +334,8 @@ int peco_place_heads_axes(const void* input, int64_t stride_batch, int64_t strid
  * int32 [batch], needs queries == keys): tokens of each sequence of a padded batch (clamped to [0, keys]); later
  * keys are not seen and later queries give 0. scale: positive, of the scores. row_max, row_log (fp32
  * [batch, q_heads, queries]) and output_rest (the output's dtype, contiguous [batch, q_heads, queries, d]; all three
- * or none) receive each row's largest unscaled score, the log2 of its sum and what the rounding of its output left,
- * for peco_window_attention_grad. workspace: peco_window_attention_workspace_size floats, 16-byte aligned (calls that
+ * or none) receive a reference near each row's largest unscaled score, the log2 of the sum of its weights relative
+ * to that and what the rounding of its output left, for peco_window_attention_grad. workspace: peco_window_attention_workspace_size floats, 16-byte aligned (calls that
  * overlap need one each; may be null when that is 0). */
 size_t peco_window_attention_workspace_size(int batch, int q_heads, int kv_heads, int queries, int keys, int left,
                                             int right, int sinks, int d);

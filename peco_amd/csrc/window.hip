@@ -8,7 +8,7 @@
 // into the other LDS buffer are in flight during the products of the current one, one barrier a tile.
 //   S^T = K Q^T (32x32x16 MFMA, A = K tile rows, B = Q^T in registers): lane l holds query l % 32, keys
 //         8 (i / 4) + 4 (l / 32) + i % 4 of a 32-key half;
-//   softmax with the running maximum and sum in fp32, a lane's query its own column;
+//   softmax with a running reference (near the maximum) and sum in fp32, a lane's query its own column;
 //   O^T += V^T P^T (A = V tile by transpose reads, B = P^T straight from the S^T accumulators).
 // Tiles that every row of a wave sees whole run without any mask; those at the edges of the window, of the
 // causal triangle and of the stream take per-element comparisons, halves that no row of the wave sees are left
@@ -16,21 +16,23 @@
 // tile each, and join their states at the end.
 //
 // Bounds: the exponentials, packing and maxima of the scores take about as long as the two products, so both have to
-// run at the same time: two workgroups a CU, one's products under the other's softmax (registers allow no third). Measured with 128 channels, bf16: 24 heads of 7006 tokens in causal windows of 2026 with 256 sinks 253 us
-// (652 TFLOP/s of the products that the mask leaves; MFMA busy 38% of the time, the last round of workgroups included),
-// 3 heads of 32896 tokens in windows of 8159 507 us (785 TFLOP/s). A large library product reaches 1252 there. No
+// run at the same time: two workgroups a CU, one's products under the other's softmax (registers allow no third). Measured with 128 channels, bf16: 24 heads of 7006 tokens in causal windows of 2026 with 256 sinks 225 us
+// (731 TFLOP/s of the products that the mask leaves, the last round of workgroups included), 3 heads of 32896 tokens in
+// windows of 8159 480 us (830 TFLOP/s). A large library product reaches 1252 there. No
 // LDS bank conflicts. Single tokens are bound by the keys' bytes: 119056 keys of 24 heads in 259 us (1.46 GB, 5.6 TB/s).
 //
 // Where items leave workgroup slots empty, their key streams are cut into `splits` parts, whose unnormalised fp32
-// outputs, maxima and sums a second launch joins.
+// outputs, references and sums a second launch joins.
 //
 // A value that a query must not see has a weight of 0, but 0 times an infinity or NaN is NaN. A workgroup whose
 // sums come out other than finite takes its item again in a careful walk, which multiplies the rows of halves that are
 // seen in part and hold such values one by one.
 //
 // Roundings: scores, softmax statistics and O are fp32. P is rounded to the type for the second product (the
-// sum takes the rounded values, so that the weights still add up to 1), out once at the end. O is rescaled at
-// every new maximum, so a row's largest weight is 1 when it is rounded.
+// sum takes the rounded values, so that the weights still add up to 1), out once at the end. Weights are relative to a
+// reference, a score that no other of the row exceeds by more than 2^8 in weight: 16-bit floats round as well at 2^8 as
+// at 1, and O is rescaled where the reference is raised, which after the first tiles is seldom (at every new maximum of
+// any of a wave's 32 rows it was in about every other half of 76 and took 253 us in place of 225, first size below).
 #include "window.hpp"
 
 #include <algorithm>
@@ -45,6 +47,9 @@ namespace {
 // rounds m * scale first, 2^-14 of an exponent off at this size.
 constexpr float kWideScores = 0x1p10f;
 
+// How far (in powers of two of the weights) a score may lie above its row's reference before that is raised.
+constexpr float kSlack = 8.0f;
+
 struct WindowArgs {
     const uint16_t *q, *k, *v;
     uint16_t* out;
@@ -53,6 +58,7 @@ struct WindowArgs {
     int batch, queries, keys;  // paged: sequences, all new tokens, capacity of a table row in keys
     int left, right, sinks;
     float scale_log2;
+    float slack;             // of a row's reference score (unscaled)
     const int32_t* lengths;  // contiguous: nullable valid tokens [batch]; paged: tokens held [batch]
     const int32_t* offsets;  // paged: first new token of each sequence [batch + 1]
     const int32_t* table;    // paged: page of each `page` tokens [batch, table_width]
@@ -62,8 +68,8 @@ struct WindowArgs {
     int splits;              // parts of every item's key stream
     int clear_tail;          // paged: rows outside every sequence are cleared
     float* part_o;           // parts' results [splits, rows, D]
-    float2* part_ml;         // and [splits, rows]: largest score, sum
-    // For the backward pass (all or none): raw maximum and log2 of the sum of every row, and what the rounding of
+    float2* part_ml;         // and [splits, rows]: reference score, sum
+    // For the backward pass (all or none): reference and log2 of the sum of every row, and what the rounding of
     // its output left (output rows one after another).
     float *row_max, *row_log;
     uint16_t* out_rest;
@@ -332,12 +338,12 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
         float tmax = sacc[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) tmax = fmaxf(tmax, sacc[i]);
-        if (__any(tmax > m_run)) {
+        if (__any(tmax > m_run + A.slack)) {
             tmax = fmaxf(tmax, __shfl_xor(tmax, 32, kWave));
-            const float m_new = fmaxf(m_run, tmax);
+            const float m_new = tmax > m_run + A.slack ? tmax : m_run;  // (by the query's own scores alone)
             const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * A.scale_log2);
             m_run = m_new;
-            // (A query that has seen nothing yet keeps its maximum at the lowest value; its weights are all 0.)
+            // (A query that has seen nothing yet keeps its reference at the lowest value; its weights are all 0.)
             neg_m = m_new == -FLT_MAX ? 0.0f : -m_new * A.scale_log2;
             wide = __any(fabsf(neg_m) > kWideScores);
             l_run *= alpha;
@@ -651,6 +657,11 @@ bool mask_ok(int left, int right, int sinks) {
 bool scale_ok(float scale) { return scale >= FLT_MIN && scale <= FLT_MAX; }
 int unbounded(int n) { return n < 0 ? kUnbounded : n; }
 
+void set_scale(WindowArgs& A, float scale) {
+    A.scale_log2 = static_cast<float>(1.4426950408889634 * static_cast<double>(scale));
+    A.slack = std::min(kSlack / A.scale_log2, 0x1p100f);  // (added to the lowest float it must stay below every score)
+}
+
 void set_parts(WindowArgs& A, const Shape& s, float* workspace, int d) {
     A.splits = s.splits;
     A.tiles = static_cast<int>(s.tiles);
@@ -705,7 +716,7 @@ PECO_API int peco_window_attention(const void* q, const void* k, const void* v, 
     A.left = unbounded(left);
     A.right = unbounded(right);
     A.sinks = sinks;
-    A.scale_log2 = static_cast<float>(1.4426950408889634 * static_cast<double>(scale));
+    set_scale(A, scale);
     A.lengths = lengths;
     A.row_max = row_max;
     A.row_log = row_log;
@@ -764,7 +775,7 @@ PECO_API int peco_paged_attention(const void* q, const void* k_pages, const void
     A.left = unbounded(left);
     A.right = 0;
     A.sinks = sinks;
-    A.scale_log2 = static_cast<float>(1.4426950408889634 * static_cast<double>(scale));
+    set_scale(A, scale);
     A.lengths = lengths;
     A.offsets = offsets;
     A.table = page_table;

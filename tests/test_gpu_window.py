@@ -154,6 +154,30 @@ def test_values_that_a_query_does_not_see(sq, sk, left, right, sinks, at, bad, a
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("step", [0.004, 0.05, 0.17, 0.7, -0.004, -0.05, -0.7])
+def test_rising_and_falling_scores(step, dtype, announce):
+    """Scores that climb along the keys by powers of two of the weight a tile, below and past the 2^8 by which a row's
+    weights may exceed its reference's, and that fall: forward and gradients."""
+    from tests.window_reference import gradients
+
+    announce()
+    g = torch.Generator().manual_seed(14)
+    signs = torch.sign(torch.randn(64, generator=g))
+    climb = step * torch.arange(1000)[:, None] / 8 * signs
+    q = (signs + 0.2 * torch.randn(1, 2, 150, 64, generator=g)).to(dtype).to(DEV)
+    k = (climb + 0.2 * torch.randn(1, 1, 1000, 64, generator=g)).to(dtype).to(DEV)
+    v = torch.randn(1, 1, 1000, 64, generator=g).to(dtype).to(DEV)
+    grad = torch.randn(1, 2, 150, 64, generator=g).to(dtype).to(DEV)
+    for left, right, sinks in ((-1, 0, 0), (400, 30, 40)):
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        out = window_attention(*leaves, (left, right), sinks)
+        _near(out, *attention(q, k, v, left, right, sinks))
+        for got, ref, bound in zip(torch.autograd.grad(out, leaves, grad), *gradients(q, k, v, grad, left, right, sinks)):
+            _near(got, ref, bound)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("size", [2.0 ** 8, 2.0 ** 30, 2.0 ** 55])
 def test_large_scores(size, announce):
     """Scores of up to 2^116 times their scale: the weights of the largest are 1, of the others 0 (they are apart by
