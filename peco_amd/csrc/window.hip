@@ -43,10 +43,6 @@
 namespace peco {
 namespace {
 
-// Scaled scores past which the maximum is subtracted before the multiplication: exp2(fma(s, scale, -m scale))
-// rounds m * scale first, 2^-14 of an exponent off at this size.
-constexpr float kWideScores = 0x1p10f;
-
 // How far (in powers of two of the weights) a score may lie above its row's reference before that is raised.
 constexpr float kSlack = 8.0f;
 

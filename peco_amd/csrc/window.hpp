@@ -26,6 +26,10 @@ constexpr int kWinTile = 64;      // rows of an LDS tile
 constexpr int kWinRows = 128;     // query rows of a forward or dQ workgroup, keys of a dK/dV workgroup
 constexpr int kUnbounded = 0x40000000;  // left or right without a limit
 
+// Scaled scores past which the reference is subtracted before the multiplication: exp2(fma(s, scale, -m scale))
+// rounds m * scale first, 2^-14 of an exponent off at this size.
+constexpr float kWideScores = 0x1p10f;
+
 template <int D> struct WinTile {
     static constexpr int CH = D / 8;                 // 16-byte chunks per row
     static constexpr int kElems = kWinTile * D;

@@ -194,7 +194,11 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
         for (int i = tid; i < A.v_blocks; i += 256) v2 = fmaxf(v2, A.v_long[static_cast<int64_t>(bh) * A.v_blocks + i]);
         dmul = dscale(g2, block_max<4>(v2, tmp));
     }
-    const float m = A.row_max[row_id], log_l = A.row_log[row_id];
+    // (A row that sees nothing has the lowest float and an infinite sum: weights of 0.) fp16: dS's factor is a power of
+    // two and goes into its weight's exponent.
+    const float m = A.row_max[row_id], log_l = A.row_log[row_id] - (DT == kF16 ? log2f(dmul) : 0.0f);
+    const bool wide = __any(m != -FLT_MAX && fabsf(m * A.scale_log2) > kWideScores);
+    const float offset = wide ? -log_l : __builtin_fmaf(-m, A.scale_log2, -log_l);
 
     const uint16_t* kh = A.k + b * A.ks.b + kvh * A.ks.h;
     const uint16_t* vh = A.v + b * A.vs.b + kvh * A.vs.h;
@@ -232,12 +236,15 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
             const int r = r0 + row;
             return r <= last_r && (r >= first_r || r < A.sinks);
         };
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sacc[i] -= m;
+        }
         float ds[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[i] - m, A.scale_log2, -log_l));
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[i], A.scale_log2, offset));
             ds[i] = p * (pacc[i] - delta);
-            if constexpr (DT == kF16) ds[i] *= dmul;
         }
         if (!whole) {
             // (Element i is row 8 (i / 4) + 4 h + i % 4: the lane's 4 h is taken off the limits, the rest is uniform.)
@@ -268,7 +275,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
         // (What the loop reads from registers has arrived: the compiler does not count the tile loads.)
 #pragma unroll
         for (int s = 0; s < S; ++s) asm volatile("" ::"v"(qf[s]), "v"(gf[s]));
-        asm volatile("" ::"v"(m), "v"(log_l));
+        asm volatile("" ::"v"(m), "v"(offset));
 #endif
         load_tile(tile0, 0);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
