@@ -16,9 +16,9 @@
 // tile each, and join their states at the end.
 //
 // Bounds: the exponentials, packing and maxima of the scores take about as long as the two products, so both have to
-// run at the same time: two workgroups a CU, one's products under the other's softmax (registers allow no third). Measured with 128 channels, bf16: 24 heads of 7006 tokens in causal windows of 2026 with 256 sinks 225 us
-// (731 TFLOP/s of the products that the mask leaves, the last round of workgroups included), 3 heads of 32896 tokens in
-// windows of 8159 480 us (830 TFLOP/s). A large library product reaches 1252 there. No
+// run at the same time: two workgroups a CU, one's products under the other's softmax (registers allow no third). Measured with 128 channels, bf16: 24 heads of 7006 tokens in causal windows of 2026 with 256 sinks 226 us
+// (728 TFLOP/s of the products that the mask leaves, the last round of workgroups included), 3 heads of 32896 tokens in
+// windows of 8159 499 us (798 TFLOP/s; calls one after another run at lower clocks than one alone). A large library product reaches 1252 there. No
 // LDS bank conflicts. Single tokens are bound by the keys' bytes: 119056 keys of 24 heads in 259 us (1.46 GB, 5.6 TB/s).
 //
 // Where items leave workgroup slots empty, their key streams are cut into `splits` parts, whose unnormalised fp32
@@ -31,8 +31,8 @@
 // Roundings: scores, softmax statistics and O are fp32. P is rounded to the type for the second product (the
 // sum takes the rounded values, so that the weights still add up to 1), out once at the end. Weights are relative to a
 // reference, a score that no other of the row exceeds by more than 2^8 in weight: 16-bit floats round as well at 2^8 as
-// at 1, and O is rescaled where the reference is raised, which after the first tiles is seldom (at every new maximum of
-// any of a wave's 32 rows it was in about every other half of 76 and took 253 us in place of 225, first size below).
+// at 1, and O is rescaled where the reference is raised, which after the first tiles is seldom (at every new
+// maximum of any of a wave's 32 rows it was in about every other half of 76, and the first size below took 253 us).
 #include "window.hpp"
 
 #include <algorithm>
@@ -43,8 +43,12 @@
 namespace peco {
 namespace {
 
-// How far (in powers of two of the weights) a score may lie above its row's reference before that is raised.
+// How far (in powers of two of the weights) a score may lie above its row's reference before that is raised, after the
+// first tiles of a walk. There the reference is the maximum: a row of few keys is mostly its largest weight, which is 1
+// then and is not rounded (with the slack from the start the gradients of windows of 16 to 256 keys are off by 1.50 to
+// 1.56 times what rounding them leaves, not 1.45 to 1.48).
 constexpr float kSlack = 8.0f;
+constexpr int kTightTiles = 4;
 
 struct WindowArgs {
     const uint16_t *q, *k, *v;
@@ -334,9 +338,10 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
         float tmax = sacc[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) tmax = fmaxf(tmax, sacc[i]);
-        if (__any(tmax > m_run + A.slack)) {
+        const float slack = t < tile0 + kTightTiles ? 0.0f : A.slack;
+        if (__any(tmax > m_run + slack)) {
             tmax = fmaxf(tmax, __shfl_xor(tmax, 32, kWave));
-            const float m_new = tmax > m_run + A.slack ? tmax : m_run;  // (by the query's own scores alone)
+            const float m_new = tmax > m_run + slack ? tmax : m_run;  // (by the query's own scores alone)
             const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * A.scale_log2);
             m_run = m_new;
             // (A query that has seen nothing yet keeps its reference at the lowest value; its weights are all 0.)
