@@ -16,10 +16,12 @@
 // tile each, and join their states at the end.
 //
 // Bounds: the exponentials, packing and maxima of the scores take about as long as the two products, so both have to
-// run at the same time: two workgroups a CU, one's products under the other's softmax (registers allow no third). Measured with 128 channels, bf16: 24 heads of 7006 tokens in causal windows of 2026 with 256 sinks 226 us
-// (728 TFLOP/s of the products that the mask leaves, the last round of workgroups included), 3 heads of 32896 tokens in
-// windows of 8159 499 us (798 TFLOP/s; calls one after another run at lower clocks than one alone). A large library product reaches 1252 there. No
-// LDS bank conflicts. Single tokens are bound by the keys' bytes: 119056 keys of 24 heads in 259 us (1.46 GB, 5.6 TB/s).
+// run at the same time: two workgroups a CU, one's products under the other's softmax (registers allow no third).
+// Measured with 128 channels, bf16: 24 heads of 7006 tokens in causal windows of 2026 with 256 sinks 226 us (728
+// TFLOP/s of the products that the mask leaves, the last round of workgroups included; MFMA busy 39% of the time), 3
+// heads of 32896 tokens in windows of 8159 499 us (798 TFLOP/s, 44%; calls one after another run at lower clocks than
+// one alone). A large library product reaches 1252 there. No LDS bank conflicts. Single tokens are bound by the keys'
+// bytes: 119056 keys of 24 heads in 259 us (1.46 GB, 5.6 TB/s).
 //
 // Where items leave workgroup slots empty, their key streams are cut into `splits` parts, whose unnormalised fp32
 // outputs, references and sums a second launch joins.

@@ -207,8 +207,8 @@ inline int64_t most_parts(int64_t keys) {
 
 // Into how many parts the walks of `items` row tiles, each over up to `keys` keys, `rows` query rows in all, are cut.
 // A call takes as long as its busiest CU: the count of workgroups there times a workgroup's tiles (and kStartTiles for
-// its start and end), in units of what a CU takes for a tile with two workgroups sharing it (1.4 us with 128 channels,
-// half with 64, in the forward and in dQ; one alone is a third faster than that, not twice), plus the join, which
+// its start and end), in units of what a CU takes for a tile with two workgroups sharing it (1.3 to 1.4 us with 128
+// channels, half with 64, in the forward and in dQ; one alone is a third faster than that, not twice), plus the join, which
 // writes and reads the parts' fp32 rows.
 inline int cut_parts(int64_t items, int64_t keys, int64_t rows, int d) {
     const int64_t cus = device_compute_units(), n = ceil_div(keys, kWinTile), most = most_parts(keys);

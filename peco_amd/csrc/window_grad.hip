@@ -370,7 +370,7 @@ __global__ __launch_bounds__(kGradWaves * kWave, 2) void window_dkv_kernel(GradA
     // in registers the compiler spills some of it to memory, whose loads wait for the tile loads before them.)
     constexpr int kSpilled = D == 128 ? 3 : 0, kHeld = S - kSpilled;
     __shared__ u16x8 operands[kGradWaves][S + kSpilled][kWave];
-    __shared__ __align__(16) float stat[2][3][kTile];  // row maxima, log2 sums and deltas of a tile
+    __shared__ __align__(16) float stat[2][3][kTile];  // references, log2 sums and deltas of a tile's rows
     __shared__ float tmp[kGradWaves];
 
     const int heads = A.batch * A.heads;

@@ -96,7 +96,7 @@ def _check(q, k, v, lengths):
 
 
 def _forward(q, k, v, lengths, left, right, sinks, scale, stats):
-    """(output, row maxima, log2 of the row sums, rest of the output); the last three None without ``stats``."""
+    """(output, row references, log2 of the row sums, rest of the output); the last three None without ``stats``."""
     batch, heads, sq, dim = q.shape
     kv_heads, sk = k.shape[1:3]
     out = torch.empty_like(q)
