@@ -117,19 +117,21 @@ inline int device_compute_units() {
 // see an LDS write in flight: it cannot tell the buffer being filled from the one being read
 // by the fragment reads and would otherwise wait for the whole prefetch in the middle of
 // every tile. The caller waits for vmcnt(0) before the barrier that publishes the tile.
+// The scalar write of M0 and the load that reads it need one wait state between them, which the compiler puts there
+// for its own builtin but not inside an asm block: the s_nop.
 __device__ __forceinline__ void dma16(const uint16_t* src, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
 }
 
 // The same with a wave-uniform base address in SGPRs and a 32-bit byte offset per lane (one
 // VALU operation per load for the offset instead of 64-bit address arithmetic).
 __device__ __forceinline__ void dma16_off(const void* base, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
 }
 
 // The same with 4 bytes per lane: lane i writes lds + 4i.
 __device__ __forceinline__ void dma4(const void* src, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
 }
 
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {
