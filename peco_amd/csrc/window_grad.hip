@@ -483,11 +483,11 @@ __global__ __launch_bounds__(kGradWaves * kWave, 2) void window_dkv_kernel(GradA
         f32x16 p{}, ds{};
         WinLane<D> at = at0.moved(qoff);
         at.fresh();
+        // (The channels in the forward's order: the references and sums are those of its scores, and where scores are
+        // large another order's rounding moves the exponents.)
 #pragma unroll
-        for (int s = S - 1; s >= kHeld; --s)
-            p = Mfma<DT>::run(at.rows(qt, s), operands[wave][S + s - kHeld][lane], p);
-#pragma unroll
-        for (int s = 0; s < kHeld; ++s) p = Mfma<DT>::run(at.rows(qt, s), kf[s], p);
+        for (int s = 0; s < S; ++s)
+            p = Mfma<DT>::run(at.rows(qt, s), s < kHeld ? kf[s < kHeld ? s : 0] : operands[wave][S + s - kHeld][lane], p);
         read_ahead<S, S + kSpilled, 6>();
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
