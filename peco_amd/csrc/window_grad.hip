@@ -70,6 +70,10 @@ __device__ __forceinline__ Sequence sequence_of(const GradArgs& A, int b) {
     return s;
 }
 
+// A row's length for the bound on dS. A row with an infinity or NaN is left out: its dS is none that a factor could keep
+// in range, and the other rows' keep theirs.
+__device__ __forceinline__ float finite_length(float sq) { return sq < INFINITY ? sq : 0.0f; }
+
 // fp16: dS is multiplied by this power of two (never more than 2^14 then).
 __device__ __forceinline__ float dscale(float g2, float v2) {
     const float bound = 2.0f * sqrtf(g2) * sqrtf(v2);
@@ -110,7 +114,7 @@ template <int D> __global__ __launch_bounds__(256) void value_lengths_kernel(Gra
         }
 #pragma unroll
         for (int m = G / 2; m; m /= 2) sq += __shfl_xor(sq, m, kWave);
-        most = fmaxf(most, sq);
+        most = fmaxf(most, finite_length(sq));
     }
     most = block_max<4>(most, tmp);
     if (threadIdx.x == 0) A.v_long[blockIdx.x] = most;
@@ -188,6 +192,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
     if constexpr (DT == kF16) {
         g2 += __shfl_xor(g2, 32, kWave);
         if (!takes) g2 = 0.0f;
+        g2 = finite_length(g2);
         const float longest = block_max<4>(g2, tmp);
         if (tid == 0 && part == 0) A.g_long[static_cast<int64_t>(bh) * A.row_tiles + tile] = longest;
         float v2 = 0.0f;

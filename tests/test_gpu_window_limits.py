@@ -46,3 +46,31 @@ def test_gradients_of_large_scores(dim, dtype, size, left, right, sinks, announc
                   for t in (g, g.abs()))
     assert ((grads[2].double() - want).abs() <= unit * want.abs() + 2.0 ** -16 * mass).all()
     assert all(torch.isfinite(t).all() for t in grads)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("which,dim", [(2, 64), (3, 64), (2, 128), (3, 128)])
+def test_fp16_gradients_beside_an_infinity(which, dim, bad, announce):
+    """An infinity or NaN in one row of v or of the gradient leaves the gradients of rows that do not meet it as they
+    were, bit for bit. Their dS is far below fp16's steps without a factor (weights of one in 1500 of gradients of
+    2^-14), and that factor comes from the lengths of the head's rows (the longest are others here)."""
+    announce()
+    gen = torch.Generator().manual_seed(15)
+    sk, left = 2600, 1500
+    q, k, v, g = (torch.randn(1, 2, sk, dim, generator=gen) for _ in range(4))
+    # (Weights as of a scale of 1 / sqrt(D), while dQ = scale dS K and dK = scale dS^T Q are 2^6 times larger.)
+    q, k = q * 2.0 ** -6, k * 2.0 ** -6
+    g[:, :, 9], v[:, :, 9] = 2 * g.norm(dim=-1).amax() * dim ** -0.5, 2 * v.norm(dim=-1).amax() * dim ** -0.5
+    clean = [t.half().to(DEV) for t in (q, k, v, g * 2.0 ** -14)]
+    scale = 2.0 ** 12 * dim ** -0.5
+    _, want = _gradients(*clean, (left, 0), 0, scale=scale)
+    changed = [t.clone() for t in clean]
+    changed[which][0, 1, 5, 3] = bad
+    out, got = _gradients(*changed, (left, 0), 0, scale=scale)
+    for i, first in enumerate((1700, 1800, 1800) if which == 2 else (200, 300, 300)):  # (whole tiles past the last reached)
+        part = got[i][:, 1, first:]
+        assert torch.isfinite(part).all() and (part != 0).float().mean() > 0.9
+        assert torch.equal(part, want[i][:, 1, first:])
+        assert torch.equal(got[i][:, 0], want[i][:, 0])
+    assert not torch.isfinite(got[0][0, 1, 5]).all()
