@@ -264,7 +264,8 @@ def plain_tensors(*tensors) -> bool:
         return False
     dual = torch.autograd.forward_ad._current_level >= 0  # (no tensor has a tangent outside a level)
     for t in tensors:
-        if type(t) not in (torch.Tensor, torch.nn.Parameter) or torch._C._functorch.is_functorch_wrapped_tensor(t):
+        if type(t) not in (torch.Tensor, torch.nn.Parameter) or torch._C._functorch.is_functorch_wrapped_tensor(t) or \
+                torch._C._functorch.is_legacy_batchedtensor(t):  # (what a batch of gradients arrives as)
             return False
         if dual and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
             return False
