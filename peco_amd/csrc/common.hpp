@@ -97,6 +97,9 @@ template <typename T> __device__ __forceinline__ T wave_shfl_xor(T v, int mask) 
 
 __host__ __device__ __forceinline__ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Whether a launch of that many workgroups is one: a grid's axis has fewer than 2^32 lanes.
+inline bool fits_grid(int64_t blocks, int threads) { return blocks * threads < (int64_t{1} << 32); }
+
 // Compute units of the current device (cached per device; 256 if the query fails).
 inline int device_compute_units() {
     static std::mutex m;

@@ -179,7 +179,7 @@ template <int DT, int D> int launch_append(const AppendArgs& a, const RotaryPlan
     const int64_t blocks = ceil_div(a.tokens, 256 / (D / 8));
     const bool wide = blocks * ceil_div(a.heads, 4) >= 2 * device_compute_units();
     const int64_t groups = wide ? ceil_div(a.heads, 4) : a.heads;
-    if (groups > 65535) return kUnsupportedShape;
+    if (groups > 65535 || !fits_grid(blocks, 256)) return kUnsupportedShape;
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(groups));
     if (wide) hipLaunchKernelGGL((append_pages_kernel<DT, D, 4>), grid, dim3(256), 0, s, a, plan);
     else hipLaunchKernelGGL((append_pages_kernel<DT, D, 1>), grid, dim3(256), 0, s, a, plan);

@@ -587,7 +587,6 @@ template <int DT, int D, int kMode> int launch_join(const WindowArgs& A, int64_t
 template <int DT, int D, int kMode> int launch_mode(const WindowArgs& A, hipStream_t s) {
     const int64_t rows = (kMode == kPaged ? int64_t{1} : int64_t{A.batch}) * A.heads * A.group * A.queries;
     const int64_t blocks = (kMode == kPaged ? int64_t{1} : int64_t{A.batch}) * A.heads * A.tiles * A.splits;
-    if (blocks > 0x7fffffff || rows > 0x7fffffff) return kUnsupportedShape;
     const dim3 grid(static_cast<unsigned>(blocks));
     hipLaunchKernelGGL((window_forward_kernel<DT, D, kMode>), grid, dim3(256), 0, s, A);
     const int status = hipGetLastError();
@@ -608,6 +607,17 @@ int launch(const WindowArgs& A, WindowMode mode, int d, int dtype, hipStream_t s
     return d == 128 ? launch_window<kF16, 128>(A, mode, s) : launch_window<kF16, 64>(A, mode, s);
 }
 
+struct Shape {
+    int64_t tiles, rows, blocks;  // row tiles of a key head, query rows, workgroups
+    int splits;
+};
+
+// Whether the forward's and the join's launches are ones (the rows' number has to be an int as well).
+bool launchable(const Shape& s, int d) {
+    const int64_t join = s.splits == 1 ? 0 : s.splits >= kWideParts ? s.rows : ceil_div(s.rows, 256 / (d / 4));
+    return s.rows <= 0x7fffffff && fits_grid(std::max(s.blocks, join), 256);
+}
+
 // Into how many parts (of at least kPartTiles tiles) the key streams are cut.
 // Items of a few rows (single tokens) are bound by what they read: about four workgroups a slot (two slots a CU) keep
 // the reads even where sequences differ in length. Measured, 128 channels: 32 x 8 heads of one token over up to 7006
@@ -615,10 +625,6 @@ int launch(const WindowArgs& A, WindowMode mode, int d, int dtype, hipStream_t s
 // in 21 (one even round, whose last workgroups read alone), 271 in 64 and 13 for the join.
 // Other items are bound by their products (cut_parts).
 constexpr int kFewRows = 32;
-struct Shape {
-    int64_t tiles, rows, blocks;  // row tiles of a key head, query rows, workgroups
-    int splits;
-};
 // `heads` key heads of `tiles` row tiles, `items` of them with rows, which hold `rows` in all.
 Shape shape_of(int64_t heads, int64_t tiles, int64_t items, int64_t seen_keys, int64_t rows, int d) {
     Shape best{tiles, rows, 0, 1};
@@ -726,7 +732,7 @@ PECO_API int peco_window_attention(const void* q, const void* k, const void* v, 
     A.out_rest = static_cast<uint16_t*>(output_rest);
     if (!aligned(output_rest)) return kInvalidValue;
     const Shape shape = window_shape(batch, q_heads, kv_heads, queries, keys, left, right, sinks, d);
-    if (shape.blocks > 0x7fffffff) return kUnsupportedShape;
+    if (!launchable(shape, d)) return kUnsupportedShape;
     if (workspace_floats(shape, d) > workspace_floats_given) return kWorkspaceTooSmall;
     if (workspace_floats(shape, d) && (!workspace || !aligned(workspace))) return kInvalidValue;
     set_parts(A, shape, workspace, d);
@@ -788,7 +794,7 @@ PECO_API int peco_paged_attention(const void* q, const void* k_pages, const void
     A.pages = pages;
     A.clear_tail = clear_tail;
     const Shape shape = paged_shape(batch, q_heads, kv_heads, tokens, capacity, left, sinks, d);
-    if (shape.blocks > 0x7fffffff) return kUnsupportedShape;
+    if (!launchable(shape, d)) return kUnsupportedShape;
     if (workspace_floats(shape, d) > workspace_floats_given) return kWorkspaceTooSmall;
     if (workspace_floats(shape, d) && (!workspace || !aligned(workspace))) return kInvalidValue;
     set_parts(A, shape, workspace, d);

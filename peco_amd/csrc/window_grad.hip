@@ -692,20 +692,21 @@ GradLayout grad_layout(const GradArgs& A, int d, int dtype) {
 template <int DT, int D> int launch_grad(const GradArgs& A, bool far, hipStream_t s) {
     const int64_t heads = static_cast<int64_t>(A.batch) * A.heads;
     const int64_t dq = heads * A.row_tiles * A.row_parts, dkv = heads * grad_items(A);
-    if (std::max(dq, dkv) > 0x7fffffff || heads * A.v_blocks > 0x7fffffff) return kUnsupportedShape;
+    const int64_t dq_join = A.row_parts > 1 ? ceil_div(heads * A.group * A.queries, 256 / (D / 4)) : 0;
+    const int64_t joined = heads * (A.parts > 1 ? A.key_tiles : A.sink_tiles) * kGradKeys;
+    const int64_t dkv_join = partial_items(A) ? ceil_div(joined, 256 / (D / 2)) : 0;
+    // (Before the first launch: a call runs whole or not at all.)
+    if (!fits_grid(std::max({dq, heads * A.v_blocks, dq_join, dkv_join}), 256) || !fits_grid(dkv, kGradWaves * kWave))
+        return kUnsupportedShape;
     if constexpr (DT == kF16)
         hipLaunchKernelGGL((value_lengths_kernel<D>), dim3(static_cast<unsigned>(heads * A.v_blocks)), dim3(256), 0, s, A);
     if (far) hipLaunchKernelGGL((window_dq_kernel<DT, D, true>), dim3(static_cast<unsigned>(dq)), dim3(256), 0, s, A);
     else hipLaunchKernelGGL((window_dq_kernel<DT, D, false>), dim3(static_cast<unsigned>(dq)), dim3(256), 0, s, A);
-    if (A.row_parts > 1)
-        hipLaunchKernelGGL((window_dq_join_kernel<DT, D>),
-                           dim3(static_cast<unsigned>(ceil_div(heads * A.group * A.queries, 256 / (D / 4)))), dim3(256), 0, s, A);
+    if (dq_join)
+        hipLaunchKernelGGL((window_dq_join_kernel<DT, D>), dim3(static_cast<unsigned>(dq_join)), dim3(256), 0, s, A);
     hipLaunchKernelGGL((window_dkv_kernel<DT, D>), dim3(static_cast<unsigned>(dkv)), dim3(kGradWaves * kWave), 0, s, A);
-    if (partial_items(A)) {
-        const int64_t rows = heads * (A.parts > 1 ? A.key_tiles : A.sink_tiles) * kGradKeys;
-        hipLaunchKernelGGL((window_dkv_join_kernel<DT, D>), dim3(static_cast<unsigned>(ceil_div(rows, 256 / (D / 2)))),
-                           dim3(256), 0, s, A);
-    }
+    if (dkv_join)
+        hipLaunchKernelGGL((window_dkv_join_kernel<DT, D>), dim3(static_cast<unsigned>(dkv_join)), dim3(256), 0, s, A);
     return hipGetLastError();
 }
 
