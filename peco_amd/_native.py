@@ -264,12 +264,19 @@ def plain_tensors(*tensors) -> bool:
         return False
     dual = torch.autograd.forward_ad._current_level >= 0  # (no tensor has a tangent outside a level)
     for t in tensors:
-        if type(t) not in (torch.Tensor, torch.nn.Parameter) or torch._C._functorch.is_functorch_wrapped_tensor(t) or \
-                torch._C._functorch.is_legacy_batchedtensor(t):  # (what a batch of gradients arrives as)
+        if type(t) not in (torch.Tensor, torch.nn.Parameter) or torch._C._functorch.is_functorch_wrapped_tensor(t):
             return False
         if dual and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
             return False
     return True
+
+
+def plain_gradient(t) -> bool:
+    """``plain_tensors`` for the gradient that a backward function is given, which may also be a batch of gradients
+    (``is_grads_batched``)."""
+    import torch
+
+    return plain_tensors(t) and not torch._C._functorch.is_legacy_batchedtensor(t)
 
 
 # hipEventDisableSystemFence (hip_runtime_api.h): the event skips the system-scope cache writeback

@@ -149,7 +149,7 @@ class _RotaryAxes(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        if not _native.plain_tensors(grad):
+        if not _native.plain_gradient(grad):
             raise RuntimeError("the gradient of rotary_axes' output must be an ordinary tensor (no tracing, transforms, "
                                "batches or tangents)")
         return _launch(grad, ctx.saved_tensors[0], ctx.axes, True), None, None

@@ -125,7 +125,7 @@ def _forward(q, k, v, lengths, left, right, sinks, scale, stats):
 
 
 def _backward(q, k, v, out, row_max, row_log, rest, lengths, grad, left, right, sinks, scale):
-    if not _native.plain_tensors(grad):
+    if not _native.plain_gradient(grad):
         raise RuntimeError("the gradient of window_attention's output must be an ordinary tensor (no tracing, transforms, "
                            "batches or tangents)")
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
