@@ -137,30 +137,46 @@ __device__ __forceinline__ void add_rows(f32x16 (&acc)[D / 32], int off, const u
 }
 
 // The same for rows with infinities or NaN that some column hides: a hidden row's weight is 0, but 0 times them is
-// NaN. Each row is multiplied by itself and added where seen(row) holds. The kernels come here only in a second walk
-// over their tiles, after the sums of a first one came out other than finite.
+// NaN. The products take such elements as 0, in add_rows' order, so that columns that hide them come out bit for bit as
+// without them; then the elements of one row after another are multiplied by themselves and added where seen(row) holds.
+// The kernels come here only in a second walk over their tiles, after the sums of a first one came out other than finite.
 template <int DT, int D, typename Seen>
 __device__ __forceinline__ void add_rows_seen(f32x16 (&acc)[D / 32], int off, const uint32_t (&w)[8],
                                               const WinLane<D>& at, int h, const Seen& seen) {
+    auto weights = [&](int kk) {
+        return __builtin_bit_cast(u16x8, u32x4{w[4 * kk], w[4 * kk + 1], w[4 * kk + 2], w[4 * kk + 3]});
+    };
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int nb = 0; nb < D / 32; ++nb) {
+            u16x8 a = at.channels(off + 32 * kk * D, nb);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (not_finite<DT>(a[e])) a[e] = 0;
+            acc[nb] = Mfma<DT>::run(a, weights(kk), acc[nb]);
+            __builtin_amdgcn_sched_barrier(0);  // (one operand at a time: the sums leave few registers)
+        }
 #pragma unroll 1
     for (int row = 0; row < 32; ++row) {
         const bool add = seen(row);
 #pragma unroll
-        for (int nb = 0; nb < D / 32; ++nb) {
-            f32x16 one{};
+        for (int nb = 0; nb < D / 32; ++nb)
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
                 u16x8 a = at.channels(off + 32 * kk * D, nb);
+                bool any = false;
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (16 * kk + 8 * (e / 4) + 4 * h + e % 4 != row) a[e] = 0;
-                const u16x8 b =
-                    __builtin_bit_cast(u16x8, u32x4{w[4 * kk], w[4 * kk + 1], w[4 * kk + 2], w[4 * kk + 3]});
-                one = Mfma<DT>::run(a, b, one);
+                for (int e = 0; e < 8; ++e) {
+                    const bool take = 16 * kk + 8 * (e / 4) + 4 * h + e % 4 == row && not_finite<DT>(a[e]);
+                    if (!take) a[e] = 0;
+                    any |= take;
+                }
+                if (!__any(any)) continue;
+                const f32x16 one = Mfma<DT>::run(a, weights(kk), f32x16{});
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[nb][i] += add ? one[i] : 0.0f;
             }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[nb][i] += add ? one[i] : 0.0f;
-        }
     }
 }
 

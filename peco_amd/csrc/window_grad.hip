@@ -23,6 +23,9 @@
 // Roundings: scores, dP, P and all sums are fp32; P and dS are rounded to the type for the products. delta takes out
 // with what its rounding left: where a query sees a few keys dS is a small difference, and out's rounding alone
 // would put as much error into it as dS's own.
+// Fine calls (fine_call: few keys a query, or little work) go by kernels of their own: weights and dS enter their
+// products as sums of two 16-bit numbers, and the weights' sum and delta are taken anew from fp32 weights by a first
+// walk of dQ's, so that the results' own rounding is what is left.
 // fp16: its smallest normal number, 2^-14, is large for a weight among thousands and for a gradient, so P enters
 // its product times 2^14 and dS times a power of two taken from |dS| <= 2 max|g_i| max|V_j| (lengths of rows); both
 // are divided out of the fp32 sums. bf16 has fp32's exponents and needs neither.
@@ -49,6 +52,8 @@ struct GradArgs {
     const int32_t* lengths;
     const float *row_max, *row_log;  // [batch, query heads, queries]
     float* delta;                    // the same shape
+    bool fine;
+    float* fine_log;                 // fine: log2 of the sums of fp32 weights, the same shape
     int row_tiles, key_tiles, v_blocks;  // tiles of kWinRows rows, of kGradKeys keys, blocks of kWinRows keys
     int row_parts;                       // of every row tile's walk
     float* row_part;                     // dQ of each part [row_parts, query rows, D]
@@ -57,6 +62,14 @@ struct GradArgs {
     int sink_tiles, sink_parts, parts;  // key tiles that hold sinks come first; parts of their walks and of the others'
     float* part;                        // [batch * heads, partial items, kGradKeys, 2, D]
 };
+
+// What the rounding of two packed values left.
+template <int DT> __device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t packed) {
+    return Mfma<DT>::pack2(a - half_to_f32<DT>(static_cast<uint16_t>(packed)),
+                           b - half_to_f32<DT>(static_cast<uint16_t>(packed >> 16)));
+}
+
+enum Walk : int { kPlainWalk, kCarefulWalk, kSumsWalk };
 
 struct Sequence {
     int queries, keys, position0;
@@ -120,7 +133,7 @@ template <int D> __global__ __launch_bounds__(256) void value_lengths_kernel(Gra
     if (threadIdx.x == 0) A.v_long[blockIdx.x] = most;
 }
 
-template <int DT, int D, bool kFar>
+template <int DT, int D, bool kFar, bool kFine>
 __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
     using T = WinTile<D>;
     constexpr int S = D / 16, NB = D / 32;
@@ -187,7 +200,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
     }
     delta += __shfl_xor(delta, 32, kWave);
     if (!takes) delta = 0.0f;
-    if (qvalid && h == 0 && part == 0) A.delta[row_id] = delta;
+    if (!kFine && qvalid && h == 0 && part == 0) A.delta[row_id] = delta;
     float dmul = 1.0f;
     if constexpr (DT == kF16) {
         g2 += __shfl_xor(g2, 32, kWave);
@@ -201,9 +214,11 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
     }
     // (A row that sees nothing has the lowest float and an infinite sum: weights of 0.) fp16: dS's factor is a power of
     // two and goes into its weight's exponent.
-    const float m = A.row_max[row_id], log_l = A.row_log[row_id] - (DT == kF16 ? log2f(dmul) : 0.0f);
+    const float m = A.row_max[row_id];
+    float log_l = A.row_log[row_id];
+    if constexpr (!kFine && DT == kF16) log_l -= log2f(dmul);
     const bool wide = __any(m != -FLT_MAX && fabsf(m * A.scale_log2) > kWideScores);
-    const float offset = wide ? -log_l : __builtin_fmaf(-m, A.scale_log2, -log_l);
+    float offset = wide ? -log_l : __builtin_fmaf(-m, A.scale_log2, -log_l);
 
     const uint16_t* kh = A.k + b * A.ks.b + kvh * A.ks.h;
     const uint16_t* vh = A.v + b * A.vs.b + kvh * A.vs.h;
@@ -221,8 +236,9 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
 #endif
     };
     f32x16 acc[NB];
+    [[maybe_unused]] float sum_p = 0.0f, sum_pdp = 0.0f;
     const WinLane<D> at(lane, kvs[0]);
-    auto compute = [&](auto careful, int t, int buf, int cb) __attribute__((always_inline)) {
+    auto compute = [&](auto kind, int t, int buf, int cb) __attribute__((always_inline)) {
         const int kt = 2 * (buf * T::kElems + 32 * cb * D), vt = kt + 4 * T::kElems;  // bytes from the first tile
         const int r0 = t * kWinTile + 32 * cb;
         if (r0 > w_any || (r0 + 31 < w_from && r0 >= A.sinks)) {
@@ -245,6 +261,16 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) sacc[i] -= m;
         }
+        if constexpr (decltype(kind)::value == kSumsWalk) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[i], A.scale_log2, offset));
+                const bool seen = whole || seen_at(8 * (i / 4) + 4 * h + i % 4);
+                sum_p += seen ? p : 0.0f;
+                sum_pdp += seen ? p * pacc[i] : 0.0f;
+            }
+            return;
+        }
         float ds[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -263,16 +289,24 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
         uint32_t w[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = Mfma<DT>::pack2(ds[2 * i], ds[2 * i + 1]);
-        if constexpr (decltype(careful)::value) {
-            if (!whole && rows_not_finite<DT, D>(kvs[0], kt, lane)) {
-                add_rows_seen<DT, D>(acc, kt, w, at, h, seen_at);
-                return;
+        auto add = [&]() __attribute__((always_inline)) {
+            if constexpr (decltype(kind)::value == kCarefulWalk) {
+                if (!whole && rows_not_finite<DT, D>(kvs[0], kt, lane)) {
+                    add_rows_seen<DT, D>(acc, kt, w, at, h, seen_at);
+                    return;
+                }
             }
+            __builtin_amdgcn_sched_barrier(0);
+            add_rows<DT, D>(acc, kt, w, at);
+        };
+        add();
+        if constexpr (kFine) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = rest2<DT>(ds[2 * i], ds[2 * i + 1], w[i]);
+            add();
         }
-        __builtin_amdgcn_sched_barrier(0);
-        add_rows<DT, D>(acc, kt, w, at);
     };
-    auto walk = [&](auto careful) __attribute__((always_inline)) {
+    auto walk = [&](auto kind) __attribute__((always_inline)) {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) acc[nb] = f32x16{};
         if (tile0 >= tile1) return;
@@ -289,19 +323,19 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
             const int buf = bufc;
             if (t + 1 < tile1) load_tile(t + 1, buf ^ 1);
             if (!wave_active) {
-            } else if constexpr (decltype(careful)::value) {
+            } else if constexpr (decltype(kind)::value != kPlainWalk) {
 #pragma unroll 1
-                for (int cb = 0; cb < 2; ++cb) compute(careful, t, buf, cb);
+                for (int cb = 0; cb < 2; ++cb) compute(kind, t, buf, cb);
             } else {
-                compute(careful, t, buf, 0);
-                compute(careful, t, buf, 1);
+                compute(kind, t, buf, 0);
+                compute(kind, t, buf, 1);
             }
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
             __builtin_amdgcn_s_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
         };
-        if constexpr (decltype(careful)::value) {
+        if constexpr (decltype(kind)::value != kPlainWalk) {
 #pragma unroll 1
             for (int t = tile0; t < tile1; ++t) step((t - tile0) & 1, t);
         } else {
@@ -311,8 +345,26 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
             }
         }
     };
-    walk(std::false_type{});
-    if (__syncthreads_or(wave_active && !all_finite(acc))) walk(std::true_type{});
+    if constexpr (kFine) {
+        // (A walk that is cut is long: its weights' roundings have averaged out in the forward's sum and output.)
+        if (A.row_parts == 1) {
+            walk(std::integral_constant<int, kSumsWalk>{});
+            sum_p += __shfl_xor(sum_p, 32, kWave);
+            sum_pdp += __shfl_xor(sum_pdp, 32, kWave);
+            if (sum_p != 0.0f) {  // (a row that sees nothing keeps its infinite sum)
+                delta = sum_pdp / sum_p;
+                log_l += log2f(sum_p);
+            }
+        }
+        if (qvalid && h == 0 && part == 0) {
+            A.delta[row_id] = delta;
+            A.fine_log[row_id] = log_l;
+        }
+        if constexpr (DT == kF16) log_l -= log2f(dmul);
+        offset = wide ? -log_l : __builtin_fmaf(-m, A.scale_log2, -log_l);
+    }
+    walk(std::integral_constant<int, kPlainWalk>{});
+    if (__syncthreads_or(wave_active && !all_finite(acc))) walk(std::integral_constant<int, kCarefulWalk>{});
     if (!qvalid) return;
     const float mul = A.scale / dmul;
     if (A.row_parts > 1) {
@@ -363,7 +415,7 @@ __host__ __device__ __forceinline__ int64_t partial_items(const GradArgs& A) {
     return A.sink_parts > 1 ? static_cast<int64_t>(A.sink_tiles) * A.sink_parts : 0;
 }
 
-template <int DT, int D>
+template <int DT, int D, bool kFine>
 __global__ __launch_bounds__(kGradWaves * kWave, 2) void window_dkv_kernel(GradArgs A) {
     using T = WinTile<D>;
     constexpr int S = D / 16, NB = D / 32;
@@ -465,7 +517,7 @@ __global__ __launch_bounds__(kGradWaves * kWave, 2) void window_dkv_kernel(GradA
         if (wave < 3 && lane < kTile) {
             const int row = min(first + lane, r_end - 1);
             const int token = A.group == 1 ? row : row / A.group, head = row - token * A.group;
-            const float* from = wave == 0 ? A.row_max : wave == 1 ? A.row_log : A.delta;
+            const float* from = wave == 0 ? A.row_max : wave == 2 ? A.delta : kFine ? A.fine_log : A.row_log;
             dma4(from + stat0 + static_cast<int64_t>(head) * A.queries + token, lds_addr(stat[buf][wave]));
         }
 #endif
@@ -518,6 +570,12 @@ __global__ __launch_bounds__(kGradWaves * kWave, 2) void window_dkv_kernel(GradA
         __builtin_amdgcn_sched_barrier(0);
         if (one_by_one) add_rows_seen<DT, D>(dv, gt, w, at, h, seen_at);
         else add_rows<DT, D>(dv, gt, w, at);
+        if constexpr (kFine) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = rest2<DT>(p[2 * i], p[2 * i + 1], w[i]);
+            if (one_by_one) add_rows_seen<DT, D>(dv, gt, w, at, h, seen_at);
+            else add_rows<DT, D>(dv, gt, w, at);
+        }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int s = 0; s < S; ++s) ds = Mfma<DT>::run(at.rows(gt, s), operands[wave][s][lane], ds);
@@ -544,6 +602,12 @@ __global__ __launch_bounds__(kGradWaves * kWave, 2) void window_dkv_kernel(GradA
         __builtin_amdgcn_sched_barrier(0);
         if (one_by_one) add_rows_seen<DT, D>(dk, qt, w, at, h, seen_at);
         else add_rows<DT, D>(dk, qt, w, at);
+        if constexpr (kFine) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = rest2<DT>(ds[2 * i], ds[2 * i + 1], w[i]);
+            if (one_by_one) add_rows_seen<DT, D>(dk, qt, w, at, h, seen_at);
+            else add_rows<DT, D>(dk, qt, w, at);
+        }
     };
     auto walk = [&](auto careful) __attribute__((always_inline)) {
 #pragma unroll
@@ -640,7 +704,22 @@ template <int DT, int D> __global__ __launch_bounds__(256) void window_dkv_join_
 // tokens in windows of 256 (32, 64 channels) 41 in 2 parts, 30 in 8.
 constexpr int kGradPartTiles = 2;  // of a part at least
 constexpr int kMaxParts = 64;
+
+// Whether a call is a fine one. Roundings of weights, delta and dS leave the gradients 1.4 to 1.5 times as far off as
+// their own rounding does; where a query sees few keys (weights are large, dS is a small difference) or rows are few
+// (nothing averages out) it was up to 2, in a quarter of short sequences above 1.5. Fine calls are at 1.00. Measured,
+// a captured step of forward and gradients, fine against not: 24 heads x 200 tokens 72 and 58 us (195 either way where
+// the host makes the call), 1 x 1000 72 and 67, 24 x 7006 in windows of 32 keys 308 and 256: larger calls only where
+// they need it, with up to 8 keys (at 16 and more the others are below 1.5).
+constexpr int kFineKeys = 8;
+constexpr int64_t kFinePairs = 1 << 20;
+bool fine_call(const GradArgs& A) {
+    const int64_t most = std::min<int64_t>(A.keys, int64_t{A.left} + A.right + 1 + A.sinks);  // keys that a query may see
+    return most <= kFineKeys || int64_t{A.batch} * A.heads * A.group * A.queries <= kFinePairs / most;
+}
+
 void plan_parts(GradArgs& A, int d) {
+    A.fine = fine_call(A);
     A.row_tiles = static_cast<int>(ceil_div(static_cast<int64_t>(A.queries) * A.group, kWinRows));
     A.key_tiles = static_cast<int>(ceil_div(A.keys, kGradKeys));
     A.v_blocks = static_cast<int>(ceil_div(A.keys, kWinRows));
@@ -674,13 +753,14 @@ void plan_parts(GradArgs& A, int d) {
 }
 
 struct GradLayout {
-    int64_t delta, v_long, g_long, part, floats;
+    int64_t fine_log, v_long, g_long, part, floats;  // (delta is at 0)
 };
 GradLayout grad_layout(const GradArgs& A, int d, int dtype) {
     const int64_t heads = static_cast<int64_t>(A.batch) * A.heads;
     auto up = [](int64_t n) { return ceil_div(n, 4) * 4; };
     GradLayout l{};
-    l.v_long = up(heads * A.group * A.queries);
+    l.fine_log = up(heads * A.group * A.queries);
+    l.v_long = l.fine_log * (A.fine ? 2 : 1);
     l.g_long = l.v_long + (dtype == kF16 ? up(heads * A.v_blocks) : 0);
     l.part = l.g_long + (dtype == kF16 ? up(heads * A.row_tiles) : 0);
     // (One after the other: the parts of dQ are joined before the next launch writes its own.)
@@ -689,7 +769,7 @@ GradLayout grad_layout(const GradArgs& A, int d, int dtype) {
     return l;
 }
 
-template <int DT, int D> int launch_grad(const GradArgs& A, bool far, hipStream_t s) {
+template <int DT, int D, bool kFine> int launch_grad(const GradArgs& A, bool far, hipStream_t s) {
     const int64_t heads = static_cast<int64_t>(A.batch) * A.heads;
     const int64_t dq = heads * A.row_tiles * A.row_parts, dkv = heads * grad_items(A);
     const int64_t dq_join = A.row_parts > 1 ? ceil_div(heads * A.group * A.queries, 256 / (D / 4)) : 0;
@@ -700,14 +780,18 @@ template <int DT, int D> int launch_grad(const GradArgs& A, bool far, hipStream_
         return kUnsupportedShape;
     if constexpr (DT == kF16)
         hipLaunchKernelGGL((value_lengths_kernel<D>), dim3(static_cast<unsigned>(heads * A.v_blocks)), dim3(256), 0, s, A);
-    if (far) hipLaunchKernelGGL((window_dq_kernel<DT, D, true>), dim3(static_cast<unsigned>(dq)), dim3(256), 0, s, A);
-    else hipLaunchKernelGGL((window_dq_kernel<DT, D, false>), dim3(static_cast<unsigned>(dq)), dim3(256), 0, s, A);
+    if (far) hipLaunchKernelGGL((window_dq_kernel<DT, D, true, kFine>), dim3(static_cast<unsigned>(dq)), dim3(256), 0, s, A);
+    else hipLaunchKernelGGL((window_dq_kernel<DT, D, false, kFine>), dim3(static_cast<unsigned>(dq)), dim3(256), 0, s, A);
     if (dq_join)
         hipLaunchKernelGGL((window_dq_join_kernel<DT, D>), dim3(static_cast<unsigned>(dq_join)), dim3(256), 0, s, A);
-    hipLaunchKernelGGL((window_dkv_kernel<DT, D>), dim3(static_cast<unsigned>(dkv)), dim3(kGradWaves * kWave), 0, s, A);
+    hipLaunchKernelGGL((window_dkv_kernel<DT, D, kFine>), dim3(static_cast<unsigned>(dkv)), dim3(kGradWaves * kWave), 0, s, A);
     if (dkv_join)
         hipLaunchKernelGGL((window_dkv_join_kernel<DT, D>), dim3(static_cast<unsigned>(dkv_join)), dim3(256), 0, s, A);
     return hipGetLastError();
+}
+
+template <int DT, int D> int launch_type(const GradArgs& A, bool far, hipStream_t s) {
+    return A.fine ? launch_grad<DT, D, true>(A, far, s) : launch_grad<DT, D, false>(A, far, s);
 }
 
 Strides strides_of(const int64_t* s) { return Strides{s[0], s[1], s[2]}; }
@@ -784,11 +868,12 @@ PECO_API int peco_window_attention_grad(const void* q, const void* k, const void
     A.scale = scale;
     A.scale_log2 = static_cast<float>(1.4426950408889634 * static_cast<double>(scale));
     A.delta = workspace;
+    A.fine_log = workspace + l.fine_log;
     A.v_long = workspace + l.v_long;
     A.g_long = workspace + l.g_long;
     A.part = A.row_part = workspace + l.part;
     const bool far = std::max(A.ks.s, A.vs.s) * 2 * keys + 2 * d >= (int64_t{1} << 32);
     const auto s = static_cast<hipStream_t>(stream);
-    if (dtype == kBF16) return d == 128 ? launch_grad<kBF16, 128>(A, far, s) : launch_grad<kBF16, 64>(A, far, s);
-    return d == 128 ? launch_grad<kF16, 128>(A, far, s) : launch_grad<kF16, 64>(A, far, s);
+    if (dtype == kBF16) return d == 128 ? launch_type<kBF16, 128>(A, far, s) : launch_type<kBF16, 64>(A, far, s);
+    return d == 128 ? launch_type<kF16, 128>(A, far, s) : launch_type<kF16, 64>(A, far, s);
 }
