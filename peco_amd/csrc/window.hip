@@ -348,7 +348,7 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
             m_run = m_new;
             // (A query that has seen nothing yet keeps its reference at the lowest value; its weights are all 0.)
             neg_m = m_new == -FLT_MAX ? 0.0f : -m_new * A.scale_log2;
-            wide = __any(fabsf(neg_m) > kWideScores);
+            wide = __any(fabsf(neg_m) > kWideScores);  // (some query of the wave's)
             l_run *= alpha;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
@@ -356,12 +356,12 @@ __global__ __launch_bounds__(256, 2) void window_forward_kernel(WindowArgs A) {
                 for (int i = 0; i < 16; ++i) oacc[nb][i] *= alpha;
         }
         float offset = neg_m;
-        if (wide) {
-            offset = 0.0f;
-            if (m_run != -FLT_MAX) {
+        if (wide) {  // (for the queries that need it: the others' weights keep their bits)
+            const bool own = fabsf(neg_m) > kWideScores;
+            const float reference = own ? m_run : 0.0f;
+            if (own) offset = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) sacc[i] -= m_run;
-            }
+            for (int i = 0; i < 16; ++i) sacc[i] -= reference;
         }
         uint32_t pp[8];
 #pragma unroll

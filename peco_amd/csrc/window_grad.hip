@@ -217,8 +217,8 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
     const float m = A.row_max[row_id];
     float log_l = A.row_log[row_id];
     if constexpr (!kFine && DT == kF16) log_l -= log2f(dmul);
-    const bool wide = __any(m != -FLT_MAX && fabsf(m * A.scale_log2) > kWideScores);
-    float offset = wide ? -log_l : __builtin_fmaf(-m, A.scale_log2, -log_l);
+    const bool own_wide = m != -FLT_MAX && fabsf(m * A.scale_log2) > kWideScores, wide = __any(own_wide);
+    float offset = own_wide ? -log_l : __builtin_fmaf(-m, A.scale_log2, -log_l);
 
     const uint16_t* kh = A.k + b * A.ks.b + kvh * A.ks.h;
     const uint16_t* vh = A.v + b * A.vs.b + kvh * A.vs.h;
@@ -257,9 +257,10 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
             const int r = r0 + row;
             return r <= last_r && (r >= first_r || r < A.sinks);
         };
-        if (wide) {
+        if (wide) {  // (for the queries that need it: the others' weights keep their bits)
+            const float reference = own_wide ? m : 0.0f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sacc[i] -= m;
+            for (int i = 0; i < 16; ++i) sacc[i] -= reference;
         }
         if constexpr (decltype(kind)::value == kSumsWalk) {
 #pragma unroll
@@ -361,7 +362,7 @@ __global__ __launch_bounds__(256, 2) void window_dq_kernel(GradArgs A) {
             A.fine_log[row_id] = log_l;
         }
         if constexpr (DT == kF16) log_l -= log2f(dmul);
-        offset = wide ? -log_l : __builtin_fmaf(-m, A.scale_log2, -log_l);
+        offset = own_wide ? -log_l : __builtin_fmaf(-m, A.scale_log2, -log_l);
     }
     walk(std::integral_constant<int, kPlainWalk>{});
     if (__syncthreads_or(wave_active && !all_finite(acc))) walk(std::integral_constant<int, kCarefulWalk>{});

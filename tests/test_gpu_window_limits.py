@@ -74,3 +74,23 @@ def test_fp16_gradients_beside_an_infinity(which, dim, bad, announce):
         assert torch.equal(part, want[i][:, 1, first:])
         assert torch.equal(got[i][:, 0], want[i][:, 0])
     assert not torch.isfinite(got[0][0, 1, 5]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("size", [float("inf"), 2.0 ** 14])
+@pytest.mark.parametrize("rows,left", [(200, 30), (1500, 800)])  # fine gradients, and not
+def test_a_row_s_neighbours_do_not_change_its_bits(rows, left, size, dtype, announce):
+    """One query is infinite, or so large that its scores take another form of the exponent: the rows beside it, in its
+    tile and in its wavefront, come out bit for bit as they did, and so does their gradient."""
+    announce()
+    gen = torch.Generator().manual_seed(16)
+    q, k, v, g = (torch.randn(1, 2, rows, 64, generator=gen).to(dtype).to(DEV) for _ in range(4))
+    q *= 2
+    changed, at = q.clone(), rows - 77
+    changed[0, 1, at] *= size
+    want, got = (_gradients(t, k, v, g, (left, 0), 3) for t in (q, changed))
+    others = torch.arange(rows, device=DEV) != at
+    assert torch.equal(got[0][:, :, others], want[0][:, :, others])
+    assert torch.equal(got[1][0][:, :, others], want[1][0][:, :, others])
+    assert not torch.equal(got[0][0, 1, at], want[0][0, 1, at])

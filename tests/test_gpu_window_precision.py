@@ -107,11 +107,11 @@ def test_which_calls_are_fine():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dim", [64, 128])
-@pytest.mark.parametrize("bad", [float("nan")])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 @pytest.mark.parametrize("which", range(4))
 @pytest.mark.parametrize("at", [3, 700, 1990])
 def test_values_that_are_not_seen_in_calls_that_are_not_fine(at, which, bad, dim, announce):
-    """A NaN in one row of q, k, v or the gradient reaches the gradients of rows that it meets, and no other
+    """A NaN or infinity in one row of q, k, v or the gradient reaches the gradients of rows that it meets, and no other
     bit of any. 4 x 2000 rows of up to 305 keys."""
     announce()
     gen = torch.Generator().manual_seed(6)
