@@ -346,8 +346,11 @@ int peco_window_attention(const void* q, const void* k, const void* v, void* out
 
 /* Its gradients: dq, dk, dv (of the shapes of q, k, v) from grad, the gradient of output, with the inputs, output,
  * row_max, row_log and output_rest of the forward call. strides: of q, k, v, output, grad, dq, dk, dv (24 values). Written with
- * lengths: every row of dq, dk and dv, 0 behind a sequence's length. workspace:
- * peco_window_attention_grad_workspace_size floats, 16-byte aligned (calls that overlap need one each). */
+ * lengths: every row of dq, dk and dv, 0 behind a sequence's length. Weights and dS are rounded to the dtype for their
+ * products, but not in calls whose queries see at most 8 keys (by left, right, sinks and keys) or of at most 2^20 pairs of
+ * a query and a key. workspace: peco_window_attention_grad_workspace_size floats, 16-byte aligned (calls that overlap
+ * need one each). Like the calls above and below, it returns 20002 before its first launch when a launch would have 2^32
+ * lanes. */
 size_t peco_window_attention_grad_workspace_size(int batch, int q_heads, int kv_heads, int queries, int keys, int left,
                                                  int right, int sinks, int d, int dtype);
 int peco_window_attention_grad(const void* q, const void* k, const void* v, const void* output, const void* grad,

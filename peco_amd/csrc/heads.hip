@@ -19,7 +19,7 @@
 // norm costs a reduction over the row's lanes by DPP moves and no memory pass; as a module of its own
 // it took 118 us per tensor of that shape (0.7 TB/s), the launch with it takes 22 us; the whole
 // double-stream call 1870 -> 1550 us. With axes in place of tables (peco_place_heads_axes) a lane computes its
-// row's four angles itself (rotary.hpp) once for its heads and no table is read: 18.3 us a tensor of that shape (16.8
+// row's four angles itself (rotary.hpp) once for its heads and no table is read: 18.2 us a tensor of that shape (16.8
 // with tables of its own, which stay in the caches when one tensor after another reads them; 13.3 unrotated).
 #include "rotary.hpp"
 

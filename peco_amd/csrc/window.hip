@@ -15,26 +15,26 @@
 // out. Items of at most 64 rows pair the waves: two waves take the same 32 rows and one 32-key half of every
 // tile each, and join their states at the end.
 //
-// Bounds: the exponentials, packing and maxima of the scores take about as long as the two products, so both have to
-// run at the same time: two workgroups a CU, one's products under the other's softmax (registers allow no third).
-// Measured with 128 channels, bf16: 24 heads of 7006 tokens in causal windows of 2026 with 256 sinks 226 us (728
-// TFLOP/s of the products that the mask leaves, the last round of workgroups included; MFMA busy 39% of the time), 3
-// heads of 32896 tokens in windows of 8159 499 us (798 TFLOP/s, 44%; calls one after another run at lower clocks than
-// one alone). A large library product reaches 1252 there. No LDS bank conflicts. Single tokens are bound by the keys'
-// bytes: 119056 keys of 24 heads in 259 us (1.46 GB, 5.6 TB/s).
+// Bounds: a wave's scores, softmax and second product follow one another, and the exponentials, packing and maxima take
+// about as long as the two products. Two workgroups a CU (registers allow no third) cover each other's in part only:
+// MFMA is busy 39 to 44% of the time, waves wait 28 to 31% of theirs. Measured with 128 channels, bf16, calls in a row:
+// 24 heads of 7006 tokens in causal windows of 2026 with 256 sinks 208 us (790 TFLOP/s of the products that the mask
+// leaves, the last round of workgroups included), 3 heads of 32896 tokens in windows of 8159 491 to 536 us (743 to 811
+// TFLOP/s; the clock goes between 1.8 and 2.05 GHz there, 2.3 in the former). A large library product reaches 1252. No
+// LDS bank conflicts. Single tokens are bound by the keys' bytes: 119056 keys of 24 heads in 260 us (1.46 GB, 5.6 TB/s).
 //
 // Where items leave workgroup slots empty, their key streams are cut into `splits` parts, whose unnormalised fp32
 // outputs, references and sums a second launch joins.
 //
 // A value that a query must not see has a weight of 0, but 0 times an infinity or NaN is NaN. A workgroup whose
-// sums come out other than finite takes its item again in a careful walk, which multiplies the rows of halves that are
-// seen in part and hold such values one by one.
+// sums come out other than finite takes its item again in a careful walk, which leaves such values out of the products
+// of halves that are seen in part and adds them row by row where they are seen.
 //
 // Roundings: scores, softmax statistics and O are fp32. P is rounded to the type for the second product (the
 // sum takes the rounded values, so that the weights still add up to 1), out once at the end. Weights are relative to a
 // reference, a score that no other of the row exceeds by more than 2^8 in weight: 16-bit floats round as well at 2^8 as
 // at 1, and O is rescaled where the reference is raised, which after the first tiles is seldom (at every new
-// maximum of any of a wave's 32 rows it was in about every other half of 76, and the first size below took 253 us).
+// maximum of any of a wave's 32 rows it was in about every other half of 76, and the first size above took a tenth longer).
 #include "window.hpp"
 
 #include <algorithm>
@@ -622,7 +622,7 @@ bool launchable(const Shape& s, int d) {
 // Items of a few rows (single tokens) are bound by what they read: about four workgroups a slot (two slots a CU) keep
 // the reads even where sequences differ in length. Measured, 128 channels: 32 x 8 heads of one token over up to 7006
 // keys 176 us uncut, 106 in 8 parts and 5 for the join; one token over 119056 keys, 24 heads, 298 us in 12 parts, 359
-// in 21 (one even round, whose last workgroups read alone), 271 in 64 and 13 for the join.
+// in 21 (one even round, whose last workgroups read alone), 271 in 64 and 13 for the join. (97 and 260 us since.)
 // Other items are bound by their products (cut_parts).
 constexpr int kFewRows = 32;
 // `heads` key heads of `tiles` row tiles, `items` of them with rows, which hold `rows` in all.

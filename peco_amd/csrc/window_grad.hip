@@ -15,10 +15,12 @@
 //       by every later row: their walk is cut into parts, which a third launch adds up in order.
 //
 // S and dP are taken in both launches: seven products where five would do, but no atomics, and no gradient is read
-// again. Measured with 128 channels, bf16, 24 heads of 7006 tokens in causal windows of 2026 with 256 sinks: dQ 261 us
-// (946 TFLOP/s of its three products, MFMA busy 53% of the time), dK/dV 417 us (789 of its four, 45%), its join 7 us.
+// again. Measured with 128 channels, bf16, 24 heads of 7006 tokens in causal windows of 2026 with 256 sinks, calls in a
+// row: dQ 261 us (946 TFLOP/s of its three products, MFMA busy 52% of the time), dK/dV 382 us (861 of its four, 45%), its
+// join 7 us.
 // Neither has LDS bank conflicts; what is left is the waves' waiting for LDS operands and for one another at the tiles'
-// ends. 4 waves of 64 keys, which read half as much from LDS, took 630 us for dK/dV (one wave a SIMD covers nothing).
+// ends. 4 waves of 64 keys, which read half as much from LDS, took half as long again for dK/dV (one wave a SIMD covers
+// nothing).
 //
 // Roundings: scores, dP, P and all sums are fp32; P and dS are rounded to the type for the products. delta takes out
 // with what its rounding left: where a query sees a few keys dS is a small difference, and out's rounding alone

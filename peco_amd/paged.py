@@ -107,7 +107,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     head h reads key head h // (HQ / HK). Keys on a page whose number in ``page_table`` is outside [0, pages) (one
     that left the window and was given back, say) are not seen. A query that sees no key gives 0. ``offsets``
     ascend; ``lengths`` are taken within [0, table's tokens]. Rows of q of no sequence, those behind
-    ``offsets[-1]`` of a padded batch, give 0, or with ``out`` (a tensor like q) are left there as they were.
+    ``offsets[-1]`` of a padded batch, give 0, or with ``out`` (a tensor like q) are left there as they were. Roundings
+    are ``window.window_attention``'s: fp32 but for the weights in their product with V and the result.
     """
     _check_cache(k_pages, v_pages, page_table, offsets, lengths, q, "q")
     tokens, heads, dim = q.shape

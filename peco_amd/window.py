@@ -173,7 +173,14 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window, 
     causal, (n - 1, 0) a causal window of n tokens, (n, n) one to both sides. A query that sees no key gives 0.
     ``lengths`` (int32 [B], needs SQ == SK): valid tokens of each sequence of a right-padded batch; later keys are
     not seen, later rows give 0 and take no gradient, whatever they hold. ``scale`` defaults to 1 / sqrt(D).
-    The result has the strides of ``empty_like(q)``. Differentiable once in Q, K and V. A backward pass may be
+    The result has the strides of ``empty_like(q)``. Scores, softmax statistics and all sums are fp32; the weights
+    are rounded to the dtype for their product with V (fp16: those below 2^-25 of a row's largest add nothing) and the
+    result once. A query whose scores are all -inf gives 0, as one that sees no key.
+
+    Differentiable once in Q, K and V. Weights and dS are rounded to the dtype for their products, which leaves the
+    gradients 1.4 to 1.5 times as far off as their own rounding does; calls whose queries see at most 8 keys, or of at
+    most 2^20 pairs of a query and a key that it may see, keep them at full precision. The gradient of the result must be
+    an ordinary tensor (no batch of gradients, no tangent). A backward pass may be
     captured into a HIP graph while no eager graph of the same leaves is alive (torch's engine would accumulate
     their gradients on that graph's stream and end the process).
     """
