@@ -389,6 +389,56 @@ int peco_append_pages(const void* k, const void* v, void* k_pages, void* v_pages
                       const double* turns, const int* axis_pairs, int axes, int halves, int inverse, int batch,
                       int heads, int tokens, int pages, int page, int table_width, int dims, int dtype, void* stream);
 
+/* Layer norm over the channels of rows. No counterpart in the reference. x and output [n0, n1, n2, channels] (fp16, bf16 or
+ * fp32; channels 1 to 16384, adjacent). strides: host memory, element strides of the three outer axes of x and of output
+ * (6 values). output = (x - mean) / sqrt(variance + eps) * weight + bias, fp32, rounded once; weight and bias
+ * (each nullable) [channels] of x's dtype, or fp32 with wide != 0, with entry_stride 0, else [n0, channels], entry_stride
+ * elements apart, for the rows of each entry of the outermost axis. around_one != 0: 1 + weight in the weight's
+ * place. stats (nullable, fp32 [n0 * n1 * n2, 2]) receives mean and 1 / sqrt(variance + eps) of each row. No alignment is
+ * needed; everything on 16 bytes with channels a multiple of 8 runs fastest. */
+int peco_layer_norm(const void* x, void* output, const int64_t* strides, const void* weight, const void* bias,
+                    int64_t entry_stride, int wide, int around_one, float eps, float* stats, int n0, int n1, int n2,
+                    int channels, int dtype, void* stream);
+
+/* The same rows quantized (from fp32) in place of an output, as peco_quantize_rows does. strides: x's 3. */
+int peco_layer_norm_rows(const void* x, const int64_t* strides, const void* weight, const void* bias,
+                         int64_t entry_stride, int wide, int around_one, float eps, int8_t* codes, int64_t pitch,
+                         float* scales, int n0, int n1, int n2, int channels, int dtype, void* stream);
+
+/* Gradients of peco_layer_norm from grad, the gradient of its output, with the forward's stats: dx (nullable) of x's
+ * shape; dweight and dbias (each nullable) contiguous [channels], or [n0, channels] with per_entry != 0, of the
+ * weight's type (fp32 with wide != 0). strides: of x, grad and dx (9 values). weight null: ones. workspace (dweight or
+ * dbias given): peco_layer_norm_grad_workspace_size floats; calls that overlap need one each. Every sum has a fixed
+ * order. per_entry takes n0 up to 65535. */
+size_t peco_layer_norm_grad_workspace_size(int n0, int n1, int n2, int channels, int per_entry);
+int peco_layer_norm_grad(const void* x, const void* grad, void* dx, const int64_t* strides, const void* weight,
+                         int64_t entry_stride, int wide, int around_one, const float* stats, void* dweight, void* dbias,
+                         int per_entry, float* workspace, size_t workspace_floats, int n0, int n1, int n2, int channels,
+                         int dtype, void* stream);
+
+/* Rows x [n0, n1, n2, channels] (as peco_layer_norm's, strides: 3) in 8 bits: with a the largest magnitude of a row,
+ * codes = rint(x * (127 / a)) and scales = a / 127 in fp32, halves to even. Rows with a < 127 * 2^-126: codes and scale 0.
+ * Rows with an infinity or a NaN: codes 0, scale NaN. codes: int8, rows in order, pitch bytes apart (a multiple of 16,
+ * at least channels; the bytes behind a row's channels are left as they are), on 16 bytes. scales: fp32, one a row. */
+int peco_quantize_rows(const void* x, const int64_t* strides, int8_t* codes, int64_t pitch, float* scales, int n0,
+                       int n1, int n2, int channels, int dtype, void* stream);
+
+/* output [rows, outputs] (dtype, contiguous, on 16 bytes) = sum over channels of codes [rows, channels] * weight [outputs,
+ * channels] (int8, exact in 32 bits: channels < 2^17), times scales [rows] times weight_scales [outputs] plus bias
+ * (nullable, [outputs] of dtype, or fp32 with bias_wide != 0) in fp32, rounded once. Rows of codes and weight start on
+ * 16 bytes, pitch and weight_pitch (up to 2^22) bytes apart; the bytes behind a row's channels, up to the next 16, are read and
+ * count for nothing. */
+int peco_int8_linear(const int8_t* codes, int64_t pitch, const float* scales, const int8_t* weight,
+                     int64_t weight_pitch, const float* weight_scales, const void* bias, int bias_wide, void* output,
+                     int rows, int channels, int outputs, int dtype, void* stream);
+
+/* The same with rows x [n0, n1, n2, channels] of x_dtype quantized first, as by peco_quantize_rows (channels up to 16384).
+ * workspace: rows * (channels rounded up to 16, + 4) bytes, on 16 bytes; calls that overlap need one each. */
+int peco_int8_linear_rows(const void* x, const int64_t* strides, int n0, int n1, int n2, int x_dtype,
+                          const int8_t* weight, int64_t weight_pitch, const float* weight_scales, const void* bias,
+                          int bias_wide, void* output, void* workspace, size_t workspace_bytes, int channels,
+                          int outputs, int dtype, void* stream);
+
 /* peco_sparse_attention without a workspace argument. No counterpart in the reference: it is
  * for callers that cannot allocate device memory (code under HIP graph capture, serving loops
  * that forbid hipMalloc). The work list lives in a static per-device array of 1048576 int32

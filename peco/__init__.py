@@ -9,7 +9,7 @@ import importlib
 import sys
 
 _MODULES = ("processor", "clustering", "quantization", "clustering_cuda", "attention_cuda", "model", "rotary",
-            "window", "paged")
+            "window", "paged", "projection", "norm")
 
 for _name in _MODULES:
     _module = importlib.import_module(f"peco_amd.{_name}")

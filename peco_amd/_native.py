@@ -154,6 +154,13 @@ SIGNATURES = {
     "peco_append_pages": (I, [P] * 4 + [LP, P, ctypes.c_int64, P, P] + PLAN + [I] * 8 + [P]),
     "peco_rotary_axes": (I, [P] + [ctypes.c_int64] * 3 + [P] + [ctypes.c_int64] * 3 + PLAN + [I] * 5 + [P]),
     "peco_place_heads_axes": (I, [P] + [ctypes.c_int64] * 3 + [P] + PLAN + [I, P, ctypes.c_float] + [I] * 7 + [P]),
+    "peco_layer_norm": (I, [P, P, LP, P, P, ctypes.c_int64, I, I, ctypes.c_float, P] + [I] * 5 + [P]),
+    "peco_layer_norm_rows": (I, [P, LP, P, P, ctypes.c_int64, I, I, ctypes.c_float, P, ctypes.c_int64, P] + [I] * 5 + [P]),
+    "peco_layer_norm_grad_workspace_size": (Z, [I] * 5),
+    "peco_layer_norm_grad": (I, [P, P, P, LP, P, ctypes.c_int64, I, I, P, P, P, I, P, Z] + [I] * 5 + [P]),
+    "peco_quantize_rows": (I, [P, LP, P, ctypes.c_int64, P] + [I] * 5 + [P]),
+    "peco_int8_linear": (I, [P, ctypes.c_int64, P, P, ctypes.c_int64, P, P, I, P] + [I] * 4 + [P]),
+    "peco_int8_linear_rows": (I, [P, LP, I, I, I, I, P, ctypes.c_int64, P, P, I, P, P, Z] + [I] * 3 + [P]),
     "peco_base_offset_attention": (I, [P, P, P, I] + [P] * 9 + [I, I] + [P] * 5 + [Z] + [I] * 8 + [P]),
 }
 

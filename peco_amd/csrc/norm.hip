@@ -1,0 +1,269 @@
+// Layer norm over a row's channels, rows quantized to 8 bits, and both at once.
+//
+// Norm: m = sum x / C, v = sum (x - m)^2 / C, r = 1 / sqrt(v + eps), y = (x - m) r f + b with f = w or 1 + w, all in fp32
+// and rounded once to the rows' type. The row is in registers, so its deviations are taken from the mean itself (the
+// difference of E[x^2] and m^2 would cancel for rows far from 0). w and b are one row for all, or one for each entry of
+// the outermost axis (a modulation).
+//
+// Quantized rows: a = max |x|, code = rint(x * (127 / a)), scale = a / 127, in fp32 with IEEE division, halves to even.
+// For 16-bit rows these are the codes of the real quotients: x * 127 / a is 2^-18 or more off any half that it does not
+// meet exactly, and the two roundings move it by 2^-23 of itself. A row whose largest magnitude is below 127 * 2^-126,
+// where the scale would leave the normal numbers, counts as 0 (codes and scale 0). A row with an infinity or a NaN gets
+// codes 0 and a NaN as its scale, which makes its products NaN and no others. The norm's rows are quantized from
+// their fp32 values.
+//
+// HBM-bound: a row is read once and its result written once. Workgroups walk over rows with the next row's loads in flight
+// while one is normalised, and keep the weight in registers for all of their rows.
+#include "rows.hpp"
+
+#include <algorithm>
+
+namespace peco {
+namespace {
+
+enum Mode { kNorm, kNormCodes, kCodes };
+
+struct NormArgs {
+    const void* x;
+    const void *weight, *bias;  // nullable
+    void* out;                  // kNorm
+    float2* stats;              // kNorm, nullable: mean and 1 / deviation of each row
+    int8_t* codes;              // the others
+    float* scales;
+    RowMap from, to;
+    int64_t pitch;              // bytes between rows of codes
+    int64_t entry;              // elements between the weights of two entries, 0: one for all
+    uint32_t rows, entry_rows;
+    int channels, waves, wide, around_one;
+    float eps, inverse_channels;
+};
+
+template <int DT, int L, int kChunks, bool kVec, int kMode>
+__global__ __launch_bounds__(512) void norm_kernel(NormArgs a) {
+    __shared__ uint32_t slots[2][8];
+    constexpr bool kAhead = kVec || kChunks < 4;  // the next row's loads in flight (as registers allow)
+    const int row_lanes = L < kWave ? L : kWave * a.waves;
+    const RowLanes r{static_cast<int>(threadIdx.x) % row_lanes, row_lanes, a.channels};
+    const uint32_t in_group = threadIdx.x / row_lanes, group = blockDim.x / row_lanes, step = gridDim.x * group;
+    RowCombine<L> over{slots, a.waves, static_cast<int>(threadIdx.x / kWave)};
+    float w[kChunks][8], b[kChunks][8];
+    uint32_t held = ~0u;  // the entry that w and b are of
+    if constexpr (kMode != kCodes) {
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[c][k] = 1.0f, b[c][k] = 0.0f;
+    }
+    Chunk<DT> next[kChunks];
+    uint32_t row = blockIdx.x * group + in_group;  // (the workgroup's rows stay together: its barriers are met by all)
+    if (kAhead) load_row<DT, kVec>(next, a.x, a.from.at(min(row, a.rows - 1)), r);
+    for (uint32_t base = blockIdx.x * group; base < a.rows; base += step, row += step) {
+        const uint32_t at = min(row, a.rows - 1);
+        if (!kAhead) load_row<DT, kVec>(next, a.x, a.from.at(at), r);
+        float x[kChunks][8];
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[c][k] = next[c].get(k);
+        if (kAhead && base + step < a.rows)
+            load_row<DT, kVec>(next, a.x, a.from.at(min(row + step, a.rows - 1)), r);
+        if constexpr (kMode != kCodes) {
+            const uint32_t entry = a.entry ? at / a.entry_rows : 0;
+            if (entry != held && (a.weight || a.bias)) {
+                held = entry;
+                if (a.weight) load_weight<DT, kVec>(w, a.weight, entry * a.entry, a.wide, r);
+                if (a.bias) load_weight<DT, kVec>(b, a.bias, entry * a.entry, a.wide, r);
+                if (a.around_one)
+#pragma unroll
+                    for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) w[c][k] += 1.0f;
+            }
+            float sum = 0.0f;
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) sum += x[c][k];
+            const float mean = over.sum(sum) * a.inverse_channels;
+            float squares = 0.0f;
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+                const float here = r.template first<true>(c) < a.channels ? mean : 0.0f;  // (0 behind the row's end)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    x[c][k] -= kVec ? here : r.template column<false>(c, k) < a.channels ? mean : 0.0f;
+                    squares = fmaf(x[c][k], x[c][k], squares);
+                }
+            }
+            const float inverse = 1.0f / sqrtf(over.sum(squares) * a.inverse_channels + a.eps);
+            if (kMode == kNorm && a.stats && r.lane == 0 && row < a.rows) a.stats[row] = make_float2(mean, inverse);
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[c][k] = fmaf(x[c][k] * inverse, w[c][k], b[c][k]);
+        }
+        if constexpr (kMode == kNorm) {
+            if (row < a.rows) {
+                const int64_t to = a.to.at(row);
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c) store_piece<DT, kVec>(round_chunk<DT>(x[c]), a.out, to, c, r);
+            }
+        } else {
+            uint32_t most = 0;  // as bits, whose order is that of the magnitudes with NaN above infinity
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (kVec || r.template column<false>(c, k) < a.channels)
+                        most = max(most, __float_as_uint(x[c][k]) & 0x7fffffffu);
+            most = over.template run<MaxU>(most);
+            const bool finite = most < 0x7f800000u;
+            const float a_max = __uint_as_float(most);
+            const bool zero = a_max < 127.0f * 0x1p-126f;
+            const float by = finite && !zero ? 127.0f / a_max : 0.0f;
+            if (row < a.rows) {
+                if (r.lane == 0) a.scales[row] = !finite ? __uint_as_float(0x7fc00000u) : zero ? 0.0f : a_max / 127.0f;
+                int8_t* to = a.codes + row * a.pitch;
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c) {
+                    int code[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) code[k] = finite ? static_cast<int>(rintf(x[c][k] * by)) : 0;
+                    if constexpr (kVec) {
+                        u32x2 packed{};
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) packed[k / 4] |= (code[k] & 0xffu) << (8 * (k % 4));
+                        const int col = r.template first<true>(c);
+                        if (col < a.channels) *reinterpret_cast<u32x2*>(to + col) = packed;
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const int col = r.template column<false>(c, k);
+                            if (col < a.channels) to[col] = static_cast<int8_t>(code[k]);
+                        }
+                    }
+                }
+            }
+        }
+    }
+}
+
+// Workgroups: enough for every CU to hold what its registers allow (measured over 2 to 16 a CU).
+template <int DT, int L, int kChunks, bool kVec, int kMode>
+int launch(const NormArgs& a, const RowShape& s, hipStream_t stream) {
+    const int64_t blocks = std::min<int64_t>(ceil_div(a.rows, s.rows), 8 * device_compute_units());
+    hipLaunchKernelGGL((norm_kernel<DT, L, kChunks, kVec, kMode>), dim3(static_cast<unsigned>(blocks)),
+                       dim3(s.threads), 0, stream, a);
+    return hipGetLastError();
+}
+
+template <int DT, bool kVec, int kMode> int launch_shape(const NormArgs& a, const RowShape& s, hipStream_t stream) {
+    if (s.lanes == 8) return launch<DT, 8, 1, kVec, kMode>(a, s, stream);
+    if (s.lanes == 16) return launch<DT, 16, 1, kVec, kMode>(a, s, stream);
+    if (s.chunks == 1) return launch<DT, 64, 1, kVec, kMode>(a, s, stream);
+    if (s.chunks == 2) return launch<DT, 64, 2, kVec, kMode>(a, s, stream);
+    return launch<DT, 64, 4, kVec, kMode>(a, s, stream);
+}
+
+template <int kMode> int launch_type(const NormArgs& a, bool vec, int dtype, hipStream_t stream) {
+    const RowShape s = row_shape(a.channels);
+    switch (dtype) {
+        case kBF16: return vec ? launch_shape<kBF16, true, kMode>(a, s, stream) : launch_shape<kBF16, false, kMode>(a, s, stream);
+        case kF16: return vec ? launch_shape<kF16, true, kMode>(a, s, stream) : launch_shape<kF16, false, kMode>(a, s, stream);
+        default: return vec ? launch_shape<kF32, true, kMode>(a, s, stream) : launch_shape<kF32, false, kMode>(a, s, stream);
+    }
+}
+
+// Sizes that every entry takes: kOk, or why not.
+int check_rows(const void* x, const int64_t* strides, int n0, int n1, int n2, int channels, int dtype) {
+    if (!x || !strides || n0 < 1 || n1 < 1 || n2 < 1 || channels < 1) return kInvalidValue;
+    if (channels > kMaxRowChannels || static_cast<int64_t>(n0) * n1 > 0x3fffffff ||
+        static_cast<int64_t>(n0) * n1 * n2 > 0x3fffffff)
+        return kUnsupportedShape;
+    if (dtype != kBF16 && dtype != kF16 && dtype != kF32) return kUnsupportedDtype;
+    return kOk;
+}
+
+void set_rows(NormArgs& a, const void* x, const int64_t* strides, int n0, int n1, int n2, int channels) {
+    a.x = x;
+    a.from = row_map(strides, n0, n1, n2);
+    a.rows = static_cast<uint32_t>(n0) * n1 * n2;
+    a.entry_rows = static_cast<uint32_t>(n1) * n2;
+    a.channels = channels;
+    a.waves = row_shape(channels).waves;
+    a.inverse_channels = 1.0f / static_cast<float>(channels);
+}
+
+void set_affine(NormArgs& a, const void* weight, const void* bias, int64_t entry, int wide, int around_one, float eps) {
+    a.weight = weight;
+    a.bias = bias;
+    a.entry = entry;
+    a.wide = wide;
+    a.around_one = around_one && weight;
+    a.eps = eps;
+}
+
+bool affine_on_16(const void* p, int64_t entry, int size) {
+    return !(reinterpret_cast<uintptr_t>(p) % 16) && !(entry * size % 16);
+}
+
+}  // namespace
+
+int launch_quantize_rows(const void* x, const int64_t* strides, int8_t* codes, int64_t pitch, float* scales, int n0,
+                         int n1, int n2, int channels, int dtype, hipStream_t stream) {
+    if (const int bad = check_rows(x, strides, n0, n1, n2, channels, dtype)) return bad;
+    if (!codes || !scales || pitch < channels || pitch % 16 || reinterpret_cast<uintptr_t>(codes) % 16) return kInvalidValue;
+    NormArgs a{};
+    set_rows(a, x, strides, n0, n1, n2, channels);
+    a.codes = codes;
+    a.scales = scales;
+    a.pitch = pitch;
+    const bool vec = channels % 8 == 0 && rows_on_16(x, strides, dtype == kF32 ? 4 : 2);
+    return launch_type<kCodes>(a, vec, dtype, stream);
+}
+
+}  // namespace peco
+
+using namespace peco;
+
+PECO_API int peco_layer_norm(const void* x, void* output, const int64_t* strides, const void* weight, const void* bias,
+                             int64_t entry_stride, int wide, int around_one, float eps, float* stats, int n0, int n1,
+                             int n2, int channels, int dtype, void* stream) {
+    if (const int bad = check_rows(x, strides, n0, n1, n2, channels, dtype)) return bad;
+    if (!output || entry_stride < 0) return kInvalidValue;
+    NormArgs a{};
+    set_rows(a, x, strides, n0, n1, n2, channels);
+    set_affine(a, weight, bias, entry_stride, wide, around_one, eps);
+    a.out = output;
+    a.to = row_map(strides + 3, n0, n1, n2);
+    a.stats = reinterpret_cast<float2*>(stats);
+    const int size = dtype == kF32 ? 4 : 2, affine = wide ? 4 : size;
+    const bool vec = channels % 8 == 0 && rows_on_16(x, strides, size) && rows_on_16(output, strides + 3, size) &&
+                     affine_on_16(weight, entry_stride, affine) && affine_on_16(bias, entry_stride, affine);
+    return launch_type<kNorm>(a, vec, dtype, static_cast<hipStream_t>(stream));
+}
+
+PECO_API int peco_layer_norm_rows(const void* x, const int64_t* strides, const void* weight, const void* bias,
+                                  int64_t entry_stride, int wide, int around_one, float eps, int8_t* codes,
+                                  int64_t pitch, float* scales, int n0, int n1, int n2, int channels, int dtype,
+                                  void* stream) {
+    if (const int bad = check_rows(x, strides, n0, n1, n2, channels, dtype)) return bad;
+    if (!codes || !scales || entry_stride < 0 || pitch < channels || pitch % 16 || reinterpret_cast<uintptr_t>(codes) % 16)
+        return kInvalidValue;
+    NormArgs a{};
+    set_rows(a, x, strides, n0, n1, n2, channels);
+    set_affine(a, weight, bias, entry_stride, wide, around_one, eps);
+    a.codes = codes;
+    a.scales = scales;
+    a.pitch = pitch;
+    const int size = dtype == kF32 ? 4 : 2, affine = wide ? 4 : size;
+    const bool vec = channels % 8 == 0 && rows_on_16(x, strides, size) &&
+                     affine_on_16(weight, entry_stride, affine) && affine_on_16(bias, entry_stride, affine);
+    return launch_type<kNormCodes>(a, vec, dtype, static_cast<hipStream_t>(stream));
+}
+
+PECO_API int peco_quantize_rows(const void* x, const int64_t* strides, int8_t* codes, int64_t pitch, float* scales,
+                                int n0, int n1, int n2, int channels, int dtype, void* stream) {
+    return launch_quantize_rows(x, strides, codes, pitch, scales, n0, n1, n2, channels, dtype,
+                                static_cast<hipStream_t>(stream));
+}

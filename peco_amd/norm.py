@@ -1,0 +1,196 @@
+"""Layer norm over the channels of rows on gfx950: forward, backward, and with rows that come out in 8 bits.
+
+``layer_norm`` is the norm of a transformer block, with a weight and a bias for all rows or a modulation of each batch
+entry; ``LayerNorm`` is torch's module on it, and ``layer_norm_rows`` quantizes the rows as it makes them, for
+``projection.int8_linear``.
+"""
+from __future__ import annotations
+
+import ctypes
+import functools
+
+import torch
+
+from . import _native
+from .projection import QuantizedRows, empty_codes, outer_axes
+
+_MOST_CHANNELS = 16384
+_LONGS = {n: ctypes.c_int64 * n for n in (3, 6, 9)}
+
+
+def _check(x, weight, bias, eps, around_one, name):
+    if not isinstance(x, torch.Tensor) or x.dim() < 1:
+        raise ValueError(f"{name} expects rows [..., C]")
+    if x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise TypeError(f"{name} supports float16, bfloat16 and float32")
+    channels = x.shape[-1]
+    if not 1 <= channels <= _MOST_CHANNELS:
+        raise ValueError(f"{name} supports rows of 1 to {_MOST_CHANNELS} channels")
+    if not isinstance(eps, (int, float)) or not 0.0 <= eps <= 1e30:
+        raise ValueError("eps must be a nonnegative finite number")
+    if around_one and weight is None:
+        raise ValueError("around_one needs a weight")
+    given = [t for t in (weight, bias) if t is not None]
+    for t in given:
+        if not isinstance(t, torch.Tensor) or t.dtype not in (x.dtype, torch.float32):
+            raise TypeError("weight and bias must be tensors of the rows' dtype or float32")
+        if t.shape != (channels,) and (x.dim() < 2 or t.shape != (x.shape[0], channels)):
+            raise ValueError("weight and bias must have shape [C], or [B, C] with B the rows' first axis")
+        if t.device != x.device:
+            raise ValueError("weight and bias must reside on the device of the rows")
+    if not x.is_cuda:
+        raise ValueError("peco_amd layer norms run on GPU tensors; CPU tensors are not supported")
+    if not _native.plain_tensors(x, *given):
+        raise RuntimeError(f"{name} takes ordinary tensors (no tracing, transforms or tangents)")
+    if x.numel() // channels >= 1 << 30:
+        raise ValueError(f"{name} supports fewer than 2^30 rows")
+    if len(given) == 2 and (weight.dtype != bias.dtype or weight.dim() != bias.dim()):  # one type, one shape
+        weight, bias = weight.float(), bias.float()
+        if weight.dim() != bias.dim():
+            weight, bias = weight.expand(x.shape[0], channels), bias.expand(x.shape[0], channels)
+    return weight, bias
+
+
+def _affine(weight, bias):
+    """(weight, bias, elements between two entries' weights, whether they are fp32) as the kernels take them."""
+    one = bias if weight is None else weight
+    if one is None:
+        return None, None, 0, 0
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    return weight, bias, one.shape[1] if one.dim() == 2 else 0, int(one.dtype == torch.float32)
+
+
+def _channels_adjacent(t):
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def _launch(x, weight, bias, eps, around_one, want_stats):
+    out = torch.empty_like(x)
+    stats = None
+    if x.numel() == 0:
+        return out, stats
+    device = x.device
+    with _native.on_device(device):
+        _native.require_gfx950(device)
+        source, sizes, strides = outer_axes(_channels_adjacent(x))
+        target = out
+        _, _, to = outer_axes(target, copy=False)
+        if to is None or out.stride(-1) != 1:
+            target = torch.empty(x.shape, dtype=x.dtype, device=device)
+            _, _, to = outer_axes(target)
+        if want_stats:
+            stats = torch.empty((x.numel() // x.shape[-1], 2), dtype=torch.float32, device=device)
+        weight, bias, entry, wide = _affine(weight, bias)
+        address = _native.address
+        _native.check(_native.library().peco_layer_norm(
+            source.data_ptr(), target.data_ptr(), _LONGS[6](*strides, *to), address(weight), address(bias), entry, wide,
+            int(around_one), eps, address(stats), *sizes, x.shape[-1], _native.dtype_code(x.dtype),
+            _native.retain(device, source, weight, bias)), "PECO HIP layer norm")
+        return (out if target is out else out.copy_(target)), stats
+
+
+@functools.lru_cache(maxsize=1024)
+def _grad_floats(device_index, *sizes):
+    """The workspace of a gradient call; it depends on the sizes and on the device's compute units alone."""
+    return _native.library().peco_layer_norm_grad_workspace_size(*sizes)
+
+
+def _gradients(x, weight, bias, stats, grad, around_one, needs):
+    """Gradients of x, weight and bias, None where ``needs`` is not set."""
+    if not _native.plain_gradient(grad):
+        raise RuntimeError("the gradient of layer_norm's output must be an ordinary tensor (no tracing, transforms, "
+                           "batches or tangents)")
+    device = x.device
+    dx = torch.empty(x.shape, dtype=x.dtype, device=device) if needs[0] else None
+    dweight, dbias = (torch.empty(t.shape, dtype=t.dtype, device=device) if n else None
+                      for t, n in zip((weight, bias), needs[1:]))
+    if x.numel() == 0:
+        return dx, *(None if t is None else t.zero_() for t in (dweight, dbias))
+    with _native.on_device(device):
+        x, sizes, strides = outer_axes(_channels_adjacent(x))
+        grad, _, by = outer_axes(_channels_adjacent(grad))
+        to = (0, 0, 0) if dx is None else outer_axes(dx)[2]
+        weight, bias, entry, wide = _affine(weight, bias)
+        workspace, floats = None, 0
+        if dweight is not None or dbias is not None:
+            floats = _grad_floats(device.index, *sizes, x.shape[-1], int(entry > 0))
+            workspace = torch.empty(floats, dtype=torch.float32, device=device)
+        address = _native.address
+        _native.check(_native.library().peco_layer_norm_grad(
+            x.data_ptr(), grad.data_ptr(), address(dx), _LONGS[9](*strides, *by, *to), address(weight),
+            entry if weight is not None else 0, wide, int(around_one), stats.data_ptr(), address(dweight),
+            address(dbias), int(entry > 0), address(workspace), floats, *sizes, x.shape[-1],
+            _native.dtype_code(x.dtype), _native.retain(device, x, grad, weight, stats)), "PECO HIP layer norm gradient")
+    return dx, dweight, dbias
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, around_one):
+        out, stats = _launch(x, weight, bias, eps, around_one, True)
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.around_one = around_one
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, weight, bias, stats = ctx.saved_tensors
+        return *_gradients(x, weight, bias, stats, grad, ctx.around_one, ctx.needs_input_grad[:3]), None, None
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+               eps: float = 1e-6, *, around_one: bool = False) -> torch.Tensor:
+    """Rows x [..., C] less their mean, over their deviation sqrt(variance + eps), times the weight, plus the bias.
+
+    fp16, bf16 or fp32 rows of 1 to 16384 channels, any strides (rows whose channels are not adjacent are copied
+    first); the result has the strides of ``empty_like(x)``. Weight and bias have the rows' dtype or float32 and shape
+    [C], or [B, C]: one for each entry of the rows' first axis, as a block's modulation gives them. ``around_one``
+    multiplies with 1 + weight. Statistics and arithmetic are fp32, the result is rounded once. A row with an
+    infinity or a NaN gives NaN and leaves the others as they are.
+
+    Differentiable once in x, weight and bias; all sums of the gradients are fp32 in a fixed order, so they repeat bit for
+    bit. The gradient of the result must be an ordinary tensor (no batch of gradients, no tangent). A backward pass may be
+    captured into a HIP graph while no eager graph of the same leaves is alive (torch's engine would accumulate their
+    gradients on that graph's stream and end the process).
+    """
+    weight, bias = _check(x, weight, bias, eps, around_one, "layer_norm")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        if any(t is not None and t.dim() == 2 for t in (weight, bias)) and x.shape[0] > 65535:
+            raise ValueError("gradients support weights of at most 65535 entries")
+        return _LayerNorm.apply(x, weight, bias, eps, around_one)
+    return _launch(x, weight, bias, eps, around_one, False)[0]
+
+
+def layer_norm_rows(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                    eps: float = 1e-6, *, around_one: bool = False) -> QuantizedRows:
+    """``projection.quantize_rows`` of ``layer_norm``'s rows in one pass, which take their codes from their fp32 values
+    (they are not rounded to x's dtype on the way). For inference: it has no gradient."""
+    weight, bias = _check(x, weight, bias, eps, around_one, "layer_norm_rows")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        raise RuntimeError("layer_norm_rows supports inference only; use torch.no_grad()")
+    codes, scales, pitch = empty_codes(x)
+    if x.numel():
+        device = x.device
+        with _native.on_device(device):
+            _native.require_gfx950(device)
+            x, sizes, strides = outer_axes(_channels_adjacent(x))
+            weight, bias, entry, wide = _affine(weight, bias)
+            _native.check(_native.library().peco_layer_norm_rows(
+                x.data_ptr(), _LONGS[3](*strides), _native.address(weight), _native.address(bias), entry, wide,
+                int(around_one), eps, codes.data_ptr(), pitch, scales.data_ptr(), *sizes, x.shape[-1],
+                _native.dtype_code(x.dtype), _native.retain(device, x, weight, bias)), "PECO HIP layer norm")
+    return QuantizedRows(codes, scales)
+
+
+class LayerNorm(torch.nn.LayerNorm):
+    """``torch.nn.LayerNorm`` over the last axis by ``layer_norm``."""
+
+    def __init__(self, *args, **kwargs):
+        super().__init__(*args, **kwargs)
+        if len(self.normalized_shape) != 1:
+            raise ValueError("LayerNorm normalises over the last axis alone")
+
+    def forward(self, x):
+        return layer_norm(x, self.weight, self.bias, self.eps)
