@@ -24,11 +24,19 @@ template <int OT> __device__ __forceinline__ float load_bias(const ProductArgs& 
     return OT == kF32 || p.bias_wide ? static_cast<const float*>(p.bias)[n] : load_elem<OT>(p.bias, n);
 }
 
+// A result in fp32, the same bits in every kernel: rounded to fp32 before the type (a mixed-precision operation would
+// round once).
+__device__ __forceinline__ float scaled(int32_t sum, float a_scale, float w_scale, float bias) {
+    float v = fmaf(static_cast<float>(sum) * a_scale, w_scale, bias);
+    asm("" : "+v"(v));
+    return v;
+}
+
 // A workgroup's tile: kTokens x kOutputs results over blocks of kBlock channels. Its wavefronts form a grid of kM x kN,
 // each with kMF x kNF products of 32 x 32, and kK of them share those results, each over every kK-th step of 32
 // channels of a block. kStages blocks are in LDS or on their way.
-template <int kM_, int kMF_, int kN_, int kNF_, int kK_, int kBlock_, int kStages_> struct Tile {
-    static constexpr int kM = kM_, kMF = kMF_, kN = kN_, kNF = kNF_, kK = kK_, kBlock = kBlock_, kStages = kStages_;
+template <int kM_, int kMF_, int kN_, int kNF_, int kK_, int kBlock_> struct Tile {
+    static constexpr int kM = kM_, kMF = kMF_, kN = kN_, kNF = kNF_, kK = kK_, kBlock = kBlock_;
     static constexpr int kTokens = kM * kMF * 32, kOutputs = kN * kNF * 32;
     static constexpr int kWaves = kM * kN * kK, kThreads = kWaves * kWave;
     static constexpr int kChunks = kBlock / 16;               // 16-byte chunks of a row of a block
@@ -40,12 +48,13 @@ template <int kM_, int kMF_, int kN_, int kNF_, int kK_, int kBlock_, int kStage
     static constexpr int kPassTiles = kK == 1 ? kNF : 1;      // 32 x 32 results a wavefront stores at once, side by side
     static constexpr int kStoreBytes = kWaves * 32 * (kPassTiles * 32 * 4 + 16);
     static constexpr int kJoinBytes = kK == 1 ? 0 : kWaves * kMF * kNF * 4096;
-    static constexpr int kLds = std::max(std::max(kStages * kStageBytes, kStoreBytes), kJoinBytes);
+    static constexpr int kLds = std::max(std::max(2 * kStageBytes, kStoreBytes), kJoinBytes);
     static_assert(kALoads * kLoadRows * kWaves == kTokens && kWLoads * kLoadRows * kWaves == kOutputs);
     static_assert(kK == 1 || (kK == kMF * kNF && kM == 1 && kN == 1));
     static_assert(kLds + 4 * (kTokens + 2 * kOutputs) <= 160 * 1024);
     // Chunk c of row r of a block lies at place c ^ swizzle(r) of the row.
-    static __device__ __forceinline__ int swizzle(int row) { return row % kChunks; }
+    static __device__ __forceinline__ int swizzle(int row) { return row / kRowsA % kChunks; }
+    static constexpr int kRowsA = kChunks >= 16 ? 1 : 16 / kChunks;
 };
 
 typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
@@ -59,6 +68,12 @@ __device__ __forceinline__ i32x4 chunk_mask(int valid) {
         m[i] = bytes == 4 ? -1 : (1 << (8 * bytes)) - 1;
     }
     return m;
+}
+
+// Waits until at most N loads are on their way, or for all where fewer than that were issued behind the ones needed.
+template <int N> __device__ __forceinline__ void wait_loads(bool some) {
+    if (N > 0 && some) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 // F 32 x 32 results of 32 tokens from m0 and 32 F outputs from n0 on: scaled, turned through LDS (the wavefront's own
@@ -78,7 +93,7 @@ __device__ __forceinline__ void store_results(const ProductArgs& p, const i32x16
             const f32x4 s = *reinterpret_cast<const f32x4*>(w_scale + n), b = *reinterpret_cast<const f32x4*>(bias + n);
             float v[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = fmaf(static_cast<float>(acc[f][4 * g + i]) * a_scale, s[i], b[i]);
+            for (int i = 0; i < 4; ++i) v[i] = scaled(acc[f][4 * g + i], a_scale, s[i], b[i]);
             char* to = span + (lane % 32) * kPitch + n * sizeof(T);
             if constexpr (OT == kF32) *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
             else *reinterpret_cast<u32x2*>(to) = u32x2{Mfma<OT>::pack2(v[0], v[1]), Mfma<OT>::pack2(v[2], v[3])};
@@ -91,7 +106,11 @@ __device__ __forceinline__ void store_results(const ProductArgs& p, const i32x16
         for (int r = 0; r < 32; r += kWave / kRowLanes) {
             const int row = r + lane / kRowLanes, col = lane % kRowLanes * kPer;
             const u32x4 v = *reinterpret_cast<const u32x4*>(span + row * kPitch + col * sizeof(T));
-            if (row < rows && col < columns) *reinterpret_cast<u32x4*>(out + static_cast<int64_t>(row) * p.n + col) = v;
+            if (row < rows && col < columns) {
+                u32x4* to = reinterpret_cast<u32x4*>(out + static_cast<int64_t>(row) * p.n + col);
+                if constexpr (F > 1) __builtin_nontemporal_store(v, to);  // (large results would push operands out of L2)
+                else *to = v;
+            }
         }
     } else {
         for (int e = lane; e < 32 * F * 32; e += kWave) {
@@ -102,12 +121,25 @@ __device__ __forceinline__ void store_results(const ProductArgs& p, const i32x16
     }
 }
 
+// Workgroup i runs on XCD i % 8, each with an L2 of its own: every XCD takes a run of tiles that lie together, in bands of
+// kBand tiles of tokens, so that its 32 CUs share rows and weights.
+constexpr int kBand = 8;
+__device__ __forceinline__ void tile_of(const ProductArgs& p, int& tile_m, int& tile_n) {
+    const int tiles = p.tiles_m * p.tiles_n, per = tiles / kXcdCount, rest = tiles % kXcdCount;
+    const int xcd = blockIdx.x % kXcdCount, t = xcd * per + min(xcd, rest) + static_cast<int>(blockIdx.x) / kXcdCount;
+    const int band = t / (kBand * p.tiles_n), in_band = t - band * kBand * p.tiles_n;
+    const int high = min(kBand, p.tiles_m - band * kBand);
+    tile_m = band * kBand + in_band % high;
+    tile_n = in_band / high;
+}
+
 template <int OT, typename T> __global__ __launch_bounds__(T::kThreads) void product_kernel(ProductArgs p) {
 #if defined(__HIP_DEVICE_COMPILE__)
     __shared__ __align__(128) char lds[T::kLds];
     __shared__ __align__(16) float a_scale[T::kTokens], w_scale[T::kOutputs], bias[T::kOutputs];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int tile_m = blockIdx.x % p.tiles_m, tile_n = blockIdx.x / p.tiles_m;
+    int tile_m, tile_n;
+    tile_of(p, tile_m, tile_n);
     const int m0 = tile_m * T::kTokens, n0 = tile_n * T::kOutputs;
     for (int i = threadIdx.x; i < T::kTokens; i += T::kThreads) a_scale[i] = p.a_scale[min(m0 + i, p.m - 1)];
     for (int i = threadIdx.x; i < T::kOutputs; i += T::kThreads) {
@@ -131,78 +163,97 @@ template <int OT, typename T> __global__ __launch_bounds__(T::kThreads) void pro
     const int8_t *a = p.a + m0 * p.a_pitch, *w = p.w + n0 * p.w_pitch;
     const int blocks = (p.k + T::kBlock - 1) / T::kBlock;
     const uint32_t lds0 = lds_addr(lds) + wave * 1024;
-    const auto load = [&](int block) {
-        const uint32_t to = lds0 + (block % T::kStages) * T::kStageBytes;
+    // Loads [first, last) of this wavefront's share of a block.
+    const auto load = [&](int block, int first, int last) {
+        const uint32_t to = lds0 + (block % 2) * T::kStageBytes;
         const int8_t *from_a = a + block * T::kBlock, *from_w = w + block * T::kBlock;
         const int left = p.k - block * T::kBlock;  // a chunk behind the row's end repeats the block's first
 #pragma unroll
-        for (int i = 0; i < T::kALoads; ++i) {
-            const int row = (i * T::kWaves + wave) * T::kLoadRows + lane / T::kChunks;
+        for (int i = first; i < last; ++i) {
+            const bool of_a = i < T::kALoads;
+            const int own = of_a ? i : i - T::kALoads;
+            const int row = (own * T::kWaves + wave) * T::kLoadRows + lane / T::kChunks;
             const int at = (chunk ^ T::swizzle(row)) * 16;
-            dma16_off(from_a, a_off[i] - (at < left ? 0 : at), to + i * T::kWaves * 1024);
-        }
-#pragma unroll
-        for (int i = 0; i < T::kWLoads; ++i) {
-            const int row = (i * T::kWaves + wave) * T::kLoadRows + lane / T::kChunks;
-            const int at = (chunk ^ T::swizzle(row)) * 16;
-            dma16_off(from_w, w_off[i] - (at < left ? 0 : at), to + T::kTokens * T::kBlock + i * T::kWaves * 1024);
+            dma16_off(of_a ? from_a : from_w, (of_a ? a_off[own] : w_off[own]) - (at < left ? 0 : at),
+                      to + (of_a ? 0 : T::kTokens * T::kBlock) + own * T::kWaves * 1024);
         }
     };
-#pragma unroll
-    for (int s = 0; s < T::kStages - 1; ++s)
-        if (s < blocks) load(s);
+    load(0, 0, T::kLoads);
+    if (blocks > 1) load(1, 0, T::kLoads);
 
     const int in_k = wave % T::kK, in_n = wave / T::kK % T::kN, in_m = wave / T::kK / T::kN;
     const int row = lane % 32, half = lane / 32;
-    const char* a_row = lds + (in_m * T::kMF * 32 + row) * T::kBlock + ((half ^ T::swizzle(row)) * 16);
-    const char* w_row = lds + (T::kTokens + in_n * T::kNF * 32 + row) * T::kBlock + ((half ^ T::swizzle(row)) * 16);
-    const uintptr_t a_at = reinterpret_cast<uintptr_t>(a_row), w_at = reinterpret_cast<uintptr_t>(w_row);
+    const int a_at = (in_m * T::kMF * 32 + row) * T::kBlock + ((half ^ T::swizzle(row)) * 16);
+    const int w_at = (T::kTokens + in_n * T::kNF * 32 + row) * T::kBlock + ((half ^ T::swizzle(row)) * 16);
     i32x16 acc[T::kMF][T::kNF];
 #pragma unroll
     for (int j = 0; j < T::kMF; ++j)
 #pragma unroll
         for (int f = 0; f < T::kNF; ++f) acc[j][f] = i32x16{};
-    const auto multiply = [&](int block, auto last) {
-        const int stage = (block % T::kStages) * T::kStageBytes;
-        i32x4 fa[2][T::kMF], fw[2][T::kNF];
-        const auto read = [&](int s, i32x4(&x)[T::kMF], i32x4(&y)[T::kNF]) {
-            const int step = s * T::kK + in_k;
-            const char* at_a = reinterpret_cast<const char*>((a_at + stage) ^ (step * 32));
-            const char* at_w = reinterpret_cast<const char*>((w_at + stage) ^ (step * 32));
+    // The operands of one step of 32 channels: in `now` while the products use them, the next step's on their way.
+    i32x4 now_a[T::kMF], now_w[T::kNF], next_a[T::kMF], next_w[T::kNF];
+    const auto read = [&](int block, int s) {
+        const int stage = (block % 2) * T::kStageBytes, step = (s * T::kK + in_k) * 32;
 #pragma unroll
-            for (int j = 0; j < T::kMF; ++j) x[j] = *reinterpret_cast<const i32x4*>(at_a + j * 32 * T::kBlock);
+        for (int f = 0; f < T::kNF; ++f)
+            next_w[f] = *reinterpret_cast<const i32x4*>(lds + stage + (w_at ^ step) + f * 32 * T::kBlock);
 #pragma unroll
-            for (int f = 0; f < T::kNF; ++f) y[f] = *reinterpret_cast<const i32x4*>(at_w + f * 32 * T::kBlock);
-            if constexpr (last.value) {
-                const i32x4 mask = chunk_mask(p.k - block * T::kBlock - step * 32 - half * 16);
-#pragma unroll
-                for (int j = 0; j < T::kMF; ++j) x[j] &= mask;
-            }
-        };
-        read(0, fa[0], fw[0]);
-#pragma unroll
-        for (int s = 0; s < T::kSteps; ++s) {
-            __builtin_amdgcn_sched_barrier(0);
-            if (s + 1 < T::kSteps) read(s + 1, fa[(s + 1) % 2], fw[(s + 1) % 2]);
-#pragma unroll
-            for (int j = 0; j < T::kMF; ++j)
-#pragma unroll
-                for (int f = 0; f < T::kNF; ++f)
-                    acc[j][f] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[s % 2][f], fa[s % 2][j], acc[j][f], 0, 0, 0);
-        }
+        for (int j = 0; j < T::kMF; ++j)
+            next_a[j] = *reinterpret_cast<const i32x4*>(lds + stage + (a_at ^ step) + j * 32 * T::kBlock);
     };
-    // A block is there when this wavefront's loads of it and every other's have landed; the barrier also says that the
-    // block before is read, whose place the next loads take.
-    for (int block = 0; block + 1 < blocks; ++block) {
-        if (block + T::kStages - 1 <= blocks) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((T::kStages - 2) * T::kLoads) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (block + T::kStages - 1 < blocks) load(block + T::kStages - 1);
-        multiply(block, std::false_type{});
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const auto advance = [&] {
+#pragma unroll
+        for (int f = 0; f < T::kNF; ++f) now_w[f] = next_w[f];
+#pragma unroll
+        for (int j = 0; j < T::kMF; ++j) now_a[j] = next_a[j];
+    };
+    const auto multiply = [&](int first, int last) {
+#pragma unroll
+        for (int i = first; i < last; ++i)
+            acc[i / T::kNF][i % T::kNF] = __builtin_amdgcn_mfma_i32_32x32x32_i8(now_w[i % T::kNF], now_a[i / T::kNF],
+                                                                               acc[i / T::kNF][i % T::kNF], 0, 0, 0);
+    };
+    constexpr int kProducts = T::kMF * T::kNF;
+    // A block's multiplication. Before its last products, whose operands are in registers: its part of LDS is read by all
+    // behind the barrier and takes the block after the next (kMore: there is one), and the next has landed. The
+    // products cover the barrier, the first reads behind it and the issue of the loads.
+    const auto run_block = [&](int block, auto more) {
+#pragma unroll
+        for (int s = 0; s + 1 < T::kSteps; ++s) {
+            read(block, s + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(0, kProducts);
+            advance();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        read(block + 1, 0);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < kProducts; ++i) {
+            multiply(i, i + 1);
+            if constexpr (more.value) load(block + 2, i * T::kLoads / kProducts, (i + 1) * T::kLoads / kProducts);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        advance();
+    };
+    wait_loads<T::kLoads>(blocks > 1);
     __syncthreads();
-    multiply(blocks - 1, std::true_type{});
+    read(0, 0);
+    advance();
+    for (int block = 0; block + 2 < blocks; ++block) run_block(block, std::true_type{});
+    if (blocks > 1) run_block(blocks - 2, std::false_type{});
+#pragma unroll
+    for (int s = 0; s < T::kSteps; ++s) {
+        if (s + 1 < T::kSteps) read(blocks - 1, s + 1);
+        const i32x4 mask = chunk_mask(p.k - (blocks - 1) * T::kBlock - (s * T::kK + in_k) * 32 - half * 16);
+#pragma unroll
+        for (int j = 0; j < T::kMF; ++j) now_a[j] &= mask;
+        multiply(0, kProducts);
+        if (s + 1 < T::kSteps) advance();
+    }
     __syncthreads();
     if constexpr (T::kK == 1) {
         char* span = lds + wave * (T::kStoreBytes / T::kWaves);
@@ -246,8 +297,133 @@ template <int OT, typename T> __global__ __launch_bounds__(T::kThreads) void pro
 #endif
 }
 
-using Wide = Tile<4, 2, 2, 4, 1, 128, 2>;   // 256 x 256
-using Small = Tile<1, 2, 1, 2, 4, 256, 2>;  // 64 x 64
+using Wide = Tile<2, 4, 4, 2, 1, 128>;   // 256 x 256
+using Small = Tile<1, 2, 1, 2, 4, 256>;  // 64 x 64
+
+// Few rows: the weight is read once, by workgroups of 16 outputs whose 8 wavefronts take segments of 256 channels in turn
+// straight into registers (v_mfma_i32_16x16x64_i8, T products of 16 rows each); their sums meet in LDS. With kFused the
+// rows come as x (of the output's type) and every workgroup quantizes them for itself into LDS while its first part of the
+// weight is on the way, which saves a launch.
+constexpr int kFewWaves = 8, kFewOutputs = 16, kSegment = 256;
+constexpr int kFusedCodes = 16384;  // rows x channels
+
+struct FewRows {
+    const void* x;
+    RowMap from;
+};
+
+__host__ __device__ inline int fused_pitch(int channels) { return (channels + kSegment - 1) / kSegment * kSegment + 16; }
+
+// x's rows as codes into LDS (0 behind a row's end), their scales into `scales`. Each row is taken by 8, 4, 2 or 1
+// wavefronts.
+template <int XT> __device__ __forceinline__ void quantize_into_lds(const ProductArgs& p, const FewRows& in, int8_t* codes,
+                                                                    float* scales, uint32_t* most) {
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, pitch = fused_pitch(p.k);
+    const int share = p.m == 1 ? 8 : p.m == 2 ? 4 : p.m <= 4 ? 2 : 1;  // wavefronts a row
+    const int part = wave % share, stride = share * kWave;
+    for (int row = wave / share; row < p.m; row += kFewWaves / share) {
+        const int64_t at = in.from.at(row);
+        uint32_t top = 0;
+        for (int k = part * kWave + lane; k < p.k; k += stride)
+            top = max(top, __float_as_uint(load_elem<XT>(in.x, at + k)) & 0x7fffffffu);
+        top = combine_lanes<MaxU, kWave>(top);
+        if (lane == 0) most[row * share + part] = top;
+    }
+    __syncthreads();
+    for (int row = wave / share; row < p.m; row += kFewWaves / share) {
+        const int64_t at = in.from.at(row);
+        uint32_t top = most[row * share];
+        for (int i = 1; i < share; ++i) top = max(top, most[row * share + i]);
+        const RowScale s(top);
+        for (int k = part * kWave + lane; k < pitch - 16; k += stride)
+            codes[row * pitch + k] = k < p.k ? static_cast<int8_t>(s.code(load_elem<XT>(in.x, at + k))) : 0;
+        if (part == 0 && lane == 0) scales[row] = s.scale();
+    }
+    __syncthreads();
+}
+
+template <int OT, int T, bool kFused>
+__global__ __launch_bounds__(kFewWaves * kWave) void few_rows_kernel(ProductArgs p, FewRows in) {
+    extern __shared__ __align__(16) int8_t few_codes[];
+    __shared__ __align__(16) int32_t sums[kFewWaves][T][kWave * 4];
+    __shared__ float scales[T * 16];
+    __shared__ uint32_t most[16];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, n0 = blockIdx.x * kFewOutputs;
+    const int row = lane % 16, quarter = lane / 16;
+    const int8_t* w = p.w + min(n0 + row, p.n - 1) * p.w_pitch;
+    const int segments = (p.k + kSegment - 1) / kSegment;
+    i32x4 weight[2][4];
+    const auto load = [&](int segment, i32x4(&to)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = segment * kSegment + i * 64 + quarter * 16;
+            to[i] = *reinterpret_cast<const i32x4*>(w + (at < p.k ? at : 0));  // (what is behind the end meets codes 0)
+        }
+    };
+    if (wave < segments) load(wave, weight[0]);
+    if constexpr (kFused) {
+        quantize_into_lds<OT>(p, in, few_codes, scales, most);
+    } else {
+        for (int i = threadIdx.x; i < T * 16; i += kFewWaves * kWave) scales[i] = p.a_scale[min(i, p.m - 1)];
+    }
+    i32x4 acc[T] = {};
+    const auto multiply = [&](int segment, const i32x4(&by)[4]) {
+        i32x4 a[T][4];
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            const int token = min(t * 16 + row, p.m - 1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at = segment * kSegment + i * 64 + quarter * 16;
+                if constexpr (kFused) a[t][i] = *reinterpret_cast<const i32x4*>(few_codes + token * fused_pitch(p.k) + at);
+                else a[t][i] = *reinterpret_cast<const i32x4*>(p.a + token * p.a_pitch + (at < p.k ? at : 0));
+            }
+        }
+        if (!kFused && (segment + 1) * kSegment > p.k) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const i32x4 mask = chunk_mask(p.k - (segment * kSegment + i * 64 + quarter * 16));
+#pragma unroll
+                for (int t = 0; t < T; ++t) a[t][i] &= mask;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int t = 0; t < T; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(by[i], a[t][i], acc[t], 0, 0, 0);
+    };
+    for (int segment = wave; segment < segments; segment += 2 * kFewWaves) {
+        if (segment + kFewWaves < segments) load(segment + kFewWaves, weight[1]);
+        multiply(segment, weight[0]);
+        if (segment + kFewWaves >= segments) break;
+        if (segment + 2 * kFewWaves < segments) load(segment + 2 * kFewWaves, weight[0]);
+        multiply(segment + kFewWaves, weight[1]);
+    }
+    // Element r of a product: row lane % 16, output 4 (lane / 16) + r.
+#pragma unroll
+    for (int t = 0; t < T; ++t) *reinterpret_cast<i32x4*>(&sums[wave][t][4 * lane]) = acc[t];
+    __syncthreads();
+    for (int e = threadIdx.x; e < T * 256; e += kFewWaves * kWave) {
+        const int token = e / 16, o = e % 16, at = 4 * (token % 16 + 16 * (o / 4)) + o % 4;
+        int32_t sum = 0;
+#pragma unroll
+        for (int i = 0; i < kFewWaves; ++i) sum += sums[i][token / 16][at];
+        const int n = n0 + o;
+        if (token >= p.m || n >= p.n) continue;
+        const float v = scaled(sum, scales[token], p.w_scale[n], load_bias<OT>(p, n));
+        const int64_t to = static_cast<int64_t>(token) * p.n + n;
+        if constexpr (OT == kF32) static_cast<float*>(p.out)[to] = v;
+        else static_cast<uint16_t*>(p.out)[to] = f32_to_half<OT>(v);
+    }
+}
+
+template <int OT, int T, bool kFused> int launch_few(const ProductArgs& p, const FewRows& in, hipStream_t s) {
+    const int64_t blocks = ceil_div(p.n, kFewOutputs);
+    if (!fits_grid(blocks, kFewWaves * kWave)) return kUnsupportedShape;
+    hipLaunchKernelGGL((few_rows_kernel<OT, T, kFused>), dim3(static_cast<unsigned>(blocks)), dim3(kFewWaves * kWave),
+                       kFused ? p.m * fused_pitch(p.k) : 0, s, p, in);
+    return hipGetLastError();
+}
 
 template <int OT, typename T> int launch_product(ProductArgs p, hipStream_t s) {
     p.tiles_m = static_cast<int>(ceil_div(p.m, T::kTokens));
@@ -259,6 +435,9 @@ template <int OT, typename T> int launch_product(ProductArgs p, hipStream_t s) {
 }
 
 template <int OT> int launch_type(const ProductArgs& p, hipStream_t s) {
+    if (p.m <= 16) return launch_few<OT, 1, false>(p, {}, s);
+    if (p.m <= 32) return launch_few<OT, 2, false>(p, {}, s);
+    if (p.m <= 64) return launch_few<OT, 4, false>(p, {}, s);
     const int64_t wide = ceil_div(p.m, Wide::kTokens) * ceil_div(p.n, Wide::kOutputs);
     return 2 * wide > device_compute_units() ? launch_product<OT, Wide>(p, s) : launch_product<OT, Small>(p, s);
 }
@@ -307,15 +486,27 @@ PECO_API int peco_int8_linear_rows(const void* x, const int64_t* strides, int n0
                                    const void* bias, int bias_wide, void* output, void* workspace,
                                    size_t workspace_bytes, int channels, int outputs, int dtype, void* stream) {
     if (!x || !strides || n0 < 1 || n1 < 1 || n2 < 1 || channels < 1) return kInvalidValue;
+    if (x_dtype != kBF16 && x_dtype != kF16 && x_dtype != kF32) return kUnsupportedDtype;
     if (static_cast<int64_t>(n0) * n1 > 0x3fffffff || static_cast<int64_t>(n0) * n1 * n2 > 0x3fffffff) return kUnsupportedShape;
     const int rows = n0 * n1 * n2;
     if (const int bad = check_product(weight, weight_pitch, weight_scales, output, rows, channels, outputs, dtype)) return bad;
+    if (channels > kMaxRowChannels) return kUnsupportedShape;
     const int64_t pitch = ceil_div(channels, 16) * 16;
     if (reinterpret_cast<uintptr_t>(workspace) % 16) return kInvalidValue;
     if (!workspace || workspace_bytes < static_cast<size_t>(rows) * (pitch + 4)) return kWorkspaceTooSmall;
     auto* codes = static_cast<int8_t*>(workspace);
     auto* scales = reinterpret_cast<float*>(codes + rows * pitch);
     const auto s = static_cast<hipStream_t>(stream);
+    if (rows <= 16 && x_dtype == dtype && static_cast<int64_t>(rows) * channels <= kFusedCodes) {
+        const ProductArgs p{nullptr, weight, nullptr, weight_scales, bias, output, 0, weight_pitch, rows, outputs, channels,
+                            bias_wide, 0, 0};
+        const FewRows in{x, row_map(strides, n0, n1, n2)};
+        switch (dtype) {
+            case kBF16: return launch_few<kBF16, 1, true>(p, in, s);
+            case kF16: return launch_few<kF16, 1, true>(p, in, s);
+            default: return launch_few<kF32, 1, true>(p, in, s);
+        }
+    }
     if (const int bad = launch_quantize_rows(x, strides, codes, pitch, scales, n0, n1, n2, channels, x_dtype, s)) return bad;
     const ProductArgs p{codes, weight, scales, weight_scales, bias, output, pitch, weight_pitch, rows, outputs, channels,
                         bias_wide, 0, 0};

@@ -109,7 +109,7 @@ __global__ __launch_bounds__(512) void norm_kernel(NormArgs a) {
                 for (int c = 0; c < kChunks; ++c) store_piece<DT, kVec>(round_chunk<DT>(x[c]), a.out, to, c, r);
             }
         } else {
-            uint32_t most = 0;  // as bits, whose order is that of the magnitudes with NaN above infinity
+            uint32_t most = 0;
 #pragma unroll
             for (int c = 0; c < kChunks; ++c)
 #pragma unroll
@@ -117,18 +117,15 @@ __global__ __launch_bounds__(512) void norm_kernel(NormArgs a) {
                     if (kVec || r.template column<false>(c, k) < a.channels)
                         most = max(most, __float_as_uint(x[c][k]) & 0x7fffffffu);
             most = over.template run<MaxU>(most);
-            const bool finite = most < 0x7f800000u;
-            const float a_max = __uint_as_float(most);
-            const bool zero = a_max < 127.0f * 0x1p-126f;
-            const float by = finite && !zero ? 127.0f / a_max : 0.0f;
+            const RowScale scale(most);
             if (row < a.rows) {
-                if (r.lane == 0) a.scales[row] = !finite ? __uint_as_float(0x7fc00000u) : zero ? 0.0f : a_max / 127.0f;
+                if (r.lane == 0) a.scales[row] = scale.scale();
                 int8_t* to = a.codes + row * a.pitch;
 #pragma unroll
                 for (int c = 0; c < kChunks; ++c) {
                     int code[8];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) code[k] = finite ? static_cast<int>(rintf(x[c][k] * by)) : 0;
+                    for (int k = 0; k < 8; ++k) code[k] = scale.code(x[c][k]);
                     if constexpr (kVec) {
                         u32x2 packed{};
 #pragma unroll

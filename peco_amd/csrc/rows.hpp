@@ -181,6 +181,21 @@ template <int L> struct RowCombine {
     __device__ __forceinline__ float sum(float v) { return __uint_as_float(run<AddF>(__float_as_uint(v))); }
 };
 
+// A row's scale and codes from the bits of its largest magnitude (whose order is that of the magnitudes, with NaN above
+// infinity): see norm.hip.
+struct RowScale {
+    float most, by;
+    bool finite, zero;
+    __device__ __forceinline__ explicit RowScale(uint32_t bits)
+        : most(__uint_as_float(bits)), finite(bits < 0x7f800000u), zero(most < 127.0f * 0x1p-126f) {
+        by = finite && !zero ? 127.0f / most : 0.0f;
+    }
+    __device__ __forceinline__ float scale() const {
+        return !finite ? __uint_as_float(0x7fc00000u) : zero ? 0.0f : most / 127.0f;
+    }
+    __device__ __forceinline__ int code(float x) const { return finite ? static_cast<int>(rintf(x * by)) : 0; }
+};
+
 // How rows of C channels are spread: lanes of a wavefront, pieces a lane, wavefronts a row, threads a workgroup.
 struct RowShape {
     int lanes, chunks, waves, threads, rows;  // rows: of a workgroup
