@@ -218,16 +218,22 @@ def address(t):
     return None if t is None else t.data_ptr()
 
 
+_STREAMS = {}
+
+
 def retain(device, *tensors) -> int:
     """``current_stream`` for callers that time their host work: the stream's handle as an integer. For tensors that
     the caller passed in; one allocated on the current stream in the same call needs no record."""
     import torch
 
-    stream = torch.cuda.current_stream(device)
+    handle = torch._C._cuda_getCurrentRawStream(device.index)
+    stream = _STREAMS.get((device.index, handle))
+    if stream is None:  # (one object a stream: making it costs more than the records)
+        stream = _STREAMS[device.index, handle] = torch.cuda.current_stream(device)
     for t in tensors:
         if t is not None:
             t.record_stream(stream)
-    return stream.cuda_stream
+    return handle
 
 
 class _Here:

@@ -40,11 +40,11 @@ struct NormArgs {
 
 template <int DT, int L, int kChunks, bool kVec, int kMode>
 __global__ __launch_bounds__(512) void norm_kernel(NormArgs a) {
-    __shared__ uint32_t slots[2][8];
+    __shared__ uint32_t slots[2][16];
     constexpr bool kAhead = kVec || kChunks < 4;  // the next row's loads in flight (as registers allow)
     const int row_lanes = L < kWave ? L : kWave * a.waves;
     const RowLanes r{static_cast<int>(threadIdx.x) % row_lanes, row_lanes, a.channels};
-    const uint32_t in_group = threadIdx.x / row_lanes, group = blockDim.x / row_lanes, step = gridDim.x * group;
+    const uint32_t in_group = row_in_group<L>(row_lanes), group = blockDim.x / row_lanes, step = gridDim.x * group;
     RowCombine<L> over{slots, a.waves, static_cast<int>(threadIdx.x / kWave)};
     float w[kChunks][8], b[kChunks][8];
     uint32_t held = ~0u;  // the entry that w and b are of
@@ -54,7 +54,7 @@ __global__ __launch_bounds__(512) void norm_kernel(NormArgs a) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) w[c][k] = 1.0f, b[c][k] = 0.0f;
     }
-    Chunk<DT> next[kChunks];
+    Piece<DT> next[kChunks];
     uint32_t row = blockIdx.x * group + in_group;  // (the workgroup's rows stay together: its barriers are met by all)
     if (kAhead) load_row<DT, kVec>(next, a.x, a.from.at(min(row, a.rows - 1)), r);
     for (uint32_t base = blockIdx.x * group; base < a.rows; base += step, row += step) {
@@ -106,7 +106,7 @@ __global__ __launch_bounds__(512) void norm_kernel(NormArgs a) {
             if (row < a.rows) {
                 const int64_t to = a.to.at(row);
 #pragma unroll
-                for (int c = 0; c < kChunks; ++c) store_piece<DT, kVec>(round_chunk<DT>(x[c]), a.out, to, c, r);
+                for (int c = 0; c < kChunks; ++c) store_piece<DT, kVec>(round_piece<DT>(x[c]), a.out, to, c, r);
             }
         } else {
             uint32_t most = 0;
@@ -162,8 +162,9 @@ template <int DT, bool kVec, int kMode> int launch_shape(const NormArgs& a, cons
     return launch<DT, 64, 4, kVec, kMode>(a, s, stream);
 }
 
-template <int kMode> int launch_type(const NormArgs& a, bool vec, int dtype, hipStream_t stream) {
-    const RowShape s = row_shape(a.channels);
+template <int kMode> int launch_type(NormArgs a, bool vec, int dtype, hipStream_t stream) {
+    const RowShape s = row_shape(a.channels, vec, 4, 4);
+    a.waves = s.waves;
     switch (dtype) {
         case kBF16: return vec ? launch_shape<kBF16, true, kMode>(a, s, stream) : launch_shape<kBF16, false, kMode>(a, s, stream);
         case kF16: return vec ? launch_shape<kF16, true, kMode>(a, s, stream) : launch_shape<kF16, false, kMode>(a, s, stream);
@@ -187,7 +188,6 @@ void set_rows(NormArgs& a, const void* x, const int64_t* strides, int n0, int n1
     a.rows = static_cast<uint32_t>(n0) * n1 * n2;
     a.entry_rows = static_cast<uint32_t>(n1) * n2;
     a.channels = channels;
-    a.waves = row_shape(channels).waves;
     a.inverse_channels = 1.0f / static_cast<float>(channels);
 }
 

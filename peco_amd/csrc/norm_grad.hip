@@ -28,13 +28,13 @@ struct GradArgs {
 };
 
 template <int DT, int L, int kChunks, bool kVec, bool kSums>
-__global__ __launch_bounds__(kGradThreads) void norm_grad_kernel(GradArgs a) {
+__global__ __launch_bounds__(kGradThreads, kChunks == 1 ? 4 : 2) void norm_grad_kernel(GradArgs a) {
     extern __shared__ float joined[];  // a row of sums
-    __shared__ uint32_t slots[2][8];
+    __shared__ uint32_t slots[2][16];
     constexpr bool kAhead = kChunks < 4 || (kVec && DT != kF32);  // the next row's loads in flight (as registers allow)
     const int row_lanes = L < kWave ? L : kWave * a.waves;
     const RowLanes r{static_cast<int>(threadIdx.x) % row_lanes, row_lanes, a.channels};
-    const uint32_t in_group = threadIdx.x / row_lanes, group = kGradThreads / row_lanes, step = a.shares * group;
+    const uint32_t in_group = row_in_group<L>(row_lanes), group = blockDim.x / row_lanes, step = a.shares * group;
     const uint32_t entry = blockIdx.x / a.shares, share = blockIdx.x - entry * a.shares, before = entry * a.entry_rows;
     RowCombine<L> over{slots, a.waves, static_cast<int>(threadIdx.x / kWave)};
     float w[kChunks][8], dw[kSums ? kChunks : 1][8], db[kSums ? kChunks : 1][8];
@@ -56,59 +56,69 @@ __global__ __launch_bounds__(kGradThreads) void norm_grad_kernel(GradArgs a) {
         for (int c = 0; c < kChunks; ++c)
 #pragma unroll
             for (int k = 0; k < 8; ++k) dw[c][k] = db[c][k] = 0.0f;
-    Chunk<DT> next_x[kChunks], next_g[kChunks];
+    Piece<DT> next_x[kChunks], next_g[kChunks];
     float2 next_stats;
     const auto load = [&](uint32_t in_entry) {
         const uint32_t at = before + min(in_entry, a.entry_rows - 1);
         load_row<DT, kVec>(next_x, a.x, a.from.at(at), r);
         load_row<DT, kVec>(next_g, a.grad, a.by.at(at), r);
         next_stats = a.stats[at];
+        if (in_entry >= a.entry_rows)  // adds nothing
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) next_g[c] = Piece<DT>{};
     };
     uint32_t row = share * group + in_group;
     if (kAhead) load(row);
     for (uint32_t base = share * group; base < a.entry_rows; base += step, row += step) {
         if (!kAhead) load(row);
-        float n[kChunks][8], g[kChunks][8];
+        Piece<DT> x[kChunks], g[kChunks];
         const float mean = next_stats.x, inverse = next_stats.y;
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) n[c][k] = next_x[c].get(k), g[c][k] = next_g[c].get(k);
+        for (int c = 0; c < kChunks; ++c) x[c] = next_x[c], g[c] = next_g[c];
         if (kAhead && base + step < a.entry_rows) load(row + step);
+        // n of an element (0 behind the row's end). It is taken from x twice, which costs less than its registers.
+        const auto normal = [&](int c, int k) {
+            const bool inside = (kVec ? r.template first<true>(c) : r.template column<false>(c, k)) < a.channels;
+            return (x[c].get(k) - (inside ? mean : 0.0f)) * inverse;
+        };
         float sum = 0.0f, along = 0.0f;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
-            const float here = r.template first<true>(c) < a.channels ? mean : 0.0f;  // (0 behind the row's end)
+            __builtin_amdgcn_sched_barrier(0);  // (piece by piece, for the registers)
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                n[c][k] = (n[c][k] - (kVec ? here : r.template column<false>(c, k) < a.channels ? mean : 0.0f)) * inverse;
+                const float n = normal(c, k), d = g[c].get(k), scaled = d * w[c][k];
                 if constexpr (kSums) {
-                    if (row < a.entry_rows) {
-                        dw[c][k] = fmaf(g[c][k], n[c][k], dw[c][k]);
-                        db[c][k] += g[c][k];
-                    }
+                    dw[c][k] = fmaf(d, n, dw[c][k]);
+                    db[c][k] += d;
                 }
-                g[c][k] *= w[c][k];
-                sum += g[c][k];
-                along = fmaf(g[c][k], n[c][k], along);
+                sum += scaled;
+                along = fmaf(scaled, n, along);
             }
         }
-        sum = over.sum(sum) * a.inverse_channels;
-        along = over.sum(along) * a.inverse_channels;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) x[c].again(), g[c].again();
+        over.sum2(sum, along);
+        sum *= a.inverse_channels;
+        along *= a.inverse_channels;
         if (row < a.entry_rows && a.dx) {
             const int64_t to = a.to.at(before + row);
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
+                __builtin_amdgcn_sched_barrier(0);
+                float dx[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) g[c][k] = fmaf(-n[c][k], along, g[c][k] - sum) * inverse;
-                store_piece<DT, kVec>(round_chunk<DT>(g[c]), a.dx, to, c, r);
+                for (int k = 0; k < 8; ++k)
+                    dx[k] = fmaf(-normal(c, k), along, g[c].get(k) * w[c][k] - sum) * inverse;
+                store_piece<DT, kVec>(round_piece<DT>(dx), a.dx, to, c, r);
             }
         }
     }
     if constexpr (kSums) {
-        const uint32_t turns = L < kWave ? kGradThreads / kWave : group;      // sets of lanes that hold a row of sums
-        const uint32_t turn = L < kWave ? threadIdx.x / kWave : in_group;
-        const bool first_rows = L == kWave || static_cast<int>(threadIdx.x % kWave) < L;
+        // The sums of the workgroup's sets of lanes side by side in LDS, then column by column.
+        const int sets = L < kWave ? blockDim.x / kWave : group, set = L < kWave ? threadIdx.x / kWave : in_group;
+        const int held = row_lanes * kChunks * 8;
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
             float(&v)[kChunks][8] = which ? db : dw;
@@ -118,20 +128,21 @@ __global__ __launch_bounds__(kGradThreads) void norm_grad_kernel(GradArgs a) {
 #pragma unroll
                     for (int far = L; far < kWave; far *= 2) v[0][k] += wave_shfl_xor(v[0][k], far);
             }
+            __syncthreads();
+            if (L == kWave || static_cast<int>(threadIdx.x % kWave) < L) {
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) joined[set * held + (c * 8 + k) * row_lanes + r.lane] = v[c][k];
+            }
+            __syncthreads();
             float* to = a.parts + (static_cast<int64_t>(blockIdx.x) * 2 + which) * a.channels;
-            for (uint32_t t = 0; t < turns; ++t) {
-                if (turn == t && first_rows) {
-#pragma unroll
-                    for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const int slot = (c * 8 + k) * row_lanes + r.lane, col = r.template column<kVec>(c, k);
-                            const float s = t ? joined[slot] + v[c][k] : v[c][k];
-                            if (t + 1 < turns) joined[slot] = s;
-                            else if (col < a.channels) to[col] = s;
-                        }
-                }
-                __syncthreads();
+            for (int e = threadIdx.x; e < held; e += blockDim.x) {
+                float sum = joined[e];
+                for (int i = 1; i < sets; ++i) sum += joined[i * held + e];
+                const int piece = e / row_lanes, lane = e - piece * row_lanes;
+                const int col = kVec ? (piece / 8 * row_lanes + lane) * 8 + piece % 8 : e;
+                if (col < a.channels) to[col] = sum;
             }
         }
     }
@@ -171,19 +182,20 @@ __global__ __launch_bounds__(kWave * kJoinWaves) void join_sums_kernel(const flo
     to[static_cast<int64_t>(blockIdx.z) * channels + col] = narrow<T>(total);
 }
 
-int grad_rows(const RowShape& s) { return kGradThreads / (s.lanes * s.waves); }
-
-// Shares of an entry's rows. One workgroup of 8 wavefronts a CU where a lane holds 4 pieces (their registers allow no
-// second one), else two; fewer where the rows are few.
+// One piece a lane as long as 8 wavefronts hold the row: two workgroups of 8 wavefronts fit a CU then. Measured over 14012
+// rows of 2048 channels in bf16 (with the second launch): 1 piece 39 us, 2 pieces 42, 4 pieces 39; of 1024 channels 25, 26 and
+// 29; fp32 rows of 2048 72, 83 and 75.
+// Shares of an entry's rows: as many workgroups as fit, fewer where the rows are few.
+RowShape grad_shape(int channels, bool vec) { return row_shape(channels, vec, 1, 8); }
 uint32_t grad_shares(const RowShape& s, int entries, uint32_t entry_rows) {
-    const int64_t blocks = (s.chunks == 4 ? 1 : 2) * device_compute_units();
-    return static_cast<uint32_t>(std::min<int64_t>(std::max<int64_t>(1, blocks / entries), ceil_div(entry_rows, grad_rows(s))));
+    const int64_t blocks = (s.chunks == 1 ? 2 : 1) * device_compute_units();
+    return static_cast<uint32_t>(std::min<int64_t>(std::max<int64_t>(1, blocks / entries), ceil_div(entry_rows, s.rows)));
 }
 
 template <int DT, int L, int kChunks, bool kVec> int launch(const GradArgs& a, const RowShape& s, int entries, hipStream_t st) {
-    const dim3 grid(a.shares * entries), block(kGradThreads);
+    const dim3 grid(a.shares * entries), block(s.threads);
     if (a.parts) {
-        const size_t lds = sizeof(float) * s.lanes * s.waves * kChunks * 8;
+        const size_t lds = sizeof(float) * (s.lanes < kWave ? s.threads / kWave : s.rows) * s.lanes * s.waves * kChunks * 8;
         hipLaunchKernelGGL((norm_grad_kernel<DT, L, kChunks, kVec, true>), grid, block, lds, st, a);
     } else {
         hipLaunchKernelGGL((norm_grad_kernel<DT, L, kChunks, kVec, false>), grid, block, 0, st, a);
@@ -220,7 +232,9 @@ PECO_API size_t peco_layer_norm_grad_workspace_size(int n0, int n1, int n2, int 
     if (!takes(n0, n1, n2, channels) || (per_entry && n0 > 65535)) return 0;
     const int entries = per_entry ? n0 : 1;
     const uint32_t rows = static_cast<uint32_t>(n1) * n2 * (per_entry ? 1 : n0);
-    return static_cast<size_t>(entries) * grad_shares(row_shape(channels), entries, rows) * 2 * channels;
+    const uint32_t shares = std::max(grad_shares(grad_shape(channels, true), entries, rows),
+                                     grad_shares(grad_shape(channels, false), entries, rows));
+    return static_cast<size_t>(entries) * shares * 2 * channels;
 }
 
 PECO_API int peco_layer_norm_grad(const void* x, const void* grad, void* dx, const int64_t* strides, const void* weight,
@@ -235,7 +249,6 @@ PECO_API int peco_layer_norm_grad(const void* x, const void* grad, void* dx, con
     const bool sums = dweight || dbias;
     if (sums && (!workspace || workspace_floats < peco_layer_norm_grad_workspace_size(n0, n1, n2, channels, per_entry)))
         return kWorkspaceTooSmall;
-    const RowShape s = row_shape(channels);
     const int entries = per_entry ? n0 : 1;
     GradArgs a{};
     a.x = x;
@@ -249,9 +262,7 @@ PECO_API int peco_layer_norm_grad(const void* x, const void* grad, void* dx, con
     if (dx) a.to = row_map(strides + 6, n0, n1, n2);
     a.entry = entry_stride;
     a.entry_rows = static_cast<uint32_t>(n1) * n2 * (per_entry ? 1 : n0);
-    a.shares = grad_shares(s, entries, a.entry_rows);
     a.channels = channels;
-    a.waves = s.waves;
     a.wide = wide;
     a.around_one = around_one;
     a.inverse_channels = 1.0f / static_cast<float>(channels);
@@ -259,6 +270,9 @@ PECO_API int peco_layer_norm_grad(const void* x, const void* grad, void* dx, con
     const bool vec = channels % 8 == 0 && rows_on_16(x, strides, size) && rows_on_16(grad, strides + 3, size) &&
                      (!dx || rows_on_16(dx, strides + 6, size)) &&
                      !(reinterpret_cast<uintptr_t>(weight) % 16) && !(entry_stride * affine % 16);
+    const RowShape s = grad_shape(channels, vec);
+    a.shares = grad_shares(s, entries, a.entry_rows);
+    a.waves = s.waves;
     const auto st = static_cast<hipStream_t>(stream);
     int status;
     switch (dtype) {

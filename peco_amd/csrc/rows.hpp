@@ -3,12 +3,10 @@
 //
 // A row of C channels is held in registers by `lanes` lanes, kChunks pieces of 8 channels each: adjacent channels
 // where everything lies on 16 bytes (kVec), else channels `lanes` apart, so that the single loads of a wavefront are
-// adjacent. Rows of up to 512 channels take 8, 16 or 64 lanes with one piece (several rows a wavefront below 64), of up
-// to 2048 one wavefront with 1, 2 or 4 pieces, so that their sums need no barrier; longer ones 2, 4 or 8 wavefronts.
+// adjacent. Short rows share a wavefront; those of one wavefront need no barrier for their sums.
 #pragma once
 
 #include "mfma.hpp"
-#include "rotary.hpp"
 
 #include <type_traits>
 
@@ -43,6 +41,39 @@ inline bool rows_on_16(const void* p, const int64_t* strides, int size) {
     return !(reinterpret_cast<uintptr_t>(p) % 16) && !(((strides[0] | strides[1] | strides[2]) * size) % 16);
 }
 
+// Eight channels as they lie in memory. (Words, not 16-bit elements: the compiler would keep each of those in a register
+// of its own across a loop.)
+template <int DT> struct Piece {
+    static constexpr int kWords = DT == kF32 ? 8 : 4;
+    uint32_t word[kWords];
+    // (A row's start, the same in a wavefront that has one row, and a 32-bit offset: one register for the address.)
+    __device__ __forceinline__ void load(const char* row, uint32_t column) {
+        const u32x4* p = reinterpret_cast<const u32x4*>(row + column * (DT == kF32 ? 4u : 2u));
+#pragma unroll
+        for (int j = 0; j < kWords / 4; ++j) {
+            const u32x4 v = p[j];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) word[4 * j + k] = v[k];
+        }
+    }
+    __device__ __forceinline__ void store(char* row, uint32_t column) const {
+        u32x4* p = reinterpret_cast<u32x4*>(row + column * (DT == kF32 ? 4u : 2u));
+#pragma unroll
+        for (int j = 0; j < kWords / 4; ++j) p[j] = u32x4{word[4 * j], word[4 * j + 1], word[4 * j + 2], word[4 * j + 3]};
+    }
+    __device__ __forceinline__ float get(int k) const {
+        if constexpr (DT == kF32) return __uint_as_float(word[k]);
+        else if constexpr (DT == kBF16) return __uint_as_float(k % 2 ? word[k / 2] & 0xffff0000u : word[k / 2] << 16);
+        else return f16_bits_to_f32(static_cast<uint16_t>(k % 2 ? word[k / 2] >> 16 : word[k / 2]));
+    }
+    // Makes the compiler take the values from the words again where it would keep them.
+    __device__ __forceinline__ void again() {
+        if constexpr (DT != kF32)
+#pragma unroll
+            for (int j = 0; j < kWords; ++j) asm("" : "+v"(word[j]));
+    }
+};
+
 // The lanes of one row: lane of lanes, and the row's length.
 struct RowLanes {
     int lane, lanes, channels;
@@ -56,65 +87,60 @@ struct RowLanes {
 
 // A lane's pieces of the row at `offset` (elements), 0 behind the row's end.
 template <int DT, bool kVec, int kChunks>
-__device__ __forceinline__ void load_row(Chunk<DT> (&x)[kChunks], const void* base, int64_t offset, const RowLanes& r) {
+__device__ __forceinline__ void load_row(Piece<DT> (&x)[kChunks], const void* base, int64_t offset, const RowLanes& r) {
+    const char* row = static_cast<const char*>(base) + offset * (DT == kF32 ? 4 : 2);
     if constexpr (kVec) {
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {  // clamped, unconditional: all loads in flight
-            const int col = r.template first<true>(c);
-            x[c].load(base, offset + min(col, r.channels - 8));
-        }
+        for (int c = 0; c < kChunks; ++c)  // clamped, unconditional: all loads in flight
+            x[c].load(row, min(r.template first<true>(c), r.channels - 8));
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
-            if (r.template first<true>(c) >= r.channels) x[c] = Chunk<DT>{};
+#pragma unroll
+            for (int k = 0; k < Piece<DT>::kWords; ++k)
+                x[c].word[k] = r.template first<true>(c) < r.channels ? x[c].word[k] : 0;
     } else {
-        using T = std::conditional_t<DT == kF32, float, uint16_t>;
+        using T = std::conditional_t<DT == kF32, uint32_t, uint16_t>;
         T v[kChunks][8];
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                v[c][k] = static_cast<const T*>(base)[offset + min(r.template column<false>(c, k), r.channels - 1)];
+                v[c][k] = reinterpret_cast<const T*>(row)[static_cast<uint32_t>(min(r.template column<false>(c, k), r.channels - 1))];
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const T w = r.template column<false>(c, k) < r.channels ? v[c][k] : T{};
-                if constexpr (DT == kF32) x[c].raw[k / 4][k % 4] = w;
-                else x[c].raw[k] = w;
+                const uint32_t w = r.template column<false>(c, k) < r.channels ? v[c][k] : 0;
+                if constexpr (DT == kF32) x[c].word[k] = w;
+                else x[c].word[k / 2] = k % 2 ? x[c].word[k / 2] | w << 16 : w;
             }
     }
 }
 
 // Eight fp32 values rounded to the type.
-template <int DT> __device__ __forceinline__ Chunk<DT> round_chunk(const float (&v)[8]) {
-    Chunk<DT> y;
-    if constexpr (DT == kF32) {
+template <int DT> __device__ __forceinline__ Piece<DT> round_piece(const float (&v)[8]) {
+    Piece<DT> y;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) y.raw[k / 4][k % 4] = v[k];
-    } else {
-        u32x4 p;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) p[k] = Mfma<DT>::pack2(v[2 * k], v[2 * k + 1]);
-        y.raw = __builtin_bit_cast(u16x8, p);
+    for (int k = 0; k < Piece<DT>::kWords; ++k) {
+        if constexpr (DT == kF32) y.word[k] = __float_as_uint(v[k]);
+        else y.word[k] = Mfma<DT>::pack2(v[2 * k], v[2 * k + 1]);
     }
     return y;
 }
 
 template <int DT, bool kVec>
-__device__ __forceinline__ void store_piece(const Chunk<DT>& y, void* base, int64_t offset, int c, const RowLanes& r) {
+__device__ __forceinline__ void store_piece(const Piece<DT>& y, void* base, int64_t offset, int c, const RowLanes& r) {
+    char* row = static_cast<char*>(base) + offset * (DT == kF32 ? 4 : 2);
     if constexpr (kVec) {
         const int col = r.template first<true>(c);
-        if (col < r.channels) y.store(base, offset + col);
+        if (col < r.channels) y.store(row, col);
     } else {
-        using T = std::conditional_t<DT == kF32, float, uint16_t>;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const int col = r.template column<false>(c, k);
-            if constexpr (DT == kF32) {
-                if (col < r.channels) static_cast<T*>(base)[offset + col] = y.raw[k / 4][k % 4];
-            } else {
-                if (col < r.channels) static_cast<T*>(base)[offset + col] = y.raw[k];
-            }
+            if (col >= r.channels) continue;
+            if constexpr (DT == kF32) reinterpret_cast<uint32_t*>(row)[static_cast<uint32_t>(col)] = y.word[k];
+            else reinterpret_cast<uint16_t*>(row)[static_cast<uint32_t>(col)] = static_cast<uint16_t>(k % 2 ? y.word[k / 2] >> 16 : y.word[k / 2]);
         }
     }
 }
@@ -124,14 +150,14 @@ template <int DT, bool kVec, int kChunks>
 __device__ __forceinline__ void load_weight(float (&w)[kChunks][8], const void* base, int64_t offset, bool wide,
                                             const RowLanes& r) {
     if (DT == kF32 || wide) {
-        Chunk<kF32> x[kChunks];
+        Piece<kF32> x[kChunks];
         load_row<kF32, kVec>(x, base, offset, r);
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
 #pragma unroll
             for (int k = 0; k < 8; ++k) w[c][k] = x[c].get(k);
     } else {
-        Chunk<DT> x[kChunks];
+        Piece<DT> x[kChunks];
         load_row<DT, kVec>(x, base, offset, r);
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
@@ -162,10 +188,10 @@ template <typename Op, int L> __device__ __forceinline__ uint32_t combine_lanes(
 }
 
 // The same over rows of `waves` whole wavefronts (every wavefront of the workgroup calls it the same number of times).
-// slots: 2 x 8 words of LDS, used in turn, so that one barrier a call is enough: a wavefront that writes a half again
+// slots: 2 x 16 words of LDS, used in turn, so that one barrier a call is enough: a wavefront that writes a half again
 // has passed the barrier of the call between, before which every wavefront had read it.
 template <int L> struct RowCombine {
-    uint32_t (*slots)[8];
+    uint32_t (*slots)[16];
     int waves, wave, half = 0;
     template <typename Op> __device__ __forceinline__ uint32_t run(uint32_t v) {
         v = combine_lanes<Op, L>(v);
@@ -179,6 +205,24 @@ template <int L> struct RowCombine {
         return v;
     }
     __device__ __forceinline__ float sum(float v) { return __uint_as_float(run<AddF>(__float_as_uint(v))); }
+    __device__ __forceinline__ void sum2(float& a, float& b) {
+        uint32_t u = combine_lanes<AddF, L>(__float_as_uint(a)), v = combine_lanes<AddF, L>(__float_as_uint(b));
+        if (L == kWave && waves > 1) {
+            slots[half][wave] = u;
+            slots[half][8 + wave] = v;
+            __syncthreads();
+            const int first = wave / waves * waves;
+            u = slots[half][first];
+            v = slots[half][8 + first];
+            for (int i = 1; i < waves; ++i) {
+                u = AddF::run(u, slots[half][first + i]);
+                v = AddF::run(v, slots[half][8 + first + i]);
+            }
+            half ^= 1;
+        }
+        a = __uint_as_float(u);
+        b = __uint_as_float(v);
+    }
 };
 
 // A row's scale and codes from the bits of its largest magnitude (whose order is that of the magnitudes, with NaN above
@@ -196,19 +240,30 @@ struct RowScale {
     __device__ __forceinline__ int code(float x) const { return finite ? static_cast<int>(rintf(x * by)) : 0; }
 };
 
-// How rows of C channels are spread: lanes of a wavefront, pieces a lane, wavefronts a row, threads a workgroup.
+// The number of a lane's row among the workgroup's.
+template <int L> __device__ __forceinline__ uint32_t row_in_group(int row_lanes) {
+    const uint32_t row = threadIdx.x / row_lanes;
+    return L == kWave ? __builtin_amdgcn_readfirstlane(row) : row;
+}
+
+// How rows of C channels are spread: lanes of a wavefront, pieces a lane, wavefronts a row, and rows and threads of a
+// workgroup of at most `most_waves`. Rows of more than a wavefront take as many as hold them with `most_chunks` pieces
+// a lane, or 4 for the longest. Single loads (vec false) take one piece a lane as long as 8 wavefronts hold the row: the
+// pieces of eight loads each cost registers, and a row of 1111 channels leaves less of three wavefronts idle.
 struct RowShape {
-    int lanes, chunks, waves, threads, rows;  // rows: of a workgroup
+    int lanes, chunks, waves, threads, rows;
 };
-inline RowShape row_shape(int channels) {
-    RowShape s{kWave, 4, 1, 256, 4};
-    if (channels <= 64) s.lanes = 8, s.chunks = 1;
-    else if (channels <= 128) s.lanes = 16, s.chunks = 1;
-    else if (channels <= 512) s.chunks = 1;
-    else if (channels <= 1024) s.chunks = 2;
-    while (s.waves * s.lanes * s.chunks * 8 < channels) s.waves *= 2;
-    if (s.waves == 8) s.threads = 512;
-    s.rows = s.threads / (s.lanes * s.waves);
+inline RowShape row_shape(int channels, bool vec, int most_chunks, int most_waves) {
+    RowShape s{kWave, 1, 1, 0, 0};
+    if (channels <= 64) s.lanes = 8;
+    else if (channels <= 128) s.lanes = 16;
+    if (!vec) most_chunks = 1;
+    while (s.chunks < most_chunks && s.lanes * s.chunks * 8 < channels) s.chunks *= 2;
+    while (s.chunks < 4 && 8 * s.lanes * s.chunks * 8 < channels) s.chunks *= 2;
+    s.waves = static_cast<int>(ceil_div(channels, s.lanes * s.chunks * 8));
+    if (s.waves > most_waves) most_waves = 8;
+    s.rows = s.lanes < kWave ? most_waves * (kWave / s.lanes) : most_waves / s.waves;
+    s.threads = s.rows * s.waves * s.lanes;
     return s;
 }
 

@@ -102,9 +102,9 @@ def _gradients(x, weight, bias, stats, grad, around_one, needs):
         raise RuntimeError("the gradient of layer_norm's output must be an ordinary tensor (no tracing, transforms, "
                            "batches or tangents)")
     device = x.device
-    dx = torch.empty(x.shape, dtype=x.dtype, device=device) if needs[0] else None
-    dweight, dbias = (torch.empty(t.shape, dtype=t.dtype, device=device) if n else None
-                      for t, n in zip((weight, bias), needs[1:]))
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if needs[0] else None
+    dweight = torch.empty_like(weight, memory_format=torch.contiguous_format) if needs[1] else None
+    dbias = torch.empty_like(bias, memory_format=torch.contiguous_format) if needs[2] else None
     if x.numel() == 0:
         return dx, *(None if t is None else t.zero_() for t in (dweight, dbias))
     with _native.on_device(device):
@@ -134,10 +134,17 @@ class _LayerNorm(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        x, weight, bias, stats = ctx.saved_tensors
-        return *_gradients(x, weight, bias, stats, grad, ctx.around_one, ctx.needs_input_grad[:3]), None, None
+        # (The wrapper costs as much as a launch; without a graph of the gradients it changes nothing.)
+        return _graph_of_gradients(ctx, grad) if torch.is_grad_enabled() else _backward(ctx, grad)
+
+
+def _backward(ctx, grad):
+    x, weight, bias, stats = ctx.saved_tensors
+    return *_gradients(x, weight, bias, stats, grad, ctx.around_one, ctx.needs_input_grad[:3]), None, None
+
+
+_graph_of_gradients = torch.autograd.function.once_differentiable(_backward)
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
