@@ -1,4 +1,5 @@
-"""Installing PECO on a transformer (the peco/model.py interface: install_attention, reset_state).
+"""Installing PECO on a transformer (the peco/model.py interface: install_attention, reset_state); its attention
+projections in 8 bits (quantize_projections).
 
 An installation is one object kept on the transformer. It owns the shared
 ``InferenceContext``, one ``PecoAttention`` per attention block (double-stream blocks first,
@@ -18,6 +19,7 @@ from dataclasses import dataclass, field
 
 import torch
 
+from . import projection
 from .processor import InferenceContext, PecoAttention, PecoConfig
 
 _ATTRIBUTE = "_peco_installation"
@@ -85,3 +87,24 @@ def install_attention(pipe, config: PecoConfig):
 def reset_state(pipe):
     """Forget the step count and every layer's cached centroids (call before each new video)."""
     getattr(pipe.transformer, _ATTRIBUTE).reset()
+
+
+_PROJECTIONS = ("to_q", "to_k", "to_v", "add_q_proj", "add_k_proj", "add_v_proj", "to_add_out")
+
+
+def quantize_projections(pipe):
+    """Put ``projection.Int8Linear`` in the place of every ``torch.nn.Linear`` among the projections of
+    ``pipe.transformer``'s attention blocks (``to_out``'s first layer too); return how many. For inference."""
+    transformer, count = pipe.transformer, 0
+    for block in (*transformer.transformer_blocks, *transformer.single_transformer_blocks):
+        attn = block.attn
+        for name in _PROJECTIONS:
+            layer = getattr(attn, name, None)
+            if type(layer) is torch.nn.Linear:
+                setattr(attn, name, projection.Int8Linear.from_linear(layer))
+                count += 1
+        out = getattr(attn, "to_out", None)
+        if out is not None and len(out) and type(out[0]) is torch.nn.Linear:
+            out[0] = projection.Int8Linear.from_linear(out[0])
+            count += 1
+    return count

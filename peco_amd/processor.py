@@ -25,6 +25,8 @@ from torch.nn.attention import SDPBackend, sdpa_kernel
 from . import _native, clustering_cuda
 from .attention_cuda import base_offset_attention, dense_supported, sparse_attention, sparse_attention_work
 from .attention_cuda import dense_attention as dense_attention_hip
+from .norm import LayerNorm
+from .projection import Int8Linear, QuantizedRows, quantize_rows
 from .quantization import _validate_bits
 from .rotary import RotaryPositions, check_positions, rotary_axes
 
@@ -127,7 +129,7 @@ def _per_channel_norm(norm):
     """True for a norm module that acts on the last axis alone, whatever the axes before it, with
     nothing attached that could see the shape it is called with."""
     hooks = torch.nn.modules.module
-    return type(norm) in (torch.nn.RMSNorm, torch.nn.LayerNorm) and len(norm.normalized_shape) == 1 and \
+    return type(norm) in (torch.nn.RMSNorm, torch.nn.LayerNorm, LayerNorm) and len(norm.normalized_shape) == 1 and \
         "forward" not in vars(norm) and not norm._forward_hooks and not norm._forward_pre_hooks and \
         not hooks._global_forward_hooks and not hooks._global_forward_pre_hooks
 
@@ -201,6 +203,22 @@ def _placeable(part, buffer):
     return part.shape[3] in (64, 128) and part.shape[2] > 0 and part.dtype in (torch.bfloat16, torch.float16) and \
         part.is_cuda and part.stride(3) == 1 and all(s % 8 == 0 for s in part.stride()[:3]) and \
         part.data_ptr() % 16 == 0 and part.shape[0] <= 65535 and _native.plain_tensors(part)
+
+
+def _shared_rows(source, projections):
+    """The rows that the projections of one source take: quantized once where all of them are 8-bit layers (with nothing
+    attached that looks at their input)."""
+    if isinstance(source, torch.Tensor) and all(
+            type(p) is Int8Linear and not p._forward_pre_hooks and not p._forward_hooks for p in projections):
+        return quantize_rows(source)
+    return source
+
+
+def _project(projection, source, rows):
+    """``projection(source)`` on the source's shared rows."""
+    if isinstance(source, torch.Tensor) and isinstance(rows, QuantizedRows):
+        return projection(rows, dtype=source.dtype)
+    return projection(rows)
 
 
 class _FitResult:
@@ -391,7 +409,9 @@ class PecoAttention:
         launch does not take). Video rows get the rotary embedding (``image_rotary_emb``: (cos, sin) tables, or a
         ``rotary.RotaryPositions`` whose angles that launch computes); text rows never do. Double-stream blocks
         (``add_q_proj`` set) project the text with their added projections and norms,
-        single-stream blocks with the same ones as the video.
+        single-stream blocks with the same ones as the video. Where a part's three projections are
+        ``projection.Int8Linear`` layers its rows are quantized once for them; a part may also come as
+        ``projection.QuantizedRows`` then (``norm.layer_norm_rows``).
         """
         rotary = _rotary_function()
         text = 0 if encoder_hidden_states is None else encoder_hidden_states.shape[1]
@@ -409,8 +429,9 @@ class PecoAttention:
         first = 0
         for source, projections, norms, freqs in parts:
             rows = source.shape[1]
+            shared = _shared_rows(source, projections)
             for slot, proj in enumerate(projections):
-                part = proj(source).unflatten(2, (attn.heads, -1)).transpose(1, 2)  # [B, H, rows, D] view
+                part = _project(proj, source, shared).unflatten(2, (attn.heads, -1)).transpose(1, 2)  # [B, H, rows, D] view
                 norm = norms[slot] if slot < 2 else None
                 turn = slot < 2 and freqs is not None
                 size = part.numel() // max(rows, 1) * length

@@ -218,7 +218,8 @@ class Int8Linear(torch.nn.Module):
     """A linear layer in 8 bits, for inference: ``int8_linear`` with a weight that is quantized once.
 
     ``Int8Linear.from_linear(layer)`` takes a ``torch.nn.Linear``'s weight and bias. It takes tensors, or
-    QuantizedRows that several layers share (and then gives the dtype of the layer it was made of).
+    QuantizedRows that several layers share; the result has ``dtype``, else the tensor's or, for QuantizedRows, the dtype
+    of the layer it was made of.
     """
 
     def __init__(self, weight: QuantizedRows, bias: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16):
@@ -242,9 +243,10 @@ class Int8Linear(torch.nn.Module):
         self.scales, self.bias = (None if t is None else t.to(self.codes.device) for t in wide)
         return self
 
-    def forward(self, x):
-        return int8_linear(x, QuantizedRows(self.codes, self.scales), self.bias,
-                           dtype=self.dtype if isinstance(x, QuantizedRows) else x.dtype)
+    def forward(self, x, dtype: torch.dtype | None = None):
+        if dtype is None:
+            dtype = self.dtype if isinstance(x, QuantizedRows) else x.dtype
+        return int8_linear(x, QuantizedRows(self.codes, self.scales), self.bias, dtype=dtype)
 
     def extra_repr(self):
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
