@@ -433,7 +433,9 @@ int peco_int8_linear(const int8_t* codes, int64_t pitch, const float* scales, co
                      int rows, int channels, int outputs, int dtype, void* stream);
 
 /* The same with rows x [n0, n1, n2, channels] of x_dtype quantized first, as by peco_quantize_rows (channels up to 16384).
- * workspace: rows * (channels rounded up to 16, + 4) bytes, on 16 bytes; calls that overlap need one each. */
+ * workspace: peco_int8_linear_rows_workspace_size bytes for rows = n0 * n1 * n2, on 16 bytes; calls that overlap need one
+ * each (may be null when that is 0: a few rows are quantized by the product's own launch). */
+size_t peco_int8_linear_rows_workspace_size(int rows, int channels, int x_dtype, int dtype);
 int peco_int8_linear_rows(const void* x, const int64_t* strides, int n0, int n1, int n2, int x_dtype,
                           const int8_t* weight, int64_t weight_pitch, const float* weight_scales, const void* bias,
                           int bias_wide, void* output, void* workspace, size_t workspace_bytes, int channels,

@@ -160,6 +160,7 @@ SIGNATURES = {
     "peco_layer_norm_grad": (I, [P, P, P, LP, P, ctypes.c_int64, I, I, P, P, P, I, P, Z] + [I] * 5 + [P]),
     "peco_quantize_rows": (I, [P, LP, P, ctypes.c_int64, P] + [I] * 5 + [P]),
     "peco_int8_linear": (I, [P, ctypes.c_int64, P, P, ctypes.c_int64, P, P, I, P] + [I] * 4 + [P]),
+    "peco_int8_linear_rows_workspace_size": (Z, [I] * 4),
     "peco_int8_linear_rows": (I, [P, LP, I, I, I, I, P, ctypes.c_int64, P, P, I, P, P, Z] + [I] * 3 + [P]),
     "peco_base_offset_attention": (I, [P, P, P, I] + [P] * 9 + [I, I] + [P] * 5 + [Z] + [I] * 8 + [P]),
 }

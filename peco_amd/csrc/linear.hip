@@ -298,6 +298,7 @@ template <int OT, typename T> __global__ __launch_bounds__(T::kThreads) void pro
 }
 
 using Wide = Tile<2, 4, 4, 2, 1, 128>;   // 256 x 256
+using Mid = Tile<4, 1, 2, 2, 1, 128>;    // 128 x 128
 using Small = Tile<1, 2, 1, 2, 4, 256>;  // 64 x 64
 
 // Few rows: the weight is read once, by workgroups of 16 outputs whose 8 wavefronts take segments of 256 channels in turn
@@ -434,12 +435,22 @@ template <int OT, typename T> int launch_product(ProductArgs p, hipStream_t s) {
     return hipGetLastError();
 }
 
+// Up to 32 rows the weight's bytes count (32 x 4096 x 4096 7.5 us, with small tiles 9.0; 64 rows so 11.5, with those 9.2).
+// Then the tile of a product. Small ones while a round of them (two workgroups a CU) holds the result: 512 x 4096 x 4096
+// takes 14.4 us with them, 20.7 with middle ones, 1024 x 2048 x 2048 9.4 and 9.6, but 512 x 6144 x 2048 14.8 and 10.3. Else by
+// rounds, in units of a middle tile a CU, which run one behind the other: a round of wide tiles costs as much
+// as 3.2 of them, the last one 2.3 and as much of 0.9 as it fills (2048 x 2048 in the channels: 768 middle tiles 31.4 us, 192
+// wide ones 27.2; 2048 x 4096 x 4096, 512 and 128, 35.9 and 41.7; 7006 x 6144 x 2048, 2640 and 672, 100 and 88).
 template <int OT> int launch_type(const ProductArgs& p, hipStream_t s) {
     if (p.m <= 16) return launch_few<OT, 1, false>(p, {}, s);
     if (p.m <= 32) return launch_few<OT, 2, false>(p, {}, s);
-    if (p.m <= 64) return launch_few<OT, 4, false>(p, {}, s);
-    const int64_t wide = ceil_div(p.m, Wide::kTokens) * ceil_div(p.n, Wide::kOutputs);
-    return 2 * wide > device_compute_units() ? launch_product<OT, Wide>(p, s) : launch_product<OT, Small>(p, s);
+    const int64_t cus = device_compute_units();
+    const auto tiles = [&](int side) { return ceil_div(p.m, side) * ceil_div(p.n, side); };
+    if (tiles(Small::kTokens) <= 2 * cus) return launch_product<OT, Small>(p, s);
+    const double wide = static_cast<double>(tiles(Wide::kTokens)) / cus, rounds = static_cast<double>(static_cast<int64_t>(wide));
+    const double rest = wide - rounds, cost = 3.2 * rounds + (rest > 0.0 ? 2.3 + 0.9 * rest : 0.0);
+    if (cost <= static_cast<double>(tiles(Mid::kTokens)) / cus) return launch_product<OT, Wide>(p, s);
+    return launch_product<OT, Mid>(p, s);
 }
 
 }  // namespace
@@ -481,6 +492,20 @@ PECO_API int peco_int8_linear(const int8_t* codes, int64_t pitch, const float* s
     return run_product(p, dtype, static_cast<hipStream_t>(stream));
 }
 
+namespace {
+
+// Whether the kernel for few rows quantizes them itself.
+bool quantizes_itself(int rows, int channels, int x_dtype, int dtype) {
+    return rows <= 16 && x_dtype == dtype && static_cast<int64_t>(rows) * channels <= kFusedCodes;
+}
+
+}  // namespace
+
+PECO_API size_t peco_int8_linear_rows_workspace_size(int rows, int channels, int x_dtype, int dtype) {
+    if (rows < 1 || channels < 1 || channels > kMaxRowChannels || quantizes_itself(rows, channels, x_dtype, dtype)) return 0;
+    return static_cast<size_t>(rows) * (ceil_div(channels, 16) * 16 + 4);
+}
+
 PECO_API int peco_int8_linear_rows(const void* x, const int64_t* strides, int n0, int n1, int n2, int x_dtype,
                                    const int8_t* weight, int64_t weight_pitch, const float* weight_scales,
                                    const void* bias, int bias_wide, void* output, void* workspace,
@@ -491,13 +516,8 @@ PECO_API int peco_int8_linear_rows(const void* x, const int64_t* strides, int n0
     const int rows = n0 * n1 * n2;
     if (const int bad = check_product(weight, weight_pitch, weight_scales, output, rows, channels, outputs, dtype)) return bad;
     if (channels > kMaxRowChannels) return kUnsupportedShape;
-    const int64_t pitch = ceil_div(channels, 16) * 16;
-    if (reinterpret_cast<uintptr_t>(workspace) % 16) return kInvalidValue;
-    if (!workspace || workspace_bytes < static_cast<size_t>(rows) * (pitch + 4)) return kWorkspaceTooSmall;
-    auto* codes = static_cast<int8_t*>(workspace);
-    auto* scales = reinterpret_cast<float*>(codes + rows * pitch);
     const auto s = static_cast<hipStream_t>(stream);
-    if (rows <= 16 && x_dtype == dtype && static_cast<int64_t>(rows) * channels <= kFusedCodes) {
+    if (quantizes_itself(rows, channels, x_dtype, dtype)) {
         const ProductArgs p{nullptr, weight, nullptr, weight_scales, bias, output, 0, weight_pitch, rows, outputs, channels,
                             bias_wide, 0, 0};
         const FewRows in{x, row_map(strides, n0, n1, n2)};
@@ -507,6 +527,12 @@ PECO_API int peco_int8_linear_rows(const void* x, const int64_t* strides, int n0
             default: return launch_few<kF32, 1, true>(p, in, s);
         }
     }
+    if (!workspace || workspace_bytes < peco_int8_linear_rows_workspace_size(rows, channels, x_dtype, dtype))
+        return kWorkspaceTooSmall;
+    if (reinterpret_cast<uintptr_t>(workspace) % 16) return kInvalidValue;
+    const int64_t pitch = ceil_div(channels, 16) * 16;
+    auto* codes = static_cast<int8_t*>(workspace);
+    auto* scales = reinterpret_cast<float*>(codes + rows * pitch);
     if (const int bad = launch_quantize_rows(x, strides, codes, pitch, scales, n0, n1, n2, channels, x_dtype, s)) return bad;
     const ProductArgs p{codes, weight, scales, weight_scales, bias, output, pitch, weight_pitch, rows, outputs, channels,
                         bias_wide, 0, 0};

@@ -10,6 +10,7 @@ codes 0 and a NaN as its scale, so its products are NaN, and no others.
 from __future__ import annotations
 
 import ctypes
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -123,6 +124,8 @@ def _code_rows(codes):
     """(codes, bytes between rows) as the kernels take them: every row on 16 bytes, a fixed distance apart."""
     stride, shape = codes.stride(), codes.shape
     if stride[-1] == 1 and codes.data_ptr() % 16 == 0:
+        if len(shape) == 2 and stride[0] % 16 == 0 and stride[0] <= 1 << 22:
+            return codes, stride[0]
         pitch, rows = 0, 1
         for n, s in zip(reversed(shape[:-1]), reversed(stride[:-1])):
             if n == 1:
@@ -137,6 +140,11 @@ def _code_rows(codes):
             return codes, pitch
     kept, _, pitch = empty_codes(codes)
     return kept.copy_(codes), pitch
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(*sizes):
+    return _native.library().peco_int8_linear_rows_workspace_size(*sizes)
 
 
 def int8_linear(x, weight: QuantizedRows, bias: torch.Tensor | None = None, *,
@@ -163,25 +171,29 @@ def int8_linear(x, weight: QuantizedRows, bias: torch.Tensor | None = None, *,
     if dtype not in _TYPES:
         raise TypeError("int8_linear gives float16, bfloat16 or float32")
     device = rows.device
-    tensors = (rows, x.scales, weight.codes, weight.scales) if quantized else (rows, weight.codes, weight.scales)
+    tensors = [rows, weight.codes, weight.scales]
+    if quantized:
+        tensors.append(x.scales)
     if bias is not None:
         if not isinstance(bias, torch.Tensor) or bias.dtype not in (dtype, torch.float32):
             raise TypeError("bias must be a tensor of the result's dtype or float32")
         if bias.shape != (outputs,):
             raise ValueError("bias must have shape [N]")
-        tensors = (*tensors, bias)
-    if not rows.is_cuda or any(t.device != device for t in tensors):
-        raise ValueError("All int8_linear inputs must reside on the same GPU device")
+        tensors.append(bias)
+    recording = torch.is_grad_enabled()
+    for t in tensors:
+        if not t.is_cuda or t.device != device:
+            raise ValueError("All int8_linear inputs must reside on the same GPU device")
+        if recording and t.requires_grad:
+            raise RuntimeError("int8_linear supports inference only; use torch.no_grad()")
     if not _native.plain_tensors(*tensors):
         raise RuntimeError("int8_linear takes ordinary tensors (no tracing, transforms or tangents)")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError("int8_linear supports inference only; use torch.no_grad()")
     if quantized:
         if channels > _MOST_PRODUCT:
             raise ValueError(f"int8_linear supports at most {_MOST_PRODUCT} channels")
         if rows.numel() // channels >= 1 << 30:
             raise ValueError("int8_linear supports fewer than 2^30 rows")
-    else:
+    elif channels > _MOST_CHANNELS or rows.numel() // channels >= 1 << 30 or x.dtype not in _TYPES:
         _check_rows(x, "int8_linear")
     if outputs >= 1 << 30:
         raise ValueError("int8_linear supports fewer than 2^30 outputs")
@@ -204,12 +216,12 @@ def int8_linear(x, weight: QuantizedRows, bias: torch.Tensor | None = None, *,
                 _native.retain(device, codes, scales, weight_codes, weight_scales, bias))
         else:
             x, sizes, strides = outer_axes(x if x.stride(-1) == 1 else x.contiguous())
-            pitch = -(-channels // 16) * 16
-            workspace = torch.empty(count * (pitch + 4), dtype=torch.int8, device=device)
+            codes = _native.dtype_code(x.dtype), _native.dtype_code(dtype)
+            size = _workspace_bytes(count, channels, *codes)
+            workspace = torch.empty(size, dtype=torch.int8, device=device) if size else None
             status = _native.library().peco_int8_linear_rows(
-                x.data_ptr(), _LONG3(*strides), *sizes, _native.dtype_code(x.dtype), *common, workspace.data_ptr(),
-                workspace.numel(), channels, outputs, _native.dtype_code(dtype),
-                _native.retain(device, x, weight_codes, weight_scales, bias))
+                x.data_ptr(), _LONG3(*strides), *sizes, codes[0], *common, _native.address(workspace), size, channels,
+                outputs, codes[1], _native.retain(device, x, weight_codes, weight_scales, bias))
         _native.check(status, "PECO HIP 8-bit projection")
     return out
 
