@@ -113,10 +113,17 @@ __device__ __forceinline__ void store_results(const ProductArgs& p, const i32x16
             }
         }
     } else {
-        for (int e = lane; e < 32 * F * 32; e += kWave) {
-            const int row = e / (F * 32), col = e % (F * 32);
-            const T v = *reinterpret_cast<const T*>(span + row * kPitch + col * sizeof(T));
-            if (row < rows && col < columns) out[static_cast<int64_t>(row) * p.n + col] = v;
+        // 16 bytes at any element, and one by one at the end of the output's rows.
+        typedef uint32_t any_u32x4 __attribute__((ext_vector_type(4), aligned(2)));
+#pragma unroll
+        for (int r = 0; r < 32; r += kWave / kRowLanes) {
+            const int row = r + lane / kRowLanes, col = lane % kRowLanes * kPer;
+            const char* from = span + row * kPitch + col * sizeof(T);
+            T* to = out + static_cast<int64_t>(row) * p.n + col;
+            if (row >= rows) continue;
+            if (col + kPer <= columns) *reinterpret_cast<any_u32x4*>(to) = *reinterpret_cast<const u32x4*>(from);
+            else
+                for (int i = 0; col + i < columns; ++i) to[i] = reinterpret_cast<const T*>(from)[i];
         }
     }
 }
@@ -494,6 +501,9 @@ PECO_API int peco_int8_linear(const int8_t* codes, int64_t pitch, const float* s
 
 namespace {
 
+// Bytes between rows of codes: whole lines for long rows (odd lengths made the loads of 1000 channels a tenth slower).
+int64_t codes_pitch(int channels) { return ceil_div(channels, channels < 512 ? 16 : 128) * (channels < 512 ? 16 : 128); }
+
 // Whether the kernel for few rows quantizes them itself.
 bool quantizes_itself(int rows, int channels, int x_dtype, int dtype) {
     return rows <= 16 && x_dtype == dtype && static_cast<int64_t>(rows) * channels <= kFusedCodes;
@@ -503,7 +513,7 @@ bool quantizes_itself(int rows, int channels, int x_dtype, int dtype) {
 
 PECO_API size_t peco_int8_linear_rows_workspace_size(int rows, int channels, int x_dtype, int dtype) {
     if (rows < 1 || channels < 1 || channels > kMaxRowChannels || quantizes_itself(rows, channels, x_dtype, dtype)) return 0;
-    return static_cast<size_t>(rows) * (ceil_div(channels, 16) * 16 + 4);
+    return static_cast<size_t>(rows) * (codes_pitch(channels) + 4);
 }
 
 PECO_API int peco_int8_linear_rows(const void* x, const int64_t* strides, int n0, int n1, int n2, int x_dtype,
@@ -530,7 +540,7 @@ PECO_API int peco_int8_linear_rows(const void* x, const int64_t* strides, int n0
     if (!workspace || workspace_bytes < peco_int8_linear_rows_workspace_size(rows, channels, x_dtype, dtype))
         return kWorkspaceTooSmall;
     if (reinterpret_cast<uintptr_t>(workspace) % 16) return kInvalidValue;
-    const int64_t pitch = ceil_div(channels, 16) * 16;
+    const int64_t pitch = codes_pitch(channels);
     auto* codes = static_cast<int8_t*>(workspace);
     auto* scales = reinterpret_cast<float*>(codes + rows * pitch);
     if (const int bad = launch_quantize_rows(x, strides, codes, pitch, scales, n0, n1, n2, channels, x_dtype, s)) return bad;

@@ -14,6 +14,7 @@ import torch
 from . import _native
 from .projection import QuantizedRows, empty_codes, outer_axes
 
+_TYPES = (torch.float16, torch.bfloat16, torch.float32)
 _MOST_CHANNELS = 16384
 _LONGS = {n: ctypes.c_int64 * n for n in (3, 6, 9)}
 
@@ -21,33 +22,35 @@ _LONGS = {n: ctypes.c_int64 * n for n in (3, 6, 9)}
 def _check(x, weight, bias, eps, around_one, name):
     if not isinstance(x, torch.Tensor) or x.dim() < 1:
         raise ValueError(f"{name} expects rows [..., C]")
-    if x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+    dtype, device, shape = x.dtype, x.device, x.shape
+    if dtype not in _TYPES:
         raise TypeError(f"{name} supports float16, bfloat16 and float32")
-    channels = x.shape[-1]
+    channels = shape[-1]
     if not 1 <= channels <= _MOST_CHANNELS:
         raise ValueError(f"{name} supports rows of 1 to {_MOST_CHANNELS} channels")
     if not isinstance(eps, (int, float)) or not 0.0 <= eps <= 1e30:
         raise ValueError("eps must be a nonnegative finite number")
     if around_one and weight is None:
         raise ValueError("around_one needs a weight")
-    given = [t for t in (weight, bias) if t is not None]
-    for t in given:
-        if not isinstance(t, torch.Tensor) or t.dtype not in (x.dtype, torch.float32):
+    for t in (weight, bias):
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or (t.dtype is not dtype and t.dtype is not torch.float32):
             raise TypeError("weight and bias must be tensors of the rows' dtype or float32")
-        if t.shape != (channels,) and (x.dim() < 2 or t.shape != (x.shape[0], channels)):
+        if t.shape[-1:] != shape[-1:] or (t.dim() != 1 and (t.dim() != 2 or len(shape) < 2 or t.shape[0] != shape[0])):
             raise ValueError("weight and bias must have shape [C], or [B, C] with B the rows' first axis")
-        if t.device != x.device:
+        if t.device != device:
             raise ValueError("weight and bias must reside on the device of the rows")
     if not x.is_cuda:
         raise ValueError("peco_amd layer norms run on GPU tensors; CPU tensors are not supported")
-    if not _native.plain_tensors(x, *given):
+    if not _native.plain_tensors(x, *(t for t in (weight, bias) if t is not None)):
         raise RuntimeError(f"{name} takes ordinary tensors (no tracing, transforms or tangents)")
-    if x.numel() // channels >= 1 << 30:
+    if x.numel() >= channels << 30:
         raise ValueError(f"{name} supports fewer than 2^30 rows")
-    if len(given) == 2 and (weight.dtype != bias.dtype or weight.dim() != bias.dim()):  # one type, one shape
-        weight, bias = weight.float(), bias.float()
+    if weight is not None and bias is not None and (weight.dtype != bias.dtype or weight.dim() != bias.dim()):
+        weight, bias = weight.float(), bias.float()  # (one type, one shape)
         if weight.dim() != bias.dim():
-            weight, bias = weight.expand(x.shape[0], channels), bias.expand(x.shape[0], channels)
+            weight, bias = weight.expand(shape[0], channels), bias.expand(shape[0], channels)
     return weight, bias
 
 
@@ -74,11 +77,12 @@ def _launch(x, weight, bias, eps, around_one, want_stats):
     with _native.on_device(device):
         _native.require_gfx950(device)
         source, sizes, strides = outer_axes(_channels_adjacent(x))
-        target = out
-        _, _, to = outer_axes(target, copy=False)
-        if to is None or out.stride(-1) != 1:
-            target = torch.empty(x.shape, dtype=x.dtype, device=device)
-            _, _, to = outer_axes(target)
+        target, to = out, strides
+        if out.stride() != source.stride():
+            _, _, to = outer_axes(target, copy=False)
+            if to is None or out.stride(-1) != 1:
+                target = torch.empty(x.shape, dtype=x.dtype, device=device)
+                _, _, to = outer_axes(target)
         if want_stats:
             stats = torch.empty((x.numel() // x.shape[-1], 2), dtype=torch.float32, device=device)
         weight, bias, entry, wide = _affine(weight, bias)
@@ -110,7 +114,8 @@ def _gradients(x, weight, bias, stats, grad, around_one, needs):
     with _native.on_device(device):
         x, sizes, strides = outer_axes(_channels_adjacent(x))
         grad, _, by = outer_axes(_channels_adjacent(grad))
-        to = (0, 0, 0) if dx is None else outer_axes(dx)[2]
+        rows = sizes[2] * x.shape[-1]
+        to = (sizes[1] * rows, rows, x.shape[-1])  # (dx is contiguous)
         weight, bias, entry, wide = _affine(weight, bias)
         workspace, floats = None, 0
         if dweight is not None or dbias is not None:

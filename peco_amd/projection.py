@@ -48,9 +48,11 @@ def outer_axes(t, copy=True):
 
 
 def empty_codes(x):
-    """Codes like x [..., K] in rows of whole 16 bytes, scales [...], and the rows' distance in bytes."""
+    """Codes like x [..., K] in rows of whole 16 bytes (whole lines for long rows), scales [...], and the rows' distance
+    in bytes."""
     *outer, channels = x.shape
-    pitch = -(-channels // 16) * 16
+    step = 16 if channels < 512 else 128
+    pitch = -(-channels // step) * step
     codes = torch.empty((*outer, pitch), dtype=torch.int8, device=x.device)
     return codes if pitch == channels else codes[..., :channels], \
         torch.empty(outer, dtype=torch.float32, device=x.device), pitch
