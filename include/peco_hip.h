@@ -395,7 +395,7 @@ int peco_append_pages(const void* k, const void* v, void* k_pages, void* v_pages
  * (each nullable) [channels] of x's dtype, or fp32 with wide != 0, with entry_stride 0, else [n0, channels], entry_stride
  * elements apart, for the rows of each entry of the outermost axis. around_one != 0: 1 + weight in the weight's
  * place. stats (nullable, fp32 [n0 * n1 * n2, 2]) receives mean and 1 / sqrt(variance + eps) of each row. No alignment is
- * needed; everything on 16 bytes with channels a multiple of 8 runs fastest. */
+ * needed. */
 int peco_layer_norm(const void* x, void* output, const int64_t* strides, const void* weight, const void* bias,
                     int64_t entry_stride, int wide, int around_one, float eps, float* stats, int n0, int n1, int n2,
                     int channels, int dtype, void* stream);
@@ -419,7 +419,7 @@ int peco_layer_norm_grad(const void* x, const void* grad, void* dx, const int64_
 /* Rows x [n0, n1, n2, channels] (as peco_layer_norm's, strides: 3) in 8 bits: with a the largest magnitude of a row,
  * codes = rint(x * (127 / a)) and scales = a / 127 in fp32, halves to even. Rows with a < 127 * 2^-126: codes and scale 0.
  * Rows with an infinity or a NaN: codes 0, scale NaN. codes: int8, rows in order, pitch bytes apart (a multiple of 16,
- * at least channels; the bytes behind a row's channels are left as they are), on 16 bytes. scales: fp32, one a row. */
+ * at least channels; the bytes behind a row's channels, up to the next 8, become 0), on 16 bytes. scales: fp32, one a row. */
 int peco_quantize_rows(const void* x, const int64_t* strides, int8_t* codes, int64_t pitch, float* scales, int n0,
                        int n1, int n2, int channels, int dtype, void* stream);
 

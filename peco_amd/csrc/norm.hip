@@ -38,10 +38,9 @@ struct NormArgs {
     float eps, inverse_channels;
 };
 
-template <int DT, int L, int kChunks, bool kVec, int kMode>
+template <int DT, int L, int kChunks, bool kWhole, int kMode>
 __global__ __launch_bounds__(512) void norm_kernel(NormArgs a) {
     __shared__ uint32_t slots[2][16];
-    constexpr bool kAhead = kVec || kChunks < 4;  // the next row's loads in flight (as registers allow)
     const int row_lanes = L < kWave ? L : kWave * a.waves;
     const RowLanes r{static_cast<int>(threadIdx.x) % row_lanes, row_lanes, a.channels};
     const uint32_t in_group = row_in_group<L>(row_lanes), group = blockDim.x / row_lanes, step = gridDim.x * group;
@@ -56,23 +55,22 @@ __global__ __launch_bounds__(512) void norm_kernel(NormArgs a) {
     }
     Piece<DT> next[kChunks];
     uint32_t row = blockIdx.x * group + in_group;  // (the workgroup's rows stay together: its barriers are met by all)
-    if (kAhead) load_row<DT, kVec>(next, a.x, a.from.at(min(row, a.rows - 1)), r);
+    load_row<DT, kWhole>(next, a.x, a.from.at(min(row, a.rows - 1)), r);
     for (uint32_t base = blockIdx.x * group; base < a.rows; base += step, row += step) {
         const uint32_t at = min(row, a.rows - 1);
-        if (!kAhead) load_row<DT, kVec>(next, a.x, a.from.at(at), r);
         float x[kChunks][8];
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
 #pragma unroll
             for (int k = 0; k < 8; ++k) x[c][k] = next[c].get(k);
-        if (kAhead && base + step < a.rows)
-            load_row<DT, kVec>(next, a.x, a.from.at(min(row + step, a.rows - 1)), r);
+        if (base + step < a.rows)
+            load_row<DT, kWhole>(next, a.x, a.from.at(min(row + step, a.rows - 1)), r);
         if constexpr (kMode != kCodes) {
             const uint32_t entry = a.entry ? at / a.entry_rows : 0;
             if (entry != held && (a.weight || a.bias)) {
                 held = entry;
-                if (a.weight) load_weight<DT, kVec>(w, a.weight, entry * a.entry, a.wide, r);
-                if (a.bias) load_weight<DT, kVec>(b, a.bias, entry * a.entry, a.wide, r);
+                if (a.weight) load_weight<DT, kWhole>(w, a.weight, entry * a.entry, a.wide, r);
+                if (a.bias) load_weight<DT, kWhole>(b, a.bias, entry * a.entry, a.wide, r);
                 if (a.around_one)
 #pragma unroll
                     for (int c = 0; c < kChunks; ++c)
@@ -87,14 +85,12 @@ __global__ __launch_bounds__(512) void norm_kernel(NormArgs a) {
             const float mean = over.sum(sum) * a.inverse_channels;
             float squares = 0.0f;
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c) {
-                const float here = r.template first<true>(c) < a.channels ? mean : 0.0f;  // (0 behind the row's end)
+            for (int c = 0; c < kChunks; ++c)
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    x[c][k] -= kVec ? here : r.template column<false>(c, k) < a.channels ? mean : 0.0f;
+                    x[c][k] -= r.template inside<kWhole>(c, k) ? mean : 0.0f;  // (0 behind the row's end)
                     squares = fmaf(x[c][k], x[c][k], squares);
                 }
-            }
             const float inverse = 1.0f / sqrtf(over.sum(squares) * a.inverse_channels + a.eps);
             if (kMode == kNorm && a.stats && r.lane == 0 && row < a.rows) a.stats[row] = make_float2(mean, inverse);
 #pragma unroll
@@ -106,16 +102,14 @@ __global__ __launch_bounds__(512) void norm_kernel(NormArgs a) {
             if (row < a.rows) {
                 const int64_t to = a.to.at(row);
 #pragma unroll
-                for (int c = 0; c < kChunks; ++c) store_piece<DT, kVec>(round_piece<DT>(x[c]), a.out, to, c, r);
+                for (int c = 0; c < kChunks; ++c) store_piece<DT, kWhole>(round_piece<DT>(x[c]), a.out, to, c, r);
             }
         } else {
             uint32_t most = 0;
 #pragma unroll
             for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (kVec || r.template column<false>(c, k) < a.channels)
-                        most = max(most, __float_as_uint(x[c][k]) & 0x7fffffffu);
+                for (int k = 0; k < 8; ++k) most = max(most, __float_as_uint(x[c][k]) & 0x7fffffffu);
             most = over.template run<MaxU>(most);
             const RowScale scale(most);
             if (row < a.rows) {
@@ -126,19 +120,11 @@ __global__ __launch_bounds__(512) void norm_kernel(NormArgs a) {
                     int code[8];
 #pragma unroll
                     for (int k = 0; k < 8; ++k) code[k] = scale.code(x[c][k]);
-                    if constexpr (kVec) {
-                        u32x2 packed{};
+                    u32x2 packed{};
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) packed[k / 4] |= (code[k] & 0xffu) << (8 * (k % 4));
-                        const int col = r.template first<true>(c);
-                        if (col < a.channels) *reinterpret_cast<u32x2*>(to + col) = packed;
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const int col = r.template column<false>(c, k);
-                            if (col < a.channels) to[col] = static_cast<int8_t>(code[k]);
-                        }
-                    }
+                    for (int k = 0; k < 8; ++k) packed[k / 4] |= (code[k] & 0xffu) << (8 * (k % 4));
+                    const int col = r.first(c);
+                    if (col < a.channels) *reinterpret_cast<u32x2*>(to + col) = packed;
                 }
             }
         }
@@ -146,29 +132,34 @@ __global__ __launch_bounds__(512) void norm_kernel(NormArgs a) {
 }
 
 // Workgroups: enough for every CU to hold what its registers allow (measured over 2 to 16 a CU).
-template <int DT, int L, int kChunks, bool kVec, int kMode>
+template <int DT, int L, int kChunks, bool kWhole, int kMode>
 int launch(const NormArgs& a, const RowShape& s, hipStream_t stream) {
     const int64_t blocks = std::min<int64_t>(ceil_div(a.rows, s.rows), 8 * device_compute_units());
-    hipLaunchKernelGGL((norm_kernel<DT, L, kChunks, kVec, kMode>), dim3(static_cast<unsigned>(blocks)),
+    hipLaunchKernelGGL((norm_kernel<DT, L, kChunks, kWhole, kMode>), dim3(static_cast<unsigned>(blocks)),
                        dim3(s.threads), 0, stream, a);
     return hipGetLastError();
 }
 
-template <int DT, bool kVec, int kMode> int launch_shape(const NormArgs& a, const RowShape& s, hipStream_t stream) {
-    if (s.lanes == 8) return launch<DT, 8, 1, kVec, kMode>(a, s, stream);
-    if (s.lanes == 16) return launch<DT, 16, 1, kVec, kMode>(a, s, stream);
-    if (s.chunks == 1) return launch<DT, 64, 1, kVec, kMode>(a, s, stream);
-    if (s.chunks == 2) return launch<DT, 64, 2, kVec, kMode>(a, s, stream);
-    return launch<DT, 64, 4, kVec, kMode>(a, s, stream);
+template <int DT, bool kWhole, int kMode> int launch_shape(const NormArgs& a, const RowShape& s, hipStream_t stream) {
+    if (s.lanes == 8) return launch<DT, 8, 1, kWhole, kMode>(a, s, stream);
+    if (s.lanes == 16) return launch<DT, 16, 1, kWhole, kMode>(a, s, stream);
+    if (s.chunks == 1) return launch<DT, 64, 1, kWhole, kMode>(a, s, stream);
+    if (s.chunks == 2) return launch<DT, 64, 2, kWhole, kMode>(a, s, stream);
+    return launch<DT, 64, 4, kWhole, kMode>(a, s, stream);
 }
 
-template <int kMode> int launch_type(NormArgs a, bool vec, int dtype, hipStream_t stream) {
-    const RowShape s = row_shape(a.channels, vec, 4, 4);
+// Pieces a lane: up to 4 of 16 bytes keep a row of 2048 channels in one wavefront, whose sums need no barrier (119056 x 4096
+// in fp16: 349 us with 4 pieces, 395 with 2; 2048 x 2048 in bf16 5.1, 5.9 and, with 1, 7.1). Two where a piece is 32 bytes or
+// rows end inside a piece, whose moves take registers (7006 x 2048 in fp32 25.2, 22.9 and 21.7, 7006 x 4096 41.4, 36.8 and 39.5;
+// 7006 x 2047 in bf16 21.5, 16.2 and 18.2).
+template <int kMode> int launch_type(NormArgs a, int dtype, hipStream_t stream) {
+    const bool whole = a.channels % 8 == 0;
+    const RowShape s = row_shape(a.channels, whole && dtype != kF32 ? 4 : 2, 4);
     a.waves = s.waves;
     switch (dtype) {
-        case kBF16: return vec ? launch_shape<kBF16, true, kMode>(a, s, stream) : launch_shape<kBF16, false, kMode>(a, s, stream);
-        case kF16: return vec ? launch_shape<kF16, true, kMode>(a, s, stream) : launch_shape<kF16, false, kMode>(a, s, stream);
-        default: return vec ? launch_shape<kF32, true, kMode>(a, s, stream) : launch_shape<kF32, false, kMode>(a, s, stream);
+        case kBF16: return whole ? launch_shape<kBF16, true, kMode>(a, s, stream) : launch_shape<kBF16, false, kMode>(a, s, stream);
+        case kF16: return whole ? launch_shape<kF16, true, kMode>(a, s, stream) : launch_shape<kF16, false, kMode>(a, s, stream);
+        default: return whole ? launch_shape<kF32, true, kMode>(a, s, stream) : launch_shape<kF32, false, kMode>(a, s, stream);
     }
 }
 
@@ -200,10 +191,6 @@ void set_affine(NormArgs& a, const void* weight, const void* bias, int64_t entry
     a.eps = eps;
 }
 
-bool affine_on_16(const void* p, int64_t entry, int size) {
-    return !(reinterpret_cast<uintptr_t>(p) % 16) && !(entry * size % 16);
-}
-
 }  // namespace
 
 int launch_quantize_rows(const void* x, const int64_t* strides, int8_t* codes, int64_t pitch, float* scales, int n0,
@@ -215,8 +202,7 @@ int launch_quantize_rows(const void* x, const int64_t* strides, int8_t* codes, i
     a.codes = codes;
     a.scales = scales;
     a.pitch = pitch;
-    const bool vec = channels % 8 == 0 && rows_on_16(x, strides, dtype == kF32 ? 4 : 2);
-    return launch_type<kCodes>(a, vec, dtype, stream);
+    return launch_type<kCodes>(a, dtype, stream);
 }
 
 }  // namespace peco
@@ -234,10 +220,7 @@ PECO_API int peco_layer_norm(const void* x, void* output, const int64_t* strides
     a.out = output;
     a.to = row_map(strides + 3, n0, n1, n2);
     a.stats = reinterpret_cast<float2*>(stats);
-    const int size = dtype == kF32 ? 4 : 2, affine = wide ? 4 : size;
-    const bool vec = channels % 8 == 0 && rows_on_16(x, strides, size) && rows_on_16(output, strides + 3, size) &&
-                     affine_on_16(weight, entry_stride, affine) && affine_on_16(bias, entry_stride, affine);
-    return launch_type<kNorm>(a, vec, dtype, static_cast<hipStream_t>(stream));
+    return launch_type<kNorm>(a, dtype, static_cast<hipStream_t>(stream));
 }
 
 PECO_API int peco_layer_norm_rows(const void* x, const int64_t* strides, const void* weight, const void* bias,
@@ -253,10 +236,7 @@ PECO_API int peco_layer_norm_rows(const void* x, const int64_t* strides, const v
     a.codes = codes;
     a.scales = scales;
     a.pitch = pitch;
-    const int size = dtype == kF32 ? 4 : 2, affine = wide ? 4 : size;
-    const bool vec = channels % 8 == 0 && rows_on_16(x, strides, size) &&
-                     affine_on_16(weight, entry_stride, affine) && affine_on_16(bias, entry_stride, affine);
-    return launch_type<kNormCodes>(a, vec, dtype, static_cast<hipStream_t>(stream));
+    return launch_type<kNormCodes>(a, dtype, static_cast<hipStream_t>(stream));
 }
 
 PECO_API int peco_quantize_rows(const void* x, const int64_t* strides, int8_t* codes, int64_t pitch, float* scales,

@@ -27,11 +27,11 @@ struct GradArgs {
     float inverse_channels;
 };
 
-template <int DT, int L, int kChunks, bool kVec, bool kSums>
+template <int DT, int L, int kChunks, bool kWhole, bool kSums>
 __global__ __launch_bounds__(kGradThreads, kChunks == 1 ? 4 : 2) void norm_grad_kernel(GradArgs a) {
     extern __shared__ float joined[];  // a row of sums
     __shared__ uint32_t slots[2][16];
-    constexpr bool kAhead = kChunks < 4 || (kVec && DT != kF32);  // the next row's loads in flight (as registers allow)
+    constexpr bool kAhead = kChunks < 4 || DT != kF32;  // the next row's loads in flight (as registers allow)
     const int row_lanes = L < kWave ? L : kWave * a.waves;
     const RowLanes r{static_cast<int>(threadIdx.x) % row_lanes, row_lanes, a.channels};
     const uint32_t in_group = row_in_group<L>(row_lanes), group = blockDim.x / row_lanes, step = a.shares * group;
@@ -39,7 +39,7 @@ __global__ __launch_bounds__(kGradThreads, kChunks == 1 ? 4 : 2) void norm_grad_
     RowCombine<L> over{slots, a.waves, static_cast<int>(threadIdx.x / kWave)};
     float w[kChunks][8], dw[kSums ? kChunks : 1][8], db[kSums ? kChunks : 1][8];
     if (a.weight) {
-        load_weight<DT, kVec>(w, a.weight, entry * a.entry, a.wide, r);
+        load_weight<DT, kWhole>(w, a.weight, entry * a.entry, a.wide, r);
         if (a.around_one)
 #pragma unroll
             for (int c = 0; c < kChunks; ++c)
@@ -60,8 +60,8 @@ __global__ __launch_bounds__(kGradThreads, kChunks == 1 ? 4 : 2) void norm_grad_
     float2 next_stats;
     const auto load = [&](uint32_t in_entry) {
         const uint32_t at = before + min(in_entry, a.entry_rows - 1);
-        load_row<DT, kVec>(next_x, a.x, a.from.at(at), r);
-        load_row<DT, kVec>(next_g, a.grad, a.by.at(at), r);
+        load_row<DT, kWhole>(next_x, a.x, a.from.at(at), r);
+        load_row<DT, kWhole>(next_g, a.grad, a.by.at(at), r);
         next_stats = a.stats[at];
         if (in_entry >= a.entry_rows)  // adds nothing
 #pragma unroll
@@ -78,8 +78,7 @@ __global__ __launch_bounds__(kGradThreads, kChunks == 1 ? 4 : 2) void norm_grad_
         if (kAhead && base + step < a.entry_rows) load(row + step);
         // n of an element (0 behind the row's end). It is taken from x twice, which costs less than its registers.
         const auto normal = [&](int c, int k) {
-            const bool inside = (kVec ? r.template first<true>(c) : r.template column<false>(c, k)) < a.channels;
-            return (x[c].get(k) - (inside ? mean : 0.0f)) * inverse;
+            return (x[c].get(k) - (r.template inside<kWhole>(c, k) ? mean : 0.0f)) * inverse;
         };
         float sum = 0.0f, along = 0.0f;
 #pragma unroll
@@ -111,7 +110,7 @@ __global__ __launch_bounds__(kGradThreads, kChunks == 1 ? 4 : 2) void norm_grad_
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
                     dx[k] = fmaf(-normal(c, k), along, g[c].get(k) * w[c][k] - sum) * inverse;
-                store_piece<DT, kVec>(round_piece<DT>(dx), a.dx, to, c, r);
+                store_piece<DT, kWhole>(round_piece<DT>(dx), a.dx, to, c, r);
             }
         }
     }
@@ -141,7 +140,7 @@ __global__ __launch_bounds__(kGradThreads, kChunks == 1 ? 4 : 2) void norm_grad_
                 float sum = joined[e];
                 for (int i = 1; i < sets; ++i) sum += joined[i * held + e];
                 const int piece = e / row_lanes, lane = e - piece * row_lanes;
-                const int col = kVec ? (piece / 8 * row_lanes + lane) * 8 + piece % 8 : e;
+                const int col = (piece / 8 * row_lanes + lane) * 8 + piece % 8;
                 if (col < a.channels) to[col] = sum;
             }
         }
@@ -186,29 +185,29 @@ __global__ __launch_bounds__(kWave * kJoinWaves) void join_sums_kernel(const flo
 // rows of 2048 channels in bf16 (with the second launch): 1 piece 39 us, 2 pieces 42, 4 pieces 39; of 1024 channels 25, 26 and
 // 29; fp32 rows of 2048 72, 83 and 75.
 // Shares of an entry's rows: as many workgroups as fit, fewer where the rows are few.
-RowShape grad_shape(int channels, bool vec) { return row_shape(channels, vec, 1, 8); }
+RowShape grad_shape(int channels) { return row_shape(channels, 1, 8); }
 uint32_t grad_shares(const RowShape& s, int entries, uint32_t entry_rows) {
     const int64_t blocks = (s.chunks == 1 ? 2 : 1) * device_compute_units();
     return static_cast<uint32_t>(std::min<int64_t>(std::max<int64_t>(1, blocks / entries), ceil_div(entry_rows, s.rows)));
 }
 
-template <int DT, int L, int kChunks, bool kVec> int launch(const GradArgs& a, const RowShape& s, int entries, hipStream_t st) {
+template <int DT, int L, int kChunks, bool kWhole> int launch(const GradArgs& a, const RowShape& s, int entries, hipStream_t st) {
     const dim3 grid(a.shares * entries), block(s.threads);
     if (a.parts) {
         const size_t lds = sizeof(float) * (s.lanes < kWave ? s.threads / kWave : s.rows) * s.lanes * s.waves * kChunks * 8;
-        hipLaunchKernelGGL((norm_grad_kernel<DT, L, kChunks, kVec, true>), grid, block, lds, st, a);
+        hipLaunchKernelGGL((norm_grad_kernel<DT, L, kChunks, kWhole, true>), grid, block, lds, st, a);
     } else {
-        hipLaunchKernelGGL((norm_grad_kernel<DT, L, kChunks, kVec, false>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((norm_grad_kernel<DT, L, kChunks, kWhole, false>), grid, block, 0, st, a);
     }
     return hipGetLastError();
 }
 
-template <int DT, bool kVec> int launch_shape(const GradArgs& a, const RowShape& s, int entries, hipStream_t st) {
-    if (s.lanes == 8) return launch<DT, 8, 1, kVec>(a, s, entries, st);
-    if (s.lanes == 16) return launch<DT, 16, 1, kVec>(a, s, entries, st);
-    if (s.chunks == 1) return launch<DT, 64, 1, kVec>(a, s, entries, st);
-    if (s.chunks == 2) return launch<DT, 64, 2, kVec>(a, s, entries, st);
-    return launch<DT, 64, 4, kVec>(a, s, entries, st);
+template <int DT, bool kWhole> int launch_shape(const GradArgs& a, const RowShape& s, int entries, hipStream_t st) {
+    if (s.lanes == 8) return launch<DT, 8, 1, kWhole>(a, s, entries, st);
+    if (s.lanes == 16) return launch<DT, 16, 1, kWhole>(a, s, entries, st);
+    if (s.chunks == 1) return launch<DT, 64, 1, kWhole>(a, s, entries, st);
+    if (s.chunks == 2) return launch<DT, 64, 2, kWhole>(a, s, entries, st);
+    return launch<DT, 64, 4, kWhole>(a, s, entries, st);
 }
 
 template <typename T>
@@ -232,9 +231,7 @@ PECO_API size_t peco_layer_norm_grad_workspace_size(int n0, int n1, int n2, int 
     if (!takes(n0, n1, n2, channels) || (per_entry && n0 > 65535)) return 0;
     const int entries = per_entry ? n0 : 1;
     const uint32_t rows = static_cast<uint32_t>(n1) * n2 * (per_entry ? 1 : n0);
-    const uint32_t shares = std::max(grad_shares(grad_shape(channels, true), entries, rows),
-                                     grad_shares(grad_shape(channels, false), entries, rows));
-    return static_cast<size_t>(entries) * shares * 2 * channels;
+    return static_cast<size_t>(entries) * grad_shares(grad_shape(channels), entries, rows) * 2 * channels;
 }
 
 PECO_API int peco_layer_norm_grad(const void* x, const void* grad, void* dx, const int64_t* strides, const void* weight,
@@ -266,19 +263,16 @@ PECO_API int peco_layer_norm_grad(const void* x, const void* grad, void* dx, con
     a.wide = wide;
     a.around_one = around_one;
     a.inverse_channels = 1.0f / static_cast<float>(channels);
-    const int size = dtype == kF32 ? 4 : 2, affine = wide ? 4 : size;
-    const bool vec = channels % 8 == 0 && rows_on_16(x, strides, size) && rows_on_16(grad, strides + 3, size) &&
-                     (!dx || rows_on_16(dx, strides + 6, size)) &&
-                     !(reinterpret_cast<uintptr_t>(weight) % 16) && !(entry_stride * affine % 16);
-    const RowShape s = grad_shape(channels, vec);
+    const bool whole = channels % 8 == 0;
+    const RowShape s = grad_shape(channels);
     a.shares = grad_shares(s, entries, a.entry_rows);
     a.waves = s.waves;
     const auto st = static_cast<hipStream_t>(stream);
     int status;
     switch (dtype) {
-        case kBF16: status = vec ? launch_shape<kBF16, true>(a, s, entries, st) : launch_shape<kBF16, false>(a, s, entries, st); break;
-        case kF16: status = vec ? launch_shape<kF16, true>(a, s, entries, st) : launch_shape<kF16, false>(a, s, entries, st); break;
-        default: status = vec ? launch_shape<kF32, true>(a, s, entries, st) : launch_shape<kF32, false>(a, s, entries, st);
+        case kBF16: status = whole ? launch_shape<kBF16, true>(a, s, entries, st) : launch_shape<kBF16, false>(a, s, entries, st); break;
+        case kF16: status = whole ? launch_shape<kF16, true>(a, s, entries, st) : launch_shape<kF16, false>(a, s, entries, st); break;
+        default: status = whole ? launch_shape<kF32, true>(a, s, entries, st) : launch_shape<kF32, false>(a, s, entries, st);
     }
     if (status || !sums) return status;
     if (wide || dtype == kF32) launch_join<float>(a, dweight, dbias, entries, st);

@@ -1,9 +1,9 @@
 // Rows of channels spread over the lanes of part of a wavefront, of one or of several, for the kernels that take
 // statistics over a row (layer norm, its gradient, quantization).
 //
-// A row of C channels is held in registers by `lanes` lanes, kChunks pieces of 8 channels each: adjacent channels
-// where everything lies on 16 bytes (kVec), else channels `lanes` apart, so that the single loads of a wavefront are
-// adjacent. Short rows share a wavefront; those of one wavefront need no barrier for their sums.
+// A row of C channels is held in registers by `lanes` lanes, kChunks pieces of 8 adjacent channels each, whatever the
+// rows' alignment: 16-byte accesses may start at any element. Short rows share a wavefront; those of one wavefront need no
+// barrier for their sums.
 #pragma once
 
 #include "mfma.hpp"
@@ -36,30 +36,44 @@ inline RowMap row_map(const int64_t* strides, int n0, int n1, int n2) {
     return m;
 }
 
-// Whether every row starts on 16 bytes.
-inline bool rows_on_16(const void* p, const int64_t* strides, int size) {
-    return !(reinterpret_cast<uintptr_t>(p) % 16) && !(((strides[0] | strides[1] | strides[2]) * size) % 16);
-}
-
 // Eight channels as they lie in memory. (Words, not 16-bit elements: the compiler would keep each of those in a register
 // of its own across a loop.)
 template <int DT> struct Piece {
     static constexpr int kWords = DT == kF32 ? 8 : 4;
     uint32_t word[kWords];
+    typedef uint32_t Any __attribute__((ext_vector_type(4), aligned(2)));  // at any element
     // (A row's start, the same in a wavefront that has one row, and a 32-bit offset: one register for the address.)
     __device__ __forceinline__ void load(const char* row, uint32_t column) {
-        const u32x4* p = reinterpret_cast<const u32x4*>(row + column * (DT == kF32 ? 4u : 2u));
+        const Any* p = reinterpret_cast<const Any*>(row + column * (DT == kF32 ? 4u : 2u));
 #pragma unroll
         for (int j = 0; j < kWords / 4; ++j) {
-            const u32x4 v = p[j];
+            const Any v = p[j];
 #pragma unroll
             for (int k = 0; k < 4; ++k) word[4 * j + k] = v[k];
         }
     }
     __device__ __forceinline__ void store(char* row, uint32_t column) const {
-        u32x4* p = reinterpret_cast<u32x4*>(row + column * (DT == kF32 ? 4u : 2u));
+        Any* p = reinterpret_cast<Any*>(row + column * (DT == kF32 ? 4u : 2u));
 #pragma unroll
-        for (int j = 0; j < kWords / 4; ++j) p[j] = u32x4{word[4 * j], word[4 * j + 1], word[4 * j + 2], word[4 * j + 3]};
+        for (int j = 0; j < kWords / 4; ++j) p[j] = Any{word[4 * j], word[4 * j + 1], word[4 * j + 2], word[4 * j + 3]};
+    }
+    __device__ __forceinline__ uint32_t bits(int k) const {
+        return DT == kF32 ? word[k] : k % 2 ? word[k / 2] >> 16 : word[k / 2] & 0xffffu;
+    }
+    // The channels moved `by` (0 to 8) places down, 0 behind them.
+    __device__ __forceinline__ void shift(int by) {
+        constexpr int kPer = DT == kF32 ? 1 : 2;  // channels a word
+#pragma unroll
+        for (int step = 8; step >= kPer; step /= 2)
+#pragma unroll
+            for (int j = 0; j < kWords; ++j) {
+                const int from = j + step / kPer;
+                word[j] = by & step ? from < kWords ? word[from] : 0u : word[j];
+            }
+        if constexpr (kPer == 2)
+#pragma unroll
+            for (int j = 0; j < kWords; ++j)
+                word[j] = by & 1 ? word[j] >> 16 | (j + 1 < kWords ? word[j + 1] << 16 : 0u) : word[j];
     }
     __device__ __forceinline__ float get(int k) const {
         if constexpr (DT == kF32) return __uint_as_float(word[k]);
@@ -77,43 +91,40 @@ template <int DT> struct Piece {
 // The lanes of one row: lane of lanes, and the row's length.
 struct RowLanes {
     int lane, lanes, channels;
-    template <bool kVec> __device__ __forceinline__ int first(int c) const {
-        return kVec ? (c * lanes + lane) * 8 : c * 8 * lanes + lane;
-    }
-    template <bool kVec> __device__ __forceinline__ int column(int c, int k) const {
-        return first<kVec>(c) + (kVec ? k : k * lanes);
+    __device__ __forceinline__ int first(int c) const { return (c * lanes + lane) * 8; }
+    // Whether element k of piece c lies in the row (kWhole: its length is a multiple of 8).
+    template <bool kWhole> __device__ __forceinline__ bool inside(int c, int k) const {
+        return first(c) + (kWhole ? 0 : k) < channels;
     }
 };
 
-// A lane's pieces of the row at `offset` (elements), 0 behind the row's end.
-template <int DT, bool kVec, int kChunks>
+// A lane's pieces of the row at `offset` (elements), 0 behind the row's end: the 8 channels before it are taken for a
+// piece that meets it, and moved.
+template <int DT, bool kWhole, int kChunks>
 __device__ __forceinline__ void load_row(Piece<DT> (&x)[kChunks], const void* base, int64_t offset, const RowLanes& r) {
     const char* row = static_cast<const char*>(base) + offset * (DT == kF32 ? 4 : 2);
-    if constexpr (kVec) {
+    if (!kWhole && r.channels < 8) {
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c)  // clamped, unconditional: all loads in flight
-            x[c].load(row, min(r.template first<true>(c), r.channels - 8));
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-            for (int k = 0; k < Piece<DT>::kWords; ++k)
-                x[c].word[k] = r.template first<true>(c) < r.channels ? x[c].word[k] : 0;
-    } else {
-        using T = std::conditional_t<DT == kF32, uint32_t, uint16_t>;
-        T v[kChunks][8];
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c)
+        for (int c = 0; c < kChunks; ++c) x[c] = Piece<DT>{};
+        if (r.lane == 0)
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                v[c][k] = reinterpret_cast<const T*>(row)[static_cast<uint32_t>(min(r.template column<false>(c, k), r.channels - 1))];
+                if (k < r.channels) {
+                    if constexpr (DT == kF32) x[0].word[k] = reinterpret_cast<const uint32_t*>(row)[k];
+                    else x[0].word[k / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[k]) << (k % 2 * 16);
+                }
+        return;
+    }
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c)
+    for (int c = 0; c < kChunks; ++c) x[c].load(row, min(r.first(c), r.channels - 8));  // all in flight
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const uint32_t w = r.template column<false>(c, k) < r.channels ? v[c][k] : 0;
-                if constexpr (DT == kF32) x[c].word[k] = w;
-                else x[c].word[k / 2] = k % 2 ? x[c].word[k / 2] | w << 16 : w;
-            }
+    for (int c = 0; c < kChunks; ++c) {
+        if constexpr (kWhole) {
+#pragma unroll
+            for (int k = 0; k < Piece<DT>::kWords; ++k) x[c].word[k] = r.first(c) < r.channels ? x[c].word[k] : 0;
+        } else {
+            x[c].shift(min(max(r.first(c) - (r.channels - 8), 0), 8));
+        }
     }
 }
 
@@ -128,37 +139,36 @@ template <int DT> __device__ __forceinline__ Piece<DT> round_piece(const float (
     return y;
 }
 
-template <int DT, bool kVec>
+template <int DT, bool kWhole>
 __device__ __forceinline__ void store_piece(const Piece<DT>& y, void* base, int64_t offset, int c, const RowLanes& r) {
     char* row = static_cast<char*>(base) + offset * (DT == kF32 ? 4 : 2);
-    if constexpr (kVec) {
-        const int col = r.template first<true>(c);
-        if (col < r.channels) y.store(row, col);
-    } else {
+    const int col = r.first(c);
+    if (col + (kWhole ? 0 : 7) < r.channels) {
+        y.store(row, col);
+    } else if (!kWhole) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int col = r.template column<false>(c, k);
-            if (col >= r.channels) continue;
-            if constexpr (DT == kF32) reinterpret_cast<uint32_t*>(row)[static_cast<uint32_t>(col)] = y.word[k];
-            else reinterpret_cast<uint16_t*>(row)[static_cast<uint32_t>(col)] = static_cast<uint16_t>(k % 2 ? y.word[k / 2] >> 16 : y.word[k / 2]);
+        for (int k = 0; k < 7; ++k) {
+            if (col + k >= r.channels) break;
+            if constexpr (DT == kF32) reinterpret_cast<uint32_t*>(row)[static_cast<uint32_t>(col + k)] = y.bits(k);
+            else reinterpret_cast<uint16_t*>(row)[static_cast<uint32_t>(col + k)] = static_cast<uint16_t>(y.bits(k));
         }
     }
 }
 
 // A lane's pieces of a weight or bias (of the rows' type, or fp32) as fp32, 0 behind the row's end.
-template <int DT, bool kVec, int kChunks>
+template <int DT, bool kWhole, int kChunks>
 __device__ __forceinline__ void load_weight(float (&w)[kChunks][8], const void* base, int64_t offset, bool wide,
                                             const RowLanes& r) {
     if (DT == kF32 || wide) {
         Piece<kF32> x[kChunks];
-        load_row<kF32, kVec>(x, base, offset, r);
+        load_row<kF32, kWhole>(x, base, offset, r);
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
 #pragma unroll
             for (int k = 0; k < 8; ++k) w[c][k] = x[c].get(k);
     } else {
         Piece<DT> x[kChunks];
-        load_row<DT, kVec>(x, base, offset, r);
+        load_row<DT, kWhole>(x, base, offset, r);
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
 #pragma unroll
@@ -248,16 +258,14 @@ template <int L> __device__ __forceinline__ uint32_t row_in_group(int row_lanes)
 
 // How rows of C channels are spread: lanes of a wavefront, pieces a lane, wavefronts a row, and rows and threads of a
 // workgroup of at most `most_waves`. Rows of more than a wavefront take as many as hold them with `most_chunks` pieces
-// a lane, or 4 for the longest. Single loads (vec false) take one piece a lane as long as 8 wavefronts hold the row: the
-// pieces of eight loads each cost registers, and a row of 1111 channels leaves less of three wavefronts idle.
+// a lane, or with more where 8 do not.
 struct RowShape {
     int lanes, chunks, waves, threads, rows;
 };
-inline RowShape row_shape(int channels, bool vec, int most_chunks, int most_waves) {
+inline RowShape row_shape(int channels, int most_chunks, int most_waves) {
     RowShape s{kWave, 1, 1, 0, 0};
     if (channels <= 64) s.lanes = 8;
     else if (channels <= 128) s.lanes = 16;
-    if (!vec) most_chunks = 1;
     while (s.chunks < most_chunks && s.lanes * s.chunks * 8 < channels) s.chunks *= 2;
     while (s.chunks < 4 && 8 * s.lanes * s.chunks * 8 < channels) s.chunks *= 2;
     s.waves = static_cast<int>(ceil_div(channels, s.lanes * s.chunks * 8));
