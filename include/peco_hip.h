@@ -394,7 +394,8 @@ int peco_append_pages(const void* k, const void* v, void* k_pages, void* v_pages
  * (6 values). output = (x - mean) / sqrt(variance + eps) * weight + bias, fp32, rounded once; weight and bias
  * (each nullable) [channels] of x's dtype, or fp32 with wide != 0, with entry_stride 0, else [n0, channels], entry_stride
  * elements apart, for the rows of each entry of the outermost axis. around_one != 0: 1 + weight in the weight's
- * place. stats (nullable, fp32 [n0 * n1 * n2, 2]) receives mean and 1 / sqrt(variance + eps) of each row. No alignment is
+ * place. stats (nullable, fp32 [n0 * n1 * n2, 3]) receives each row's mean, what
+ * rounding left of it and 1 / sqrt(variance + eps). No alignment is
  * needed. */
 int peco_layer_norm(const void* x, void* output, const int64_t* strides, const void* weight, const void* bias,
                     int64_t entry_stride, int wide, int around_one, float eps, float* stats, int n0, int n1, int n2,

@@ -2,7 +2,9 @@
 //
 // Norm: m = sum x / C, v = sum (x - m)^2 / C, r = 1 / sqrt(v + eps), y = (x - m) r f + b with f = w or 1 + w, all in fp32
 // and rounded once to the rows' type. The row is in registers, so its deviations are taken from the mean itself (the
-// difference of E[x^2] and m^2 would cancel for rows far from 0). w and b are one row for all, or one for each entry of
+// difference of E[x^2] and m^2 would cancel for rows far from 0), and the mean is kept in two parts: what rounding left of
+// it is the mean of those deviations. An error of half a step of the mean would stay in every deviation, which for
+// rows much further from 0 than they are wide is no small part of them. w and b are one row for all, or one for each entry of
 // the outermost axis (a modulation).
 //
 // Quantized rows: a = max |x|, code = rint(x * (127 / a)), scale = a / 127, in fp32 with IEEE division, halves to even.
@@ -27,7 +29,7 @@ struct NormArgs {
     const void* x;
     const void *weight, *bias;  // nullable
     void* out;                  // kNorm
-    float2* stats;              // kNorm, nullable: mean and 1 / deviation of each row
+    RowStats* stats;            // kNorm, nullable
     int8_t* codes;              // the others
     float* scales;
     RowMap from, to;
@@ -83,16 +85,24 @@ __global__ __launch_bounds__(512) void norm_kernel(NormArgs a) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) sum += x[c][k];
             const float mean = over.sum(sum) * a.inverse_channels;
-            float squares = 0.0f;
+            float rest = 0.0f, squares = 0.0f;
 #pragma unroll
             for (int c = 0; c < kChunks; ++c)
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     x[c][k] -= r.template inside<kWhole>(c, k) ? mean : 0.0f;  // (0 behind the row's end)
+                    rest += x[c][k];
                     squares = fmaf(x[c][k], x[c][k], squares);
                 }
-            const float inverse = 1.0f / sqrtf(over.sum(squares) * a.inverse_channels + a.eps);
-            if (kMode == kNorm && a.stats && r.lane == 0 && row < a.rows) a.stats[row] = make_float2(mean, inverse);
+            over.sum2(rest, squares);
+            rest *= a.inverse_channels;
+            const float variance = squares * a.inverse_channels - rest * rest;
+            const float inverse = 1.0f / sqrtf((variance < 0.0f ? 0.0f : variance) + a.eps);
+            if (kMode == kNorm && a.stats && r.lane == 0 && row < a.rows) a.stats[row] = RowStats{mean, rest, inverse};
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[c][k] -= r.template inside<kWhole>(c, k) ? rest : 0.0f;
 #pragma unroll
             for (int c = 0; c < kChunks; ++c)
 #pragma unroll
@@ -219,7 +229,7 @@ PECO_API int peco_layer_norm(const void* x, void* output, const int64_t* strides
     set_affine(a, weight, bias, entry_stride, wide, around_one, eps);
     a.out = output;
     a.to = row_map(strides + 3, n0, n1, n2);
-    a.stats = reinterpret_cast<float2*>(stats);
+    a.stats = reinterpret_cast<RowStats*>(stats);
     return launch_type<kNorm>(a, dtype, static_cast<hipStream_t>(stream));
 }
 

@@ -18,7 +18,7 @@ constexpr int kGradThreads = 512;
 struct GradArgs {
     const void *x, *grad, *weight;  // weight nullable: ones
     void* dx;                       // nullable
-    const float2* stats;
+    const RowStats* stats;
     float* parts;                   // [entries, shares, 2, C], nullable: rows only
     RowMap from, by, to;
     int64_t entry;
@@ -57,7 +57,7 @@ __global__ __launch_bounds__(kGradThreads, kChunks == 1 ? 4 : 2) void norm_grad_
 #pragma unroll
             for (int k = 0; k < 8; ++k) dw[c][k] = db[c][k] = 0.0f;
     Piece<DT> next_x[kChunks], next_g[kChunks];
-    float2 next_stats;
+    RowStats next_stats;
     const auto load = [&](uint32_t in_entry) {
         const uint32_t at = before + min(in_entry, a.entry_rows - 1);
         load_row<DT, kWhole>(next_x, a.x, a.from.at(at), r);
@@ -72,13 +72,14 @@ __global__ __launch_bounds__(kGradThreads, kChunks == 1 ? 4 : 2) void norm_grad_
     for (uint32_t base = share * group; base < a.entry_rows; base += step, row += step) {
         if (!kAhead) load(row);
         Piece<DT> x[kChunks], g[kChunks];
-        const float mean = next_stats.x, inverse = next_stats.y;
+        const RowStats stats = next_stats;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) x[c] = next_x[c], g[c] = next_g[c];
         if (kAhead && base + step < a.entry_rows) load(row + step);
         // n of an element (0 behind the row's end). It is taken from x twice, which costs less than its registers.
         const auto normal = [&](int c, int k) {
-            return (x[c].get(k) - (r.template inside<kWhole>(c, k) ? mean : 0.0f)) * inverse;
+            const bool inside = r.template inside<kWhole>(c, k);
+            return (x[c].get(k) - (inside ? stats.mean : 0.0f) - (inside ? stats.rest : 0.0f)) * stats.inverse;
         };
         float sum = 0.0f, along = 0.0f;
 #pragma unroll
@@ -109,7 +110,7 @@ __global__ __launch_bounds__(kGradThreads, kChunks == 1 ? 4 : 2) void norm_grad_
                 float dx[8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
-                    dx[k] = fmaf(-normal(c, k), along, g[c].get(k) * w[c][k] - sum) * inverse;
+                    dx[k] = fmaf(-normal(c, k), along, g[c].get(k) * w[c][k] - sum) * stats.inverse;
                 store_piece<DT, kWhole>(round_piece<DT>(dx), a.dx, to, c, r);
             }
         }
@@ -252,7 +253,7 @@ PECO_API int peco_layer_norm_grad(const void* x, const void* grad, void* dx, con
     a.grad = grad;
     a.weight = weight;
     a.dx = dx;
-    a.stats = reinterpret_cast<const float2*>(stats);
+    a.stats = reinterpret_cast<const RowStats*>(stats);
     a.parts = sums ? workspace : nullptr;
     a.from = row_map(strides, n0, n1, n2);
     a.by = row_map(strides + 3, n0, n1, n2);

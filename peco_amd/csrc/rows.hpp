@@ -250,6 +250,11 @@ struct RowScale {
     __device__ __forceinline__ int code(float x) const { return finite ? static_cast<int>(rintf(x * by)) : 0; }
 };
 
+// What the norm keeps of a row: its mean in two parts, and 1 / sqrt(variance + eps).
+struct RowStats {
+    float mean, rest, inverse;
+};
+
 // The number of a lane's row among the workgroup's.
 template <int L> __device__ __forceinline__ uint32_t row_in_group(int row_lanes) {
     const uint32_t row = threadIdx.x / row_lanes;

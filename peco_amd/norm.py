@@ -84,7 +84,7 @@ def _launch(x, weight, bias, eps, around_one, want_stats):
                 target = torch.empty(x.shape, dtype=x.dtype, device=device)
                 _, _, to = outer_axes(target)
         if want_stats:
-            stats = torch.empty((x.numel() // x.shape[-1], 2), dtype=torch.float32, device=device)
+            stats = torch.empty((x.numel() // x.shape[-1], 3), dtype=torch.float32, device=device)
         weight, bias, entry, wide = _affine(weight, bias)
         address = _native.address
         _native.check(_native.library().peco_layer_norm(

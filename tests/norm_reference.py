@@ -20,15 +20,17 @@ class Norm:
         self.x, self.x_type = x.double(), x.dtype
         self.factor = torch.ones((), dtype=torch.float64, device=x.device) if weight is None else \
             broadcast(weight, x) + float(around_one)
-        shift = torch.zeros((), dtype=torch.float64, device=x.device) if bias is None else broadcast(bias, x)
+        plus = torch.zeros((), dtype=torch.float64, device=x.device) if bias is None else broadcast(bias, x)
         self.mean = self.x.mean(-1, keepdim=True)
         self.inverse = ((self.x - self.mean).square().mean(-1, keepdim=True) + eps).rsqrt()
         self.n = (self.x - self.mean) * self.inverse
-        self.out = self.n * self.factor + shift
-        # The mean is off by at most ROW U mean|x|, which stays in every deviation; the inverse by half of what a sum of
-        # squares is, and a few operations.
-        self.n_off = ROW * U * (self.inverse * self.x.abs().mean(-1, keepdim=True) + self.n.abs())
-        self.out_off = self.n_off * self.factor.abs() + 3 * U * ((self.n * self.factor).abs() + shift.abs())
+        self.out = self.n * self.factor + plus
+        # The deviations are taken from a mean that is off by `shift` and their own mean, which is good to ROW U of
+        # their size; the sum of squares less that square is good to ROW U of either.
+        shift = ROW * U * self.x.abs().mean(-1, keepdim=True)
+        wide = (self.x - self.mean).abs().mean(-1, keepdim=True) + shift
+        self.n_off = ROW * U * (self.inverse * wide + self.n.abs() * (2 + (shift * self.inverse).square()))
+        self.out_off = self.n_off * self.factor.abs() + 3 * U * ((self.n * self.factor).abs() + plus.abs())
 
     def out_bound(self):
         return HALF_STEP[self.x_type] * 1.01 * self.out.abs() + self.out_off + SMALLEST[self.x_type]

@@ -183,6 +183,30 @@ def test_rows_that_are_not_finite_or_constant(channels, dtype, announce):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("channels", [8, 100, 128, 777, 2048, 5000])
+def test_rows_far_from_zero(channels, announce):
+    """fp32 rows 10^4 to 10^6 times as far from 0 as they are wide (steps of 2^-10 around 2^13, of 2^-4 around
+    -2^17), and constant ones: the bounds hold no term of the distance but its square."""
+    announce()
+    g = torch.Generator().manual_seed(channels)
+    steps = torch.randint(-3, 4, (3, 40, channels), generator=g).float()
+    x = torch.stack((8192 + steps[0] / 1024, -131072 + steps[1] / 16, torch.full((40, channels), 1000.1))).to(DEV)
+    weight, bias = (torch.randn(3, channels, generator=g).to(DEV) for _ in range(2))
+    grad = torch.randn(3, 40, channels, generator=g).to(DEV)
+    leaves = [t.requires_grad_() for t in (x, weight, bias)]
+    out = layer_norm(*leaves, 1e-6)
+    ref = Norm(x.detach(), weight.detach(), bias.detach(), 1e-6, False)
+    assert ((out.double() - ref.out).abs() <= ref.out_bound()).all()
+    (dx, dx_bound), (dw, dw_off), _ = ref.gradients(grad, True)
+    got = torch.autograd.grad(out, leaves, grad)
+    assert ((got[0].double() - dx).abs() <= dx_bound).all()
+    assert ((got[1].double() - dw).abs() <= 2.0 ** -24 * dw.abs() + dw_off).all()
+    # A check of the bounds themselves. Rows at 8192: a plain mean is good to 48 2^-24 8192 = 0.023, which times the
+    # inverse (up to 1000 for these steps) leaves 23 in n. Here its square, 550, stands at 48 2^-24 |n f|: 0.0016 of at most 9.
+    assert float(ref.out_bound()[0].max()) < 0.0016 * 9 * 1.1
+
+
+@pytest.mark.gpu
 def test_mixed_weights_empty_rows_and_module(announce):
     announce()
     x = torch.randn(2, 6, 64, device=DEV).bfloat16()
