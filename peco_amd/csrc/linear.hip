@@ -323,17 +323,21 @@ struct FewRows {
 __host__ __device__ inline int fused_pitch(int channels) { return (channels + kSegment - 1) / kSegment * kSegment + 16; }
 
 // x's rows as codes into LDS (0 behind a row's end), their scales into `scales`. Each row is taken by 8, 4, 2 or 1
-// wavefronts.
+// wavefronts, 8 channels a lane at a time, and read twice (the second time from the caches).
 template <int XT> __device__ __forceinline__ void quantize_into_lds(const ProductArgs& p, const FewRows& in, int8_t* codes,
                                                                     float* scales, uint32_t* most) {
     const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, pitch = fused_pitch(p.k);
     const int share = p.m == 1 ? 8 : p.m == 2 ? 4 : p.m <= 4 ? 2 : 1;  // wavefronts a row
-    const int part = wave % share, stride = share * kWave;
+    const int part = wave % share, lanes = share * kWave;
     for (int row = wave / share; row < p.m; row += kFewWaves / share) {
         const int64_t at = in.from.at(row);
         uint32_t top = 0;
-        for (int k = part * kWave + lane; k < p.k; k += stride)
-            top = max(top, __float_as_uint(load_elem<XT>(in.x, at + k)) & 0x7fffffffu);
+        for (int first = 0; first < p.k; first += lanes * 8) {
+            Piece<XT> x[1];
+            load_row<XT, false>(x, in.x, at, RowLanes{first / 8 + part * kWave + lane, lanes, p.k});
+#pragma unroll
+            for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(x[0].get(k)) & 0x7fffffffu);
+        }
         top = combine_lanes<MaxU, kWave>(top);
         if (lane == 0) most[row * share + part] = top;
     }
@@ -343,8 +347,15 @@ template <int XT> __device__ __forceinline__ void quantize_into_lds(const Produc
         uint32_t top = most[row * share];
         for (int i = 1; i < share; ++i) top = max(top, most[row * share + i]);
         const RowScale s(top);
-        for (int k = part * kWave + lane; k < pitch - 16; k += stride)
-            codes[row * pitch + k] = k < p.k ? static_cast<int8_t>(s.code(load_elem<XT>(in.x, at + k))) : 0;
+        for (int first = 0; first < pitch - 16; first += lanes * 8) {
+            const RowLanes r{first / 8 + part * kWave + lane, lanes, p.k};
+            Piece<XT> x[1];
+            load_row<XT, false>(x, in.x, at, r);
+            u32x2 packed{};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) packed[k / 4] |= (s.code(x[0].get(k)) & 0xffu) << (8 * (k % 4));
+            if (r.first(0) < pitch - 16) *reinterpret_cast<u32x2*>(codes + row * pitch + r.first(0)) = packed;
+        }
         if (part == 0 && lane == 0) scales[row] = s.scale();
     }
     __syncthreads();
