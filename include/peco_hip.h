@@ -418,7 +418,7 @@ int peco_layer_norm_grad(const void* x, const void* grad, void* dx, const int64_
                          int dtype, void* stream);
 
 /* Rows x [n0, n1, n2, channels] (as peco_layer_norm's, strides: 3) in 8 bits: with a the largest magnitude of a row,
- * codes = rint(x * (127 / a)) and scales = a / 127 in fp32, halves to even. Rows with a < 127 * 2^-126: codes and scale 0.
+ * codes = rint(x * (127 * (1 / a))) and scales = a * (1 / 127), each operation in fp32, halves to even. Rows with a < 127 * 2^-126: codes and scale 0.
  * Rows with an infinity or a NaN: codes 0, scale NaN. codes: int8, rows in order, pitch bytes apart (a multiple of 16,
  * at least channels; the bytes behind a row's channels, up to the next 8, become 0), on 16 bytes. scales: fp32, one a row. */
 int peco_quantize_rows(const void* x, const int64_t* strides, int8_t* codes, int64_t pitch, float* scales, int n0,

@@ -7,9 +7,10 @@
 // rows much further from 0 than they are wide is no small part of them. w and b are one row for all, or one for each entry of
 // the outermost axis (a modulation).
 //
-// Quantized rows: a = max |x|, code = rint(x * (127 / a)), scale = a / 127, in fp32 with IEEE division, halves to even.
-// For 16-bit rows these are the codes of the real quotients: x * 127 / a is 2^-18 or more off any half that it does not
-// meet exactly, and the two roundings move it by 2^-23 of itself. A row whose largest magnitude is below 127 * 2^-126,
+// Quantized rows: a = max |x|, code = rint(x * (127 * (1 / a))), scale = a * (1 / 127), each operation in fp32 (IEEE), halves
+// to even. For 16-bit rows these are the codes of the real quotients: x * 127 / a is 2^-20 or more off any half that it
+// does not meet exactly, the three roundings move it by 2^-22 of itself, and those that meet one have a = 127 * 2^e, for
+// which 127 * (1 / a) is exact. A row whose largest magnitude is below 127 * 2^-126,
 // where the scale would leave the normal numbers, counts as 0 (codes and scale 0). A row with an infinity or a NaN gets
 // codes 0 and a NaN as its scale, which makes its products NaN and no others. The norm's rows are quantized from
 // their fp32 values.

@@ -242,10 +242,10 @@ struct RowScale {
     bool finite, zero;
     __device__ __forceinline__ explicit RowScale(uint32_t bits)
         : most(__uint_as_float(bits)), finite(bits < 0x7f800000u), zero(most < 127.0f * 0x1p-126f) {
-        by = finite && !zero ? 127.0f / most : 0.0f;
+        by = finite && !zero ? 127.0f * (1.0f / most) : 0.0f;
     }
     __device__ __forceinline__ float scale() const {
-        return !finite ? __uint_as_float(0x7fc00000u) : zero ? 0.0f : most / 127.0f;
+        return !finite ? __uint_as_float(0x7fc00000u) : zero ? 0.0f : most * (1.0f / 127.0f);
     }
     __device__ __forceinline__ int code(float x) const { return finite ? static_cast<int>(rintf(x * by)) : 0; }
 };

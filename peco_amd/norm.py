@@ -69,11 +69,11 @@ def _channels_adjacent(t):
 
 
 def _launch(x, weight, bias, eps, around_one, want_stats):
+    """(output, statistics, what a gradient call takes again); the last two None without ``want_stats``."""
     out = torch.empty_like(x)
-    stats = None
     if x.numel() == 0:
-        return out, stats
-    device = x.device
+        return out, None, None
+    device, channels, stats, plan = x.device, x.shape[-1], None, None
     with _native.on_device(device):
         _native.require_gfx950(device)
         source, sizes, strides = outer_axes(_channels_adjacent(x))
@@ -83,15 +83,17 @@ def _launch(x, weight, bias, eps, around_one, want_stats):
             if to is None or out.stride(-1) != 1:
                 target = torch.empty(x.shape, dtype=x.dtype, device=device)
                 _, _, to = outer_axes(target)
-        if want_stats:
-            stats = torch.empty((x.numel() // x.shape[-1], 3), dtype=torch.float32, device=device)
         weight, bias, entry, wide = _affine(weight, bias)
+        code = _native.dtype_code(x.dtype)
+        if want_stats:
+            stats = torch.empty((x.numel() // channels, 3), dtype=torch.float32, device=device)
+            plan = sizes, channels, strides if source is x else None, entry, wide, code
         address = _native.address
         _native.check(_native.library().peco_layer_norm(
             source.data_ptr(), target.data_ptr(), _LONGS[6](*strides, *to), address(weight), address(bias), entry, wide,
-            int(around_one), eps, address(stats), *sizes, x.shape[-1], _native.dtype_code(x.dtype),
+            int(around_one), eps, address(stats), *sizes, channels, code,
             _native.retain(device, source, weight, bias)), "PECO HIP layer norm")
-        return (out if target is out else out.copy_(target)), stats
+        return out if target is out else out.copy_(target), stats, plan
 
 
 @functools.lru_cache(maxsize=1024)
@@ -100,56 +102,59 @@ def _grad_floats(device_index, *sizes):
     return _native.library().peco_layer_norm_grad_workspace_size(*sizes)
 
 
-def _gradients(x, weight, bias, stats, grad, around_one, needs):
-    """Gradients of x, weight and bias, None where ``needs`` is not set."""
+def _gradients(ctx, grad):
+    """Gradients of x, weight and bias, None where none is asked for.
+
+    Few steps: torch's engine calls this on a thread of its own, whose core has to fetch everything that it touches (a
+    step costs two to three times what it does on the caller's). The engine has made the forward's device and stream
+    the current ones, on which the forward recorded the tensors it saved.
+    """
     if not _native.plain_gradient(grad):
         raise RuntimeError("the gradient of layer_norm's output must be an ordinary tensor (no tracing, transforms, "
                            "batches or tangents)")
-    device = x.device
-    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if needs[0] else None
-    dweight = torch.empty_like(weight, memory_format=torch.contiguous_format) if needs[1] else None
-    dbias = torch.empty_like(bias, memory_format=torch.contiguous_format) if needs[2] else None
-    if x.numel() == 0:
-        return dx, *(None if t is None else t.zero_() for t in (dweight, dbias))
-    with _native.on_device(device):
-        x, sizes, strides = outer_axes(_channels_adjacent(x))
-        grad, _, by = outer_axes(_channels_adjacent(grad))
-        rows = sizes[2] * x.shape[-1]
-        to = (sizes[1] * rows, rows, x.shape[-1])  # (dx is contiguous)
-        weight, bias, entry, wide = _affine(weight, bias)
-        workspace, floats = None, 0
-        if dweight is not None or dbias is not None:
-            floats = _grad_floats(device.index, *sizes, x.shape[-1], int(entry > 0))
-            workspace = torch.empty(floats, dtype=torch.float32, device=device)
-        address = _native.address
-        _native.check(_native.library().peco_layer_norm_grad(
-            x.data_ptr(), grad.data_ptr(), address(dx), _LONGS[9](*strides, *by, *to), address(weight),
-            entry if weight is not None else 0, wide, int(around_one), stats.data_ptr(), address(dweight),
-            address(dbias), int(entry > 0), address(workspace), floats, *sizes, x.shape[-1],
-            _native.dtype_code(x.dtype), _native.retain(device, x, grad, weight, stats)), "PECO HIP layer norm gradient")
-    return dx, dweight, dbias
+    x, weight, bias, stats = ctx.saved_tensors
+    needs, dense = ctx.needs_input_grad, torch.contiguous_format
+    dx = torch.empty_like(x, memory_format=dense) if needs[0] else None
+    dweight = torch.empty_like(weight, memory_format=dense) if needs[1] else None
+    dbias = torch.empty_like(bias, memory_format=dense) if needs[2] else None
+    if ctx.plan is None:  # no rows
+        return dx, *(None if t is None else t.zero_() for t in (dweight, dbias)), None, None
+    sizes, channels, strides, entry, wide, code = ctx.plan
+    if strides is None:
+        x, _, strides = outer_axes(x.contiguous())
+    grad, _, by = outer_axes(_channels_adjacent(grad))
+    rows = sizes[2] * channels
+    workspace, floats, device = None, 0, x.device
+    if needs[1] or needs[2]:
+        floats = _grad_floats(device.index, *sizes, channels, int(entry > 0))
+        workspace = torch.empty(floats, dtype=torch.float32, device=device)
+    if weight is not None:
+        weight = weight.contiguous()
+    address = _native.address
+    status = _native.library().peco_layer_norm_grad(
+        x.data_ptr(), grad.data_ptr(), address(dx), _LONGS[9](*strides, *by, sizes[1] * rows, rows, channels),
+        address(weight), 0 if weight is None else entry, wide, ctx.around_one, stats.data_ptr(), address(dweight),
+        address(dbias), int(entry > 0), address(workspace), floats, *sizes, channels, code, _native.retain(device, grad))
+    if status:
+        _native.check(status, "PECO HIP layer norm gradient")
+    return dx, dweight, dbias, None, None
+
+
+_graph_of_gradients = torch.autograd.function.once_differentiable(_gradients)
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, around_one):
-        out, stats = _launch(x, weight, bias, eps, around_one, True)
+        out, stats, ctx.plan = _launch(x, weight, bias, eps, around_one, True)
         ctx.save_for_backward(x, weight, bias, stats)
-        ctx.around_one = around_one
+        ctx.around_one = int(around_one)
         return out
 
     @staticmethod
     def backward(ctx, grad):
         # (The wrapper costs as much as a launch; without a graph of the gradients it changes nothing.)
-        return _graph_of_gradients(ctx, grad) if torch.is_grad_enabled() else _backward(ctx, grad)
-
-
-def _backward(ctx, grad):
-    x, weight, bias, stats = ctx.saved_tensors
-    return *_gradients(x, weight, bias, stats, grad, ctx.around_one, ctx.needs_input_grad[:3]), None, None
-
-
-_graph_of_gradients = torch.autograd.function.once_differentiable(_backward)
+        return _graph_of_gradients(ctx, grad) if torch.is_grad_enabled() else _gradients(ctx, grad)
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,

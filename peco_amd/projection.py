@@ -3,9 +3,10 @@
 ``quantize_rows`` makes the codes, ``int8_linear`` the product, ``Int8Linear`` is a layer of it in place of
 ``torch.nn.Linear`` (``model.quantize_projections`` puts it into every attention block of a transformer).
 
-A row's codes are ``rint(x * (127 / a))`` with a its largest magnitude, and its scale is ``a / 127``: fp32 arithmetic,
-halves to even. A row whose largest magnitude is below 127 * 2^-126 counts as 0. A row with an infinity or a NaN has
-codes 0 and a NaN as its scale, so its products are NaN, and no others.
+A row's codes are ``rint(x * (127 * (1 / a)))`` with a its largest magnitude, and its scale is ``a * (1 / 127)``, each
+operation in fp32, halves to even (for 16-bit rows these are the nearest codes to ``127 x / a``). A row whose largest
+magnitude is below 127 * 2^-126 counts as 0. A row with an infinity or a NaN has codes 0 and a NaN as its scale, so its
+products are NaN, and no others.
 """
 from __future__ import annotations
 

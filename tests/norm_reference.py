@@ -65,8 +65,9 @@ def quantized(x):
     x = x.float().cpu()
     most = x.abs().amax(-1, keepdim=True)
     kept = most >= 127 * 2.0 ** -126
-    by = torch.where(kept, torch.tensor(127.0) / most, torch.zeros(()))
-    return (x * by).round().to(torch.int8), torch.where(kept, most / torch.tensor(127.0), torch.zeros(()))[..., 0]
+    one, steps = torch.tensor(1.0), torch.tensor(127.0)
+    by = torch.where(kept, steps * (one / most), torch.zeros(()))
+    return (x * by).round().to(torch.int8), torch.where(kept, most * (one / steps), torch.zeros(()))[..., 0]
 
 
 def product(codes, scales, weight, weight_scales, bias, dtype):

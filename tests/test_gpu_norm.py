@@ -113,7 +113,8 @@ def test_gradients_against_differences(announce):
 @pytest.mark.parametrize("shape,entries", SHAPES)
 def test_quantized_rows(shape, entries, dtype, announce):
     """Codes of the norm's fp32 rows: every value within half a step of the row, and what fp32 leaves of the norm; the
-    largest has code 127."""
+    largest has code 127. (The factor of the codes has three roundings, the scale two: 127 steps * 3 2^-24 and 2^-23
+    of the largest value are together below 2^-21 of it.)"""
     announce()
     x, weight, bias, _ = _inputs(shape, entries, dtype, False, 2)
     for part in _layouts(x):
@@ -121,7 +122,7 @@ def test_quantized_rows(shape, entries, dtype, announce):
         rows = layer_norm_rows(part, weight, bias, 1e-5, around_one=True)
         assert rows.shape == part.shape and rows.scales.shape == part.shape[:-1]
         most = ref.out.abs().amax(-1, keepdim=True)
-        off = ref.out_off.amax(-1, keepdim=True) + 2.0 ** -22 * most
+        off = ref.out_off.amax(-1, keepdim=True) + 2.0 ** -21 * most
         assert ((rows.dequantize(torch.float64) - ref.out).abs() <= most / 254 + off).all()
         assert ((rows.scales.double() * 127)[..., None] - most).abs().le(off).all()
         assert (rows.codes.abs().amax(-1) == 127).all()
