@@ -8,15 +8,16 @@
 // the outermost axis (a modulation).
 //
 // Quantized rows: a = max |x|, code = rint(x * (127 * (1 / a))), scale = a * (1 / 127), each operation in fp32 (IEEE), halves
-// to even. For 16-bit rows these are the codes of the real quotients: x * 127 / a is 2^-20 or more off any half that it
-// does not meet exactly, the three roundings move it by 2^-22 of itself, and those that meet one have a = 127 * 2^e, for
-// which 127 * (1 / a) is exact. A row whose largest magnitude is below 127 * 2^-126,
-// where the scale would leave the normal numbers, counts as 0 (codes and scale 0). A row with an infinity or a NaN gets
-// codes 0 and a NaN as its scale, which makes its products NaN and no others. The norm's rows are quantized from
-// their fp32 values.
+// to even. For 16-bit rows these are the codes nearest to the real quotients: x * 127 / a is 2^-20 or more off any half
+// that it does not meet exactly, and the three roundings move it by 2^-22 of itself; where it is a half (x = a / 2), both
+// neighbours are. A row whose largest magnitude is below 127 * 2^-126, where the scale would leave the normal numbers,
+// counts as 0 (codes and scale 0). A row with an infinity or a NaN gets codes 0 and a NaN as its scale, which makes its
+// products NaN and no others. The norm's rows are quantized from their fp32 values.
 //
 // HBM-bound: a row is read once and its result written once. Workgroups walk over rows with the next row's loads in flight
-// while one is normalised, and keep the weight in registers for all of their rows.
+// while one is normalised, and keep the weight in registers for all of their rows. Measured: norm of 119056 x 4096 in fp16
+// 348-357 us (1.95 GB, 5.5 TB/s; a copy of 1 GB runs at 5.05-5.08), 7006 x 2048 in bf16 15 us (3.8), 24 x 7006 rows of 128 with
+// their statistics 19 us (4.6); codes of 119056 x 4096 270 us (1.46 GB, 5.4), of 7006 x 2048 9.5 us, of its norm 16 us.
 #include "rows.hpp"
 
 #include <algorithm>
@@ -142,7 +143,7 @@ __global__ __launch_bounds__(512) void norm_kernel(NormArgs a) {
     }
 }
 
-// Workgroups: enough for every CU to hold what its registers allow (measured over 2 to 16 a CU).
+// Workgroups: as many as a CU holds of the smallest kinds; of those that hold fewer, the rest start as they end.
 template <int DT, int L, int kChunks, bool kWhole, int kMode>
 int launch(const NormArgs& a, const RowShape& s, hipStream_t stream) {
     const int64_t blocks = std::min<int64_t>(ceil_div(a.rows, s.rows), 8 * device_compute_units());
