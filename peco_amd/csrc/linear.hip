@@ -497,7 +497,8 @@ int check_product(const int8_t* weight, int64_t weight_pitch, const float* weigh
     if (dtype != kBF16 && dtype != kF16 && dtype != kF32) return kUnsupportedDtype;
     // Sums of 2^17 products of -128 would leave 32 bits, and a tile's offsets are 32 bits.
     if (channels >= 1 << 17 || weight_pitch > 1 << 22 || rows > 0x3fffffff || outputs > 0x3fffffff) return kUnsupportedShape;
-    return kOk;
+    // (Results that large take wide tiles.)
+    return fits_grid(ceil_div(rows, Wide::kTokens) * ceil_div(outputs, Wide::kOutputs), Wide::kThreads) ? kOk : kUnsupportedShape;
 }
 
 int run_product(const ProductArgs& p, int dtype, hipStream_t s) {

@@ -184,6 +184,55 @@ def test_rows_that_are_not_finite_or_constant(channels, dtype, announce):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape,entries", [((2, 9, 3, 64), 2), ((1, 3, 37, 128), 0), ((2, 5, 1111), 0), ((3, 3, 2048), 3)])
+def test_gradients_without_a_weight_or_a_bias(shape, entries, dtype, announce):
+    announce()
+    x, weight, bias, grad = _inputs(shape, entries, dtype, False, 7)
+    half = HALF_STEP[dtype] * 1.01
+    for w, b in ((None, None), (None, bias), (weight, None)):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b) if t is not None]
+        given = iter(leaves[1:])
+        out = layer_norm(leaves[0], None if w is None else next(given), None if b is None else next(given), 1e-5)
+        got = torch.autograd.grad(out, leaves, grad)
+        (dx, dx_bound), (dw, dw_off), (db, db_off) = Norm(x, w, b, 1e-5, False).gradients(grad, entries > 0)
+        assert ((got[0].double() - dx).abs() <= dx_bound).all()
+        if w is not None:
+            assert ((got[1].double() - dw).abs() <= half * dw.abs() + dw_off + 2.0 ** -25).all()
+        if b is not None:
+            assert ((got[1].double() - db).abs() <= half * db.abs() + db_off + 2.0 ** -25).all()
+    frozen = x.detach()
+    leaf = weight.detach().requires_grad_()
+    only, = torch.autograd.grad(layer_norm(frozen, leaf, bias, 1e-5), leaf, grad)  # rows without a gradient
+    assert ((only.double() - dw).abs() <= half * dw.abs() + dw_off + 2.0 ** -25).all()
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once(announce):
+    """Forward and backward of two inputs on two streams, several in flight, against one after the other."""
+    announce()
+    g = torch.Generator().manual_seed(11)
+    inputs = [tuple(torch.randn(2, 900, 1024, generator=g).to(DEV) for _ in range(2)) for _ in range(2)]
+    weight, bias = (torch.randn(2, 1024, generator=g).to(DEV).requires_grad_() for _ in range(2))
+
+    def step(x, grad):
+        x = x.detach().requires_grad_()
+        out = layer_norm(x, weight, bias)
+        return out.detach(), *torch.autograd.grad(out, (x, weight, bias), grad)
+
+    want = [step(*i) for i in inputs]
+    streams = [torch.cuda.Stream() for _ in inputs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for k, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[k].append(step(*inputs[k]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for k in range(2) for out in got[k] for a, b in zip(out, want[k]))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("channels", [8, 100, 128, 777, 2048, 5000])
 def test_rows_far_from_zero(channels, announce):
     """fp32 rows 10^4 to 10^6 times as far from 0 as they are wide (steps of 2^-10 around 2^13, of 2^-4 around

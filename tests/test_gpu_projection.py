@@ -149,6 +149,24 @@ def test_streams_and_graphs(rows, announce):
 
 
 @pytest.mark.gpu
+def test_calls_on_two_streams_at_once(announce):
+    announce()
+    g = torch.Generator().manual_seed(13)
+    weight = quantize_rows(torch.randn(1100, 900, generator=g).to(DEV))
+    inputs = [torch.randn(n, 900, generator=g).to(DEV).bfloat16() for n in (1500, 9)]
+    want = [int8_linear(x, weight) for x in inputs]
+    streams = [torch.cuda.Stream() for _ in inputs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for k, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[k].append(int8_linear(inputs[k], weight))
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want[k]) for k in range(2) for out in got[k])
+
+
+@pytest.mark.gpu
 def test_results_past_32_bit_offsets(announce):
     """A result of more than 2^32 elements, and rows of codes more than 2^32 bytes behind the first."""
     announce()
