@@ -16,8 +16,8 @@
 //
 // HBM-bound: a row is read once and its result written once. Workgroups walk over rows with the next row's loads in flight
 // while one is normalised, and keep the weight in registers for all of their rows. Measured: norm of 119056 x 4096 in fp16
-// 348-357 us (1.95 GB, 5.5 TB/s; a copy of 1 GB runs at 5.05-5.08), 7006 x 2048 in bf16 15 us (3.8), 24 x 7006 rows of 128 with
-// their statistics 19 us (4.6); codes of 119056 x 4096 270 us (1.46 GB, 5.4), of 7006 x 2048 9.5 us, of its norm 16 us.
+// 336-348 us (1.95 GB, 5.7 TB/s; a copy of 1 GB runs at 5.05-5.08), 7006 x 2048 in bf16 12-13 us (4.6), 24 x 7006 rows of 128
+// with their statistics 16-20 us; codes of 119056 x 4096 247 us (1.46 GB, 5.9), of 7006 x 2048 8-10 us, of its norm 12-14 us.
 #include "rows.hpp"
 
 #include <algorithm>
@@ -160,8 +160,14 @@ template <int DT, int L, int kChunks, bool kWhole, int kMode> int resident(int t
 // 8 a CU, where 3 fit, most had one row: 7006 x 2048 in bf16 14.6 us for 12.5, 2 x 7006 with statistics 25.9 for 21.9.
 template <int DT, int L, int kChunks, bool kWhole, int kMode>
 int launch(const NormArgs& a, const RowShape& s, hipStream_t stream) {
-    const int64_t most = static_cast<int64_t>(resident<DT, L, kChunks, kWhole, kMode>(s.threads)) * device_compute_units();
-    const int64_t blocks = std::min(ceil_div(a.rows, s.rows), most);
+    int groups = resident<DT, L, kChunks, kWhole, kMode>(s.threads);
+    if (kMode == kCodes && kWhole) {
+        // Codes alone are quickest with 3 a CU (300000 x 1024 in bf16 165 us, with 4 or 8 176 and 181), rows of 4 pieces that
+        // do not stay in the 256 MB of the last cache with 2 (119056 x 4096 247 us, 272 with 3; 7006 x 4096 16.8 and 15.7).
+        const int64_t bytes = static_cast<int64_t>(a.rows) * a.channels * (DT == kF32 ? 4 : 2);
+        groups = std::min(groups, kChunks == 4 && bytes > int64_t{256} << 20 ? 2 : 3);
+    }
+    const int64_t blocks = std::min<int64_t>(ceil_div(a.rows, s.rows), static_cast<int64_t>(groups) * device_compute_units());
     hipLaunchKernelGGL((norm_kernel<DT, L, kChunks, kWhole, kMode>), dim3(static_cast<unsigned>(blocks)),
                        dim3(s.threads), 0, stream, a);
     return hipGetLastError();

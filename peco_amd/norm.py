@@ -43,7 +43,8 @@ def _check(x, weight, bias, eps, around_one, name):
             raise ValueError("weight and bias must reside on the device of the rows")
     if not x.is_cuda:
         raise ValueError("peco_amd layer norms run on GPU tensors; CPU tensors are not supported")
-    if not _native.plain_tensors(x, *(t for t in (weight, bias) if t is not None)):
+    tensors = (x,) if weight is None else (x, weight)
+    if not _native.plain_tensors(*(tensors if bias is None else (*tensors, bias))):
         raise RuntimeError(f"{name} takes ordinary tensors (no tracing, transforms or tangents)")
     if x.numel() >= channels << 30:
         raise ValueError(f"{name} supports fewer than 2^30 rows")
@@ -52,6 +53,12 @@ def _check(x, weight, bias, eps, around_one, name):
         if weight.dim() != bias.dim():
             weight, bias = weight.expand(shape[0], channels), bias.expand(shape[0], channels)
     return weight, bias
+
+
+def _records(x, weight, bias):
+    """Whether a gradient of some input is recorded."""
+    return torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                        (bias is not None and bias.requires_grad))
 
 
 def _affine(weight, bias):
@@ -173,8 +180,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     gradients on that graph's stream and end the process).
     """
     weight, bias = _check(x, weight, bias, eps, around_one, "layer_norm")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
-        if any(t is not None and t.dim() == 2 for t in (weight, bias)) and x.shape[0] > 65535:
+    if _records(x, weight, bias):
+        if x.dim() > 1 and x.shape[0] > 65535 and any(t is not None and t.dim() == 2 for t in (weight, bias)):
             raise ValueError("gradients support weights of at most 65535 entries")
         return _LayerNorm.apply(x, weight, bias, eps, around_one)
     return _launch(x, weight, bias, eps, around_one, False)[0]
@@ -185,7 +192,7 @@ def layer_norm_rows(x: torch.Tensor, weight: torch.Tensor | None = None, bias: t
     """``projection.quantize_rows`` of ``layer_norm``'s rows in one pass, which take their codes from their fp32 values
     (they are not rounded to x's dtype on the way). For inference: it has no gradient."""
     weight, bias = _check(x, weight, bias, eps, around_one, "layer_norm_rows")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if _records(x, weight, bias):
         raise RuntimeError("layer_norm_rows supports inference only; use torch.no_grad()")
     codes, scales, pitch = empty_codes(x)
     if x.numel():
