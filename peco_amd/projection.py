@@ -55,7 +55,7 @@ def empty_codes(x):
     step = 16 if channels < 512 else 128
     pitch = -(-channels // step) * step
     codes = torch.empty((*outer, pitch), dtype=torch.int8, device=x.device)
-    return codes if pitch == channels else codes[..., :channels], \
+    return codes if pitch == channels else codes.narrow(-1, 0, channels), \
         torch.empty(outer, dtype=torch.float32, device=x.device), pitch
 
 
