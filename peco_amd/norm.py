@@ -94,7 +94,7 @@ def _launch(x, weight, bias, eps, around_one, want_stats):
         code = _native.dtype_code(x.dtype)
         if want_stats:
             stats = torch.empty((x.numel() // channels, 3), dtype=torch.float32, device=device)
-            plan = sizes, channels, strides if source is x else None, entry, wide, code
+            plan = sizes, channels, entry, wide, code
         address = _native.address
         _native.check(_native.library().peco_layer_norm(
             source.data_ptr(), target.data_ptr(), _LONGS[6](*strides, *to), address(weight), address(bias), entry, wide,
@@ -109,6 +109,10 @@ def _grad_floats(device_index, *sizes):
     return _native.library().peco_layer_norm_grad_workspace_size(*sizes)
 
 
+def _kind(t):
+    return None if t is None else (t.shape, t.dtype, t.device)
+
+
 def _gradients(ctx, grad):
     """Gradients of x, weight and bias, None where none is asked for.
 
@@ -119,17 +123,19 @@ def _gradients(ctx, grad):
     if not _native.plain_gradient(grad):
         raise RuntimeError("the gradient of layer_norm's output must be an ordinary tensor (no tracing, transforms, "
                            "batches or tangents)")
-    x, weight, bias, stats = ctx.saved_tensors
+    x, weight, bias, stats = saved = ctx.saved_tensors
+    if tuple(map(_kind, saved)) != ctx.kinds:
+        raise RuntimeError("a tensor that layer_norm saved for its gradient has another shape, dtype or device now")
     needs, dense = ctx.needs_input_grad, torch.contiguous_format
     dx = torch.empty_like(x, memory_format=dense) if needs[0] else None
     dweight = torch.empty_like(weight, memory_format=dense) if needs[1] else None
     dbias = torch.empty_like(bias, memory_format=dense) if needs[2] else None
     if ctx.plan is None:  # no rows
         return dx, *(None if t is None else t.zero_() for t in (dweight, dbias)), None, None
-    sizes, channels, strides, entry, wide, code = ctx.plan
-    if strides is None:
-        x, _, strides = outer_axes(x.contiguous())
-    grad, _, by = outer_axes(_channels_adjacent(grad))
+    sizes, channels, entry, wide, code = ctx.plan
+    source, _, strides = outer_axes(_channels_adjacent(x))  # (hooks of saved tensors may lay out x and stats anew)
+    stats = stats.contiguous()
+    above, _, by = outer_axes(_channels_adjacent(grad))
     rows = sizes[2] * channels
     workspace, floats, device = None, 0, x.device
     if needs[1] or needs[2]:
@@ -139,7 +145,7 @@ def _gradients(ctx, grad):
         weight = weight.contiguous()
     address = _native.address
     status = _native.library().peco_layer_norm_grad(
-        x.data_ptr(), grad.data_ptr(), address(dx), _LONGS[9](*strides, *by, sizes[1] * rows, rows, channels),
+        source.data_ptr(), above.data_ptr(), address(dx), _LONGS[9](*strides, *by, sizes[1] * rows, rows, channels),
         address(weight), 0 if weight is None else entry, wide, ctx.around_one, stats.data_ptr(), address(dweight),
         address(dbias), int(entry > 0), address(workspace), floats, *sizes, channels, code, _native.retain(device, grad))
     if status:
@@ -154,7 +160,9 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, around_one):
         out, stats, ctx.plan = _launch(x, weight, bias, eps, around_one, True)
-        ctx.save_for_backward(x, weight, bias, stats)
+        saved = x, weight, bias, stats
+        ctx.save_for_backward(*saved)
+        ctx.kinds = tuple(map(_kind, saved))
         ctx.around_one = int(around_one)
         return out
 

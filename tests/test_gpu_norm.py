@@ -208,6 +208,45 @@ def test_gradients_without_a_weight_or_a_bias(shape, entries, dtype, announce):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape,entries", [((2, 7, 3, 64), 2), ((3, 5, 1111), 0), ((2, 9, 2048), 2)])
+def test_saved_tensors_that_come_back_laid_out_anew(shape, entries, dtype, announce):
+    """Hooks of saved tensors keep their sizes and values, not their strides: the gradients are the same bits."""
+    announce()
+    x, weight, bias, grad = _inputs(shape, entries, dtype, False, 2)
+
+    def apart(t):  # the same values, every second element
+        return torch.zeros(*t.shape, 2, dtype=t.dtype, device=DEV)[..., 0].copy_(t.detach())
+
+    def dense(t):
+        return t.detach().clone(memory_format=torch.contiguous_format)
+
+    for part in _layouts(x):
+        leaves = [t.detach().requires_grad_() for t in (part, weight, bias)]
+        want = torch.autograd.grad(layer_norm(*leaves, 1e-5), leaves, grad)
+        for pack in (dense, apart):
+            with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+                out = layer_norm(*leaves, 1e-5)
+            assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, leaves, grad), want))
+    with torch.autograd.graph.save_on_cpu():
+        out = layer_norm(*leaves, 1e-5)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, leaves, grad), want))
+
+
+@pytest.mark.gpu
+def test_leaves_that_change_before_the_gradient_are_refused(announce):
+    """A module may be cast or moved between its forward and its backward call."""
+    announce()
+    for change in (torch.Tensor.bfloat16, torch.Tensor.cpu, lambda t: t[:32].clone()):
+        for which in range(3):
+            leaves = [torch.ones(64, device=DEV).requires_grad_() for _ in range(3)]
+            out = layer_norm(*leaves)
+            leaves[which].data = change(leaves[which].data)
+            with pytest.raises(RuntimeError):
+                torch.autograd.grad(out, [t for i, t in enumerate(leaves) if i != which], torch.ones_like(out))
+
+
+@pytest.mark.gpu
 def test_calls_on_two_streams_at_once(announce):
     """Forward and backward of two inputs on two streams, several in flight, against one after the other."""
     announce()
