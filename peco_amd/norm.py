@@ -49,7 +49,8 @@ def _check(x, weight, bias, eps, around_one, name):
     if x.numel() >= channels << 30:
         raise ValueError(f"{name} supports fewer than 2^30 rows")
     if weight is not None and bias is not None and (weight.dtype != bias.dtype or weight.dim() != bias.dim()):
-        weight, bias = weight.float(), bias.float()  # (one type, one shape)
+        _native.retain(x.device, weight, bias)  # (read by what follows)
+        weight, bias = weight.float(), bias.float()  # one type, one shape
         if weight.dim() != bias.dim():
             weight, bias = weight.expand(shape[0], channels), bias.expand(shape[0], channels)
     return weight, bias
@@ -90,6 +91,7 @@ def _launch(x, weight, bias, eps, around_one, want_stats):
             if to is None or out.stride(-1) != 1:
                 target = torch.empty(x.shape, dtype=x.dtype, device=device)
                 _, _, to = outer_axes(target)
+        given = weight, bias
         weight, bias, entry, wide = _affine(weight, bias)
         code = _native.dtype_code(x.dtype)
         if want_stats:
@@ -99,7 +101,7 @@ def _launch(x, weight, bias, eps, around_one, want_stats):
         _native.check(_native.library().peco_layer_norm(
             source.data_ptr(), target.data_ptr(), _LONGS[6](*strides, *to), address(weight), address(bias), entry, wide,
             int(around_one), eps, address(stats), *sizes, channels, code,
-            _native.retain(device, source, weight, bias)), "PECO HIP layer norm")
+            _native.retain(device, x, *given)), "PECO HIP layer norm")
         return out if target is out else out.copy_(target), stats, plan
 
 
@@ -207,12 +209,13 @@ def layer_norm_rows(x: torch.Tensor, weight: torch.Tensor | None = None, bias: t
         device = x.device
         with _native.on_device(device):
             _native.require_gfx950(device)
-            x, sizes, strides = outer_axes(_channels_adjacent(x))
+            source, sizes, strides = outer_axes(_channels_adjacent(x))
+            given = weight, bias
             weight, bias, entry, wide = _affine(weight, bias)
             _native.check(_native.library().peco_layer_norm_rows(
-                x.data_ptr(), _LONGS[3](*strides), _native.address(weight), _native.address(bias), entry, wide,
+                source.data_ptr(), _LONGS[3](*strides), _native.address(weight), _native.address(bias), entry, wide,
                 int(around_one), eps, codes.data_ptr(), pitch, scales.data_ptr(), *sizes, x.shape[-1],
-                _native.dtype_code(x.dtype), _native.retain(device, x, weight, bias)), "PECO HIP layer norm")
+                _native.dtype_code(x.dtype), _native.retain(device, x, *given)), "PECO HIP layer norm")
     return QuantizedRows(codes, scales)
 
 

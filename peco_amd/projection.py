@@ -116,9 +116,9 @@ def quantize_rows(x: torch.Tensor) -> QuantizedRows:
         device = x.device
         with _native.on_device(device):
             _native.require_gfx950(device)
-            x, sizes, strides = outer_axes(x if x.stride(-1) == 1 else x.contiguous())
+            source, sizes, strides = outer_axes(x if x.stride(-1) == 1 else x.contiguous())
             _native.check(_native.library().peco_quantize_rows(
-                x.data_ptr(), _LONG3(*strides), codes.data_ptr(), pitch, scales.data_ptr(), *sizes, x.shape[-1],
+                source.data_ptr(), _LONG3(*strides), codes.data_ptr(), pitch, scales.data_ptr(), *sizes, x.shape[-1],
                 _native.dtype_code(x.dtype), _native.retain(device, x)), "PECO HIP row quantization")
     return QuantizedRows(codes, scales)
 
@@ -208,23 +208,24 @@ def int8_linear(x, weight: QuantizedRows, bias: torch.Tensor | None = None, *,
         _native.require_gfx950(device)
         weight_codes, weight_pitch = _code_rows(weight.codes)
         weight_scales = weight.scales.contiguous()
-        bias = None if bias is None else bias.contiguous()
-        common = (weight_codes.data_ptr(), weight_pitch, weight_scales.data_ptr(), _native.address(bias),
+        added = None if bias is None else bias.contiguous()
+        common = (weight_codes.data_ptr(), weight_pitch, weight_scales.data_ptr(), _native.address(added),
                   int(bias is not None and bias.dtype == torch.float32), out.data_ptr())
+        stream = _native.retain(device, *tensors)  # (copies of them are this stream's own)
         if quantized:
             codes, pitch = _code_rows(rows)
             scales = x.scales.contiguous()
             status = _native.library().peco_int8_linear(
                 codes.data_ptr(), pitch, scales.data_ptr(), *common, count, channels, outputs, _native.dtype_code(dtype),
-                _native.retain(device, codes, scales, weight_codes, weight_scales, bias))
+                stream)
         else:
-            x, sizes, strides = outer_axes(x if x.stride(-1) == 1 else x.contiguous())
+            source, sizes, strides = outer_axes(x if x.stride(-1) == 1 else x.contiguous())
             codes = _native.dtype_code(x.dtype), _native.dtype_code(dtype)
             size = _workspace_bytes(count, channels, *codes)
             workspace = torch.empty(size, dtype=torch.int8, device=device) if size else None
             status = _native.library().peco_int8_linear_rows(
-                x.data_ptr(), _LONG3(*strides), *sizes, codes[0], *common, _native.address(workspace), size, channels,
-                outputs, codes[1], _native.retain(device, x, weight_codes, weight_scales, bias))
+                source.data_ptr(), _LONG3(*strides), *sizes, codes[0], *common, _native.address(workspace), size, channels,
+                outputs, codes[1], stream)
         _native.check(status, "PECO HIP 8-bit projection")
     return out
 

@@ -272,6 +272,38 @@ def test_calls_on_two_streams_at_once(announce):
 
 
 @pytest.mark.gpu
+def test_inputs_that_are_freed_while_a_copy_of_them_is_due(announce):
+    """Inputs that the call copies (channels apart, weights of two types or apart) belong to another stream, and are freed
+    there before the call's stream has come to the copy: their memory must not be handed out until it has."""
+    announce()
+    g = torch.Generator().manual_seed(17)
+    x = torch.randn(6, 500, 1024, generator=g).to(DEV)
+    weight, bias = (torch.randn(6, 1024, generator=g).to(DEV) for _ in range(2))
+
+    def apart(t):
+        return torch.zeros(*t.shape, 2, dtype=t.dtype, device=DEV)[..., 0].copy_(t)
+
+    calls = [(layer_norm, lambda: (apart(x), apart(weight), apart(bias))),
+             (layer_norm, lambda: (apart(x.half()), weight.clone(), bias.half())),
+             (lambda *t: layer_norm_rows(*t).codes, lambda: (apart(x), apart(weight), apart(bias))),
+             (lambda *t: quantize_rows(*t).codes, lambda: (apart(x),))]
+    side = torch.cuda.Stream()
+    for call, make in calls:
+        want = call(*make())
+        inputs = make()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+            got = call(*inputs)
+        sizes = [(t.untyped_storage().nbytes(), t.untyped_storage().data_ptr()) for t in inputs]
+        del inputs
+        others = [torch.full((size,), 119, dtype=torch.uint8, device=DEV) for size, _ in sizes]
+        assert not {t.data_ptr() for t in others} & {at for _, at in sizes}
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("channels", [8, 100, 128, 777, 2048, 5000])
 def test_rows_far_from_zero(channels, announce):
     """fp32 rows 10^4 to 10^6 times as far from 0 as they are wide (steps of 2^-10 around 2^13, of 2^-4 around

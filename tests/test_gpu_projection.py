@@ -167,6 +167,44 @@ def test_calls_on_two_streams_at_once(announce):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("quantized", [False, True])
+def test_inputs_that_are_freed_while_a_copy_of_them_is_due(quantized, announce):
+    """Inputs that the call copies (channels, codes, scales or the bias apart) belong to another stream, and are freed there
+    before the call's stream has come to the copy: their memory must not be handed out until it has."""
+    announce()
+    g = torch.Generator().manual_seed(19)
+    x = torch.randn(3000, 640, generator=g).to(DEV)
+    weight, rows = quantize_rows(torch.randn(1200, 640, generator=g).to(DEV)), quantize_rows(x)
+    bias = torch.randn(1200, generator=g).to(DEV)
+
+    def apart(t):
+        return torch.zeros(*t.shape, 2, dtype=t.dtype, device=DEV)[..., 0].copy_(t)
+
+    def make():
+        first = [apart(rows.codes), apart(rows.scales)] if quantized else [apart(x)]
+        return first + [apart(weight.codes), apart(weight.scales), apart(bias)]
+
+    def call(inputs):
+        *first, codes, scales, added = inputs
+        return int8_linear(QuantizedRows(*first) if quantized else first[0], QuantizedRows(codes, scales), added,
+                           dtype=torch.float32)
+
+    want = call(make())
+    inputs = make()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        got = call(inputs)
+    sizes = [(t.untyped_storage().nbytes(), t.untyped_storage().data_ptr()) for t in inputs]
+    del inputs
+    others = [torch.full((size,), 119, dtype=torch.uint8, device=DEV) for size, _ in sizes]
+    assert not {t.data_ptr() for t in others} & {at for _, at in sizes}
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
 def test_results_past_32_bit_offsets(announce):
     """A result of more than 2^32 elements, and rows of codes more than 2^32 bytes behind the first."""
     announce()
