@@ -228,4 +228,6 @@ class LayerNorm(torch.nn.LayerNorm):
             raise ValueError("LayerNorm normalises over the last axis alone")
 
     def forward(self, x):
+        if x.shape[-1:] != self.normalized_shape:
+            raise ValueError(f"Expected rows of {self.normalized_shape[0]} channels, got {tuple(x.shape)}")
         return layer_norm(x, self.weight, self.bias, self.eps)
