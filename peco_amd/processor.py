@@ -125,13 +125,18 @@ def _apply_rotary_emb(x, freqs_cis):
     return (x.float() * cos + rotated.float() * sin).to(x.dtype)
 
 
+def _unwatched(module):
+    """True where nothing is attached to a call of ``module`` that could see what it is called with."""
+    hooks = torch.nn.modules.module
+    return "forward" not in vars(module) and not module._forward_hooks and not module._forward_pre_hooks and \
+        not hooks._global_forward_hooks and not hooks._global_forward_pre_hooks
+
+
 def _per_channel_norm(norm):
     """True for a norm module that acts on the last axis alone, whatever the axes before it, with
     nothing attached that could see the shape it is called with."""
-    hooks = torch.nn.modules.module
     return type(norm) in (torch.nn.RMSNorm, torch.nn.LayerNorm, LayerNorm) and len(norm.normalized_shape) == 1 and \
-        "forward" not in vars(norm) and not norm._forward_hooks and not norm._forward_pre_hooks and \
-        not hooks._global_forward_hooks and not hooks._global_forward_pre_hooks
+        _unwatched(norm)
 
 
 def _rms_norm(norm, part):
@@ -208,8 +213,7 @@ def _placeable(part, buffer):
 def _shared_rows(source, projections):
     """The rows that the projections of one source take: quantized once where all of them are 8-bit layers (with nothing
     attached that looks at their input)."""
-    if isinstance(source, torch.Tensor) and all(
-            type(p) is Int8Linear and not p._forward_pre_hooks and not p._forward_hooks for p in projections):
+    if isinstance(source, torch.Tensor) and all(type(p) is Int8Linear and _unwatched(p) for p in projections):
         return quantize_rows(source)
     return source
 
