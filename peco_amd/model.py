@@ -92,19 +92,47 @@ def reset_state(pipe):
 _PROJECTIONS = ("to_q", "to_k", "to_v", "add_q_proj", "add_k_proj", "add_v_proj", "to_add_out")
 
 
+def _projection_places(transformer):
+    """(block's number, owner, name or index, layer) of every ``torch.nn.Linear`` among the blocks' projections."""
+    places = {}
+    for number, block in enumerate((*transformer.transformer_blocks, *transformer.single_transformer_blocks)):
+        attn = block.attn
+        out = getattr(attn, "to_out", None)
+        own = [(attn, name, getattr(attn, name, None)) for name in (*_PROJECTIONS, "to_out")]
+        if isinstance(out, (torch.nn.ModuleList, torch.nn.Sequential, list)) and len(out):
+            own.append((out, 0, out[0]))
+        for owner, key, layer in own:
+            if type(layer) is torch.nn.Linear:
+                places.setdefault((id(owner), key), (number, owner, key, layer))
+    return list(places.values())
+
+
+def _attached(layer):
+    """Whether something hangs on this module that would be lost with it."""
+    return "forward" in vars(layer) or any(
+        (layer._forward_hooks, layer._forward_pre_hooks, layer._backward_hooks, layer._backward_pre_hooks))
+
+
 def quantize_projections(pipe):
     """Put ``projection.Int8Linear`` in the place of every ``torch.nn.Linear`` among the projections of
-    ``pipe.transformer``'s attention blocks (``to_out``'s first layer too); return how many. For inference."""
-    transformer, count = pipe.transformer, 0
-    for block in (*transformer.transformer_blocks, *transformer.single_transformer_blocks):
-        attn = block.attn
-        for name in _PROJECTIONS:
-            layer = getattr(attn, name, None)
-            if type(layer) is torch.nn.Linear:
-                setattr(attn, name, projection.Int8Linear.from_linear(layer))
-                count += 1
-        out = getattr(attn, "to_out", None)
-        if out is not None and len(out) and type(out[0]) is torch.nn.Linear:
-            out[0] = projection.Int8Linear.from_linear(out[0])
-            count += 1
-    return count
+    ``pipe.transformer``'s attention blocks (``to_out`` or its first layer too); return how many places. For inference.
+
+    All layers are made before the first is replaced, so a layer that is refused (on the CPU, of more than 16384
+    channels, with hooks or a ``forward`` of its own, which would be lost) leaves the transformer as it was. A layer in
+    several places stays one.
+    """
+    places, made = _projection_places(pipe.transformer), {}
+    for number, owner, key, layer in places:
+        if _attached(layer):
+            name = key if isinstance(key, str) else f"to_out.{key}"
+            raise RuntimeError(f"attention of block {number}: {name} has hooks or a forward of its own, which an 8-bit "
+                               "layer in its place would not have")
+    for *_, layer in places:
+        if id(layer) not in made:
+            made[id(layer)] = projection.Int8Linear.from_linear(layer)
+    for _, owner, key, layer in places:
+        if isinstance(key, str):
+            setattr(owner, key, made[id(layer)])
+        else:
+            owner[key] = made[id(layer)]
+    return len(places)

@@ -1,9 +1,11 @@
 """The modules around a block's attention, as far as they go without a GPU: what they refuse, what they keep and what they
 leave alone."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 
-from peco_amd import processor
+from peco_amd import model, processor, projection
 from peco_amd.norm import LayerNorm
 from peco_amd.projection import Int8Linear, QuantizedRows
 
@@ -52,3 +54,76 @@ def test_layers_that_something_watches_share_no_rows(watch, monkeypatch):
         assert processor._shared_rows(source, layers) is source
     finally:
         remove()
+
+
+class _Attn(torch.nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.to_q, self.to_k, self.to_v = (torch.nn.Linear(32, 32) for _ in range(3))
+        self.to_out = torch.nn.ModuleList([torch.nn.Linear(32, 32), torch.nn.Dropout(0.0)])
+
+
+def _pipe(*attns):
+    blocks = [SimpleNamespace(attn=a) for a in attns]
+    return SimpleNamespace(transformer=SimpleNamespace(transformer_blocks=blocks[:1], single_transformer_blocks=blocks[1:]))
+
+
+def _layers(attn):
+    return attn.to_q, attn.to_k, attn.to_v, attn.to_out[0]
+
+
+def _stand_in(monkeypatch, refused=lambda: None):
+    """from_linear without a GPU; ``refused()`` is a layer that it does not take."""
+    def make(layer):
+        if layer is refused():
+            raise ValueError("not this one")
+        return _int8_layer(layer.out_features, layer.in_features)
+
+    monkeypatch.setattr(projection.Int8Linear, "from_linear", make)
+
+
+def test_a_refused_layer_leaves_the_transformer_as_it_was(monkeypatch):
+    attns = _Attn(), _Attn()
+    _stand_in(monkeypatch, lambda: attns[1].to_out[0])
+    before = [_layers(a) for a in attns]
+    with pytest.raises(ValueError, match="not this one"):
+        model.quantize_projections(_pipe(*attns))
+    assert all(a is b for attn, old in zip(attns, before) for a, b in zip(_layers(attn), old))
+    _stand_in(monkeypatch)
+    assert model.quantize_projections(_pipe(*attns)) == 8
+    assert all(type(layer) is Int8Linear for attn in attns for layer in _layers(attn))
+    assert model.quantize_projections(_pipe(*attns)) == 0
+
+
+@pytest.mark.parametrize("attach", [
+    lambda layer: layer.register_forward_hook(lambda *a: None),
+    lambda layer: layer.register_forward_pre_hook(lambda *a: None),
+    lambda layer: layer.register_full_backward_hook(lambda *a: None),
+    lambda layer: layer.register_full_backward_pre_hook(lambda *a: None),
+    lambda layer: setattr(layer, "forward", torch.nn.functional.relu),
+])
+def test_a_layer_with_something_attached_is_refused(attach, monkeypatch):
+    """It would be lost with the layer."""
+    _stand_in(monkeypatch)
+    attns = _Attn(), _Attn()
+    attach(attns[1].to_v)
+    before = [_layers(a) for a in attns]
+    with pytest.raises(RuntimeError, match=r"block 1.*to_v"):
+        model.quantize_projections(_pipe(*attns))
+    assert all(a is b for attn, old in zip(attns, before) for a, b in zip(_layers(attn), old))
+
+
+def test_a_layer_in_several_places_stays_one(monkeypatch):
+    _stand_in(monkeypatch)
+    attns = _Attn(), _Attn()
+    attns[1].to_q = attns[0].to_k = attns[0].to_q
+    assert model.quantize_projections(_pipe(*attns, attns[0])) == 8  # (a block's attention that comes twice)
+    assert attns[1].to_q is attns[0].to_q and attns[0].to_k is attns[0].to_q and attns[0].to_v is not attns[0].to_q
+
+
+def test_an_output_projection_without_a_list(monkeypatch):
+    _stand_in(monkeypatch)
+    attns = _Attn(), _Attn(), _Attn()
+    attns[0].to_out, attns[1].to_out, attns[2].to_out = torch.nn.Linear(32, 32), torch.nn.Identity(), None
+    assert model.quantize_projections(_pipe(*attns)) == 10
+    assert type(attns[0].to_out) is Int8Linear and type(attns[1].to_out) is torch.nn.Identity
