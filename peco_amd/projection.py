@@ -230,6 +230,13 @@ def int8_linear(x, weight: QuantizedRows, bias: torch.Tensor | None = None, *,
     return out
 
 
+def _laid_out(codes):
+    """A weight's codes [N, K] in rows that the product takes without a copy."""
+    if codes.stride(-1) == 1 and codes.stride(0) % 16 == 0:
+        return codes
+    return empty_codes(codes)[0].copy_(codes)
+
+
 class Int8Linear(torch.nn.Module):
     """A linear layer in 8 bits, for inference: ``int8_linear`` with a weight that is quantized once.
 
@@ -242,8 +249,8 @@ class Int8Linear(torch.nn.Module):
         super().__init__()
         self.out_features, self.in_features = weight.shape
         self.dtype = dtype
-        # (The scales and the bias stay fp32, whatever the module is cast to.)
-        self.register_buffer("codes", weight.codes)
+        # (The scales and the bias stay fp32, whatever the module is cast to, and the codes' rows on 16 bytes.)
+        self.register_buffer("codes", _laid_out(weight.codes))
         self.register_buffer("scales", weight.scales)
         self.register_buffer("bias", None if bias is None else bias.float())
 
@@ -254,9 +261,11 @@ class Int8Linear(torch.nn.Module):
         return cls(quantize_rows(layer.weight.detach()), bias, layer.weight.dtype)
 
     def _apply(self, fn, recurse=True):
-        wide = self.scales, self.bias
+        before = self.scales, self.bias
         super()._apply(fn, recurse)
-        self.scales, self.bias = (None if t is None else t.to(self.codes.device) for t in wide)
+        self.codes = _laid_out(self.codes)  # (a move to another device makes them dense)
+        self.scales, self.bias = (now if now is None or now.dtype == torch.float32 else was.to(now.device)
+                                  for was, now in zip(before, (self.scales, self.bias)))
         return self
 
     def forward(self, x, dtype: torch.dtype | None = None):

@@ -127,3 +127,34 @@ def test_an_output_projection_without_a_list(monkeypatch):
     attns[0].to_out, attns[1].to_out, attns[2].to_out = torch.nn.Linear(32, 32), torch.nn.Identity(), None
     assert model.quantize_projections(_pipe(*attns)) == 10
     assert type(attns[0].to_out) is Int8Linear and type(attns[1].to_out) is torch.nn.Identity
+
+
+def test_a_layer_that_moves_keeps_its_rows_on_16_bytes():
+    """(Rows a fixed number of 16 bytes apart are what a call takes without a copy.)"""
+    for channels, pitch in ((20, 32), (32, 32), (600, 640)):
+        layer = _int8_layer(8, channels)
+        codes, scales, bias = layer.codes.clone(), layer.scales.clone(), layer.bias.clone()
+        assert layer.codes.stride() == (pitch, 1)
+        for move in (lambda: layer.to("meta"), lambda: layer.to_empty(device="cpu"), layer.half, layer.double,
+                     lambda: layer.to("cpu", torch.bfloat16)):
+            move()
+            assert layer.codes.shape == (8, channels) and layer.codes.stride() == (pitch, 1)
+            assert layer.codes.dtype == torch.int8 and layer.scales.dtype == layer.bias.dtype == torch.float32
+            assert layer.codes.device == layer.scales.device == layer.bias.device
+            if layer.codes.device.type == "cpu":
+                for kept, t in ((layer.codes, codes), (layer.scales, scales), (layer.bias, bias)):
+                    assert kept.copy_(t) is kept
+    layer = _int8_layer(8, 20, bias=False)
+    assert layer.half().bias is None
+    codes = layer.codes
+    layer.float()
+    assert layer.codes is codes  # (as it was)
+
+
+def test_values_stay_through_a_cast():
+    layer = _int8_layer(8, 20)
+    codes, scales, bias = layer.codes.clone(), layer.scales.clone(), layer.bias.clone()
+    for change in (layer.half, layer.double, layer.bfloat16):
+        change()
+        assert torch.equal(layer.codes, codes) and torch.equal(layer.scales, scales) and torch.equal(layer.bias, bias)
+    assert layer.share_memory() is layer and layer.codes.is_shared() and layer.scales.is_shared()
