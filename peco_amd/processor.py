@@ -221,7 +221,7 @@ def _shared_rows(source, projections):
 def _project(projection, source, rows):
     """``projection(source)`` on the source's shared rows."""
     if isinstance(source, torch.Tensor) and isinstance(rows, QuantizedRows):
-        return projection(rows, dtype=source.dtype)
+        return projection(rows, dtype=projection.result_dtype(source))
     return projection(rows)
 
 

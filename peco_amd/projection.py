@@ -241,8 +241,8 @@ class Int8Linear(torch.nn.Module):
     """A linear layer in 8 bits, for inference: ``int8_linear`` with a weight that is quantized once.
 
     ``Int8Linear.from_linear(layer)`` takes a ``torch.nn.Linear``'s weight and bias. It takes tensors, or
-    QuantizedRows that several layers share; the result has ``dtype``, else the tensor's or, for QuantizedRows, the dtype
-    of the layer it was made of.
+    QuantizedRows that several layers share; the result has ``dtype``, else autocast's where that is enabled, else the
+    tensor's or, for QuantizedRows, the dtype of the layer it was made of.
     """
 
     def __init__(self, weight: QuantizedRows, bias: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16):
@@ -268,10 +268,15 @@ class Int8Linear(torch.nn.Module):
                                   for was, now in zip(before, (self.scales, self.bias)))
         return self
 
+    def result_dtype(self, x) -> torch.dtype:
+        """The dtype of ``forward(x)``."""
+        if torch.is_autocast_enabled("cuda"):
+            return torch.get_autocast_dtype("cuda")
+        return self.dtype if isinstance(x, QuantizedRows) else x.dtype
+
     def forward(self, x, dtype: torch.dtype | None = None):
-        if dtype is None:
-            dtype = self.dtype if isinstance(x, QuantizedRows) else x.dtype
-        return int8_linear(x, QuantizedRows(self.codes, self.scales), self.bias, dtype=dtype)
+        return int8_linear(x, QuantizedRows(self.codes, self.scales), self.bias,
+                           dtype=self.result_dtype(x) if dtype is None else dtype)
 
     def extra_repr(self):
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"

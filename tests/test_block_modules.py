@@ -158,3 +158,30 @@ def test_values_stay_through_a_cast():
         change()
         assert torch.equal(layer.codes, codes) and torch.equal(layer.scales, scales) and torch.equal(layer.bias, bias)
     assert layer.share_memory() is layer and layer.codes.is_shared() and layer.scales.is_shared()
+
+
+def test_results_under_autocast_have_its_dtype(monkeypatch):
+    """As those of the torch.nn.Linear whose place a layer takes; without it the rows' (codes: the layer's)."""
+    asked = []
+    monkeypatch.setattr(projection, "int8_linear", lambda x, weight, bias, dtype: asked.append(dtype))
+    monkeypatch.setattr(processor, "quantize_rows", lambda x: codes)
+    layers, x = [_int8_layer() for _ in range(3)], torch.zeros(2, 32)
+    codes = QuantizedRows(torch.zeros(2, 32, dtype=torch.int8), torch.zeros(2))
+
+    def calls():
+        asked.clear()
+        layers[0](x), layers[0](codes), layers[0](x, dtype=torch.float32)
+        processor._project(layers[0], x, processor._shared_rows(x, layers))
+        processor._project(layers[0], codes, processor._shared_rows(codes, layers))
+        return asked
+
+    assert calls() == [torch.float32, torch.bfloat16, torch.float32, torch.float32, torch.bfloat16]
+    kept = torch.get_autocast_dtype("cuda")
+    try:  # (what torch.autocast sets, which does nothing without a GPU)
+        torch.set_autocast_enabled("cuda", True)
+        for dtype in (torch.float16, torch.bfloat16):
+            torch.set_autocast_dtype("cuda", dtype)
+            assert calls() == [dtype, dtype, torch.float32, dtype, dtype]
+    finally:
+        torch.set_autocast_enabled("cuda", False)
+        torch.set_autocast_dtype("cuda", kept)
