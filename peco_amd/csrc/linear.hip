@@ -470,16 +470,41 @@ template <int OT, typename T> int launch_product(ProductArgs p, hipStream_t s) {
 // rounds, in units of a middle tile a CU, which run one behind the other: a round of wide tiles costs as much
 // as 3.2 of them, the last one 2.3 and as much of 0.9 as it fills (2048 x 2048 in the channels: 768 middle tiles 31.4 us, 192
 // wide ones 27.2; 2048 x 4096 x 4096, 512 and 128, 35.9 and 41.7; 7006 x 6144 x 2048, 2640 and 672, 100 and 88).
-template <int OT> int launch_type(const ProductArgs& p, hipStream_t s) {
-    if (p.m <= 16) return launch_few<OT, 1, false>(p, {}, s);
-    if (p.m <= 32) return launch_few<OT, 2, false>(p, {}, s);
+enum class Form { kFew, kFew2, kSmall, kMid, kWide };
+Form form_of(int64_t m, int64_t n) {
+    if (m <= 16) return Form::kFew;
+    if (m <= 32) return Form::kFew2;
     const int64_t cus = device_compute_units();
-    const auto tiles = [&](int side) { return ceil_div(p.m, side) * ceil_div(p.n, side); };
-    if (tiles(Small::kTokens) <= 2 * cus) return launch_product<OT, Small>(p, s);
+    const auto tiles = [&](int side) { return ceil_div(m, side) * ceil_div(n, side); };
+    if (tiles(Small::kTokens) <= 2 * cus) return Form::kSmall;
     const double wide = static_cast<double>(tiles(Wide::kTokens)) / cus, rounds = static_cast<double>(static_cast<int64_t>(wide));
     const double rest = wide - rounds, cost = 3.2 * rounds + (rest > 0.0 ? 2.3 + 0.9 * rest : 0.0);
-    if (cost <= static_cast<double>(tiles(Mid::kTokens)) / cus) return launch_product<OT, Wide>(p, s);
-    return launch_product<OT, Mid>(p, s);
+    return cost <= static_cast<double>(tiles(Mid::kTokens)) / cus ? Form::kWide : Form::kMid;
+}
+
+// Whether the product's launch is one (asked before the rows' launch).
+bool fits_launch(int64_t m, int64_t n) {
+    const auto tiles = [&](auto tile) {
+        using T = decltype(tile);
+        return fits_grid(ceil_div(m, T::kTokens) * ceil_div(n, T::kOutputs), T::kThreads);
+    };
+    switch (form_of(m, n)) {
+        case Form::kFew:
+        case Form::kFew2: return fits_grid(ceil_div(n, kFewOutputs), kFewWaves * kWave);
+        case Form::kSmall: return tiles(Small{});
+        case Form::kMid: return tiles(Mid{});
+        default: return tiles(Wide{});
+    }
+}
+
+template <int OT> int launch_type(const ProductArgs& p, hipStream_t s) {
+    switch (form_of(p.m, p.n)) {
+        case Form::kFew: return launch_few<OT, 1, false>(p, {}, s);
+        case Form::kFew2: return launch_few<OT, 2, false>(p, {}, s);
+        case Form::kSmall: return launch_product<OT, Small>(p, s);
+        case Form::kMid: return launch_product<OT, Mid>(p, s);
+        default: return launch_product<OT, Wide>(p, s);
+    }
 }
 
 }  // namespace
@@ -497,8 +522,7 @@ int check_product(const int8_t* weight, int64_t weight_pitch, const float* weigh
     if (dtype != kBF16 && dtype != kF16 && dtype != kF32) return kUnsupportedDtype;
     // Sums of 2^17 products of -128 would leave 32 bits, and a tile's offsets are 32 bits.
     if (channels >= 1 << 17 || weight_pitch > 1 << 22 || rows > 0x3fffffff || outputs > 0x3fffffff) return kUnsupportedShape;
-    // (Results that large take wide tiles.)
-    return fits_grid(ceil_div(rows, Wide::kTokens) * ceil_div(outputs, Wide::kOutputs), Wide::kThreads) ? kOk : kUnsupportedShape;
+    return fits_launch(rows, outputs) ? kOk : kUnsupportedShape;
 }
 
 int run_product(const ProductArgs& p, int dtype, hipStream_t s) {
