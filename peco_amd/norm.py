@@ -182,7 +182,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     first); the result has the strides of ``empty_like(x)``. Weight and bias have the rows' dtype or float32 and shape
     [C], or [B, C]: one for each entry of the rows' first axis, as a block's modulation gives them. ``around_one``
     multiplies with 1 + weight. Statistics and arithmetic are fp32, the result is rounded once. A row with an
-    infinity or a NaN gives NaN and leaves the others as they are.
+    infinity or a NaN gives NaN and leaves the others as they are. Rows with deviations past 10^19, whose squares leave
+    fp32, are out of its range.
 
     Differentiable once in x, weight and bias; all sums of the gradients are fp32 in a fixed order, so they repeat bit for
     bit. The gradient of the result must be an ordinary tensor (no batch of gradients, no tangent). A backward pass may be
@@ -220,7 +221,7 @@ def layer_norm_rows(x: torch.Tensor, weight: torch.Tensor | None = None, bias: t
 
 
 class LayerNorm(torch.nn.LayerNorm):
-    """``torch.nn.LayerNorm`` over the last axis by ``layer_norm``."""
+    """``torch.nn.LayerNorm`` over the last axis by ``layer_norm``; its results have the rows' dtype, under autocast too."""
 
     def __init__(self, *args, **kwargs):
         super().__init__(*args, **kwargs)
