@@ -156,8 +156,8 @@ def int8_linear(x, weight: QuantizedRows, bias: torch.Tensor | None = None, *,
 
     x is a tensor (fp16, bf16 or fp32, up to 16384 channels), whose rows are quantized as ``quantize_rows`` does, or
     ``QuantizedRows`` (K below 2^17). The sums over K are exact integers; scales and bias (of the result's dtype or
-    float32) are applied in fp32, the row's scale first, and the result is rounded once, to ``dtype`` (default: x's, bfloat16 for
-    QuantizedRows). For inference: it has no gradient. Weight rows that do not start on 16 bytes a fixed distance
+    float32) are applied in fp32, the row's scale first (the sum times it has to be a number of fp32), and the result is
+    rounded once, to ``dtype`` (default: x's, bfloat16 for QuantizedRows). For inference: it has no gradient. Weight rows that do not start on 16 bytes a fixed distance
     apart are copied by each call (``quantize_rows`` lays them out so).
     """
     if not isinstance(weight, QuantizedRows):
