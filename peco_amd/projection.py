@@ -157,8 +157,9 @@ def int8_linear(x, weight: QuantizedRows, bias: torch.Tensor | None = None, *,
     x is a tensor (fp16, bf16 or fp32, up to 16384 channels), whose rows are quantized as ``quantize_rows`` does, or
     ``QuantizedRows`` (K below 2^17). The sums over K are exact integers; scales and bias (of the result's dtype or
     float32) are applied in fp32, the row's scale first (the sum times it has to be a number of fp32), and the result is
-    rounded once, to ``dtype`` (default: x's, bfloat16 for QuantizedRows). For inference: it has no gradient. Weight rows that do not start on 16 bytes a fixed distance
-    apart are copied by each call (``quantize_rows`` lays them out so).
+    rounded once, to ``dtype`` (default: x's, bfloat16 for QuantizedRows). N is below 2^30, for up to 32 rows below 2^27.
+    For inference: it has no gradient. Weight rows that do not start on 16 bytes a fixed distance apart are copied by each
+    call (``quantize_rows`` lays them out so).
     """
     if not isinstance(weight, QuantizedRows):
         raise TypeError("weight must be QuantizedRows")
@@ -200,8 +201,10 @@ def int8_linear(x, weight: QuantizedRows, bias: torch.Tensor | None = None, *,
         _check_rows(x, "int8_linear")
     if outputs >= 1 << 30:
         raise ValueError("int8_linear supports fewer than 2^30 outputs")
-    out = torch.empty((*rows.shape[:-1], outputs), dtype=dtype, device=device)
     count = rows.numel() // channels
+    if 1 <= count <= 32 and outputs >= 1 << 27:  # (16 a workgroup of 512 lanes, 2^32 lanes a launch)
+        raise ValueError("int8_linear supports fewer than 2^27 outputs of up to 32 rows")
+    out = torch.empty((*rows.shape[:-1], outputs), dtype=dtype, device=device)
     if count == 0:
         return out
     with _native.on_device(device):

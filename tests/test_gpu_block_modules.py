@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from peco_amd import model
-from peco_amd.projection import Int8Linear, quantize_rows
+from peco_amd.projection import Int8Linear, QuantizedRows, int8_linear, quantize_rows
 from test_gpu_block_projection import DEV, DIM, HEADS, TEXT, VIDEO, _call, _pipe
 from test_processor_call import _Attn
 
@@ -86,3 +86,17 @@ def test_autocast(dtype, announce):
         want = attn.to_v(quantize_rows(x), dtype=dtype).unflatten(2, (HEADS, DIM)).transpose(1, 2)
         assert torch.equal(v[:, :, :VIDEO], want)
         assert attn.to_q(x).dtype == torch.float32
+
+
+@pytest.mark.gpu
+def test_results_of_few_rows_that_no_launch_holds(announce):
+    """Refused before the result's gigabytes are allocated."""
+    announce()
+    weight = QuantizedRows(torch.zeros(1, 16, dtype=torch.int8, device=DEV).expand(1 << 27, 16),
+                           torch.zeros(1, device=DEV).expand(1 << 27))
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    for rows in (1, 17, 32):
+        with pytest.raises(ValueError, match="2\\^27"):
+            int8_linear(torch.zeros(rows, 16, device=DEV), weight)
+    assert torch.cuda.max_memory_allocated() - before < 1 << 20
