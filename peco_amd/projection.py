@@ -235,7 +235,8 @@ def int8_linear(x, weight: QuantizedRows, bias: torch.Tensor | None = None, *,
 
 def _laid_out(codes):
     """A weight's codes [N, K] in rows that the product takes without a copy."""
-    if codes.stride(-1) == 1 and codes.stride(0) % 16 == 0:
+    if codes.stride(-1) == 1 and codes.stride(0) % 16 == 0 and codes.stride(0) <= 1 << 22 and \
+            codes.storage_offset() % 16 == 0:  # (a storage starts on 16 bytes; on the meta device there is no address)
         return codes
     return empty_codes(codes)[0].copy_(codes)
 

@@ -100,3 +100,14 @@ def test_results_of_few_rows_that_no_launch_holds(announce):
         with pytest.raises(ValueError, match="2\\^27"):
             int8_linear(torch.zeros(rows, 16, device=DEV), weight)
     assert torch.cuda.max_memory_allocated() - before < 1 << 20
+
+
+@pytest.mark.gpu
+def test_a_layer_of_codes_off_16_bytes(announce):
+    announce()
+    flat = torch.randint(-127, 128, (200 * 32 + 8,), device=DEV).to(torch.int8)
+    scales, x = torch.rand(200, device=DEV), torch.randn(40, 32, device=DEV)
+    weight = QuantizedRows(flat[8:].view(200, 32), scales)
+    layer = Int8Linear(weight)
+    assert layer.codes.data_ptr() % 16 == 0 and torch.equal(layer.codes, weight.codes)
+    assert torch.equal(layer(x), int8_linear(x, weight))
