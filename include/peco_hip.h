@@ -428,7 +428,8 @@ int peco_quantize_rows(const void* x, const int64_t* strides, int8_t* codes, int
  * channels] (int8, exact in 32 bits: channels < 2^17), times scales [rows] times weight_scales [outputs] plus bias
  * (nullable, [outputs] of dtype, or fp32 with bias_wide != 0) in fp32, rounded once. Rows of codes and weight start on
  * 16 bytes, pitch and weight_pitch (up to 2^22) bytes apart; the bytes behind a row's channels, up to the next 16, are read and
- * count for nothing. */
+ * count for nothing. Results of more workgroups than a launch holds (2^27 outputs of up to 32 rows) are refused before any
+ * launch. */
 int peco_int8_linear(const int8_t* codes, int64_t pitch, const float* scales, const int8_t* weight,
                      int64_t weight_pitch, const float* weight_scales, const void* bias, int bias_wide, void* output,
                      int rows, int channels, int outputs, int dtype, void* stream);
